@@ -224,6 +224,57 @@ XTG_CUDA_API int xtg_cuda_kv_store(const float* k, const float* v, int64_t pos, 
                       int dtype, uint8_t* k_codes, uint8_t* v_codes, float* k_scales, float* v_scales, void* stream,
                       char* err, int err_len);
 
+// ---- a paged key/value cache held in 4 bits (no counterpart in the reference, whose caches are 8-bit) ----
+// pool: `pages` pages x kv_heads blocks of 72 head_dim bytes (16-byte aligned, head_dim 64, 128 or 256): 64 positions
+// of one KV head, K and V, 4.5 bits a value. Each group of 64 head dims of a position has a scale s and an offset z
+// (bf16), and a code c in 0 .. 15 stands for s (c - 8) + z:
+//   lo, hi = min, max of the group;  s = bf16, rounded up, of max(2^-100, (hi - lo) (1 / 15));  z = bf16(lo + 8 s);
+//   c = clamp(rint((x - z) (1 / s)), -8, 7) + 8, all in f32; a group that holds a NaN or an infinity reads back as NaN.
+// A block's bytes (csrc/kv4.h has the order of the codes): K codes, K's (s, z) words, V codes, V's (s, z) words.
+//
+// A call covers rows of several sequences: rows cu_rows[i] .. cu_rows[i + 1] - 1 of its arrays are sequence i's, at
+// positions pos[i], pos[i] + 1, ... Position p of sequence i is slot p % 64 of page table[i][p / 64]. A negative table
+// entry or position holds nothing: a store skips it, a load gives zeros, attention does not see it. table, pos, cu_rows
+// and err are device memory, read when the call runs on `stream` (a captured call follows their later contents); the
+// calls allocate nothing and do not wait. Rows past cu_rows[seqs] are left alone. A position past the table or a page
+// past the pool is treated as nothing there and recorded in *err (6, 7; 1 when a device wait timed out).
+// Two sequences of one store must not write the same page. Sequences may share pages that are only read.
+typedef struct {
+  uint8_t* pool;
+  int64_t pages;
+  int kv_heads, head_dim;
+  const int32_t* table;     // [seqs][max_pages]
+  int max_pages, seqs;
+  const int32_t* pos;       // [seqs]
+  const int32_t* cu_rows;   // [seqs + 1], from 0, not decreasing
+  int64_t rows;             // rows of this call's arrays, below 2^31
+  int32_t* err;             // one word, or NULL
+} xtg_cuda_kv4;
+
+// dtype of rows: 0 f32, 1 bf16, 2 f16. Pointers start on 16-byte boundaries and strides (in elements) are multiples of
+// 16 bytes; the head_dim values of a row's head are contiguous.
+//
+// Quantise rows k, v [rows][kv_heads][head_dim] into the cache. The other slots of the pages keep their contents.
+XTG_CUDA_API int xtg_cuda_kv4_store(const xtg_cuda_kv4* c, const void* k, const void* v, int dtype, int64_t k_row,
+                                    int64_t k_head, int64_t v_row, int64_t v_head, void* stream, char* err,
+                                    int err_len);
+// Read the rows' positions back into k, v [rows][kv_heads][head_dim] (contiguous).
+XTG_CUDA_API int xtg_cuda_kv4_load(const xtg_cuda_kv4* c, void* k, void* v, int dtype, void* stream, char* err,
+                                   int err_len);
+// Bytes of xtg_cuda_kv4_attention's workspace on the current device; -1 for bad arguments.
+XTG_CUDA_API int64_t xtg_cuda_kv4_workspace(int heads, int kv_heads, int head_dim, int rows_per_seq);
+// out [rows][heads][head_dim] (contiguous, q's type): softmax(scale q . K) V of each row over the cached positions up
+// to its own (with window > 0 only the last `window` of these); the row's own position counts, so the call's keys and
+// values are stored first. heads a multiple of kv_heads, q head j reads KV head j / (heads / kv_heads). A row that
+// sees nothing gives zeros. rows_per_seq >= 1: about how many rows a sequence has; it chooses the tiling, the result
+// holds for any. workspace: device memory of at least xtg_cuda_kv4_workspace bytes, 16-byte aligned, not shared by
+// calls that may overlap. Sums, softmax and outputs before their last rounding are f32; a call's result does not
+// depend on timing (no atomics).
+XTG_CUDA_API int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, void* out, int dtype, int heads,
+                                        int64_t q_row, int64_t q_head, float scale, int window, int rows_per_seq,
+                                        void* workspace, int64_t workspace_bytes, void* stream, char* err,
+                                        int err_len);
+
 // The seeded generators (device; bit-identical with the oracle's xo_gen_*): what 0 normal bf16 (a = stddev),
 // 1 uniform f32 in [a, b), 2 int8 in [-127, 127].
 XTG_CUDA_API int xtg_cuda_gen(int what, uint64_t seed, uint64_t stream_id, float a, float b, void* out, int64_t n, void* stream,

@@ -38,6 +38,13 @@ class AttnArgs(C.Structure):
                 ("ring_pos", C.c_void_p), ("dtype", C.c_int), ("out", C.c_void_p)]
 
 
+class Kv4(C.Structure):
+    """xtg_cuda_kv4: a 4-bit paged cache and where a call's rows stand in it."""
+    _fields_ = [("pool", C.c_void_p), ("pages", C.c_int64), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("table", C.c_void_p), ("max_pages", C.c_int), ("seqs", C.c_int), ("pos", C.c_void_p),
+                ("cu_rows", C.c_void_p), ("rows", C.c_int64), ("err", C.c_void_p)]
+
+
 class Sampling(C.Structure):
     """xtg_cuda_sampling: Sampler::sample's parameters."""
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("min_p", C.c_float)]
@@ -123,6 +130,17 @@ def lib():
         L.xtg_cuda_kv_store.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int64, C.c_int,
                                         C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, E,
                                         C.c_int]
+        L.xtg_cuda_kv4_store.restype = C.c_int
+        L.xtg_cuda_kv4_store.argtypes = [C.POINTER(Kv4), C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64,
+                                         C.c_int64, C.c_int64, C.c_void_p, E, C.c_int]
+        L.xtg_cuda_kv4_load.restype = C.c_int
+        L.xtg_cuda_kv4_load.argtypes = [C.POINTER(Kv4), C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, E, C.c_int]
+        L.xtg_cuda_kv4_workspace.restype = C.c_int64
+        L.xtg_cuda_kv4_workspace.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int]
+        L.xtg_cuda_kv4_attention.restype = C.c_int
+        L.xtg_cuda_kv4_attention.argtypes = [C.POINTER(Kv4), C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int64,
+                                             C.c_int64, C.c_float, C.c_int, C.c_int, C.c_void_p, C.c_int64,
+                                             C.c_void_p, E, C.c_int]
         L.xtg_cuda_gen.restype = C.c_int
         L.xtg_cuda_gen.argtypes = [C.c_int, C.c_uint64, C.c_uint64, C.c_float, C.c_float, C.c_void_p, C.c_int64,
                                    C.c_void_p, E, C.c_int]
@@ -566,4 +584,139 @@ def kv_store(k, v, pos, slots, ring, dtype, k_codes, v_codes, k_scales, v_scales
 def gen(what, seed, stream_id, a, b, out):
     err = _err()
     _check(lib().xtg_cuda_gen(what, seed, stream_id, a, b, _ptr(out), out.numel(), _stream(), err, len(err)), err)
+    return out
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# A paged key/value cache held in 4 bits (include/xtg_cuda.h: xtg_cuda_kv4_*)
+#
+# pool: uint8 [pages][kv_heads][72 head_dim]. A call covers rows of several sequences: rows cu_rows[i] ..
+# cu_rows[i + 1] - 1 are sequence i's, at positions pos[i], pos[i] + 1, ...; position p of sequence i is slot p % 64 of
+# page table[i][p // 64], and a negative table entry or position holds nothing. table [seqs][max_pages], pos [seqs] and
+# cu_rows [seqs + 1] are int32 CUDA tensors, read when the call runs on the current stream of pool's device. err (an
+# int32 CUDA tensor of one word, or None) records positions past the table and pages past the pool, which hold nothing;
+# kv4_check raises what it holds.
+# ----------------------------------------------------------------------------------------------------------------
+
+KV4_PAGE = 64
+
+_KV4_ERRORS = {1: "a device wait timed out", 6: "a position lies past its sequence's page table",
+               7: "a page table entry lies past the pool"}
+_kv4_workspace_bytes = {}
+
+
+def _kv4_dtypes():
+    import torch
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def kv4_pool(pages, kv_heads, head_dim, device="cuda"):
+    """An empty pool (every value reads back as 0)."""
+    import torch
+    return torch.zeros((pages, kv_heads, 72 * head_dim), dtype=torch.uint8, device=device)
+
+
+def kv4_check(err):
+    """Wait for err's device, raise XtgError for a recorded error and clear it."""
+    code = int(err.item())
+    if code:
+        err.zero_()
+        raise XtgError("kv4: " + _KV4_ERRORS.get(code, f"error {code}"))
+
+
+def _kv4_where(pool, table, pos, cu_rows, rows, err):
+    import torch
+    dev = pool.device
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or not pool.is_contiguous() or not pool.is_cuda:
+        raise XtgError("kv4: pool is a contiguous uint8 CUDA tensor [pages][kv_heads][72 head_dim]")
+    pages, kvh, block = pool.shape
+    if block % 72 or block // 72 not in (64, 128, 256):
+        raise XtgError("kv4: head_dim 64, 128 or 256 (pool.shape[2] / 72)")
+    for name, t, dims in (("table", table, 2), ("pos", pos, 1), ("cu_rows", cu_rows, 1)):
+        if t.dtype != torch.int32 or t.dim() != dims or t.device != dev or not t.is_contiguous():
+            raise XtgError(f"kv4: {name} is a contiguous int32 tensor of {dims} dimension(s) on the pool's device")
+    seqs, max_pages = table.shape
+    if pos.shape[0] != seqs or cu_rows.shape[0] != seqs + 1:
+        raise XtgError("kv4: table [seqs][max_pages], pos [seqs], cu_rows [seqs + 1]")
+    if err is not None and (err.dtype != torch.int32 or err.numel() != 1 or err.device != dev):
+        raise XtgError("kv4: err is one int32 on the pool's device")
+    return Kv4(pool.data_ptr(), pages, kvh, block // 72, table.data_ptr(), max_pages, seqs, pos.data_ptr(),
+               cu_rows.data_ptr(), rows, err.data_ptr() if err is not None else None)
+
+
+def _kv4_rows(name, t, pool, heads):
+    """dtype code of rows t [rows][heads][head_dim] with contiguous head dims on the pool's device."""
+    dtype = _kv4_dtypes().get(t.dtype)
+    if dtype is None:
+        raise XtgError(f"kv4: {name} is float32, bfloat16 or float16")
+    if t.dim() != 3 or t.shape[2] * 72 != pool.shape[2] or (heads and t.shape[1] != heads) or t.device != pool.device:
+        raise XtgError(f"kv4: {name} is [rows][heads][head_dim] of the pool's head_dim on the pool's device")
+    if t.stride(2) != 1 and t.numel():
+        raise XtgError(f"kv4: {name}'s head dims must be contiguous")
+    return dtype
+
+
+def _kv4_call(pool, f, *args):
+    """Call entry point f with the pool's device current, on its current stream."""
+    import torch
+    err = _err()
+    if torch.cuda.current_device() == pool.device.index:
+        rc = f(*args, torch.cuda.current_stream().cuda_stream, err, len(err))
+    else:
+        with torch.cuda.device(pool.device):
+            rc = f(*args, torch.cuda.current_stream().cuda_stream, err, len(err))
+    _check(rc, err)
+
+
+def kv4_store(pool, k, v, table, pos, cu_rows, err=None):
+    """Quantise rows k, v [rows][kv_heads][head_dim] (float32, bfloat16 or float16; row and head strides of 16-byte
+    multiples) into the pool. Two sequences of a call must not write the same page."""
+    dtype = _kv4_rows("k", k, pool, pool.shape[1])
+    if _kv4_rows("v", v, pool, pool.shape[1]) != dtype or k.shape[0] != v.shape[0]:
+        raise XtgError("kv4: k and v have the same type and rows")
+    c = _kv4_where(pool, table, pos, cu_rows, k.shape[0], err)
+    _kv4_call(pool, lib().xtg_cuda_kv4_store, C.byref(c), k.data_ptr(), v.data_ptr(), dtype, k.stride(0), k.stride(1),
+              v.stride(0), v.stride(1))
+
+
+def kv4_load(pool, table, pos, cu_rows, rows, dtype=None, err=None):
+    """The cached keys and values of `rows` rows (cu_rows' last entry): (k, v) [rows][kv_heads][head_dim] of dtype
+    (default bfloat16)."""
+    import torch
+    dtype = dtype or torch.bfloat16
+    code = _kv4_dtypes().get(dtype)
+    if code is None:
+        raise XtgError("kv4: dtype is float32, bfloat16 or float16")
+    c = _kv4_where(pool, table, pos, cu_rows, rows, err)
+    k = torch.empty((rows, pool.shape[1], pool.shape[2] // 72), dtype=dtype, device=pool.device)
+    v = torch.empty_like(k)
+    _kv4_call(pool, lib().xtg_cuda_kv4_load, C.byref(c), k.data_ptr(), v.data_ptr(), code)
+    return k, v
+
+
+def kv4_attention(q, pool, table, pos, cu_rows, scale, window=0, rows_per_seq=None, out=None, err=None):
+    """Attention of rows q [rows][heads][head_dim] over the cached positions up to each row's own (window > 0: the last
+    `window` of these), after the call's rows were stored: [rows][heads][head_dim] in q's type. rows_per_seq: about how
+    many rows a sequence has (default rows / seqs); it chooses the tiling only."""
+    import torch
+    dtype = _kv4_rows("q", q, pool, 0)
+    rows, heads, d = q.shape
+    c = _kv4_where(pool, table, pos, cu_rows, rows, err)
+    if out is None:
+        out = torch.empty((rows, heads, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise XtgError("kv4: out is contiguous, of q's shape and type")
+    if rows_per_seq is None:
+        rows_per_seq = max(1, -(-rows // max(1, c.seqs)))
+    key = (pool.device.index, heads, c.kv_heads, d, rows_per_seq)
+    size = _kv4_workspace_bytes.get(key)
+    if size is None:
+        with torch.cuda.device(pool.device):
+            size = lib().xtg_cuda_kv4_workspace(heads, c.kv_heads, d, rows_per_seq)
+        if size < 0:
+            raise XtgError("kv4: q heads a multiple of KV heads, rows_per_seq at least 1")
+        _kv4_workspace_bytes[key] = size
+    work = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _kv4_call(pool, lib().xtg_cuda_kv4_attention, C.byref(c), q.data_ptr(), out.data_ptr(), dtype, heads, q.stride(0),
+              q.stride(1), scale, window, rows_per_seq, work.data_ptr(), size)
     return out

@@ -14,6 +14,7 @@
 #include "sampling.h"
 #include "fp4mma.cuh"
 #include "kernels.h"
+#include "kv4.h"
 
 using namespace xtg;
 
@@ -367,6 +368,96 @@ int xtg_cuda_kv_store(const float* k, const float* v, int64_t pos, int n, int kv
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     launch_kv_store(a, s);
     XTG_CUDA(cudaStreamSynchronize(s));
+  });
+}
+
+namespace {
+
+// The checks of a 4-bit cache call that need no device work; the kernels check what the device arrays hold.
+Kv4Where kv4_where(const xtg_cuda_kv4* c) {
+  XTG_REQUIRE(c, "kv4: no cache");
+  XTG_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "kv4: head_dim 64, 128 or 256");
+  XTG_REQUIRE(c->kv_heads >= 1 && c->kv_heads <= 65535, "kv4: 1..65535 KV heads");
+  XTG_REQUIRE(c->pages >= 1 && c->max_pages >= 1, "kv4: at least one page in the pool and per sequence");
+  XTG_REQUIRE(c->seqs >= 0 && c->rows >= 0 && c->rows < (1ll << 31), "kv4: sequences and rows in 0 .. 2^31 - 1");
+  XTG_REQUIRE(c->seqs < (1 << 29), "kv4: fewer than 2^29 sequences");
+  XTG_REQUIRE(c->pool && (c->seqs == 0 || (c->table && c->pos && c->cu_rows)), "kv4: null pointer");
+  XTG_REQUIRE(aligned16(c->pool), "kv4: the pool must start on a 16-byte boundary");
+  return {c->pool, c->pages, c->kv_heads, c->head_dim, c->table, c->max_pages, c->seqs, c->pos, c->cu_rows, c->rows,
+          c->err};
+}
+
+void kv4_require_rows(int dtype, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> strides) {
+  XTG_REQUIRE(dtype == kKv4F32 || dtype == kKv4Bf16 || dtype == kKv4F16, "kv4: rows of f32 (0), bf16 (1) or f16 (2)");
+  for (const void* p : pointers) {
+    XTG_REQUIRE(p, "kv4: null pointer");
+    XTG_REQUIRE(aligned16(p), "kv4: rows must start on a 16-byte boundary");
+  }
+  for (int64_t s : strides)
+    XTG_REQUIRE(s >= 0 && s % (dtype == kKv4F32 ? 4 : 8) == 0, "kv4: row and head strides must be multiples of 16 bytes");
+}
+
+int device_sms() {
+  int dev = 0, sms = 0;
+  XTG_CUDA(cudaGetDevice(&dev));
+  XTG_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  return sms;
+}
+
+void kv4_require_heads(int heads, int kv_heads, int rows_per_seq) {
+  XTG_REQUIRE(heads >= 1 && heads % kv_heads == 0, "kv4: q heads a multiple of KV heads");
+  XTG_REQUIRE(rows_per_seq >= 1, "kv4: rows_per_seq at least 1");
+}
+
+}  // namespace
+
+int xtg_cuda_kv4_store(const xtg_cuda_kv4* c, const void* k, const void* v, int dtype, int64_t k_row, int64_t k_head,
+                       int64_t v_row, int64_t v_head, void* stream, char* err, int err_len) {
+  return guarded(err, err_len, [&] {
+    const Kv4Where w = kv4_where(c);
+    if (w.rows == 0 || w.seqs == 0) return;
+    kv4_require_rows(dtype, {k, v}, {k_row, k_head, v_row, v_head});
+    launch_kv4_store(w, {const_cast<void*>(k), const_cast<void*>(v), dtype, k_row, k_head, v_row, v_head},
+                     static_cast<cudaStream_t>(stream));
+  });
+}
+
+int xtg_cuda_kv4_load(const xtg_cuda_kv4* c, void* k, void* v, int dtype, void* stream, char* err, int err_len) {
+  return guarded(err, err_len, [&] {
+    const Kv4Where w = kv4_where(c);
+    if (w.rows == 0 || w.seqs == 0) return;
+    kv4_require_rows(dtype, {k, v}, {});
+    const int64_t head = w.head_dim, row = head * w.kv_heads;
+    launch_kv4_load(w, {k, v, dtype, row, head, row, head}, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int64_t xtg_cuda_kv4_workspace(int heads, int kv_heads, int head_dim, int rows_per_seq) {
+  int64_t bytes = -1;
+  guarded(nullptr, 0, [&] {
+    XTG_REQUIRE(kv_heads >= 1 && (head_dim == 64 || head_dim == 128 || head_dim == 256), "kv4: bad shape");
+    kv4_require_heads(heads, kv_heads, rows_per_seq);
+    bytes = kv4_workspace_bytes(head_dim, heads / kv_heads, rows_per_seq, device_sms());
+  });
+  return bytes;
+}
+
+int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, void* out, int dtype, int heads, int64_t q_row,
+                           int64_t q_head, float scale, int window, int rows_per_seq, void* workspace,
+                           int64_t workspace_bytes, void* stream, char* err, int err_len) {
+  return guarded(err, err_len, [&] {
+    const Kv4Where w = kv4_where(c);
+    kv4_require_heads(heads, w.kv_heads, rows_per_seq);
+    XTG_REQUIRE(window >= 0, "kv4: window 0 (none) or more");
+    if (w.rows == 0 || w.seqs == 0) return;
+    kv4_require_rows(dtype, {q, out}, {q_row, q_head});
+    const int sms = device_sms();
+    XTG_REQUIRE(workspace && aligned16(workspace) &&
+                    workspace_bytes >= kv4_workspace_bytes(w.head_dim, heads / w.kv_heads, rows_per_seq, sms),
+                "kv4: a workspace of xtg_cuda_kv4_workspace bytes on a 16-byte boundary");
+    launch_kv4_attention({w, q, out, dtype, q_row, q_head, heads, window, scale, rows_per_seq,
+                          static_cast<float*>(workspace)},
+                         sms, static_cast<cudaStream_t>(stream));
   });
 }
 
