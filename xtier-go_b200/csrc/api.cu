@@ -380,6 +380,7 @@ Kv4Where kv4_where(const xtg_cuda_kv4* c) {
   XTG_REQUIRE(c->kv_heads >= 1 && c->kv_heads <= 65535, "kv4: 1..65535 KV heads");
   XTG_REQUIRE(c->pages >= 1 && c->max_pages >= 1, "kv4: at least one page in the pool and per sequence");
   XTG_REQUIRE(c->seqs >= 0 && c->rows >= 0 && c->rows < (1ll << 31), "kv4: sequences and rows in 0 .. 2^31 - 1");
+  XTG_REQUIRE(c->max_pages < (1 << 25), "kv4: a sequence's table holds fewer than 2^25 pages");
   XTG_REQUIRE(c->seqs < (1 << 29), "kv4: fewer than 2^29 sequences");
   XTG_REQUIRE(c->pool && (c->seqs == 0 || (c->table && c->pos && c->cu_rows)), "kv4: null pointer");
   XTG_REQUIRE(aligned16(c->pool), "kv4: the pool must start on a 16-byte boundary");
@@ -449,13 +450,14 @@ int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, void* out, int 
     const Kv4Where w = kv4_where(c);
     kv4_require_heads(heads, w.kv_heads, rows_per_seq);
     XTG_REQUIRE(window >= 0, "kv4: window 0 (none) or more");
+    XTG_REQUIRE(w.rows * heads < (1ll << 31), "kv4: rows x heads below 2^31");
     if (w.rows == 0 || w.seqs == 0) return;
     kv4_require_rows(dtype, {q, out}, {q_row, q_head});
     const int sms = device_sms();
     XTG_REQUIRE(workspace && aligned16(workspace) &&
                     workspace_bytes >= kv4_workspace_bytes(w.head_dim, heads / w.kv_heads, rows_per_seq, sms),
                 "kv4: a workspace of xtg_cuda_kv4_workspace bytes on a 16-byte boundary");
-    launch_kv4_attention({w, q, out, dtype, q_row, q_head, heads, window, scale, rows_per_seq,
+    launch_kv4_attention({w, q, out, dtype, q_row, q_head, heads, heads / w.kv_heads, window, scale, rows_per_seq,
                           static_cast<float*>(workspace)},
                          sms, static_cast<cudaStream_t>(stream));
   });

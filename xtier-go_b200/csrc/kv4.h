@@ -59,7 +59,7 @@ struct Kv4Attn {
   void* out;       // [rows][heads][D] contiguous, q's type
   int dtype;
   int64_t q_row, q_head;
-  int heads, window;
+  int heads, group, window;   // group: q heads per KV head
   float scale;
   int rows_per_seq;   // about how many rows a sequence has: chooses the tiling, not the result
   float* part;        // workspace, kv4_workspace_bytes

@@ -4,23 +4,28 @@
 //   o[r] = sum_p P[r][p] V[p] / sum_p P[r][p],  P[r][p] = 2^(S[r][p] - max_p S[r][p]),  S = log2(e) scale q[r] . K[p]
 //
 // with K and V as s (code - 8) + z per group of 64 head dims. Both products run on mma.m16n8k16 (f16 in, f32 out)
-// straight from the codes: a query row's 16-row tile is 8 rows in two f16 planes, x = hi + lo (22 bits), the hi parts
-// in the tile's rows 0-7 and the lo parts in rows 8-15, so that one instruction multiplies both and a lane holds both
-// sums of the same (row, column). The scales and offsets enter in f32:
+// straight from the codes, transposed, so that the few query rows are the instruction's 8 columns and no part of it is
+// idle: S^T = K Q^T takes 16 slots x 16 dims of K, o^T = V^T P^T 16 dims x 16 slots of V. A lane then holds the scores
+// of slots g, g + 8 and rows 2 a, 2 a + 1 (lane = 4 g + a); movmatrix turns the probabilities into the second
+// product's operand. The scales and offsets enter in f32:
 //   q . K[p] = sum_G s[p][G] (q . code - 8 sum q)_G + z[p][G] (sum q)_G        (-8 sum q: the accumulator's start)
-//   o[r]     = sum_p (P[r][p] s[p][G]) (code - 8) + P[r][p] z[p][G]            (P s: the A operand, by group G)
-// K's codes enter as f16 subnormals, the nibble itself: code 2^-24 (bits 0-3) or code 2^-20 (bits 4-7), exact; the
-// query planes of the dims at bits 4-7 carry the factor 1/16. V's become 1024 + code less 1032: there the sum runs
-// over positions whose terms cancel, and an uncentred code would cost the bits that cancel.
-// P s is brought below 2^15 by a power of two per chunk and group (its largest scale); a chunk's product starts from
-// zero and is added to the row's f32 accumulator with that power, so the matrix unit sums at most 64 positions.
+//   o[r]     = sum_p (P[r][p] s[p][G]) (code - 8) + P[r][p] z[p][G]            (P s: the operand, by group G)
+// K's codes enter as f16 subnormals, the nibble itself: code 2^-24 (bits 0-3) or code 2^-20 (bits 4-7), exact; q
+// carries 1/16 where they lie at bits 4-7. V's are centred first (64 + c / 16 less 64.5): a sum of uncentred codes over
+// positions would put an error of about 2^-20 of the group's range into components far smaller than it.
+// Precision of the f16 operands: q of 16-bit rows is exact in one plane (a power of two brings the row's largest value
+// to 2^14 .. 2^15); of f32 rows it is hi + lo, 22 bits. P s is brought below 2^15 by a power of two per chunk and
+// group (its largest scale) and always has two planes: one would put 2^-12 of the largest value into the result, which
+// a small component beside large values of other positions shows even after bf16's rounding. A chunk's product starts from zero and is added to the row's f32
+// accumulator, so the matrix unit itself sums at most 64 positions.
 //
 // What bounds it: the cache's bytes with few rows, the instructions around the matrix products with many. One CTA per
 // SM takes an equal share of all (sequence, row block, KV head, 64-position chunk) items in that order, whatever the
 // sequences' lengths: shares start and end inside a sequence, whose parts a second kernel joins. A producer warp
-// brings chunks (one bulk copy of a page's block of the head) into a ring; 8 consumer warps take them: a row block is
-// 1, 2, 4 or 8 tiles of 8 rows, one per warp, and the 8 / tiles warps of a tile take every other chunk, each with a
-// running maximum of its own, so that no warp waits for another before the end of a sequence's part.
+// brings chunks (one bulk copy of a page's block of the head) into a ring of shared memory; the consumer warps take
+// half chunks (32 positions). A warp holds 8 rows, or 16 (the codes unpacked once for both); a row block is 1, 2, 4 or 8
+// warps' rows, and the warps with the same rows take the half chunks in turn, each with a running maximum of its own,
+// so that no warp waits for another before the end of a sequence's part.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -32,84 +37,95 @@ namespace xtg {
 
 namespace {
 
-constexpr int kWarps = 8;                         // consumer warps
-constexpr int kThreads = 32 * (kWarps + 1);       // and the producer
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kUnit = 32;                        // positions a warp takes at once: half a chunk
+constexpr int kUnits = kKv4Page / kUnit, kSteps = kUnit / 16;
 
-template <int D>
+// Consumer warps and registers. The producer's warpgroup has one working warp; setmaxnreg moves registers from it to the
+// consumers, whose sum with its share must not pass what the CTA started with (threads x kStart).
+template <int D, int RT>
 struct Kv4Shape {
+  static constexpr int kWarps = RT == 1 && D <= 128 ? 12 : 8;
+  static constexpr int kThreads = 32 * (kWarps + 4);
+  static constexpr int kStart = 65536 / kThreads / 8 * 8;
+  static constexpr int kProducerRegs = 40;
+  static constexpr int kConsumerRegs = (kThreads * kStart - 128 * kProducerRegs) / (32 * kWarps) / 8 * 8;
+  static_assert(32 * kWarps * kConsumerRegs + 128 * kProducerRegs <= kThreads * kStart, "more registers than launched");
   static constexpr int kBlock = kv4_block_bytes(D);
-  static constexpr int kStages = D == 256 ? 8 : D == 128 ? 16 : 24;   // a multiple of 8; about 110 or 147 KB
-  static constexpr int kMergeStride = D + 8;                          // floats of a row's accumulator being merged
+  static constexpr int kStages = D == 256 ? 8 : D == 128 ? (RT == 1 ? 16 : 15) : 24;   // 110 to 147 KB
+  static constexpr int kMergeStride = D + 4;   // floats of a row's accumulator being merged
 };
 
-template <int D>
+template <int D, int RT>
 struct Kv4Smem {
-  uint8_t stage[Kv4Shape<D>::kStages][Kv4Shape<D>::kBlock];
-  float acc[kWarps][8][Kv4Shape<D>::kMergeStride];
-  float m[kWarps][8], l[kWarps][8];
-  uint64_t full[Kv4Shape<D>::kStages], empty[Kv4Shape<D>::kStages];
-  int present[Kv4Shape<D>::kStages];   // 0: no page, nothing was copied
-  int64_t scan[kThreads / 32];
-  int64_t start_base;   // items before the sequence that the CTA's share starts in
+  using Shape = Kv4Shape<D, RT>;
+  uint8_t stage[Shape::kStages][Shape::kBlock];
+  float acc[Shape::kWarps][8 * RT][Shape::kMergeStride];
+  float m[Shape::kWarps][8 * RT], l[Shape::kWarps][8 * RT];
+  uint64_t full[Shape::kStages], empty[Shape::kStages];
+  int present[Shape::kStages];   // 0: no page, nothing was copied
+  uint64_t scan[Shape::kThreads / 32];
+  uint64_t start_base;   // items before the sequence that the CTA's share starts in
   int start_seq;
-  int failed;           // a wait ran out: the rest of the call waits only briefly and computes nothing
+  int failed;            // a wait ran out: the rest of the call waits only briefly and computes nothing
 };
 
 // A part of a sequence's items: row block b of KV head h, chunks c0 .. c0 + take - 1 of the sequence's cnt from page lo.
+// Positions are below 2^31 (the table holds fewer).
 struct Part {
-  int seq, b, h;
-  int64_t row0, n, pos, lo, cnt, c0, take;
+  int seq, b, h, row0, n, pos, lo, cnt, c0, take;
 };
 
 // What the combine reads: the split (sequence, row block, head) that a CTA's share ends in, and the last CTA with a
 // part of it.
 struct Kv4Split {
-  int64_t row0;
-  int n, h, b, last;   // last < 0: none
+  int row0, n, h, b, last;   // last < 0: none
 };
+
+__device__ __forceinline__ uint64_t divide(uint64_t a, uint32_t b) {
+  return a >> 32 ? a / b : (uint32_t)a / b;
+}
 
 // The items of sequence s: row blocks x KV heads x chunks. Sequences with rows have at least one chunk (it may hold
 // nothing), so that every row is written.
-__device__ __forceinline__ int64_t kv4_items(const Kv4Attn& a, int s, int rows_per_block, Part& p) {
-  p.row0 = kv4_row_bound(a.w, s);
-  p.n = kv4_row_bound(a.w, s + 1) - p.row0;
+__device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, int rows_per_block, Part& p) {
+  p.pos = a.w.pos[s];
+  p.row0 = (int)kv4_row_bound(a.w, s);
+  p.n = (int)kv4_row_bound(a.w, s + 1) - p.row0;
   if (p.n <= 0) return 0;
   p.seq = s;
-  p.pos = a.w.pos[s];
-  const int64_t end = p.pos + p.n;
-  const int64_t first = a.window > 0 ? p.pos - a.window + 1 : 0;
-  p.lo = first > 0 ? first / kKv4Page : 0;
-  p.cnt = end > 0 ? (end + kKv4Page - 1) / kKv4Page - p.lo : 1;
-  const int64_t most = (int64_t)a.w.max_pages - p.lo;
-  if (end > (int64_t)a.w.max_pages * kKv4Page) {   // rows past the table see what the table holds
+  const int64_t held = (int64_t)a.w.max_pages * kKv4Page;
+  int64_t end = (int64_t)p.pos + p.n;
+  if (end > held) {   // rows past the table see what the table holds
     if (a.w.err && threadIdx.x == 0) atomicExch(a.w.err, 6);
-    p.cnt = most;
+    end = held;
   }
-  if (p.cnt < 1) p.cnt = 1;
-  const int64_t qrows = p.n * (a.heads / a.w.kv_heads);
-  return (qrows + rows_per_block - 1) / rows_per_block * a.w.kv_heads * p.cnt;
+  const int first = a.window > 0 && p.pos >= a.window ? p.pos - a.window + 1 : 0;
+  p.lo = first / kKv4Page;
+  p.cnt = max((int)((end + kKv4Page - 1) >> 6) - p.lo, 1);
+  const uint32_t qrows = (uint32_t)p.n * (uint32_t)a.group;
+  return (uint64_t)((qrows + rows_per_block - 1) / (uint32_t)rows_per_block) * (uint32_t)a.w.kv_heads * (uint32_t)p.cnt;
 }
 
-// Walks a CTA's share [start, end) of the items part by part.
+// Walks a CTA's share of the items part by part.
 struct Walk {
   int s;
-  int64_t off, left;
+  uint64_t off, left;   // from sequence s's first item
 };
 
 __device__ __forceinline__ bool kv4_next(const Kv4Attn& a, int rows_per_block, Walk& k, Part& p) {
   while (k.left > 0 && k.s < a.w.seqs) {
-    const int64_t items = kv4_items(a, k.s, rows_per_block, p);
+    const uint64_t items = kv4_items(a, k.s, rows_per_block, p);
     if (k.off >= items) {
       k.off -= items;
       ++k.s;
       continue;
     }
-    const int64_t seg = k.off / p.cnt;
-    p.c0 = k.off - seg * p.cnt;
-    p.h = (int)(seg % a.w.kv_heads);
-    p.b = (int)(seg / a.w.kv_heads);
-    p.take = p.cnt - p.c0 < k.left ? p.cnt - p.c0 : k.left;
+    const uint64_t seg = divide(k.off, p.cnt);
+    p.c0 = (int)(k.off - seg * (uint32_t)p.cnt);
+    p.b = (int)divide(seg, a.w.kv_heads);
+    p.h = (int)(seg - (uint64_t)p.b * (uint32_t)a.w.kv_heads);
+    p.take = (int)((uint64_t)(p.cnt - p.c0) < k.left ? (uint64_t)(p.cnt - p.c0) : k.left);
     k.off += p.take;
     k.left -= p.take;
     return true;
@@ -140,18 +156,13 @@ __device__ __forceinline__ void load_q8(const void* base, int64_t at, int dtype,
   }
 }
 
-// 4 neighbouring output values
-__device__ __forceinline__ void store_out4(void* base, int64_t at, int dtype, float4 v) {
-  if (dtype == kKv4F32) {
-    *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = v;
-  } else if (dtype == kKv4Bf16) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-  } else {
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) =
-        make_uint2(pack_f16x2(v.x, v.y), pack_f16x2(v.z, v.w));
-  }
+__device__ __forceinline__ void store_out(void* base, int64_t at, int dtype, float x) {
+  if (dtype == kKv4F32)
+    static_cast<float*>(base)[at] = x;
+  else if (dtype == kKv4Bf16)
+    static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(x);
+  else
+    static_cast<__half*>(base)[at] = __float2half_rn(x);
 }
 
 // x = hi + lo in f16: two values' hi parts and lo parts, packed
@@ -171,13 +182,32 @@ __device__ __forceinline__ uint32_t hadd2_u32(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// The codes of two slots at bits 0-3 (SHIFTED false) or 4-7 of each half, less 8, as f16: 1024 + c - 1032, and
-// (1024 + 16 c) / 16 - 72; exact.
+// The V codes at bits 0-3 (low) or 4-7 (high) of a word's halves as (code - 8) 2^-4 in f16: 64 + c / 16 less 64.5, and
+// (1024 + 16 c) / 256 less 4.5; exact.
 __device__ __forceinline__ uint32_t v_codes_low(uint32_t w) {
-  return hadd2_u32((w & 0x000f000fu) | 0x64006400u, 0xe408e408u);
+  return hadd2_u32((w & 0x000f000fu) | 0x54005400u, 0xd408d408u);
 }
 __device__ __forceinline__ uint32_t v_codes_high(uint32_t w) {
-  return hfma2_u32((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
+  return hfma2_u32((w & 0x00f000f0u) | 0x64006400u, 0x1c001c00u, 0xc480c480u);
+}
+
+// D = A B + C with C apart from D
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                             const float (&c)[4]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+__device__ __forceinline__ void mma_f16_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  mma_f16(d, a[0], a[1], a[2], a[3], b0, b1);
+}
+
+// The transpose of an 8 x 8 matrix of 16-bit values (lane 4 g + a holds row g, columns 2 a and 2 a + 1)
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 
 __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)biased << 23); }
@@ -203,126 +233,140 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 // floats of a part's row in the workspace: m, l, 2 pads, acc[D]
 __host__ __device__ constexpr int part_row(int D) { return D + 4; }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, 1) kv4_attention_kernel(const Kv4Attn a, const int tiles, float* part,
-                                                                   Kv4Split* splits) {
-  using Shape = Kv4Shape<D>;
-  constexpr int kStages = Shape::kStages;
+// RT: 8-row tiles per warp; TYPE: q's and out's. tiles: warps per row block.
+template <int D, int RT, int TYPE>
+__global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
+    kv4_attention_kernel(const Kv4Attn a, const int tiles, float* part, Kv4Split* splits) {
+  using Shape = Kv4Shape<D, RT>;
+  constexpr int kStages = Shape::kStages, kWarps = Shape::kWarps, kThreads = Shape::kThreads;
   constexpr int kGroups = D / kKv4Group, kBlocks = D / 32, H = D < 128 ? D : 128;
+  constexpr int kQPlanes = TYPE == kKv4F32 ? 2 : 1;
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  Kv4Smem<D>& sm = *reinterpret_cast<Kv4Smem<D>*>(smem_raw);
+  Kv4Smem<D, RT>& sm = *reinterpret_cast<Kv4Smem<D, RT>*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, tq = lane & 3;
-  const int group = a.heads / a.w.kv_heads, block_rows = 8 * tiles, lanes = kWarps / tiles;
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sm.full[s], 1);
-      mbar_init(&sm.empty[s], tiles);
-    }
-    mbar_init_fence();
-    sm.failed = 0;
-    sm.start_seq = a.w.seqs;
-    sm.start_base = 0;
-  }
-  __syncthreads();
+  const int warp_rows = 8 * RT, block_rows = warp_rows * tiles, lanes = kWarps / tiles;
 
   // ---- this CTA's share of the items: an equal part of their sum over the sequences ----
-  int64_t total = 0, share = 0, share_end = 0;
-  int64_t ctas = gridDim.x;   // with fewer items than CTAs one each, so that no share between two others is empty
+  uint64_t total = 0, share = 0;
+  uint32_t share_items = 0, most = 0, extra = 0;   // CTAs below `extra` have `most` + 1 items, the others `most`
+  const bool one_pass = a.w.seqs <= kThreads;
   for (int pass = 0; pass < 2; ++pass) {   // the sum, then where the share starts
-    int64_t base = 0;
+    uint64_t base = 0;
     for (int s0 = 0; s0 < a.w.seqs; s0 += kThreads) {
       const int s = s0 + threadIdx.x;
       Part p;
-      const int64_t mine = s < a.w.seqs ? kv4_items(a, s, block_rows, p) : 0;
-      int64_t x = mine;
+      const uint64_t mine = s < a.w.seqs ? kv4_items(a, s, block_rows, p) : 0;
+      uint64_t x = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      __syncthreads();
       if (lane == 31) sm.scan[warp] = x;
+      if (threadIdx.x == 0 && pass == 0 && s0 == 0) {
+        for (int st = 0; st < kStages; ++st) {
+          mbar_init(&sm.full[st], 1);
+          mbar_init(&sm.empty[st], kUnits * tiles);
+        }
+        mbar_init_fence();
+        sm.failed = 0;
+        sm.start_seq = a.w.seqs;
+        sm.start_base = 0;
+      }
       __syncthreads();
-      int64_t sum = 0;
+      uint64_t sum = 0;
+#pragma unroll
       for (int v = 0; v < kThreads / 32; ++v) {
         if (v < warp) x += sm.scan[v];
         sum += sm.scan[v];
       }
-      if (pass == 1 && base + x - mine <= share && share < base + x) {
+      if (one_pass || pass == 0) {
+        total = base + sum;
+        if (s0 + kThreads >= a.w.seqs) {
+          // with fewer items than CTAs one each, so that no share between two others is empty
+          const uint32_t ctas = total < gridDim.x ? (uint32_t)total : gridDim.x;
+          if (blockIdx.x < ctas) {
+            most = (uint32_t)divide(total, ctas);
+            extra = (uint32_t)(total - (uint64_t)most * ctas);
+            share = (uint64_t)most * blockIdx.x + min(blockIdx.x, extra);
+            share_items = most + (blockIdx.x < extra);
+          }
+        }
+      }
+      if ((one_pass || pass == 1) && base + x - mine <= share && share < base + x) {
         sm.start_seq = s;
         sm.start_base = base + x - mine;
       }
       base += sum;
+      __syncthreads();
     }
-    if (pass == 0) {
-      total = base;
-      if (total < ctas) ctas = total;
-      if (blockIdx.x < ctas) {
-        share = total * blockIdx.x / ctas;
-        share_end = total * (blockIdx.x + 1) / ctas;
-      }
-    }
+    if (one_pass) break;
   }
-  __syncthreads();
-  Walk walk = {sm.start_seq, share - sm.start_base, share_end - share};
+  Walk walk = {sm.start_seq, share - sm.start_base, share_items};
   Part p;
 
-  if (warp == kWarps) {
+  if (warp >= kWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kProducerRegs));
+    if (warp > kWarps) return;
     // ---- producer: the chunks of every part in order, a page's block of the head per stage ----
-    int64_t it = 0;
+    int st = 0;
+    uint32_t turn = 0;   // how often the ring has gone round
     while (kv4_next(a, block_rows, walk, p)) {
-      for (int64_t k0 = 0; k0 < p.take; k0 += 32) {
+      const uint8_t* head = a.w.pool + (int64_t)p.h * Shape::kBlock;
+      for (int k0 = 0; k0 < p.take; k0 += 32) {
         const int64_t mine = k0 + lane < p.take ? kv4_page(a.w, p.seq, p.lo + p.c0 + k0 + lane) : -1;
-        const int count = (int)(p.take - k0 < 32 ? p.take - k0 : 32);
-        for (int j = 0; j < count; ++j, ++it) {
+        const int count = min(p.take - k0, 32);
+        for (int j = 0; j < count; ++j) {
           const int64_t page = __shfl_sync(0xffffffffu, mine, j);
-          if (lane == 0) {
-            const int st = (int)(it % kStages);
-            const int64_t turn = it / kStages;
-            const bool free_ = turn == 0 || kv4_wait(&sm.empty[st], (uint32_t)((turn - 1) & 1), &sm.failed, a.w.err);
-            if (free_) {
-              sm.present[st] = page >= 0;
-              if (page >= 0) {
-                mbar_expect_tx(&sm.full[st], Shape::kBlock);
-                bulk_g2s(sm.stage[st], a.w.pool + (page * a.w.kv_heads + p.h) * (int64_t)Shape::kBlock, Shape::kBlock,
-                         &sm.full[st]);
-              } else {
-                mbar_arrive(&sm.full[st]);
-              }
+          if (lane == 0 && (turn == 0 || kv4_wait(&sm.empty[st], (turn - 1) & 1, &sm.failed, a.w.err))) {
+            sm.present[st] = page >= 0;
+            if (page >= 0) {
+              mbar_expect_tx(&sm.full[st], Shape::kBlock);
+              bulk_g2s(sm.stage[st], head + page * a.w.kv_heads * (int64_t)Shape::kBlock, Shape::kBlock, &sm.full[st]);
+            } else {
+              mbar_arrive(&sm.full[st]);
             }
+          }
+          if (++st == kStages) {
+            st = 0;
+            ++turn;
           }
           __syncwarp();
         }
       }
     }
-    if (lane == 0 && share_end <= share) splits[blockIdx.x].last = -1;
+    if (lane == 0 && share_items == 0) splits[blockIdx.x].last = -1;
   } else {
-    const int rt = warp % tiles, sl = warp / tiles;   // this warp's tile of the row block, its turn among the chunks
-    int64_t it = 0;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kConsumerRegs));
+    const int rt = warp % tiles, sl = warp / tiles;   // this warp's rows of the row block, its turn among the units
+    const uint32_t group = a.group;
+    uint32_t it = 0;            // chunks of the parts before
     bool split_after = false;   // the last part goes on in the next CTA
     while (kv4_next(a, block_rows, walk, p)) {
-      // ---- the tile's rows: row r of the sequence and KV head is (row r / group of the sequence, q head r % group) ----
-      const int64_t qrows = p.n * group, r0 = (int64_t)p.b * block_rows + 8 * rt, r = r0 + g;
-      const bool live = r < qrows, any = r0 < qrows;
-      const int64_t i = live ? r / group : 0;
-      const int64_t t = live ? p.pos + i : -1;   // the row's position; dead rows see nothing
-      // the tile's first and last position
-      const int64_t tmin = p.pos + r0 / group, tmax = p.pos + (r0 + 7 < qrows ? r0 + 7 : qrows - 1) / group;
+      // ---- the warp's rows: row r of the sequence and KV head is (row r / group of the sequence, q head r % group) ----
+      const uint32_t qrows = (uint32_t)p.n * group, r0 = (uint32_t)p.b * block_rows + warp_rows * rt;
+      const bool any = r0 < qrows;
+      // the position of the sequence's row i (past 2^31 - 1 the table holds nothing more to see)
+      auto position = [&](uint32_t i) { return (int)min((int64_t)p.pos + i, (int64_t)0x7fffffff); };
+      // the warp's first and last position
+      const int tmin = position(r0 / group), tmax = position((min(r0 + warp_rows, qrows) - 1) / group);
 
-      // Q in two f16 planes, scaled by the power of two that brings the row's largest value to 2^14 .. 2^15; a lane has
-      // the 8 dims of one K word per block of 32: nibble pair i (dims i, i + 4) is a register of step i / 2
-      uint32_t qa[kBlocks][2][4];
-      float qsum[kGroups], rf;   // (sum q)_G and the factor from the products' unit to base-2 scores
-      {
-        float x[kBlocks][8];
-        float mx = 0.f;
-        const int64_t at = (p.row0 + i) * a.q_row + (p.h * group + (live ? r % group : 0)) * a.q_head;
+      // Q as the operand of row 8 j + g: the 8 dims of one K word per block of 32, nibble pair i (dims i, i + 4) is a
+      // register of step i / 2. Then what belongs to rows 8 j + 2 tq + {0, 1}, this lane's scores' rows.
+      uint32_t qb[RT][kBlocks][2][kQPlanes][2];
+      float qsum[RT][2][kGroups], rf[RT][2];   // (sum q)_G and the factor from the products' unit to base-2 scores
+      int t[RT][2];                            // the row's position; dead rows see nothing
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        const uint32_t r = r0 + 8 * j + g, i = r / group;
+        const bool live = r < qrows;
+        float x[kBlocks][8], mx = 0.f, sums[kGroups];
+        const int64_t at = ((int64_t)p.row0 + i) * a.q_row + (int64_t)(p.h * group + (r - i * group)) * a.q_head;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
           if (live)
-            load_q8(a.q, at + 32 * b + 8 * tq, a.dtype, x[b]);
+            load_q8(a.q, at + 32 * b + 8 * tq, TYPE, x[b]);
           else
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[b][e] = 0.f;
@@ -331,362 +375,459 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attention_kernel(const Kv4Att
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        int e2 = (int)(__float_as_uint(mx) >> 23);   // biased exponent of the largest value
-        if (e2 < 16) e2 = 16;
-        if (e2 > 254) e2 = 254;
-        const float up = pow2_bits(127 + 14 + 127 - e2 > 254 ? 254 : 268 - e2);
-        rf = a.scale * kLog2e * (16777216.f / up);   // 2^24: the codes' unit
+        const int e2 = min(max((int)(__float_as_uint(mx) >> 23), 16), 254);   // biased exponent of the largest value
+        // the factor is not negative (a maximum of scores stays one): a negative scale turns q's sign
+        const float up = a.scale < 0.f ? -pow2_bits(min(268 - e2, 254)) : pow2_bits(min(268 - e2, 254));
+        const float f = fmaxf(fabsf(a.scale) * kLog2e * (16777216.f / fabsf(up)), 1.1754944e-38f);   // 2^24: the codes' unit
 #pragma unroll
-        for (int G = 0; G < kGroups; ++G) qsum[G] = 0.f;
+        for (int G = 0; G < kGroups; ++G) sums[G] = 0.f;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             x[b][e] *= up;
-            qsum[b / 2] += x[b][e];
+            sums[b / 2] += x[b][e];
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            split_f16x2(x[b][2 * e], x[b][2 * e + 4], qa[b][e][0], qa[b][e][1]);
-            split_f16x2(x[b][2 * e + 1] * 0.0625f, x[b][2 * e + 5] * 0.0625f, qa[b][e][2], qa[b][e][3]);
+            const float lo0 = x[b][2 * e], lo1 = x[b][2 * e + 4], hi0 = x[b][2 * e + 1] * 0.0625f,
+                        hi1 = x[b][2 * e + 5] * 0.0625f;
+            if constexpr (kQPlanes == 2) {
+              split_f16x2(lo0, lo1, qb[j][b][e][0][0], qb[j][b][e][kQPlanes - 1][0]);
+              split_f16x2(hi0, hi1, qb[j][b][e][0][1], qb[j][b][e][kQPlanes - 1][1]);
+            } else {
+              qb[j][b][e][0][0] = pack_f16x2(lo0, lo1);
+              qb[j][b][e][0][1] = pack_f16x2(hi0, hi1);
+            }
           }
         }
 #pragma unroll
         for (int G = 0; G < kGroups; ++G) {
-          qsum[G] += __shfl_xor_sync(0xffffffffu, qsum[G], 1);
-          qsum[G] += __shfl_xor_sync(0xffffffffu, qsum[G], 2);
-          qsum[G] *= 1.f / 16777216.f;
+          sums[G] += __shfl_xor_sync(0xffffffffu, sums[G], 1);
+          sums[G] += __shfl_xor_sync(0xffffffffu, sums[G], 2);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int from = 4 * (2 * tq + e);
+          rf[j][e] = __shfl_sync(0xffffffffu, f, from);
+#pragma unroll
+          for (int G = 0; G < kGroups; ++G) qsum[j][e][G] = __shfl_sync(0xffffffffu, sums[G], from) * (1.f / 16777216.f);
+          t[j][e] = __shfl_sync(0xffffffffu, live ? position(i) : -1, from);
         }
       }
 
-      float o[kBlocks][4][2];   // the row's dims 32 c + 8 t + 2 tq + {0, 1}, without the offsets' part
-      float oz[kGroups];        // sum of P z over this lane's slots
-      float run_m = -INFINITY, run_l = 0.f;
+      // the rows' dims 32 c + 16 m + g (+ 8: the last two), rows 8 j + 2 tq + {0, 1}, without the offsets' part
+      float o[RT][kBlocks][2][4];
+      float oz[RT][2][kGroups];   // sum of P z over this lane's slots
+      float run_m[RT][2], run_l[RT][2];
 #pragma unroll
-      for (int c = 0; c < kBlocks; ++c)
+      for (int j = 0; j < RT; ++j) {
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) o[c][tt][0] = o[c][tt][1] = 0.f;
+        for (int c = 0; c < kBlocks; ++c)
 #pragma unroll
-      for (int G = 0; G < kGroups; ++G) oz[G] = 0.f;
+          for (int m = 0; m < 2; ++m) o[j][c][m][0] = o[j][c][m][1] = o[j][c][m][2] = o[j][c][m][3] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          run_m[j][e] = -INFINITY;
+          run_l[j][e] = 0.f;
+#pragma unroll
+          for (int G = 0; G < kGroups; ++G) oz[j][e][G] = 0.f;
+        }
+      }
 
-      auto chunk = [&](const uint8_t* stg, int64_t p0, auto masked_) {
+      // half chunk hh of a stage, its first position p0
+      auto unit = [&](const uint8_t* stg, int hh, int p0, auto masked_) {
         constexpr bool kMasked = decltype(masked_)::value;
-        const uint32_t* kw = reinterpret_cast<const uint32_t*>(stg);
-        const uint32_t* kpar = reinterpret_cast<const uint32_t*>(stg + kv4_k_params(D));
-        const uint32_t* vw = reinterpret_cast<const uint32_t*>(stg + kv4_v_codes(D));
-        const uint32_t* vpar = reinterpret_cast<const uint32_t*>(stg + kv4_v_params(D));
-        // ---- scores: 8 tiles of 8 slots; this lane: slots 8 j + 2 tq + {0, 1} of its row ----
-        float s[8][2];
+        const uint32_t* kw = reinterpret_cast<const uint32_t*>(stg) + hh * kUnit * (H / 8);
+        const uint32_t* kpar = reinterpret_cast<const uint32_t*>(stg + kv4_k_params(D)) + hh * kUnit;
+        const uint32_t* vw = reinterpret_cast<const uint32_t*>(stg + kv4_v_codes(D)) + hh * kUnit * (D / 8);
+        const uint32_t* vpar = reinterpret_cast<const uint32_t*>(stg + kv4_v_params(D)) + hh * kUnit;
+        // ---- scores of 16 slots each: [0, 1] slot 16 u + g, [2, 3] slot 16 u + 8 + g; rows 2 tq, 2 tq + 1 ----
+        float s[RT][kSteps][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int slot = 8 * j + g;
-          float c[kGroups][4];
-#pragma unroll
-          for (int G = 0; G < kGroups; ++G) {
-            c[G][0] = c[G][1] = -8.f * qsum[G];
-            c[G][2] = c[G][3] = 0.f;
-          }
+        for (int u = 0; u < kSteps; ++u) {
+          float c[RT][kGroups][4];
 #pragma unroll
           for (int hf = 0; hf < D / H; ++hf) {
-            uint32_t w[H / 32];
-            if constexpr (H == 128) {
-              const uint4 v = *reinterpret_cast<const uint4*>(kw + ((hf * kKv4Page + slot) * 4 + tq) * 4);
-              w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-            } else {
-              const uint2 v = *reinterpret_cast<const uint2*>(kw + (slot * 4 + tq) * 2);
-              w[0] = v.x, w[1] = v.y;
-            }
-#pragma unroll
-            for (int b = 0; b < H / 32; ++b) {
-              const int blk = hf * (H / 32) + b;
-              const uint32_t w8 = w[b] >> 8;
-              mma_f16(c[blk / 2], qa[blk][0][0], qa[blk][0][1], qa[blk][0][2], qa[blk][0][3], w[b] & 0x000f000fu,
-                      w[b] & 0x00f000f0u);
-              mma_f16(c[blk / 2], qa[blk][1][0], qa[blk][1][1], qa[blk][1][2], qa[blk][1][3], w8 & 0x000f000fu,
-                      w8 & 0x00f000f0u);
-            }
-          }
-          s[j][0] = s[j][1] = 0.f;
-#pragma unroll
-          for (int G = 0; G < kGroups; ++G) {
-            const uint2 w = *reinterpret_cast<const uint2*>(kpar + G * kKv4Page + 8 * j + 2 * tq);
-            s[j][0] = fmaf(__uint_as_float(w.x & 0xffff0000u), c[G][0] + c[G][2], s[j][0]);
-            s[j][1] = fmaf(__uint_as_float(w.y & 0xffff0000u), c[G][1] + c[G][3], s[j][1]);
-            s[j][0] = fmaf(__uint_as_float(w.x << 16), qsum[G], s[j][0]);
-            s[j][1] = fmaf(__uint_as_float(w.y << 16), qsum[G], s[j][1]);
-          }
-          s[j][0] *= rf;
-          s[j][1] *= rf;
-          if constexpr (kMasked) {
+            uint32_t w[2][H / 32];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int64_t pp = p0 + 8 * j + 2 * tq + e;
-              if (pp > t || (a.window > 0 && pp <= t - a.window)) s[j][e] = -INFINITY;
-            }
-          }
-        }
-        // ---- the running maximum and sum ----
-        float mx = s[0][0];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fmaxf(s[j][0], s[j][1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float new_m = fmaxf(run_m, mx), ref = new_m == -INFINITY ? 0.f : new_m;
-        const float alpha = ex2_approx(run_m - ref);
-        run_m = new_m;
-        run_l *= alpha;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          s[j][0] = ex2_approx(s[j][0] - ref);
-          s[j][1] = ex2_approx(s[j][1] - ref);
-          run_l += s[j][0] + s[j][1];
-        }
-        // ---- P V by group of 64 dims ----
-#pragma unroll
-        for (int G = 0; G < kGroups; ++G) {
-          uint2 w[8];
-          int top = 0;   // the largest scale's word: positive f32 order is integer order, NaN's word is negative
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            w[j] = *reinterpret_cast<const uint2*>(vpar + G * kKv4Page + 8 * j + 2 * tq);
-            if constexpr (kMasked) {   // what no row of the tile sees may hold anything
-              const int64_t pp = p0 + 8 * j + 2 * tq;
-              if (pp > tmax || (a.window > 0 && pp <= tmin - a.window)) w[j].x = 0;
-              if (pp + 1 > tmax || (a.window > 0 && pp + 1 <= tmin - a.window)) w[j].y = 0;
-            }
-            top = max(top, max((int)w[j].x, (int)w[j].y));
-          }
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          int e2 = top >> 23;
-          if (e2 < 27) e2 = 27;
-          if (e2 > 254) e2 = 254;
-          const float down = pow2_bits(268 - e2), up = pow2_bits(e2 - 14);
-          uint32_t pa[4][4];
-          oz[G] *= alpha;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float s0 = __uint_as_float(w[j].x & 0xffff0000u), s1 = __uint_as_float(w[j].y & 0xffff0000u);
-            float x0 = s[j][0] * (s0 * down), x1 = s[j][1] * (s1 * down);
-            if constexpr (kMasked) {   // a masked NaN scale gives nothing
-              x0 = s[j][0] == 0.f ? 0.f : x0;
-              x1 = s[j][1] == 0.f ? 0.f : x1;
-            }
-            split_f16x2(x0, x1, pa[j / 2][2 * (j & 1)], pa[j / 2][2 * (j & 1) + 1]);
-            oz[G] = fmaf(s[j][0], __uint_as_float(w[j].x << 16), oz[G]);
-            oz[G] = fmaf(s[j][1], __uint_as_float(w[j].y << 16), oz[G]);
-          }
-#pragma unroll
-          for (int c = 2 * G; c < 2 * G + 2; ++c) {
-            float d[4][4];
-#pragma unroll
-            for (int tt = 0; tt < 4; ++tt) d[tt][0] = d[tt][1] = d[tt][2] = d[tt][3] = 0.f;
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              const uint4 v = *reinterpret_cast<const uint4*>(vw + (((hh * kBlocks + c) * 8 + g) * 4 + tq) * 4);
-              const uint32_t word[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int tt = 0; tt < 4; ++tt) {
-                const uint32_t w8 = word[tt] >> 8;
-                const uint32_t(&p0_)[4] = pa[2 * hh];
-                const uint32_t(&p1_)[4] = pa[2 * hh + 1];
-                mma_f16(d[tt], p0_[0], p0_[1], p0_[2], p0_[3], v_codes_low(word[tt]), v_codes_high(word[tt]));
-                mma_f16(d[tt], p1_[0], p1_[1], p1_[2], p1_[3], v_codes_low(w8), v_codes_high(w8));
+              const int slot = 16 * u + 8 * e + g;
+              if constexpr (H == 128) {
+                const uint4 v = *reinterpret_cast<const uint4*>(kw + ((hf * kKv4Page + slot) * 4 + tq) * 4);
+                w[e][0] = v.x, w[e][1] = v.y, w[e][2] = v.z, w[e][3] = v.w;
+              } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(kw + (slot * 4 + tq) * 2);
+                w[e][0] = v.x, w[e][1] = v.y;
               }
             }
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
-              o[c][tt][0] = fmaf(d[tt][0] + d[tt][2], up, o[c][tt][0] * alpha);
-              o[c][tt][1] = fmaf(d[tt][1] + d[tt][3], up, o[c][tt][1] * alpha);
+            for (int b = 0; b < H / 32; ++b) {
+              const int blk = hf * (H / 32) + b, G = blk / 2;
+#pragma unroll
+              for (int st = 0; st < 2; ++st) {
+                const uint32_t w0 = st ? w[0][b] >> 8 : w[0][b], w1 = st ? w[1][b] >> 8 : w[1][b];
+                const uint32_t ka[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                  if (blk % 2 == 0 && st == 0) {
+                    const float q0 = -8.f * qsum[j][0][G], q1 = -8.f * qsum[j][1][G];
+                    const float start[4] = {q0, q1, q0, q1};
+                    mma_f16_from(c[j][G], ka, qb[j][blk][st][0][0], qb[j][blk][st][0][1], start);
+                  } else {
+                    mma_f16_add(c[j][G], ka, qb[j][blk][st][0][0], qb[j][blk][st][0][1]);
+                  }
+                  if constexpr (kQPlanes == 2)
+                    mma_f16_add(c[j][G], ka, qb[j][blk][st][kQPlanes - 1][0], qb[j][blk][st][kQPlanes - 1][1]);
+                }
+              }
             }
+          }
+#pragma unroll
+          for (int G = 0; G < kGroups; ++G) {
+            const uint32_t w0 = kpar[G * kKv4Page + 16 * u + g], w1 = kpar[G * kKv4Page + 16 * u + 8 + g];
+            const float s0 = __uint_as_float(w0 & 0xffff0000u), s1 = __uint_as_float(w1 & 0xffff0000u);
+            const float z0 = __uint_as_float(w0 << 16), z1 = __uint_as_float(w1 << 16);
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float sc = e < 2 ? s0 : s1, of = e < 2 ? z0 : z1, q1 = qsum[j][e % 2][G];
+                s[j][u][e] = fmaf(sc, c[j][G][e], G == 0 ? of * q1 : fmaf(of, q1, s[j][u][e]));
+              }
+          }
+          if constexpr (kMasked) {
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int pp = p0 + 16 * u + 8 * (e / 2) + g;
+                if (pp > t[j][e % 2] || (a.window > 0 && pp <= t[j][e % 2] - a.window)) s[j][u][e] = -INFINITY;
+              }
+          }
+        }
+        // ---- the running maxima and sums ----
+        float alpha[RT][2];
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(s[j][0][e], s[j][0][e + 2]);
+#pragma unroll
+            for (int u = 1; u < kSteps; ++u) mx = fmaxf(mx, fmaxf(s[j][u][e], s[j][u][e + 2]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float new_m = fmaxf(run_m[j][e], mx * rf[j][e]), ref = new_m == -INFINITY ? 0.f : new_m;
+            alpha[j][e] = ex2_approx(run_m[j][e] - ref);
+            run_m[j][e] = new_m;
+            float l = run_l[j][e] * alpha[j][e];
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u) {
+              s[j][u][e] = ex2_approx(fmaf(s[j][u][e], rf[j][e], -ref));
+              s[j][u][e + 2] = ex2_approx(fmaf(s[j][u][e + 2], rf[j][e], -ref));
+              l += s[j][u][e] + s[j][u][e + 2];
+            }
+            run_l[j][e] = l;
+          }
+        // ---- P V by group of 64 dims ----
+#pragma unroll
+        for (int G = 0; G < kGroups; ++G) {
+          uint32_t w[2 * kSteps];   // slots 8 i + g
+          int top = 0;   // the largest scale's word: positive f32 order is integer order, NaN's word is negative
+#pragma unroll
+          for (int i = 0; i < 2 * kSteps; ++i) {
+            w[i] = vpar[G * kKv4Page + 8 * i + g];
+            if constexpr (kMasked) {   // what no row of the warp sees may hold anything
+              const int pp = p0 + 8 * i + g;
+              if (pp > tmax || (a.window > 0 && pp <= tmin - a.window)) w[i] = 0;
+            }
+            top = max(top, (int)w[i]);
+          }
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+          const int e2 = min(max(top >> 23, 27), 254);
+          const float down = pow2_bits(268 - e2), up = pow2_bits(e2 - 14) * 16.f;   // P s below 2^15 and back
+          uint32_t pb[RT][2][2 * kSteps];
+#pragma unroll
+          for (int i = 0; i < 2 * kSteps; ++i) {
+            const float sc = __uint_as_float(w[i] & 0xffff0000u) * down;
+            const float of = __uint_as_float(w[i] << 16);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+              const float p0_ = s[j][i / 2][2 * (i % 2)], p1_ = s[j][i / 2][2 * (i % 2) + 1];
+              float x0 = p0_ * sc, x1 = p1_ * sc;
+              if constexpr (kMasked) {   // a masked NaN scale gives nothing
+                x0 = p0_ == 0.f ? 0.f : x0;
+                x1 = p1_ == 0.f ? 0.f : x1;
+              }
+              // hi: the leading 11 bits (cut, so that an AND gives them), lo: the next 11
+              const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffffe000u);
+              const float h1 = __uint_as_float(__float_as_uint(x1) & 0xffffe000u);
+              pb[j][0][i] = transpose8(pack_f16x2(h0, h1));
+              pb[j][1][i] = transpose8(pack_f16x2(x0 - h0, x1 - h1));
+              oz[j][0][G] = i == 0 ? fmaf(p0_, of, oz[j][0][G] * alpha[j][0]) : fmaf(p0_, of, oz[j][0][G]);
+              oz[j][1][G] = i == 0 ? fmaf(p1_, of, oz[j][1][G] * alpha[j][1]) : fmaf(p1_, of, oz[j][1][G]);
+            }
+          }
+#pragma unroll
+          for (int c = 2 * G; c < 2 * G + 2; ++c) {
+            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+            float d[RT][2][4];
+            const uint4 v = *reinterpret_cast<const uint4*>(vw + ((c * 8 + g) * 4 + tq) * 4);
+            const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+              for (int st = 0; st < 2; ++st) {
+                const uint32_t w0 = st ? word[2 * m] >> 8 : word[2 * m], w1 = st ? word[2 * m + 1] >> 8 : word[2 * m + 1];
+                const uint32_t va[4] = {v_codes_low(w0), v_codes_low(w1), v_codes_high(w0), v_codes_high(w1)};
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                  if (st == 0)
+                    mma_f16_from(d[j][m], va, pb[j][0][0], pb[j][0][1], zero);
+                  else
+                    mma_f16_add(d[j][m], va, pb[j][0][2], pb[j][0][3]);
+                  mma_f16_add(d[j][m], va, pb[j][1][2 * st], pb[j][1][2 * st + 1]);
+                }
+              }
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+              for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  o[j][c][m][e] = fmaf(d[j][m][e], up, o[j][c][m][e] * alpha[j][e % 2]);
           }
         }
       };
 
-      // ---- this warp's chunks of the part ----
-      for (int64_t k = (sl - it % lanes + lanes) % lanes; k < p.take; k += lanes) {
-        const int st = (int)((it + k) % kStages);
-        const bool ok = kv4_wait(&sm.full[st], (uint32_t)(((it + k) / kStages) & 1), &sm.failed, a.w.err);
-        const int64_t p0 = (p.lo + p.c0 + k) * kKv4Page;
-        const bool seen = ok && any && sm.present[st] && p0 <= tmax && (a.window <= 0 || p0 + 63 > tmin - a.window);
+      // ---- this warp's half chunks of the part: every `lanes`-th of the CTA's ----
+      for (int x = (int)((sl + lanes - kUnits * it % lanes) % lanes); x < kUnits * p.take; x += lanes) {
+        const uint32_t k = it + x / kUnits;
+        const int st = (int)(k % kStages), hh = x % kUnits;
+        const bool ok = kv4_wait(&sm.full[st], (k / kStages) & 1, &sm.failed, a.w.err);
+        const int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x;
+        const bool seen =
+            ok && any && sm.present[st] && p0 <= tmax && (a.window <= 0 || p0 + kUnit - 1 > tmin - a.window);
         if (seen) {
-          if (p0 + 63 <= tmin && (a.window <= 0 || p0 > tmax - a.window))
-            chunk(sm.stage[st], p0, std::false_type());
+          if (p0 + kUnit - 1 <= tmin && (a.window <= 0 || p0 > tmax - a.window))
+            unit(sm.stage[st], hh, p0, std::false_type());
           else
-            chunk(sm.stage[st], p0, std::true_type());
+            unit(sm.stage[st], hh, p0, std::true_type());
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[st]);
       }
       it += p.take;
 
-      // ---- the part's warps meet: per row, the warps of its tile by their maxima ----
-      run_l += __shfl_xor_sync(0xffffffffu, run_l, 1);
-      run_l += __shfl_xor_sync(0xffffffffu, run_l, 2);
+      // ---- the part's warps meet: per row, the warps with that row by their maxima ----
 #pragma unroll
-      for (int G = 0; G < kGroups; ++G) {
-        oz[G] += __shfl_xor_sync(0xffffffffu, oz[G], 1);
-        oz[G] += __shfl_xor_sync(0xffffffffu, oz[G], 2);
-      }
-      if (tq == 0) {
-        sm.m[warp][g] = run_m;
-        sm.l[warp][g] = run_l;
-      }
+      for (int j = 0; j < RT; ++j)
 #pragma unroll
-      for (int c = 0; c < kBlocks; ++c)
+        for (int e = 0; e < 2; ++e) {
+          const int row = 8 * j + 2 * tq + e;
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-          *reinterpret_cast<float2*>(&sm.acc[warp][g][32 * c + 8 * tt + 2 * tq]) =
-              make_float2(o[c][tt][0] + oz[c / 2], o[c][tt][1] + oz[c / 2]);
+          for (int x = 4; x < 32; x <<= 1) {
+            run_l[j][e] += __shfl_xor_sync(0xffffffffu, run_l[j][e], x);
+#pragma unroll
+            for (int G = 0; G < kGroups; ++G) oz[j][e][G] += __shfl_xor_sync(0xffffffffu, oz[j][e][G], x);
+          }
+          if (g == 0) {
+            sm.m[warp][row] = run_m[j][e];
+            sm.l[warp][row] = run_l[j][e];
+          }
+#pragma unroll
+          for (int c = 0; c < kBlocks; ++c)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              sm.acc[warp][row][32 * c + 16 * m + g] = o[j][c][m][e] + oz[j][e][c / 2];
+              sm.acc[warp][row][32 * c + 16 * m + 8 + g] = o[j][c][m][e + 2] + oz[j][e][c / 2];
+            }
+        }
       named_bar_sync(1, 32 * kWarps);
+      // a warp per row: lane v has the row's maximum in the v-th of its `lanes` warps
       const bool whole = p.c0 == 0 && p.take == p.cnt;
       float* mine = part + (int64_t)(2 * blockIdx.x + (p.c0 == 0 ? 1 : 0)) * block_rows * part_row(D);
-      for (int x = threadIdx.x; x < block_rows * (D / 4); x += 32 * kWarps) {
-        const int row = x / (D / 4), d0 = 4 * (x % (D / 4)), tile = row / 8, gg = row % 8;
-        const int64_t rr = (int64_t)p.b * block_rows + row;
-        if (rr >= qrows) continue;
-        float M = -INFINITY;
-        for (int v = 0; v < lanes; ++v) M = fmaxf(M, sm.m[v * tiles + tile][gg]);
-        float l = 0.f;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int row = warp; row < block_rows; row += kWarps) {
+        const uint32_t rr = (uint32_t)p.b * block_rows + row;
+        if (rr >= qrows) break;
+        const int tile = row / warp_rows, from = row % warp_rows;
+        const float mv = lane < lanes ? sm.m[lane * tiles + tile][from] : -INFINITY, M = warp_max(mv);
+        const float wt = mv == M ? 1.f : ex2_approx(mv - M);
+        const float l = warp_sum(lane < lanes ? wt * sm.l[lane * tiles + tile][from] : 0.f);
+        float y[D / 32];
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) y[e] = 0.f;
         for (int v = 0; v < lanes; ++v) {
-          const int from = v * tiles + tile;
-          const float mv = sm.m[from][gg], wt = mv == M ? 1.f : ex2_approx(mv - M);
-          const float4 u = *reinterpret_cast<const float4*>(&sm.acc[from][gg][d0]);
-          l = fmaf(wt, sm.l[from][gg], l);
-          y.x = fmaf(wt, u.x, y.x);
-          y.y = fmaf(wt, u.y, y.y);
-          y.z = fmaf(wt, u.z, y.z);
-          y.w = fmaf(wt, u.w, y.w);
+          const float f = __shfl_sync(0xffffffffu, wt, v);
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) y[e] = fmaf(f, sm.acc[v * tiles + tile][from][32 * e + lane], y[e]);
         }
         if (whole) {
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          const int64_t at = ((p.row0 + rr / group) * a.heads + p.h * group + rr % group) * D + d0;
-          store_out4(a.out, at, a.dtype, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+          const uint32_t i = rr / group;
+          const int64_t at = (((int64_t)p.row0 + i) * a.heads + p.h * group + (rr - i * group)) * D + lane;
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) store_out(a.out, at + 32 * e, TYPE, y[e] * inv);
         } else {
           float* to = mine + (int64_t)row * part_row(D);
-          *reinterpret_cast<float4*>(to + 4 + d0) = y;
-          if (d0 == 0) *reinterpret_cast<float2*>(to) = make_float2(M, l);
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) to[4 + 32 * e + lane] = y[e];
+          if (lane == 0) *reinterpret_cast<float2*>(to) = make_float2(M, l);
         }
       }
       split_after = p.c0 == 0 && !whole;
       if (split_after && threadIdx.x == 0) {
         // the last item of this (sequence, row block, head), and the CTA whose share holds it
-        const int64_t end = share_end - p.take + p.cnt - 1;
-        Kv4Split sp;
-        sp.row0 = p.row0;
-        sp.n = (int)(p.n < 0x7fffffff ? p.n : 0x7fffffff);
-        sp.h = p.h;
-        sp.b = p.b;
-        sp.last = (int)(((end + 1) * ctas - 1) / total);
-        splits[blockIdx.x] = sp;
+        const uint64_t end = share + share_items - p.take + p.cnt - 1, longer = (uint64_t)extra * (most + 1);
+        splits[blockIdx.x] = {p.row0, p.n, p.h, p.b,
+                              (int)(end < longer ? divide(end, most + 1) : extra + divide(end - longer, most))};
       }
       named_bar_sync(1, 32 * kWarps);   // before the next part's sums
     }
-    if (threadIdx.x == 0 && !split_after && share_end > share) splits[blockIdx.x].last = -1;
+    if (threadIdx.x == 0 && !split_after && share_items > 0) splits[blockIdx.x].last = -1;
   }
   pdl_launch_next();
 }
 
-// The parts of a split (sequence, row block, KV head): the last part of CTA blockIdx.x and the first parts of the CTAs
-// after it, joined by their maxima in that order. blockIdx.y: rows y, y + 8, ... of the block; 4 warps take every
-// fourth part.
+// The splits (sequence, row block, KV head) that ended inside a CTA's share: the last part of CTA `first` and the first
+// parts of the CTAs after it, joined by their maxima in that order. A row is joined by `per` warps of a block, which
+// take every per-th part: 8 when there are fewer rows than blocks (the parts' latency counts), else 1.
+constexpr int kCombineWarps = 8, kCombineBlocksPerSm = 4, kMostSms = 1024;
+
 template <int D>
-__global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4Attn a, const int tiles, const float* part,
-                                                        const Kv4Split* splits) {
+__global__ void __launch_bounds__(32 * kCombineWarps)
+    kv4_combine_kernel(const Kv4Attn a, const int block_rows, const int ctas, const float* part, const Kv4Split* splits) {
   constexpr int kPer = D / 32;
-  __shared__ float red[4];
-  __shared__ float acc[4][D];
-  __shared__ float sum[4];
+  __shared__ short found[kMostSms];
+  __shared__ int count;
+  __shared__ float acc[kCombineWarps][D];
+  __shared__ float sum[kCombineWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
-  const Kv4Split sp = splits[blockIdx.x];
-  if (sp.last < 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, block_rows = 8 * tiles;
-  const int group = a.heads / a.w.kv_heads, first = blockIdx.x, count = sp.last - first + 1;
-  for (int row = blockIdx.y; row < block_rows; row += gridDim.y) {
-    const int64_t rr = (int64_t)sp.b * block_rows + row;
-    if (rr >= (int64_t)sp.n * group) return;   // the same for the whole block
-    auto at = [&](int k) {   // the k-th part's row
-      return part + ((int64_t)(2 * (first + k) + (k == 0 ? 1 : 0)) * block_rows + row) * part_row(D);
-    };
-    float M = -INFINITY;
-    for (int k = threadIdx.x; k < count; k += 128) M = fmaxf(M, at(k)[0]);
-    M = warp_max(M);
-    if (lane == 0) red[warp] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (warp == 0) {   // the CTAs with a split, in order
+    int n = 0;
+    for (int c0 = 0; c0 < ctas; c0 += 32) {
+      const bool has = c0 + lane < ctas && splits[c0 + lane].last >= 0;
+      const uint32_t all = __ballot_sync(0xffffffffu, has);
+      if (has) found[n + __popc(all & ((1u << lane) - 1))] = (short)(c0 + lane);
+      n += __popc(all);
+    }
+    if (lane == 0) count = n;
+  }
+  __syncthreads();
+  const int rows = count * block_rows, per = rows <= (int)gridDim.x ? kCombineWarps : 1;
+  const uint32_t group = a.group;
+  for (int r0 = blockIdx.x * (kCombineWarps / per); r0 < rows; r0 += gridDim.x * (kCombineWarps / per)) {
+    const int r = r0 + warp / per, mine = warp % per;
     float y[kPer] = {}, l = 0.f;
-    for (int k = warp; k < count; k += 4) {
-      const float* from = at(k);
-      const float mv = from[0], wt = mv == M ? 1.f : ex2_approx(mv - M);
-      l = fmaf(wt, from[1], l);
+    int64_t to = -1;
+    if (r < rows) {
+      const int first = found[r / block_rows], row = r % block_rows;
+      const Kv4Split sp = splits[first];
+      const uint32_t rr = (uint32_t)sp.b * block_rows + row;
+      if (rr < (uint32_t)sp.n * group) {
+        const uint32_t i = rr / group;
+        to = (((int64_t)sp.row0 + i) * a.heads + sp.h * group + (rr - i * group)) * D + lane;
+        const int parts = sp.last - first + 1;
+        auto at = [&](int k) {   // the k-th part's row
+          return part + ((int64_t)(2 * (first + k) + (k == 0 ? 1 : 0)) * block_rows + row) * part_row(D);
+        };
+        float M = -INFINITY;
+        for (int k = lane; k < parts; k += 32) M = fmaxf(M, at(k)[0]);
+        M = warp_max(M);
+#pragma unroll 4
+        for (int k = mine; k < parts; k += per) {
+          const float* from = at(k);
+          const float mv = from[0], wt = mv == M ? 1.f : ex2_approx(mv - M);
+          l = fmaf(wt, from[1], l);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) y[e] = fmaf(wt, from[4 + 32 * e + lane], y[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) acc[warp][32 * e + lane] = y[e];
-    if (lane == 0) sum[warp] = l;
-    __syncthreads();
-    l = sum[0] + sum[1] + sum[2] + sum[3];
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int64_t to = ((sp.row0 + rr / group) * a.heads + sp.h * group + rr % group) * D;
-    for (int d0 = 4 * threadIdx.x; d0 < D; d0 += 512) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = 0; k < 4; ++k) {
-        const float4 u = *reinterpret_cast<const float4*>(&acc[k][d0]);
-        v.x += u.x;
-        v.y += u.y;
-        v.z += u.z;
-        v.w += u.w;
+          for (int e = 0; e < kPer; ++e) y[e] = fmaf(wt, from[4 + 32 * e + lane], y[e]);
+        }
       }
-      store_out4(a.out, to + d0, a.dtype, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
     }
-    __syncthreads();
+    if (per > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[warp][32 * e + lane] = y[e];
+      if (lane == 0) sum[warp] = l;
+      __syncthreads();
+      if (warp != 0) continue;
+      for (int v = 1; v < kCombineWarps; ++v) {
+        l += sum[v];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) y[e] += acc[v][32 * e + lane];
+      }
+    }
+    if (to < 0) continue;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) store_out(a.out, to + 32 * e, a.dtype, y[e] * inv);
   }
 }
 
-// Tiles of 8 query rows that a CTA takes at once: as many as a sequence's rows fill, up to one per warp.
-int row_tiles(int group, int rows_per_seq) {
-  const int64_t need = ((int64_t)group * std::max(1, rows_per_seq) + 7) / 8;
-  return need >= 5 ? 8 : need >= 3 ? 4 : (int)need;
+// A row block: `tiles` warps of rt x 8 rows each, as many as a sequence's rows fill, up to one per warp. 16 rows per warp
+// beyond 8 rows in all (head dim 256 has no registers for them).
+struct RowBlock {
+  int rt, tiles;
+};
+
+RowBlock row_block(int head_dim, int group, int rows_per_seq) {
+  const int64_t rows = (int64_t)group * std::max(1, rows_per_seq);
+  const int rt = head_dim <= 128 && rows > 8 ? 2 : 1;
+  const int64_t need = (rows + 8 * rt - 1) / (8 * rt);
+  return {rt, need >= 5 ? 8 : need >= 3 ? 4 : (int)need};
 }
 
-template <int D>
-void launch(const Kv4Attn& a, int sms, cudaStream_t s) {
-  const int tiles = row_tiles(a.heads / a.w.kv_heads, a.rows_per_seq);
+template <int D, int RT, int TYPE>
+void launch(const Kv4Attn& a, int tiles, int sms, cudaStream_t s) {
+  const int block_rows = 8 * RT * tiles;
   float* part = a.part;
-  Kv4Split* splits = reinterpret_cast<Kv4Split*>(part + (int64_t)sms * 2 * 8 * tiles * part_row(D));
+  Kv4Split* splits = reinterpret_cast<Kv4Split*>(part + (int64_t)sms * 2 * block_rows * part_row(D));
   static std::atomic<uint64_t> optin;
-  const int smem = (int)sizeof(Kv4Smem<D>);
-  ensure_smem_optin((const void*)kv4_attention_kernel<D>, smem, optin);
-  kv4_attention_kernel<D><<<sms, kThreads, smem, s>>>(a, tiles, part, splits);
+  const int smem = (int)sizeof(Kv4Smem<D, RT>);
+  ensure_smem_optin((const void*)kv4_attention_kernel<D, RT, TYPE>, smem, optin);
+  kv4_attention_kernel<D, RT, TYPE><<<sms, Kv4Shape<D, RT>::kThreads, smem, s>>>(a, tiles, part, splits);
   XTG_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sms, 8);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(sms * kCombineBlocksPerSm);
+  cfg.blockDim = dim3(32 * kCombineWarps);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  XTG_CUDA(cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D>, a, tiles, (const float*)part, (const Kv4Split*)splits));
+  XTG_CUDA(cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D>, a, block_rows, sms, (const float*)part,
+                              (const Kv4Split*)splits));
+}
+
+template <int D, int RT>
+void launch_type(const Kv4Attn& a, int tiles, int sms, cudaStream_t s) {
+  if (a.dtype == kKv4F32)
+    launch<D, RT, kKv4F32>(a, tiles, sms, s);
+  else if (a.dtype == kKv4Bf16)
+    launch<D, RT, kKv4Bf16>(a, tiles, sms, s);
+  else
+    launch<D, RT, kKv4F16>(a, tiles, sms, s);
 }
 
 }  // namespace
 
 int64_t kv4_workspace_bytes(int head_dim, int group, int rows_per_seq, int sms) {
-  return (int64_t)sms * (2 * 8 * row_tiles(group, rows_per_seq) * part_row(head_dim) * (int64_t)sizeof(float) +
-                         (int64_t)sizeof(Kv4Split));
+  const RowBlock b = row_block(head_dim, group, rows_per_seq);
+  return (int64_t)sms * (2 * 8 * b.rt * b.tiles * part_row(head_dim) * (int64_t)sizeof(float) + (int64_t)sizeof(Kv4Split));
 }
 
 void launch_kv4_attention(const Kv4Attn& a, int sms, cudaStream_t s) {
-  if (a.w.head_dim == 64)
-    launch<64>(a, sms, s);
+  XTG_REQUIRE(sms <= kMostSms, "kv4: more SMs than the combine lists");
+  const RowBlock b = row_block(a.w.head_dim, a.group, a.rows_per_seq);
+  if (a.w.head_dim == 256)
+    launch_type<256, 1>(a, b.tiles, sms, s);
   else if (a.w.head_dim == 128)
-    launch<128>(a, sms, s);
+    b.rt == 2 ? launch_type<128, 2>(a, b.tiles, sms, s) : launch_type<128, 1>(a, b.tiles, sms, s);
   else
-    launch<256>(a, sms, s);
+    b.rt == 2 ? launch_type<64, 2>(a, b.tiles, sms, s) : launch_type<64, 1>(a, b.tiles, sms, s);
 }
 
 }  // namespace xtg
