@@ -21,8 +21,8 @@
 //
 // What bounds it: the cache's bytes with few rows, the instructions around the matrix products with many. One CTA per
 // SM takes an equal share of all (sequence, row block, KV head, 64-position chunk) items in that order, whatever the
-// sequences' lengths: shares start and end inside a sequence, whose parts a second kernel joins. A producer warp
-// brings chunks (one bulk copy of a page's block of the head) into a ring of shared memory; the consumer warps take
+// sequences' lengths: shares start and end inside a sequence, whose parts a second kernel joins. Producer warps
+// bring chunks (one bulk copy of a page's block of the head) into a ring of shared memory; the consumer warps take
 // half chunks (32 positions). A warp holds 8 rows, or 16 (the codes unpacked once for both); a row block is 1, 2, 4 or 8
 // warps' rows, and the warps with the same rows take the half chunks in turn, each with a running maximum of its own,
 // so that no warp waits for another before the end of a sequence's part.
@@ -40,19 +40,23 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kUnit = 32;                        // positions a warp takes at once: half a chunk
 constexpr int kUnits = kKv4Page / kUnit, kSteps = kUnit / 16;
+// What the start of another part costs a CTA (its rows, its sums), in chunks: counted as items before the part's first,
+// so that a CTA with several parts gets fewer chunks, and few sequences' parts go to CTAs of their own.
+constexpr int kPartCost = 8;
 
-// Consumer warps and registers. The producer's warpgroup has one working warp; setmaxnreg moves registers from it to the
-// consumers, whose sum with its share must not pass what the CTA started with (threads x kStart).
+// Consumer warps and registers: a warpgroup of producers beside them, from which setmaxnreg moves registers to the
+// consumers; the sum of both shares must not pass what the CTA started with (threads x kStart).
 template <int D, int RT>
 struct Kv4Shape {
   static constexpr int kWarps = RT == 1 && D <= 128 ? 12 : 8;
   static constexpr int kThreads = 32 * (kWarps + 4);
+  static constexpr int kRows = 8 * RT * (kWarps == 8 ? 8 : 1);   // of a row block at most
   static constexpr int kStart = 65536 / kThreads / 8 * 8;
   static constexpr int kProducerRegs = 40;
   static constexpr int kConsumerRegs = (kThreads * kStart - 128 * kProducerRegs) / (32 * kWarps) / 8 * 8;
   static_assert(32 * kWarps * kConsumerRegs + 128 * kProducerRegs <= kThreads * kStart, "more registers than launched");
   static constexpr int kBlock = kv4_block_bytes(D);
-  static constexpr int kStages = D == 256 ? 8 : D == 128 ? (RT == 1 ? 16 : 15) : 24;   // 110 to 147 KB
+  static constexpr int kStages = D == 256 ? 8 : D == 128 ? 16 : 24;   // a multiple of 4; 110 or 147 KB
   static constexpr int kMergeStride = D + 4;   // floats of a row's accumulator being merged
 };
 
@@ -60,8 +64,13 @@ template <int D, int RT>
 struct Kv4Smem {
   using Shape = Kv4Shape<D, RT>;
   uint8_t stage[Shape::kStages][Shape::kBlock];
+  // a part's start: the rows' operands [8-row tile][plane][32-dim block][lane], its end: the warps' accumulators
   float acc[Shape::kWarps][8 * RT][Shape::kMergeStride];
+  float qsum[Shape::kRows][D / kKv4Group], qfac[Shape::kRows];   // what belongs to a row's scores
+  int qpos[Shape::kRows];
+  // the warps' maxima (then their weights) and sums; per row the joined maximum, sum and factor
   float m[Shape::kWarps][8 * RT], l[Shape::kWarps][8 * RT];
+  float row_m[Shape::kRows], row_l[Shape::kRows];
   uint64_t full[Shape::kStages], empty[Shape::kStages];
   int present[Shape::kStages];   // 0: no page, nothing was copied
   uint64_t scan[Shape::kThreads / 32];
@@ -86,7 +95,7 @@ __device__ __forceinline__ uint64_t divide(uint64_t a, uint32_t b) {
   return a >> 32 ? a / b : (uint32_t)a / b;
 }
 
-// The items of sequence s: row blocks x KV heads x chunks. Sequences with rows have at least one chunk (it may hold
+// The items of sequence s: row blocks x KV heads x (kPartCost + chunks). Sequences with rows have at least one chunk (it may hold
 // nothing), so that every row is written.
 __device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, int rows_per_block, Part& p) {
   p.pos = a.w.pos[s];
@@ -104,7 +113,8 @@ __device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, int rows_
   p.lo = first / kKv4Page;
   p.cnt = max((int)((end + kKv4Page - 1) >> 6) - p.lo, 1);
   const uint32_t qrows = (uint32_t)p.n * (uint32_t)a.group;
-  return (uint64_t)((qrows + rows_per_block - 1) / (uint32_t)rows_per_block) * (uint32_t)a.w.kv_heads * (uint32_t)p.cnt;
+  return (uint64_t)((qrows + rows_per_block - 1) / (uint32_t)rows_per_block) * (uint32_t)a.w.kv_heads *
+         (uint32_t)(p.cnt + kPartCost);
 }
 
 // Walks a CTA's share of the items part by part.
@@ -121,12 +131,16 @@ __device__ __forceinline__ bool kv4_next(const Kv4Attn& a, int rows_per_block, W
       ++k.s;
       continue;
     }
-    const uint64_t seg = divide(k.off, p.cnt);
-    p.c0 = (int)(k.off - seg * (uint32_t)p.cnt);
+    const uint64_t seg = divide(k.off, p.cnt + kPartCost);
+    const int at = (int)(k.off - seg * (uint32_t)(p.cnt + kPartCost));
+    const int skip = max(kPartCost - at, 0);
+    if (skip >= k.left) break;
+    p.c0 = at + skip - kPartCost;
     p.b = (int)divide(seg, a.w.kv_heads);
     p.h = (int)(seg - (uint64_t)p.b * (uint32_t)a.w.kv_heads);
+    k.left -= skip;
     p.take = (int)((uint64_t)(p.cnt - p.c0) < k.left ? (uint64_t)(p.cnt - p.c0) : k.left);
-    k.off += p.take;
+    k.off += skip + p.take;
     k.left -= p.take;
     return true;
   }
@@ -156,13 +170,18 @@ __device__ __forceinline__ void load_q8(const void* base, int64_t at, int dtype,
   }
 }
 
-__device__ __forceinline__ void store_out(void* base, int64_t at, int dtype, float x) {
-  if (dtype == kKv4F32)
-    static_cast<float*>(base)[at] = x;
-  else if (dtype == kKv4Bf16)
-    static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(x);
-  else
-    static_cast<__half*>(base)[at] = __float2half_rn(x);
+// 4 neighbouring output values
+__device__ __forceinline__ void store_out4(void* base, int64_t at, int dtype, float4 v) {
+  if (dtype == kKv4F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = v;
+  } else if (dtype == kKv4Bf16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) =
+        make_uint2(pack_f16x2(v.x, v.y), pack_f16x2(v.z, v.w));
+  }
 }
 
 // x = hi + lo in f16: two values' hi parts and lo parts, packed
@@ -308,17 +327,19 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 
   if (warp >= kWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kProducerRegs));
-    if (warp > kWarps) return;
-    // ---- producer: the chunks of every part in order, a page's block of the head per stage ----
-    int st = 0;
-    uint32_t turn = 0;   // how often the ring has gone round
+    // ---- producers: chunk k of the parts in order is warp k % 4's, a page's block of the head into stage k % kStages;
+    // 32 chunks' pages are looked up at once ----
+    const int pw = warp - kWarps;
+    uint32_t it = 0;
     while (kv4_next(a, block_rows, walk, p)) {
       const uint8_t* head = a.w.pool + (int64_t)p.h * Shape::kBlock;
-      for (int k0 = 0; k0 < p.take; k0 += 32) {
-        const int64_t mine = k0 + lane < p.take ? kv4_page(a.w, p.seq, p.lo + p.c0 + k0 + lane) : -1;
-        const int count = min(p.take - k0, 32);
-        for (int j = 0; j < count; ++j) {
+      int x = (pw - (int)it) & 3;   // this warp's next chunk of the part
+      while (x < p.take) {
+        const int count = min((p.take - x + 3) / 4, 32);
+        const int64_t mine = lane < count ? kv4_page(a.w, p.seq, p.lo + p.c0 + x + 4 * lane) : -1;
+        for (int j = 0; j < count; ++j, x += 4) {
           const int64_t page = __shfl_sync(0xffffffffu, mine, j);
+          const uint32_t k = it + x, st = k % kStages, turn = k / kStages;
           if (lane == 0 && (turn == 0 || kv4_wait(&sm.empty[st], (turn - 1) & 1, &sm.failed, a.w.err))) {
             sm.present[st] = page >= 0;
             if (page >= 0) {
@@ -328,15 +349,11 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
               mbar_arrive(&sm.full[st]);
             }
           }
-          if (++st == kStages) {
-            st = 0;
-            ++turn;
-          }
           __syncwarp();
         }
       }
+      it += p.take;
     }
-    if (lane == 0 && share_items == 0) splits[blockIdx.x].last = -1;
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kConsumerRegs));
     const int rt = warp % tiles, sl = warp / tiles;   // this warp's rows of the row block, its turn among the units
@@ -352,69 +369,77 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
       // the warp's first and last position
       const int tmin = position(r0 / group), tmax = position((min(r0 + warp_rows, qrows) - 1) / group);
 
-      // Q as the operand of row 8 j + g: the 8 dims of one K word per block of 32, nibble pair i (dims i, i + 4) is a
-      // register of step i / 2. Then what belongs to rows 8 j + 2 tq + {0, 1}, this lane's scores' rows.
+      // ---- Q as the first product's operand for every row of the block, by all consumer warps: a thread takes 8
+      // neighbouring dims, the word of K codes that lane 4 g + (dims / 8) % 4 multiplies: nibble pair i (dims i, i + 4)
+      // is a register of step i / 2 ----
+      uint4* qfrag = reinterpret_cast<uint4*>(sm.acc);
+      constexpr int kPieces = D / 8;   // threads per row
+      for (int x = threadIdx.x; x < block_rows * kPieces; x += 32 * kWarps) {   // whole warps: block_rows x D / 8 >= 64
+        const int row = x / kPieces, d8 = x % kPieces;
+        const uint32_t r = (uint32_t)p.b * block_rows + row, i = r / group;
+        const bool live = r < qrows;
+        float v[8] = {};
+        if (live)
+          load_q8(a.q, ((int64_t)p.row0 + i) * a.q_row + (int64_t)(p.h * group + (r - i * group)) * a.q_head + 8 * d8, TYPE,
+                  v);
+        float mx = 0.f, sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[e]));
+#pragma unroll
+        for (int o = 1; o < kPieces; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const int e2 = min(max((int)(__float_as_uint(mx) >> 23), 16), 254);   // biased exponent of the largest value
+        // the factor is not negative (a maximum of scores stays one): a negative scale turns q's sign
+        const float up = a.scale < 0.f ? -pow2_bits(min(268 - e2, 254)) : pow2_bits(min(268 - e2, 254));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] *= up;
+          sum += v[e];
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);   // the group's 8 threads
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float f = e % 2 ? 0.0625f : 1.f;   // the codes at bits 4-7 stand for 16 times the others
+          if constexpr (kQPlanes == 2)
+            split_f16x2(v[e] * f, v[e + 4] * f, hi[e], lo[e]);
+          else
+            hi[e] = pack_f16x2(v[e] * f, v[e + 4] * f);
+        }
+        const int at = (row / 8 * kQPlanes * kBlocks + d8 / 4) * 32 + 4 * (row % 8) + d8 % 4;
+        qfrag[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (kQPlanes == 2) qfrag[at + kBlocks * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (d8 % 8 == 0) sm.qsum[row][d8 / 8] = sum * (1.f / 16777216.f);
+        if (d8 == 0) {
+          sm.qfac[row] = fmaxf(fabsf(a.scale) * kLog2e * (16777216.f / fabsf(up)), 1.1754944e-38f);   // 2^24: the codes' unit
+          sm.qpos[row] = live ? position(i) : -1;
+        }
+      }
+      named_bar_sync(1, 32 * kWarps);
+      // the operands of rows 8 j + g, and what belongs to rows 8 j + 2 tq + {0, 1}, this lane's scores' rows
       uint32_t qb[RT][kBlocks][2][kQPlanes][2];
       float qsum[RT][2][kGroups], rf[RT][2];   // (sum q)_G and the factor from the products' unit to base-2 scores
       int t[RT][2];                            // the row's position; dead rows see nothing
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
-        const uint32_t r = r0 + 8 * j + g, i = r / group;
-        const bool live = r < qrows;
-        float x[kBlocks][8], mx = 0.f, sums[kGroups];
-        const int64_t at = ((int64_t)p.row0 + i) * a.q_row + (int64_t)(p.h * group + (r - i * group)) * a.q_head;
+        const int tile = rt * RT + j;
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          if (live)
-            load_q8(a.q, at + 32 * b + 8 * tq, TYPE, x[b]);
-          else
+        for (int pl = 0; pl < kQPlanes; ++pl)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[b][e] = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[b][e]));
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e2 = min(max((int)(__float_as_uint(mx) >> 23), 16), 254);   // biased exponent of the largest value
-        // the factor is not negative (a maximum of scores stays one): a negative scale turns q's sign
-        const float up = a.scale < 0.f ? -pow2_bits(min(268 - e2, 254)) : pow2_bits(min(268 - e2, 254));
-        const float f = fmaxf(fabsf(a.scale) * kLog2e * (16777216.f / fabsf(up)), 1.1754944e-38f);   // 2^24: the codes' unit
-#pragma unroll
-        for (int G = 0; G < kGroups; ++G) sums[G] = 0.f;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[b][e] *= up;
-            sums[b / 2] += x[b][e];
+          for (int b = 0; b < kBlocks; ++b) {
+            const uint4 v = qfrag[((tile * kQPlanes + pl) * kBlocks + b) * 32 + lane];
+            qb[j][b][0][pl][0] = v.x, qb[j][b][0][pl][1] = v.y, qb[j][b][1][pl][0] = v.z, qb[j][b][1][pl][1] = v.w;
           }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float lo0 = x[b][2 * e], lo1 = x[b][2 * e + 4], hi0 = x[b][2 * e + 1] * 0.0625f,
-                        hi1 = x[b][2 * e + 5] * 0.0625f;
-            if constexpr (kQPlanes == 2) {
-              split_f16x2(lo0, lo1, qb[j][b][e][0][0], qb[j][b][e][kQPlanes - 1][0]);
-              split_f16x2(hi0, hi1, qb[j][b][e][0][1], qb[j][b][e][kQPlanes - 1][1]);
-            } else {
-              qb[j][b][e][0][0] = pack_f16x2(lo0, lo1);
-              qb[j][b][e][0][1] = pack_f16x2(hi0, hi1);
-            }
-          }
-        }
-#pragma unroll
-        for (int G = 0; G < kGroups; ++G) {
-          sums[G] += __shfl_xor_sync(0xffffffffu, sums[G], 1);
-          sums[G] += __shfl_xor_sync(0xffffffffu, sums[G], 2);
-        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int from = 4 * (2 * tq + e);
-          rf[j][e] = __shfl_sync(0xffffffffu, f, from);
+          const int row = 8 * tile + 2 * tq + e;
+          rf[j][e] = sm.qfac[row];
+          t[j][e] = sm.qpos[row];
 #pragma unroll
-          for (int G = 0; G < kGroups; ++G) qsum[j][e][G] = __shfl_sync(0xffffffffu, sums[G], from) * (1.f / 16777216.f);
-          t[j][e] = __shfl_sync(0xffffffffu, live ? position(i) : -1, from);
+          for (int G = 0; G < kGroups; ++G) qsum[j][e][G] = sm.qsum[row][G];
         }
       }
+      named_bar_sync(1, 32 * kWarps);   // before the accumulators take the operands' place
 
       // the rows' dims 32 c + 16 m + g (+ 8: the last two), rows 8 j + 2 tq + {0, 1}, without the offsets' part
       float o[RT][kBlocks][2][4];
@@ -645,35 +670,46 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
             }
         }
       named_bar_sync(1, 32 * kWarps);
-      // a warp per row: lane v has the row's maximum in the v-th of its `lanes` warps
       const bool whole = p.c0 == 0 && p.take == p.cnt;
       float* mine = part + (int64_t)(2 * blockIdx.x + (p.c0 == 0 ? 1 : 0)) * block_rows * part_row(D);
-      for (int row = warp; row < block_rows; row += kWarps) {
+      if (threadIdx.x < block_rows) {   // a thread per row: the weights of its warps' accumulators
+        const int tile = threadIdx.x / warp_rows, from = threadIdx.x % warp_rows;
+        float M = -INFINITY, l = 0.f;
+        for (int v = 0; v < lanes; ++v) M = fmaxf(M, sm.m[v * tiles + tile][from]);
+        for (int v = 0; v < lanes; ++v) {
+          float* mv = &sm.m[v * tiles + tile][from];
+          const float wt = *mv == M ? 1.f : ex2_approx(*mv - M);
+          *mv = wt;
+          l = fmaf(wt, sm.l[v * tiles + tile][from], l);
+        }
+        sm.row_l[threadIdx.x] = whole ? (l == 0.f ? 0.f : 1.f / l) : l;
+        sm.row_m[threadIdx.x] = M;
+      }
+      named_bar_sync(1, 32 * kWarps);
+      constexpr int kQuads = D / 4;   // threads per row
+#pragma unroll 2
+      for (int x = threadIdx.x; x < block_rows * kQuads; x += 32 * kWarps) {
+        const int row = x / kQuads, d0 = 4 * (x % kQuads), tile = row / warp_rows, from = row % warp_rows;
         const uint32_t rr = (uint32_t)p.b * block_rows + row;
         if (rr >= qrows) break;
-        const int tile = row / warp_rows, from = row % warp_rows;
-        const float mv = lane < lanes ? sm.m[lane * tiles + tile][from] : -INFINITY, M = warp_max(mv);
-        const float wt = mv == M ? 1.f : ex2_approx(mv - M);
-        const float l = warp_sum(lane < lanes ? wt * sm.l[lane * tiles + tile][from] : 0.f);
-        float y[D / 32];
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) y[e] = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int v = 0; v < lanes; ++v) {
-          const float f = __shfl_sync(0xffffffffu, wt, v);
-#pragma unroll
-          for (int e = 0; e < D / 32; ++e) y[e] = fmaf(f, sm.acc[v * tiles + tile][from][32 * e + lane], y[e]);
+          const float wt = sm.m[v * tiles + tile][from];
+          const float4 u = *reinterpret_cast<const float4*>(&sm.acc[v * tiles + tile][from][d0]);
+          y.x = fmaf(wt, u.x, y.x);
+          y.y = fmaf(wt, u.y, y.y);
+          y.z = fmaf(wt, u.z, y.z);
+          y.w = fmaf(wt, u.w, y.w);
         }
         if (whole) {
-          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const float inv = sm.row_l[row];
           const uint32_t i = rr / group;
-          const int64_t at = (((int64_t)p.row0 + i) * a.heads + p.h * group + (rr - i * group)) * D + lane;
-#pragma unroll
-          for (int e = 0; e < D / 32; ++e) store_out(a.out, at + 32 * e, TYPE, y[e] * inv);
+          store_out4(a.out, (((int64_t)p.row0 + i) * a.heads + p.h * group + (rr - i * group)) * D + d0, TYPE,
+                     make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
         } else {
           float* to = mine + (int64_t)row * part_row(D);
-#pragma unroll
-          for (int e = 0; e < D / 32; ++e) to[4 + 32 * e + lane] = y[e];
-          if (lane == 0) *reinterpret_cast<float2*>(to) = make_float2(M, l);
+          *reinterpret_cast<float4*>(to + 4 + d0) = y;
+          if (d0 == 0) *reinterpret_cast<float2*>(to) = make_float2(sm.row_m[row], sm.row_l[row]);
         }
       }
       split_after = p.c0 == 0 && !whole;
@@ -685,84 +721,105 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
       }
       named_bar_sync(1, 32 * kWarps);   // before the next part's sums
     }
-    if (threadIdx.x == 0 && !split_after && share_items > 0) splits[blockIdx.x].last = -1;
+    if (threadIdx.x == 0 && !split_after) splits[blockIdx.x].last = -1;
   }
   pdl_launch_next();
 }
 
-// The splits (sequence, row block, KV head) that ended inside a CTA's share: the last part of CTA `first` and the first
-// parts of the CTAs after it, joined by their maxima in that order. A row is joined by `per` warps of a block, which
-// take every per-th part: 8 when there are fewer rows than blocks (the parts' latency counts), else 1.
-constexpr int kCombineWarps = 8, kCombineBlocksPerSm = 4, kMostSms = 1024;
+// The splits (sequence, row block, KV head) that a CTA's share ended in: the last part of that CTA and the first parts
+// of the CTAs after it, joined by their maxima. A set of D / 4 threads takes 4 dims each of a part's row. With few rows
+// (the parts' latency counts) a block's sets share a row and take every kSets-th part, else a set has a row of its own.
+constexpr int kCombineThreads = 256, kCombineBlocksPerSm = 4, kMostSms = 256;
 
 template <int D>
-__global__ void __launch_bounds__(32 * kCombineWarps)
+__global__ void __launch_bounds__(kCombineThreads)
     kv4_combine_kernel(const Kv4Attn a, const int block_rows, const int ctas, const float* part, const Kv4Split* splits) {
-  constexpr int kPer = D / 32;
-  __shared__ short found[kMostSms];
-  __shared__ int count;
-  __shared__ float acc[kCombineWarps][D];
-  __shared__ float sum[kCombineWarps];
+  constexpr int kQuads = D / 4, kSets = kCombineThreads / kQuads;   // 4, 8 or 16 sets of threads
+  __shared__ Kv4Split found[kMostSms];
+  __shared__ short cta[kMostSms];
+  __shared__ int before[kMostSms / 32 + 1];
+  __shared__ __align__(16) float acc[kSets][D];
+  __shared__ float sm_m[kSets], sm_l[kSets];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
-  if (warp == 0) {   // the CTAs with a split, in order
-    int n = 0;
-    for (int c0 = 0; c0 < ctas; c0 += 32) {
-      const bool has = c0 + lane < ctas && splits[c0 + lane].last >= 0;
-      const uint32_t all = __ballot_sync(0xffffffffu, has);
-      if (has) found[n + __popc(all & ((1u << lane) - 1))] = (short)(c0 + lane);
-      n += __popc(all);
-    }
-    if (lane == 0) count = n;
+  // the CTAs with a split, in order
+  Kv4Split mine;
+  mine.last = -1;
+  if (threadIdx.x < ctas) mine = splits[threadIdx.x];
+  const uint32_t has = __ballot_sync(0xffffffffu, mine.last >= 0);
+  if (lane == 0) before[warp + 1] = __popc(has);
+  if (threadIdx.x == 0) before[0] = 0;
+  __syncthreads();
+  int n = 0, count = 0;
+  for (int v = 1; v <= kMostSms / 32; ++v) {
+    if (v <= warp) n += before[v];
+    count += before[v];
+  }
+  if (mine.last >= 0) {
+    n += __popc(has & ((1u << lane) - 1));
+    found[n] = mine;
+    cta[n] = (short)threadIdx.x;
   }
   __syncthreads();
-  const int rows = count * block_rows, per = rows <= (int)gridDim.x ? kCombineWarps : 1;
   const uint32_t group = a.group;
-  for (int r0 = blockIdx.x * (kCombineWarps / per); r0 < rows; r0 += gridDim.x * (kCombineWarps / per)) {
-    const int r = r0 + warp / per, mine = warp % per;
-    float y[kPer] = {}, l = 0.f;
+  const int rows = count * block_rows, set = threadIdx.x / kQuads, d0 = 4 * (threadIdx.x % kQuads);
+  const bool together = rows <= (int)gridDim.x;   // a block per row
+  const int step = together ? 1 : kSets;
+  for (int r0 = blockIdx.x * step; r0 < rows; r0 += gridDim.x * step) {
+    const int r = together ? r0 : r0 + set;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -INFINITY, l = 0.f;
     int64_t to = -1;
     if (r < rows) {
-      const int first = found[r / block_rows], row = r % block_rows;
-      const Kv4Split sp = splits[first];
+      const Kv4Split sp = found[r / block_rows];
+      const int first = cta[r / block_rows], row = r % block_rows;
       const uint32_t rr = (uint32_t)sp.b * block_rows + row;
       if (rr < (uint32_t)sp.n * group) {
         const uint32_t i = rr / group;
-        to = (((int64_t)sp.row0 + i) * a.heads + sp.h * group + (rr - i * group)) * D + lane;
+        to = (((int64_t)sp.row0 + i) * a.heads + sp.h * group + (rr - i * group)) * D + d0;
         const int parts = sp.last - first + 1;
-        auto at = [&](int k) {   // the k-th part's row
-          return part + ((int64_t)(2 * (first + k) + (k == 0 ? 1 : 0)) * block_rows + row) * part_row(D);
-        };
-        float M = -INFINITY;
-        for (int k = lane; k < parts; k += 32) M = fmaxf(M, at(k)[0]);
-        M = warp_max(M);
 #pragma unroll 4
-        for (int k = mine; k < parts; k += per) {
-          const float* from = at(k);
-          const float mv = from[0], wt = mv == M ? 1.f : ex2_approx(mv - M);
-          l = fmaf(wt, from[1], l);
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) y[e] = fmaf(wt, from[4 + 32 * e + lane], y[e]);
+        for (int k = together ? set : 0; k < parts; k += together ? kSets : 1) {
+          const float* from = part + ((int64_t)(2 * (first + k) + (k == 0 ? 1 : 0)) * block_rows + row) * part_row(D);
+          const float2 ml = *reinterpret_cast<const float2*>(from);
+          const float4 u = *reinterpret_cast<const float4*>(from + 4 + d0);
+          const float top = fmaxf(M, ml.x);
+          const float old = M == top ? 1.f : ex2_approx(M - top), add = ml.x == top ? 1.f : ex2_approx(ml.x - top);
+          M = top;
+          l = fmaf(add, ml.y, l * old);
+          y.x = fmaf(add, u.x, y.x * old);
+          y.y = fmaf(add, u.y, y.y * old);
+          y.z = fmaf(add, u.z, y.z * old);
+          y.w = fmaf(add, u.w, y.w * old);
         }
       }
     }
-    if (per > 1) {
+    if (together) {
       __syncthreads();
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[warp][32 * e + lane] = y[e];
-      if (lane == 0) sum[warp] = l;
+      *reinterpret_cast<float4*>(&acc[set][d0]) = y;
+      if (d0 == 0) {
+        sm_m[set] = M;
+        sm_l[set] = l;
+      }
       __syncthreads();
-      if (warp != 0) continue;
-      for (int v = 1; v < kCombineWarps; ++v) {
-        l += sum[v];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) y[e] += acc[v][32 * e + lane];
+      if (set != 0) continue;
+      float top = M;
+      for (int v = 1; v < kSets; ++v) top = fmaxf(top, sm_m[v]);
+      y = make_float4(0.f, 0.f, 0.f, 0.f);
+      l = 0.f;
+      for (int v = 0; v < kSets; ++v) {
+        const float wt = sm_m[v] == top ? 1.f : ex2_approx(sm_m[v] - top);
+        const float4 u = *reinterpret_cast<const float4*>(&acc[v][d0]);
+        l = fmaf(wt, sm_l[v], l);
+        y.x = fmaf(wt, u.x, y.x);
+        y.y = fmaf(wt, u.y, y.y);
+        y.z = fmaf(wt, u.z, y.z);
+        y.w = fmaf(wt, u.w, y.w);
       }
     }
     if (to < 0) continue;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) store_out(a.out, to + 32 * e, a.dtype, y[e] * inv);
+    store_out4(a.out, to, a.dtype, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
   }
 }
 
@@ -791,7 +848,7 @@ void launch(const Kv4Attn& a, int tiles, int sms, cudaStream_t s) {
   XTG_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sms * kCombineBlocksPerSm);
-  cfg.blockDim = dim3(32 * kCombineWarps);
+  cfg.blockDim = dim3(kCombineThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
