@@ -38,6 +38,7 @@ namespace xtg {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 6.f;   // how far, in powers of two, a row's probabilities may pass 1 before its sums are scaled
 constexpr int kUnit = 32;                        // positions a warp takes at once: half a chunk
 constexpr int kUnits = kKv4Page / kUnit, kSteps = kUnit / 16;
 // What the start of another part costs a CTA (its rows, its sums), in chunks: counted as items before the part's first,
@@ -260,6 +261,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
   constexpr int kStages = Shape::kStages, kWarps = Shape::kWarps, kThreads = Shape::kThreads;
   constexpr int kGroups = D / kKv4Group, kBlocks = D / 32, H = D < 128 ? D : 128;
   constexpr int kQPlanes = TYPE == kKv4F32 ? 2 : 1;
+  constexpr bool kDirect = TYPE != kKv4F32;   // P V added up in the matrix unit
   extern __shared__ __align__(128) unsigned char smem_raw[];
   Kv4Smem<D, RT>& sm = *reinterpret_cast<Kv4Smem<D, RT>*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -444,7 +446,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
       // the rows' dims 32 c + 16 m + g (+ 8: the last two), rows 8 j + 2 tq + {0, 1}, without the offsets' part
       float o[RT][kBlocks][2][4];
       float oz[RT][2][kGroups];   // sum of P z over this lane's slots
-      float run_m[RT][2], run_l[RT][2];
+      float ref[RT][2], run_l[RT][2];
+      int unit_e[kGroups];   // P s 2^(136 - unit_e) is below 2^15
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
 #pragma unroll
@@ -453,12 +456,15 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
           for (int m = 0; m < 2; ++m) o[j][c][m][0] = o[j][c][m][1] = o[j][c][m][2] = o[j][c][m][3] = 0.f;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          run_m[j][e] = -INFINITY;
+          ref[j][e] = -INFINITY;
           run_l[j][e] = 0.f;
 #pragma unroll
           for (int G = 0; G < kGroups; ++G) oz[j][e][G] = 0.f;
         }
       }
+
+#pragma unroll
+      for (int G = 0; G < kGroups; ++G) unit_e[G] = 27;
 
       // half chunk hh of a stage, its first position p0
       auto unit = [&](const uint8_t* stg, int hh, int p0, auto masked_) {
@@ -531,52 +537,93 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
               }
           }
         }
-        // ---- the running maxima and sums ----
-        float alpha[RT][2];
+        // ---- the scales of V: their largest exponent per group ----
+        uint32_t w[kGroups][2 * kSteps];   // slots 8 i + g
+        bool move = false;
+        int next_e[kGroups];
+#pragma unroll
+        for (int G = 0; G < kGroups; ++G) {
+          int top = 0;   // the largest scale's word: positive f32 order is integer order, NaN's word is negative
+#pragma unroll
+          for (int i = 0; i < 2 * kSteps; ++i) {
+            w[G][i] = vpar[G * kKv4Page + 8 * i + g];
+            if constexpr (kMasked) {   // what no row of the warp sees may hold anything
+              const int pp = p0 + 8 * i + g;
+              if (pp > tmax || (a.window > 0 && pp <= tmin - a.window)) w[G][i] = 0;
+            }
+            top = max(top, (int)w[G][i]);
+          }
+          next_e[G] = top >> 23;
+          move |= next_e[G] > unit_e[G];
+        }
+        // ---- the rows' references: a row's probabilities are 2^(score - ref), at most 2^kSlack; a reference (and V's
+        // exponent) moves up when a maximum passes it by more, and then the sums are scaled ----
+        float mx[RT][2];
 #pragma unroll
         for (int j = 0; j < RT; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(s[j][0][e], s[j][0][e + 2]);
+            float m = fmaxf(s[j][0][e], s[j][0][e + 2]);
 #pragma unroll
-            for (int u = 1; u < kSteps; ++u) mx = fmaxf(mx, fmaxf(s[j][u][e], s[j][u][e + 2]));
+            for (int u = 1; u < kSteps; ++u) m = fmaxf(m, fmaxf(s[j][u][e], s[j][u][e + 2]));
+            mx[j][e] = m * rf[j][e];
+            move |= mx[j][e] > ref[j][e] + kSlack;
+          }
+        if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            const float new_m = fmaxf(run_m[j][e], mx * rf[j][e]), ref = new_m == -INFINITY ? 0.f : new_m;
-            alpha[j][e] = ex2_approx(run_m[j][e] - ref);
-            run_m[j][e] = new_m;
-            float l = run_l[j][e] * alpha[j][e];
+          for (int G = 0; G < kGroups; ++G) {
+            int e2 = min(max(next_e[G], unit_e[G]), 254);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) e2 = max(e2, __shfl_xor_sync(0xffffffffu, e2, x));
+            next_e[G] = e2;
+          }
+#pragma unroll
+          for (int j = 0; j < RT; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float m = fmaxf(mx[j][e], ref[j][e]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+              const float alpha = m == ref[j][e] ? 1.f : ex2_approx(ref[j][e] - m);
+              ref[j][e] = m;
+              run_l[j][e] *= alpha;
+#pragma unroll
+              for (int G = 0; G < kGroups; ++G) {
+                oz[j][e][G] *= alpha;
+                const float f = kDirect ? alpha * ex2_approx((float)(unit_e[G] - next_e[G])) : alpha;
+#pragma unroll
+                for (int c = 2 * G; c < 2 * G + 2; ++c)
+#pragma unroll
+                  for (int m2 = 0; m2 < 2; ++m2) {
+                    o[j][c][m2][e] *= f;
+                    o[j][c][m2][e + 2] *= f;
+                  }
+              }
+            }
+#pragma unroll
+          for (int G = 0; G < kGroups; ++G) unit_e[G] = next_e[G];
+        }
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float r = ref[j][e] == -INFINITY ? 0.f : ref[j][e];
 #pragma unroll
             for (int u = 0; u < kSteps; ++u) {
-              s[j][u][e] = ex2_approx(fmaf(s[j][u][e], rf[j][e], -ref));
-              s[j][u][e + 2] = ex2_approx(fmaf(s[j][u][e + 2], rf[j][e], -ref));
-              l += s[j][u][e] + s[j][u][e + 2];
+              s[j][u][e] = ex2_approx(fmaf(s[j][u][e], rf[j][e], -r));
+              s[j][u][e + 2] = ex2_approx(fmaf(s[j][u][e + 2], rf[j][e], -r));
+              run_l[j][e] += s[j][u][e] + s[j][u][e + 2];
             }
-            run_l[j][e] = l;
           }
         // ---- P V by group of 64 dims ----
 #pragma unroll
         for (int G = 0; G < kGroups; ++G) {
-          uint32_t w[2 * kSteps];   // slots 8 i + g
-          int top = 0;   // the largest scale's word: positive f32 order is integer order, NaN's word is negative
-#pragma unroll
-          for (int i = 0; i < 2 * kSteps; ++i) {
-            w[i] = vpar[G * kKv4Page + 8 * i + g];
-            if constexpr (kMasked) {   // what no row of the warp sees may hold anything
-              const int pp = p0 + 8 * i + g;
-              if (pp > tmax || (a.window > 0 && pp <= tmin - a.window)) w[i] = 0;
-            }
-            top = max(top, (int)w[i]);
-          }
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
-          const int e2 = min(max(top >> 23, 27), 254);
-          const float down = pow2_bits(268 - e2), up = pow2_bits(e2 - 14) * 16.f;   // P s below 2^15 and back
+          const float down = pow2_bits(136 + 127 - unit_e[G]), up = pow2_bits(unit_e[G] - 9) * 16.f;
           uint32_t pb[RT][2][2 * kSteps];
 #pragma unroll
           for (int i = 0; i < 2 * kSteps; ++i) {
-            const float sc = __uint_as_float(w[i] & 0xffff0000u) * down;
-            const float of = __uint_as_float(w[i] << 16);
+            const float sc = __uint_as_float(w[G][i] & 0xffff0000u) * down;
+            const float of = __uint_as_float(w[G][i] << 16);
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
               const float p0_ = s[j][i / 2][2 * (i % 2)], p1_ = s[j][i / 2][2 * (i % 2) + 1];
@@ -590,14 +637,13 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
               const float h1 = __uint_as_float(__float_as_uint(x1) & 0xffffe000u);
               pb[j][0][i] = transpose8(pack_f16x2(h0, h1));
               pb[j][1][i] = transpose8(pack_f16x2(x0 - h0, x1 - h1));
-              oz[j][0][G] = i == 0 ? fmaf(p0_, of, oz[j][0][G] * alpha[j][0]) : fmaf(p0_, of, oz[j][0][G]);
-              oz[j][1][G] = i == 0 ? fmaf(p1_, of, oz[j][1][G] * alpha[j][1]) : fmaf(p1_, of, oz[j][1][G]);
+              oz[j][0][G] = fmaf(p0_, of, oz[j][0][G]);
+              oz[j][1][G] = fmaf(p1_, of, oz[j][1][G]);
             }
           }
 #pragma unroll
           for (int c = 2 * G; c < 2 * G + 2; ++c) {
-            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-            float d[RT][2][4];
+            float d[RT][2][4] = {};
             const uint4 v = *reinterpret_cast<const uint4*>(vw + ((c * 8 + g) * 4 + tq) * 4);
             const uint32_t word[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -608,20 +654,18 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
                 const uint32_t va[4] = {v_codes_low(w0), v_codes_low(w1), v_codes_high(w0), v_codes_high(w1)};
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
-                  if (st == 0)
-                    mma_f16_from(d[j][m], va, pb[j][0][0], pb[j][0][1], zero);
-                  else
-                    mma_f16_add(d[j][m], va, pb[j][0][2], pb[j][0][3]);
-                  mma_f16_add(d[j][m], va, pb[j][1][2 * st], pb[j][1][2 * st + 1]);
+                  float(&to)[4] = kDirect ? o[j][c][m] : d[j][m];
+                  mma_f16_add(to, va, pb[j][0][2 * st], pb[j][0][2 * st + 1]);
+                  mma_f16_add(to, va, pb[j][1][2 * st], pb[j][1][2 * st + 1]);
                 }
               }
+            if constexpr (!kDirect)
 #pragma unroll
-            for (int j = 0; j < RT; ++j)
+              for (int j = 0; j < RT; ++j)
 #pragma unroll
-              for (int m = 0; m < 2; ++m)
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  o[j][c][m][e] = fmaf(d[j][m][e], up, o[j][c][m][e] * alpha[j][e % 2]);
+                  for (int e = 0; e < 4; ++e) o[j][c][m][e] = fmaf(d[j][m][e], up, o[j][c][m][e]);
           }
         }
       };
@@ -658,15 +702,16 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
             for (int G = 0; G < kGroups; ++G) oz[j][e][G] += __shfl_xor_sync(0xffffffffu, oz[j][e][G], x);
           }
           if (g == 0) {
-            sm.m[warp][row] = run_m[j][e];
+            sm.m[warp][row] = ref[j][e];
             sm.l[warp][row] = run_l[j][e];
           }
 #pragma unroll
           for (int c = 0; c < kBlocks; ++c)
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-              sm.acc[warp][row][32 * c + 16 * m + g] = o[j][c][m][e] + oz[j][e][c / 2];
-              sm.acc[warp][row][32 * c + 16 * m + 8 + g] = o[j][c][m][e + 2] + oz[j][e][c / 2];
+              const float up = kDirect ? pow2_bits(unit_e[c / 2] - 9) * 16.f : 1.f;
+              sm.acc[warp][row][32 * c + 16 * m + g] = fmaf(o[j][c][m][e], up, oz[j][e][c / 2]);
+              sm.acc[warp][row][32 * c + 16 * m + 8 + g] = fmaf(o[j][c][m][e + 2], up, oz[j][e][c / 2]);
             }
         }
       named_bar_sync(1, 32 * kWarps);
