@@ -10,6 +10,7 @@ import ctypes as C
 import json
 import os
 import subprocess
+import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libxtg_cuda.so")
@@ -602,12 +603,17 @@ KV4_PAGE = 64
 
 _KV4_ERRORS = {1: "a device wait timed out", 6: "a position lies past its sequence's page table",
                7: "a page table entry lies past the pool"}
-_kv4_workspace_bytes = {}
+_kv4_dtypes = {}            # torch dtype -> the C ABI's code
+_kv4_workspace_bytes = {}   # by shape and device
+_kv4_local = threading.local()
 
 
-def _kv4_dtypes():
-    import torch
-    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+def _kv4_dtype(t):
+    """The C ABI's code of a torch dtype, None for one it does not take."""
+    if not _kv4_dtypes:
+        import torch
+        _kv4_dtypes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    return _kv4_dtypes.get(t)
 
 
 def kv4_pool(pages, kv_heads, head_dim, device="cuda"):
@@ -624,59 +630,71 @@ def kv4_check(err):
         raise XtgError("kv4: " + _KV4_ERRORS.get(code, f"error {code}"))
 
 
-def _kv4_where(pool, table, pos, cu_rows, rows, err):
+def _kv4_index(name, t, dims, dev):
+    """The shape of an index tensor (contiguous int32 on device dev)."""
     import torch
-    dev = pool.device
-    if pool.dtype != torch.uint8 or pool.dim() != 3 or not pool.is_contiguous() or not pool.is_cuda:
+    shape = t.shape
+    if t.dtype is not torch.int32 or len(shape) != dims or t.get_device() != dev or not t.is_contiguous():
+        raise XtgError(f"kv4: {name} is a contiguous int32 tensor of {dims} dimension(s) on the pool's device")
+    return shape
+
+
+def _kv4_where(pool, table, pos, cu_rows, rows, err):
+    """(xtg_cuda_kv4, the pool's device) after the checks that need no device work."""
+    import torch
+    dev = pool.get_device()
+    shape = pool.shape
+    if pool.dtype is not torch.uint8 or len(shape) != 3 or not pool.is_contiguous() or dev < 0:
         raise XtgError("kv4: pool is a contiguous uint8 CUDA tensor [pages][kv_heads][72 head_dim]")
-    pages, kvh, block = pool.shape
-    if block % 72 or block // 72 not in (64, 128, 256):
+    pages, kvh, block = shape
+    if block not in (72 * 64, 72 * 128, 72 * 256):
         raise XtgError("kv4: head_dim 64, 128 or 256 (pool.shape[2] / 72)")
-    for name, t, dims in (("table", table, 2), ("pos", pos, 1), ("cu_rows", cu_rows, 1)):
-        if t.dtype != torch.int32 or t.dim() != dims or t.device != dev or not t.is_contiguous():
-            raise XtgError(f"kv4: {name} is a contiguous int32 tensor of {dims} dimension(s) on the pool's device")
-    seqs, max_pages = table.shape
-    if pos.shape[0] != seqs or cu_rows.shape[0] != seqs + 1:
+    seqs, max_pages = _kv4_index("table", table, 2, dev)
+    if _kv4_index("pos", pos, 1, dev)[0] != seqs or _kv4_index("cu_rows", cu_rows, 1, dev)[0] != seqs + 1:
         raise XtgError("kv4: table [seqs][max_pages], pos [seqs], cu_rows [seqs + 1]")
-    if err is not None and (err.dtype != torch.int32 or err.numel() != 1 or err.device != dev):
+    if err is not None and (err.dtype is not torch.int32 or err.numel() != 1 or err.get_device() != dev):
         raise XtgError("kv4: err is one int32 on the pool's device")
     return Kv4(pool.data_ptr(), pages, kvh, block // 72, table.data_ptr(), max_pages, seqs, pos.data_ptr(),
-               cu_rows.data_ptr(), rows, err.data_ptr() if err is not None else None)
+               cu_rows.data_ptr(), rows, None if err is None else err.data_ptr()), dev
 
 
-def _kv4_rows(name, t, pool, heads):
-    """dtype code of rows t [rows][heads][head_dim] with contiguous head dims on the pool's device."""
-    dtype = _kv4_dtypes().get(t.dtype)
+def _kv4_rows(name, t, heads, c, dev):
+    """(dtype code, strides) of rows t [rows][heads][head_dim] with contiguous head dims on device dev; heads 0: any."""
+    dtype = _kv4_dtype(t.dtype)
     if dtype is None:
         raise XtgError(f"kv4: {name} is float32, bfloat16 or float16")
-    if t.dim() != 3 or t.shape[2] * 72 != pool.shape[2] or (heads and t.shape[1] != heads) or t.device != pool.device:
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != c.head_dim or (heads and shape[1] != heads) or t.get_device() != dev:
         raise XtgError(f"kv4: {name} is [rows][heads][head_dim] of the pool's head_dim on the pool's device")
-    if t.stride(2) != 1 and t.numel():
+    if strides[2] != 1:
         raise XtgError(f"kv4: {name}'s head dims must be contiguous")
-    return dtype
+    return dtype, strides
 
 
-def _kv4_call(pool, f, *args):
-    """Call entry point f with the pool's device current, on its current stream."""
+def _kv4_call(dev, f, *args):
+    """Call entry point f with device dev current, on its current stream."""
     import torch
-    err = _err()
-    if torch.cuda.current_device() == pool.device.index:
-        rc = f(*args, torch.cuda.current_stream().cuda_stream, err, len(err))
-    else:
-        with torch.cuda.device(pool.device):
-            rc = f(*args, torch.cuda.current_stream().cuda_stream, err, len(err))
-    _check(rc, err)
+    err = getattr(_kv4_local, "err", None)
+    if err is None:
+        err = _kv4_local.err = _err()
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return _kv4_call(dev, f, *args)
+    # torch.cuda.current_stream() builds a Stream object for the same handle: 3 us a call
+    if f(*args, torch._C._cuda_getCurrentRawStream(dev), err, 1024):
+        raise XtgError(err.value.decode(errors="replace"))
 
 
 def kv4_store(pool, k, v, table, pos, cu_rows, err=None):
     """Quantise rows k, v [rows][kv_heads][head_dim] (float32, bfloat16 or float16; row and head strides of 16-byte
     multiples) into the pool. Two sequences of a call must not write the same page."""
-    dtype = _kv4_rows("k", k, pool, pool.shape[1])
-    if _kv4_rows("v", v, pool, pool.shape[1]) != dtype or k.shape[0] != v.shape[0]:
+    rows = k.shape[0]
+    c, dev = _kv4_where(pool, table, pos, cu_rows, rows, err)
+    dtype, ks = _kv4_rows("k", k, c.kv_heads, c, dev)
+    other, vs = _kv4_rows("v", v, c.kv_heads, c, dev)
+    if other != dtype or v.shape[0] != rows:
         raise XtgError("kv4: k and v have the same type and rows")
-    c = _kv4_where(pool, table, pos, cu_rows, k.shape[0], err)
-    _kv4_call(pool, lib().xtg_cuda_kv4_store, C.byref(c), k.data_ptr(), v.data_ptr(), dtype, k.stride(0), k.stride(1),
-              v.stride(0), v.stride(1))
+    _kv4_call(dev, lib().xtg_cuda_kv4_store, c, k.data_ptr(), v.data_ptr(), dtype, ks[0], ks[1], vs[0], vs[1])
 
 
 def kv4_load(pool, table, pos, cu_rows, rows, dtype=None, err=None):
@@ -684,13 +702,13 @@ def kv4_load(pool, table, pos, cu_rows, rows, dtype=None, err=None):
     (default bfloat16)."""
     import torch
     dtype = dtype or torch.bfloat16
-    code = _kv4_dtypes().get(dtype)
+    code = _kv4_dtype(dtype)
     if code is None:
         raise XtgError("kv4: dtype is float32, bfloat16 or float16")
-    c = _kv4_where(pool, table, pos, cu_rows, rows, err)
-    k = torch.empty((rows, pool.shape[1], pool.shape[2] // 72), dtype=dtype, device=pool.device)
+    c, dev = _kv4_where(pool, table, pos, cu_rows, rows, err)
+    k = torch.empty((rows, c.kv_heads, c.head_dim), dtype=dtype, device=pool.device)
     v = torch.empty_like(k)
-    _kv4_call(pool, lib().xtg_cuda_kv4_load, C.byref(c), k.data_ptr(), v.data_ptr(), code)
+    _kv4_call(dev, lib().xtg_cuda_kv4_load, c, k.data_ptr(), v.data_ptr(), code)
     return k, v
 
 
@@ -699,24 +717,25 @@ def kv4_attention(q, pool, table, pos, cu_rows, scale, window=0, rows_per_seq=No
     `window` of these), after the call's rows were stored: [rows][heads][head_dim] in q's type. rows_per_seq: about how
     many rows a sequence has (default rows / seqs); it chooses the tiling only."""
     import torch
-    dtype = _kv4_rows("q", q, pool, 0)
-    rows, heads, d = q.shape
-    c = _kv4_where(pool, table, pos, cu_rows, rows, err)
+    rows = q.shape[0]
+    c, dev = _kv4_where(pool, table, pos, cu_rows, rows, err)
+    dtype, qs = _kv4_rows("q", q, 0, c, dev)
+    heads = q.shape[1]
     if out is None:
-        out = torch.empty((rows, heads, d), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
         raise XtgError("kv4: out is contiguous, of q's shape and type")
     if rows_per_seq is None:
         rows_per_seq = max(1, -(-rows // max(1, c.seqs)))
-    key = (pool.device.index, heads, c.kv_heads, d, rows_per_seq)
+    key = (dev, heads, c.kv_heads, c.head_dim, rows_per_seq)
     size = _kv4_workspace_bytes.get(key)
     if size is None:
-        with torch.cuda.device(pool.device):
-            size = lib().xtg_cuda_kv4_workspace(heads, c.kv_heads, d, rows_per_seq)
+        with torch.cuda.device(dev):
+            size = lib().xtg_cuda_kv4_workspace(heads, c.kv_heads, c.head_dim, rows_per_seq)
         if size < 0:
             raise XtgError("kv4: q heads a multiple of KV heads, rows_per_seq at least 1")
         _kv4_workspace_bytes[key] = size
     work = torch.empty(size, dtype=torch.uint8, device=q.device)
-    _kv4_call(pool, lib().xtg_cuda_kv4_attention, C.byref(c), q.data_ptr(), out.data_ptr(), dtype, heads, q.stride(0),
-              q.stride(1), scale, window, rows_per_seq, work.data_ptr(), size)
+    _kv4_call(dev, lib().xtg_cuda_kv4_attention, c, q.data_ptr(), out.data_ptr(), dtype, heads, qs[0], qs[1], scale,
+              window, rows_per_seq, work.data_ptr(), size)
     return out

@@ -202,13 +202,21 @@ __device__ __forceinline__ uint32_t hadd2_u32(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// The V codes at bits 0-3 (low) or 4-7 (high) of a word's halves as (code - 8) 2^-4 in f16: 64 + c / 16 less 64.5, and
-// (1024 + 16 c) / 256 less 4.5; exact.
-__device__ __forceinline__ uint32_t v_codes_low(uint32_t w) {
-  return hadd2_u32((w & 0x000f000fu) | 0x54005400u, 0xd408d408u);
+// (a & b) | c in one instruction: with two immediates the compiler takes two
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "n"(MASK), "r"(c));
+  return r;
 }
-__device__ __forceinline__ uint32_t v_codes_high(uint32_t w) {
-  return hfma2_u32((w & 0x00f000f0u) | 0x64006400u, 0x1c001c00u, 0xc480c480u);
+
+// The V codes at bits 0-3 (low) or 4-7 (high) of a word's halves as (code - 8) 2^-4 in f16: 64 + c / 16 less 64.5, and
+// (1024 + 16 c) / 256 less 4.5; exact. base: 64 (low) and 1024 (high) in both halves.
+__device__ __forceinline__ uint32_t v_codes_low(uint32_t w, uint32_t base) {
+  return hadd2_u32(and_or<0x000f000fu>(w, base), 0xd408d408u);
+}
+__device__ __forceinline__ uint32_t v_codes_high(uint32_t w, uint32_t base) {
+  return hfma2_u32(and_or<0x00f000f0u>(w, base), 0x1c001c00u, 0xc480c480u);
 }
 
 // D = A B + C with C apart from D
@@ -360,6 +368,9 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kConsumerRegs));
     const int rt = warp % tiles, sl = warp / tiles;   // this warp's rows of the row block, its turn among the units
     const uint32_t group = a.group;
+    uint32_t base_low, base_high;   // kept in registers (v_codes_low)
+    asm volatile("mov.b32 %0, 0x54005400;" : "=r"(base_low));
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(base_high));
     uint32_t it = 0;            // chunks of the parts before
     bool split_after = false;   // the last part goes on in the next CTA
     while (kv4_next(a, block_rows, walk, p)) {
@@ -651,7 +662,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
               for (int st = 0; st < 2; ++st) {
                 const uint32_t w0 = st ? word[2 * m] >> 8 : word[2 * m], w1 = st ? word[2 * m + 1] >> 8 : word[2 * m + 1];
-                const uint32_t va[4] = {v_codes_low(w0), v_codes_low(w1), v_codes_high(w0), v_codes_high(w1)};
+                const uint32_t va[4] = {v_codes_low(w0, base_low), v_codes_low(w1, base_low), v_codes_high(w0, base_high),
+                                        v_codes_high(w1, base_high)};
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                   float(&to)[4] = kDirect ? o[j][c][m] : d[j][m];
