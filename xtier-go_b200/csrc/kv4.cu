@@ -7,9 +7,10 @@
 // cut an end. The offset sits at the middle of the levels and not at lo, so that sums of s (code - 8) over many
 // positions stay as small as the values' own sums.
 //
-// Both kernels are bound by memory: one pass over the rows and the pages. A CTA takes one page of one KV head. The
-// page is the unit because neighbouring positions share the bytes of V: a CTA that owns the page merges all the
-// call's rows into it without atomics, whatever their number.
+// Both kernels are bound by memory: one pass over the rows and the pages. A CTA takes one page of one KV head, the heads
+// of a page by neighbouring CTAs, which share the rows' DRAM pages. The page is the unit because neighbouring positions
+// share the bytes of V: a CTA that owns the page merges all the call's rows into it without atomics, whatever their
+// number. A thread requests what it needs of several rows before it works on the first.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -20,42 +21,101 @@ namespace xtg {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBatch = 4;   // rows of K and of V that a thread requests at once
 
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+__device__ __forceinline__ uint32_t min_nan2(uint32_t a, uint32_t b, __nv_bfloat16) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t min_nan2(uint32_t a, uint32_t b, __half) {
+  uint32_t r;
+  asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
-// 8 neighbouring values (16-byte aligned) to and from f32
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+// 8 neighbouring values as they lie in memory (16-byte aligned)
+template <class T>
+struct Piece {
+  uint4 w;
+};
+template <>
+struct Piece<float> {
+  uint4 w, w2;
+};
+template <class T>
+__device__ __forceinline__ void load(const T* p, Piece<T>& x) {
+  x.w = *reinterpret_cast<const uint4*>(p);
+  if constexpr (sizeof(T) == 4) x.w2 = *reinterpret_cast<const uint4*>(p + 4);
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+
+__device__ __forceinline__ void to_f32(const Piece<float>& p, float (&x)[8]) {
+  const uint32_t w[8] = {p.w.x, p.w.y, p.w.z, p.w.w, p.w2.x, p.w2.y, p.w2.z, p.w2.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+}
+__device__ __forceinline__ void to_f32(const Piece<__nv_bfloat16>& p, float (&x)[8]) {
+  const uint32_t w[4] = {p.w.x, p.w.y, p.w.z, p.w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     x[2 * i] = __uint_as_float(w[i] << 16);
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
-__device__ __forceinline__ void load8(const __half* p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ float2 halves(uint32_t w, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float2 halves(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ void to_f32(const Piece<__half>& p, float (&x)[8]) {
+  const uint32_t w[4] = {p.w.x, p.w.y, p.w.z, p.w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    const float2 f = halves(w[i], __half());
     x[2 * i] = f.x;
     x[2 * i + 1] = f.y;
   }
 }
+
+// The least and the greatest value of a group, NaN if it holds one: over the 8 lanes that have a piece each. 16-bit
+// values are compared in pairs, the greatest as the least of the negated.
+__device__ __forceinline__ void range(const Piece<float>& p, float& lo, float& hi) {
+  float x[8];
+  to_f32(p, x);
+  lo = x[0];
+  hi = -x[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) {
+    lo = min_nan(lo, x[e]);
+    hi = min_nan(hi, -x[e]);
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = min_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  hi = -hi;
+}
+template <class T>
+__device__ __forceinline__ void range(const Piece<T>& p, float& lo, float& hi) {
+  constexpr uint32_t kSigns = 0x80008000u;
+  const T t = T();
+  const uint32_t l = min_nan2(min_nan2(p.w.x, p.w.y, t), min_nan2(p.w.z, p.w.w, t), t);
+  const uint32_t h = min_nan2(min_nan2(p.w.x ^ kSigns, p.w.y ^ kSigns, t), min_nan2(p.w.z ^ kSigns, p.w.w ^ kSigns, t), t);
+  uint32_t both = min_nan2(__byte_perm(l, h, 0x5410), __byte_perm(l, h, 0x7632), t);   // least, negated greatest
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) both = min_nan2(both, __shfl_xor_sync(0xffffffffu, both, o), t);
+  const float2 f = halves(both, t);
+  lo = f.x;
+  hi = -f.y;
+}
+
 __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
   *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
   *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
@@ -74,7 +134,41 @@ __device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
       make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
 }
 
-// The (sequence, page) of task blockIdx.x. A sequence of n rows touches at most n / 64 + 2 pages, so task numbers
+// The values of 8 codes (nibbles of word) with the parameters p: 16 + code as the f32 whose mantissa starts with the
+// nibble, less 24, then s (code - 8) + z with one rounding
+__device__ __forceinline__ void values8(uint32_t word, uint32_t p, float (&x)[8]) {
+  const float s = __uint_as_float(p & 0xffff0000u), z = __uint_as_float(p << 16);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t at19 = e < 5 ? word << (19 - 4 * e) : word >> (4 * e - 19);
+    x[e] = fmaf(__uint_as_float((at19 & 0x00780000u) | 0x41800000u) - 24.f, s, z);
+  }
+}
+
+// The transpose of 8 words of 8 nibbles: nibble c of word r becomes nibble r of word c
+__device__ __forceinline__ void transpose_nibbles(uint32_t (&w)[8]) {
+  constexpr uint32_t kLow = 0x0f0f0f0fu;
+#pragma unroll
+  for (int r = 0; r < 8; r += 2) {
+    const uint32_t a = w[r], b = w[r + 1];
+    w[r] = (a & kLow) | ((b << 4) & ~kLow);
+    w[r + 1] = ((a >> 4) & kLow) | (b & ~kLow);
+  }
+#pragma unroll
+  for (int r = 0; r < 8; r += r % 4 == 1 ? 3 : 1) {   // 0, 1, 4, 5
+    const uint32_t a = w[r], b = w[r + 2];
+    w[r] = __byte_perm(a, b, 0x6240);
+    w[r + 2] = __byte_perm(a, b, 0x7351);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint32_t a = w[r], b = w[r + 4];
+    w[r] = __byte_perm(a, b, 0x5410);
+    w[r + 4] = __byte_perm(a, b, 0x7632);
+  }
+}
+
+// The (sequence, page) of task blockIdx.x / kv_heads. A sequence of n rows touches at most n / 64 + 2 pages, so task numbers
 // start at cu_rows[s] / 64 + 2 s for sequence s: found without a prefix sum over the sequences' positions.
 struct Task {
   int64_t row0;   // the call's row at the page's first touched slot
@@ -83,7 +177,7 @@ struct Task {
 };
 
 __device__ __forceinline__ bool find_task(const Kv4Where& w, int* shared_seq, Task& t) {
-  const int64_t task = blockIdx.x;
+  const int64_t task = blockIdx.x / (uint32_t)w.kv_heads;
   if (threadIdx.x == 0) *shared_seq = -1;
   __syncthreads();
   for (int s = threadIdx.x; s < w.seqs; s += kThreads) {
@@ -107,88 +201,107 @@ __device__ __forceinline__ bool find_task(const Kv4Where& w, int* shared_seq, Ta
   return true;
 }
 
+// Quantises the 8 values that this lane has of a group: their codes as nibbles, the group's parameters.
+template <class T>
+__device__ __forceinline__ void quantise(const Piece<T>& p, uint32_t& word, uint32_t& par) {
+  float x[8], lo, hi;
+  range(p, lo, hi);
+  to_f32(p, x);
+  const float raw = __fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f);
+  const float s = fmaxf(__uint_as_float((__float_as_uint(raw) + 0xffffu) & 0xffff0000u), kKv4MinScale);
+  const float z = __bfloat162float(__float2bfloat16_rn(__fadd_rn(lo, __fmul_rn(8.f, s))));
+  const bool fine = raw < INFINITY && fabsf(z) < INFINITY;   // false for NaN too
+  const float inv = __frcp_rn(s);
+  // adding 1.5 2^23 + 8 rounds to an integer, ties to even, in the low bits: the code. Codes outside 0 .. 15 come only
+  // from z's rounding where |z| passes 2^8 s: the least and the greatest value, which bound the others, tell.
+  constexpr float kRound = 12582920.f;
+  constexpr uint32_t kBits = 0x4b400000u;   // of code 0
+  auto code = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(v, z), inv), kRound)); };
+  word = 0;
+  if (code(lo) >= kBits && code(hi) <= kBits + 15) {
+    // sum of 16^e bits(e) less that of code 0's bits
+#pragma unroll
+    for (int e = 7; e >= 0; --e) word = 16u * word + code(x[e]);
+    word -= kBits * 0x11111111u;
+  } else {
+#pragma unroll
+    for (int e = 7; e >= 0; --e) word = 16u * word + (min(max((int)(code(x[e]) - kBits), 0), 15));
+  }
+  if (!fine) word = 0;
+  par = fine ? (__float_as_uint(s) & 0xffff0000u) | (__float_as_uint(z) >> 16) : kKv4NanParam;
+}
+
 template <class T, int D>
 __global__ void __launch_bounds__(kThreads) kv4_store_kernel(const Kv4Where w, const Kv4Rows r) {
-  constexpr int H = D < 128 ? D : 128, kPerRow = D / 8;
-  constexpr int kStride = D + 16;   // of a slot's codes in shared memory: 8 slots x 4 dims without bank conflicts
-  __shared__ __align__(16) uint8_t codes[kKv4Page * kStride];
+  constexpr int H = D < 128 ? D : 128, kPerRow = D / 8, kRowsAtOnce = kThreads / kPerRow;
+  constexpr int kStride = D / 8 + 4;   // of a slot's words in shared memory: 4 slots x 8 words without bank conflicts
+  __shared__ uint32_t codes[kKv4Page * kStride];
   __shared__ int seq;
   Task t;
   if (!find_task(w, &seq, t) || t.page < 0) return;
-  const int h = blockIdx.y;
+  const int h = blockIdx.x % (uint32_t)w.kv_heads;
   uint8_t* block = w.pool + (t.page * w.kv_heads + h) * (int64_t)kv4_block_bytes(D);
   uint32_t* kcodes = reinterpret_cast<uint32_t*>(block);
   uint32_t* kpar = reinterpret_cast<uint32_t*>(block + kv4_k_params(D));
   uint32_t* vcodes = reinterpret_cast<uint32_t*>(block + kv4_v_codes(D));
   uint32_t* vpar = reinterpret_cast<uint32_t*>(block + kv4_v_params(D));
 
-  // one lane: 8 neighbouring dims of one row of K or V; 8 lanes: a group
-  const int per = t.count * kPerRow;
-  for (int u0 = 0; u0 < 2 * per; u0 += kThreads) {
-    const int u = u0 + threadIdx.x;
-    const bool live = u < 2 * per, isv = u >= per;
-    const int i = (isv ? u - per : u) / kPerRow, d0 = 8 * (u % kPerRow), slot = t.slot0 + i;   // per: whole rows
-    float x[8] = {};
-    if (live) {
-      const T* src = isv ? static_cast<const T*>(r.v) + (t.row0 + i) * r.v_row + h * r.v_head
-                         : static_cast<const T*>(r.k) + (t.row0 + i) * r.k_row + h * r.k_head;
-      load8(src + d0, x);
-    }
-    float lo = x[0], hi = x[0];
+  // a thread has dims d0 .. d0 + 7 of every kRowsAtOnce-th row, 8 threads a group; kBatch rows of K and V at a time
+  const int d0 = 8 * (threadIdx.x % kPerRow), first = threadIdx.x / kPerRow;
+  const T* ksrc = static_cast<const T*>(r.k) + t.row0 * r.k_row + h * r.k_head + d0;
+  const T* vsrc = static_cast<const T*>(r.v) + t.row0 * r.v_row + h * r.v_head + d0;
+  for (int i0 = 0; i0 < t.count; i0 += kBatch * kRowsAtOnce) {
+    Piece<T> k[kBatch] = {}, v[kBatch] = {};
 #pragma unroll
-    for (int e = 1; e < 8; ++e) {
-      lo = min_nan(lo, x[e]);
-      hi = max_nan(hi, x[e]);
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b * kRowsAtOnce + first;
+      if (i < t.count) {
+        load(ksrc + i * r.k_row, k[b]);
+        load(vsrc + i * r.v_row, v[b]);
+      }
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const float raw = __fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f);
-    const float s = fmaxf(__uint_as_float((__float_as_uint(raw) + 0xffffu) & 0xffff0000u), kKv4MinScale);
-    const float z = bf16_bits_to_f32(f32_to_bf16_bits(__fadd_rn(lo, __fmul_rn(8.f, s))));
-    const bool fine = raw < INFINITY && fabsf(z) < INFINITY;   // false for NaN too
-    const float inv = __frcp_rn(s);
-    uint32_t word = 0;
-    uint32_t bytes[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[e], z), inv), -8.f), 7.f);
-      // + 1.5 2^23 rounds to an integer, ties to even; + 8 makes it the code (0 .. 15, the low bits)
-      const uint32_t code = fine ? __float_as_uint(__fadd_rn(c, 12582920.f)) & 15u : 0u;
-      word |= code << (4 * e);
-      bytes[e / 4] |= code << (8 * (e % 4));
-    }
-    if (live) {
-      uint32_t* par = isv ? vpar : kpar;
-      if ((d0 & 63) == 0)
-        par[(d0 / 64) * kKv4Page + slot] =
-            fine ? (__float_as_uint(s) & 0xffff0000u) | (__float_as_uint(z) >> 16) : kKv4NanParam;
-      if (isv)
-        *reinterpret_cast<uint2*>(codes + slot * kStride + d0) = make_uint2(bytes[0], bytes[1]);
-      else
-        kcodes[((d0 / H * kKv4Page + slot) * 4 + d0 % 32 / 8) * (H / 32) + d0 % H / 32] = word;
+    for (int b = 0; b < kBatch; ++b) {
+      if (i0 + b * kRowsAtOnce >= t.count) break;   // the same for all threads
+      const int i = i0 + b * kRowsAtOnce + first, slot = t.slot0 + i;
+      uint32_t kw, kp, vw, vp;
+      quantise(k[b], kw, kp);
+      quantise(v[b], vw, vp);
+      if (i < t.count) {
+        kcodes[((d0 / H * kKv4Page + slot) * 4 + d0 % 32 / 8) * (H / 32) + d0 % H / 32] = kw;
+        codes[slot * kStride + d0 / 8] = vw;
+        if (d0 % 64 == 0) {
+          kpar[d0 / 64 * kKv4Page + slot] = kp;
+          vpar[d0 / 64 * kKv4Page + slot] = vp;
+        }
+      }
     }
   }
   __syncthreads();
-  // V's words: 8 slots of a head dim each; the slots that this call does not write keep their codes
-  for (int i = threadIdx.x; i < 8 * D; i += kThreads) {
-    const int tt = i & 3, a = (i >> 2) & 3, g = (i >> 4) & 7, c = (i >> 7) % (D / 32), hh = i / (4 * D);
-    const int first = 32 * hh + 2 * a, dim = 32 * c + 8 * tt + g;
-    uint32_t word = 0, mask = 0;
+  // V's words, of a head dim each, from 8 slots' words of 8 dims. The slots that this call does not write keep their
+  // codes.
+  for (int i = threadIdx.x; i < D; i += kThreads) {
+    const int tt = i & 3, a = (i >> 2) & 3, c = (i >> 4) % (D / 32), hh = i / (D / 2);
+    uint32_t words[8], mask = 0;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      const int slot = first + 8 * (n % 4) + n / 4;
-      if (slot >= t.slot0 && slot < t.slot0 + t.count) {
-        word |= (uint32_t)codes[slot * kStride + dim] << (4 * n);
-        mask |= 15u << (4 * n);
-      }
+      const int slot = 32 * hh + 2 * a + 8 * (n % 4) + n / 4;
+      if (slot >= t.slot0 && slot < t.slot0 + t.count) mask |= 15u << (4 * n);
+      words[n] = codes[slot * kStride + 4 * c + tt];
     }
-    if (mask == 0xffffffffu)
-      vcodes[i] = word;
-    else if (mask)
-      vcodes[i] = (vcodes[i] & ~mask) | word;
+    if (mask == 0) continue;
+    transpose_nibbles(words);
+    uint32_t* to = vcodes + ((hh * (D / 32) + c) * 8 * 4 + a) * 4 + tt;
+    if (mask == 0xffffffffu) {
+#pragma unroll
+      for (int g = 0; g < 8; ++g) to[16 * g] = words[g];
+    } else {
+      uint32_t old[8];
+#pragma unroll
+      for (int g = 0; g < 8; ++g) old[g] = to[16 * g];
+#pragma unroll
+      for (int g = 0; g < 8; ++g) to[16 * g] = (old[g] & ~mask) | (words[g] & mask);
+    }
   }
 }
 
@@ -196,11 +309,10 @@ template <class T, int D>
 __global__ void __launch_bounds__(kThreads) kv4_load_kernel(const Kv4Where w, const Kv4Rows r) {
   constexpr int H = D < 128 ? D : 128, kPerRow = D / 8;
   __shared__ __align__(16) uint32_t par[2][D / 64][kKv4Page];   // K's, V's
-  __shared__ __align__(16) uint32_t vcodes[8 * D];
   __shared__ int seq;
   Task t;
   if (!find_task(w, &seq, t)) return;
-  const int h = blockIdx.y;
+  const int h = blockIdx.x % (uint32_t)w.kv_heads;
   T* kout = static_cast<T*>(r.k) + t.row0 * r.k_row + h * r.k_head;
   T* vout = static_cast<T*>(r.v) + t.row0 * r.v_row + h * r.v_head;
   if (t.page < 0) {   // nothing there: zeros
@@ -212,40 +324,60 @@ __global__ void __launch_bounds__(kThreads) kv4_load_kernel(const Kv4Where w, co
     return;
   }
   const uint8_t* block = w.pool + (t.page * w.kv_heads + h) * (int64_t)kv4_block_bytes(D);
-  for (int i = threadIdx.x; i < 2 * D; i += kThreads)
-    reinterpret_cast<uint4*>(vcodes)[i] = reinterpret_cast<const uint4*>(block + kv4_v_codes(D))[i];
+  auto written = [&](int slot) { return slot >= t.slot0 && slot < t.slot0 + t.count; };
+  // 2 D items of 64 values, 8 words each, D of K and D of V: K's two uint4 (of one slot each), V's of 8 dims at 8 slots
+  constexpr int kItems = (2 * D + kThreads - 1) / kThreads;
+  uint32_t words[kItems][8];
+#pragma unroll
+  for (int x = 0; x < kItems; ++x) {
+    const int item = x * kThreads + threadIdx.x;
+    if (item < D) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {   // uint4 item + D e: coalesced
+        const uint4 v = reinterpret_cast<const uint4*>(block)[item + D * e];
+        words[x][4 * e] = v.x, words[x][4 * e + 1] = v.y, words[x][4 * e + 2] = v.z, words[x][4 * e + 3] = v.w;
+      }
+    } else if (item < 2 * D) {
+      const int i = item - D, tt = i & 3, a = (i >> 2) & 3, c = (i >> 4) % (D / 32), hh = i / (D / 2);
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(block + kv4_v_codes(D)) +
+                             ((hh * (D / 32) + c) * 8 * 4 + a) * 4 + tt;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) words[x][g] = from[16 * g];
+    }
+  }
   for (int i = threadIdx.x; i < D / 2; i += kThreads) {   // D / 4 16-byte pieces each
     const bool isv = i >= D / 4;
     reinterpret_cast<uint4*>(par)[i] = reinterpret_cast<const uint4*>(
         block + (isv ? kv4_v_params(D) : kv4_k_params(D)))[isv ? i - D / 4 : i];
   }
   __syncthreads();
-  const uint32_t* kcodes = reinterpret_cast<const uint32_t*>(block);
-  for (int u = threadIdx.x; u < t.count * kPerRow; u += kThreads) {   // K: the words in their own order
-    const int b = u % (H / 32), a = u / (H / 32) % 4, hh = u / (H / 8) % (D / H), i = u / kPerRow;
-    const int slot = t.slot0 + i, d0 = H * hh + 32 * b + 8 * a;
-    const uint32_t word = kcodes[((hh * kKv4Page + slot) * 4 + a) * (H / 32) + b], p = par[0][d0 / 64][slot];
-    const float s = __uint_as_float(p & 0xffff0000u), z = __uint_as_float(p << 16);
-    float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((int)((word >> (4 * e)) & 15u) - 8), s, z);
-    store8(kout + i * r.k_row + d0, x);
-  }
-  // V: a warp takes 8 neighbouring slots (2 a + j) x 4 pieces of 8 dims, 16 words of each shared-memory row
-  const int lane = threadIdx.x & 31;
-  for (int o = threadIdx.x >> 5; o < 8 * (D / 32); o += kThreads / 32) {
-    const int octet = o / (D / 32), c = o % (D / 32), tt = lane & 3, slot = 8 * octet + (lane >> 2);
-    if (slot < t.slot0 || slot >= t.slot0 + t.count) continue;
-    const int d0 = 32 * c + 8 * tt, n = octet % 4 + 4 * (slot % 2);
-    const uint32_t p = par[1][d0 / 64][slot];
-    const float s = __uint_as_float(p & 0xffff0000u), z = __uint_as_float(p << 16);
-    float x[8];
+  for (int x = 0; x < kItems; ++x) {
+    const int item = x * kThreads + threadIdx.x;
+    if (item < D) {
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      const uint32_t word = vcodes[(((octet / 4 * (D / 32) + c) * 8 + g) * 4 + slot % 8 / 2) * 4 + tt];
-      x[g] = fmaf((float)((int)((word >> (4 * n)) & 15u) - 8), s, z);
+      for (int e = 0; e < 8; ++e) {   // word [hh][slot][a][b]: dims H hh + 32 b + 8 a ..
+        const int i = 4 * (item + D * (e / 4)) + e % 4;
+        const int b = i % (H / 32), a = i / (H / 32) % 4, slot = i / (H / 8) % kKv4Page, hh = i / (8 * H);
+        if (!written(slot)) continue;
+        const int d0 = H * hh + 32 * b + 8 * a;
+        float v[8];
+        values8(words[x][e], par[0][d0 / 64][slot], v);
+        store8(kout + (slot - t.slot0) * r.k_row + d0, v);
+      }
+    } else if (item < 2 * D) {
+      const int i = item - D, tt = i & 3, a = (i >> 2) & 3, c = (i >> 4) % (D / 32), hh = i / (D / 2);
+      const int d0 = 32 * c + 8 * tt;
+      transpose_nibbles(words[x]);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int slot = 32 * hh + 2 * a + 8 * (n % 4) + n / 4;
+        if (!written(slot)) continue;
+        float v[8];
+        values8(words[x][n], par[1][d0 / 64][slot], v);
+        store8(vout + (slot - t.slot0) * r.v_row + d0, v);
+      }
     }
-    store8(vout + (slot - t.slot0) * r.v_row + d0, x);
   }
 }
 
@@ -268,7 +400,9 @@ void by_type_and_dim(int dtype, int head_dim, F&& f) {
 }
 
 dim3 task_grid(const Kv4Where& w) {
-  return dim3((unsigned)(w.rows / kKv4Page + 2 * (int64_t)w.seqs), (unsigned)w.kv_heads);
+  const int64_t ctas = (w.rows / kKv4Page + 2 * (int64_t)w.seqs) * w.kv_heads;
+  XTG_REQUIRE(ctas < (1ll << 31), "kv4: too many pages x KV heads in one call");
+  return dim3((unsigned)ctas);
 }
 
 }  // namespace
