@@ -23,9 +23,10 @@
 // SM takes an equal share of all (sequence, row block, KV head, 64-position chunk) items in that order, whatever the
 // sequences' lengths: shares start and end inside a sequence, whose parts a second kernel joins. Producer warps
 // bring chunks (one bulk copy of a page's block of the head) into a ring of shared memory; the consumer warps take
-// half chunks (32 positions). A warp holds 8 rows, or 16 (the codes unpacked once for both); a row block is 1, 2, 4 or 8
-// warps' rows, and the warps with the same rows take the half chunks in turn, each with a running maximum of its own,
-// so that no warp waits for another before the end of a sequence's part.
+// half chunks (32 positions) in turn, each with a running maximum of its own, so that no warp waits for another before
+// the end of a sequence's part. A row block is 8 rows, or 16 (the codes unpacked once for both), all held by every
+// warp: more rows read the chunks again, from L2 when the row blocks of a head run at the same time, which costs less
+// than the products of 16 rows take, and larger blocks would cost more at every part's start and end.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -51,7 +52,7 @@ template <int D, int RT>
 struct Kv4Shape {
   static constexpr int kWarps = RT == 1 && D <= 128 ? 12 : 8;
   static constexpr int kThreads = 32 * (kWarps + 4);
-  static constexpr int kRows = 8 * RT * (kWarps == 8 ? 8 : 1);   // of a row block at most
+  static constexpr int kRows = 8 * RT;   // of a row block
   static constexpr int kStart = 65536 / kThreads / 8 * 8;
   static constexpr int kProducerRegs = 40;
   static constexpr int kConsumerRegs = (kThreads * kStart - 128 * kProducerRegs) / (32 * kWarps) / 8 * 8;
@@ -66,11 +67,11 @@ struct Kv4Smem {
   using Shape = Kv4Shape<D, RT>;
   uint8_t stage[Shape::kStages][Shape::kBlock];
   // a part's start: the rows' operands [8-row tile][plane][32-dim block][lane], its end: the warps' accumulators
-  float acc[Shape::kWarps][8 * RT][Shape::kMergeStride];
+  float acc[Shape::kWarps][Shape::kRows][Shape::kMergeStride];
   float qsum[Shape::kRows][D / kKv4Group], qfac[Shape::kRows];   // what belongs to a row's scores
   int qpos[Shape::kRows];
   // the warps' maxima (then their weights) and sums; per row the joined maximum, sum and factor
-  float m[Shape::kWarps][8 * RT], l[Shape::kWarps][8 * RT];
+  float m[Shape::kWarps][Shape::kRows], l[Shape::kWarps][Shape::kRows];
   float row_m[Shape::kRows], row_l[Shape::kRows];
   uint64_t full[Shape::kStages], empty[Shape::kStages];
   int present[Shape::kStages];   // 0: no page, nothing was copied
@@ -84,6 +85,7 @@ struct Kv4Smem {
 // Positions are below 2^31 (the table holds fewer).
 struct Part {
   int seq, b, h, row0, n, pos, lo, cnt, c0, take;
+  uint32_t blocks;   // of the sequence
 };
 
 // What the combine reads: the split (sequence, row block, head) that a CTA's share ends in, and the last CTA with a
@@ -96,9 +98,10 @@ __device__ __forceinline__ uint64_t divide(uint64_t a, uint32_t b) {
   return a >> 32 ? a / b : (uint32_t)a / b;
 }
 
-// The items of sequence s: row blocks x KV heads x (kPartCost + chunks). Sequences with rows have at least one chunk (it may hold
+// The items of sequence s: KV heads x row blocks x (kPartCost + chunks). Sequences with rows have at least one chunk (it may hold
 // nothing), so that every row is written.
-__device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, int rows_per_block, Part& p) {
+template <int ROWS>
+__device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, Part& p) {
   p.pos = a.w.pos[s];
   p.row0 = (int)kv4_row_bound(a.w, s);
   p.n = (int)kv4_row_bound(a.w, s + 1) - p.row0;
@@ -113,9 +116,8 @@ __device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, int rows_
   const int first = a.window > 0 && p.pos >= a.window ? p.pos - a.window + 1 : 0;
   p.lo = first / kKv4Page;
   p.cnt = max((int)((end + kKv4Page - 1) >> 6) - p.lo, 1);
-  const uint32_t qrows = (uint32_t)p.n * (uint32_t)a.group;
-  return (uint64_t)((qrows + rows_per_block - 1) / (uint32_t)rows_per_block) * (uint32_t)a.w.kv_heads *
-         (uint32_t)(p.cnt + kPartCost);
+  p.blocks = ((uint32_t)p.n * (uint32_t)a.group + ROWS - 1) / ROWS;
+  return (uint64_t)p.blocks * (uint32_t)a.w.kv_heads * (uint32_t)(p.cnt + kPartCost);
 }
 
 // Walks a CTA's share of the items part by part.
@@ -124,9 +126,10 @@ struct Walk {
   uint64_t off, left;   // from sequence s's first item
 };
 
-__device__ __forceinline__ bool kv4_next(const Kv4Attn& a, int rows_per_block, Walk& k, Part& p) {
+template <int ROWS>
+__device__ __forceinline__ bool kv4_next(const Kv4Attn& a, Walk& k, Part& p) {
   while (k.left > 0 && k.s < a.w.seqs) {
-    const uint64_t items = kv4_items(a, k.s, rows_per_block, p);
+    const uint64_t items = kv4_items<ROWS>(a, k.s, p);
     if (k.off >= items) {
       k.off -= items;
       ++k.s;
@@ -137,8 +140,8 @@ __device__ __forceinline__ bool kv4_next(const Kv4Attn& a, int rows_per_block, W
     const int skip = max(kPartCost - at, 0);
     if (skip >= k.left) break;
     p.c0 = at + skip - kPartCost;
-    p.b = (int)divide(seg, a.w.kv_heads);
-    p.h = (int)(seg - (uint64_t)p.b * (uint32_t)a.w.kv_heads);
+    p.h = (int)divide(seg, p.blocks);
+    p.b = (int)(seg - (uint64_t)p.h * p.blocks);
     k.left -= skip;
     p.take = (int)((uint64_t)(p.cnt - p.c0) < k.left ? (uint64_t)(p.cnt - p.c0) : k.left);
     k.off += skip + p.take;
@@ -261,12 +264,12 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 // floats of a part's row in the workspace: m, l, 2 pads, acc[D]
 __host__ __device__ constexpr int part_row(int D) { return D + 4; }
 
-// RT: 8-row tiles per warp; TYPE: q's and out's. tiles: warps per row block.
+// RT: 8-row tiles of a row block; TYPE: q's and out's.
 template <int D, int RT, int TYPE>
 __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
-    kv4_attention_kernel(const Kv4Attn a, const int tiles, float* part, Kv4Split* splits) {
+    kv4_attention_kernel(const Kv4Attn a, float* part, Kv4Split* splits) {
   using Shape = Kv4Shape<D, RT>;
-  constexpr int kStages = Shape::kStages, kWarps = Shape::kWarps, kThreads = Shape::kThreads;
+  constexpr int kStages = Shape::kStages, kWarps = Shape::kWarps, kThreads = Shape::kThreads, kRows = Shape::kRows;
   constexpr int kGroups = D / kKv4Group, kBlocks = D / 32, H = D < 128 ? D : 128;
   constexpr int kQPlanes = TYPE == kKv4F32 ? 2 : 1;
   constexpr bool kDirect = TYPE != kKv4F32;   // P V added up in the matrix unit
@@ -274,7 +277,6 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
   Kv4Smem<D, RT>& sm = *reinterpret_cast<Kv4Smem<D, RT>*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, tq = lane & 3;
-  const int warp_rows = 8 * RT, block_rows = warp_rows * tiles, lanes = kWarps / tiles;
 
   // ---- this CTA's share of the items: an equal part of their sum over the sequences ----
   uint64_t total = 0, share = 0;
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
     for (int s0 = 0; s0 < a.w.seqs; s0 += kThreads) {
       const int s = s0 + threadIdx.x;
       Part p;
-      const uint64_t mine = s < a.w.seqs ? kv4_items(a, s, block_rows, p) : 0;
+      const uint64_t mine = s < a.w.seqs ? kv4_items<kRows>(a, s, p) : 0;
       uint64_t x = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
       if (threadIdx.x == 0 && pass == 0 && s0 == 0) {
         for (int st = 0; st < kStages; ++st) {
           mbar_init(&sm.full[st], 1);
-          mbar_init(&sm.empty[st], kUnits * tiles);
+          mbar_init(&sm.empty[st], kUnits);
         }
         mbar_init_fence();
         sm.failed = 0;
@@ -340,8 +342,9 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
     // ---- producers: chunk k of the parts in order is warp k % 4's, a page's block of the head into stage k % kStages;
     // 32 chunks' pages are looked up at once ----
     const int pw = warp - kWarps;
+    const uint64_t once = l2_evict_first();
     uint32_t it = 0;
-    while (kv4_next(a, block_rows, walk, p)) {
+    while (kv4_next<kRows>(a, walk, p)) {
       const uint8_t* head = a.w.pool + (int64_t)p.h * Shape::kBlock;
       int x = (pw - (int)it) & 3;   // this warp's next chunk of the part
       while (x < p.take) {
@@ -354,7 +357,11 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
             sm.present[st] = page >= 0;
             if (page >= 0) {
               mbar_expect_tx(&sm.full[st], Shape::kBlock);
-              bulk_g2s(sm.stage[st], head + page * a.w.kv_heads * (int64_t)Shape::kBlock, Shape::kBlock, &sm.full[st]);
+              const uint8_t* from = head + page * a.w.kv_heads * (int64_t)Shape::kBlock;
+              if (p.blocks == 1)   // read once: the first to leave L2
+                bulk_g2s_hint(sm.stage[st], from, Shape::kBlock, &sm.full[st], once);
+              else
+                bulk_g2s(sm.stage[st], from, Shape::kBlock, &sm.full[st]);
             } else {
               mbar_arrive(&sm.full[st]);
             }
@@ -366,30 +373,28 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kConsumerRegs));
-    const int rt = warp % tiles, sl = warp / tiles;   // this warp's rows of the row block, its turn among the units
     const uint32_t group = a.group;
     uint32_t base_low, base_high;   // kept in registers (v_codes_low)
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(base_low));
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(base_high));
     uint32_t it = 0;            // chunks of the parts before
     bool split_after = false;   // the last part goes on in the next CTA
-    while (kv4_next(a, block_rows, walk, p)) {
-      // ---- the warp's rows: row r of the sequence and KV head is (row r / group of the sequence, q head r % group) ----
-      const uint32_t qrows = (uint32_t)p.n * group, r0 = (uint32_t)p.b * block_rows + warp_rows * rt;
-      const bool any = r0 < qrows;
+    while (kv4_next<kRows>(a, walk, p)) {
+      // ---- the rows: row r of the sequence and KV head is (row r / group of the sequence, q head r % group) ----
+      const uint32_t qrows = (uint32_t)p.n * group, r0 = (uint32_t)p.b * kRows;
       // the position of the sequence's row i (past 2^31 - 1 the table holds nothing more to see)
       auto position = [&](uint32_t i) { return (int)min((int64_t)p.pos + i, (int64_t)0x7fffffff); };
-      // the warp's first and last position
-      const int tmin = position(r0 / group), tmax = position((min(r0 + warp_rows, qrows) - 1) / group);
+      // the block's first and last position
+      const int tmin = position(r0 / group), tmax = position((min(r0 + kRows, qrows) - 1) / group);
 
       // ---- Q as the first product's operand for every row of the block, by all consumer warps: a thread takes 8
       // neighbouring dims, the word of K codes that lane 4 g + (dims / 8) % 4 multiplies: nibble pair i (dims i, i + 4)
       // is a register of step i / 2 ----
       uint4* qfrag = reinterpret_cast<uint4*>(sm.acc);
       constexpr int kPieces = D / 8;   // threads per row
-      for (int x = threadIdx.x; x < block_rows * kPieces; x += 32 * kWarps) {   // whole warps: block_rows x D / 8 >= 64
+      for (int x = threadIdx.x; x < kRows * kPieces; x += 32 * kWarps) {   // whole warps: kRows x D / 8 >= 64
         const int row = x / kPieces, d8 = x % kPieces;
-        const uint32_t r = (uint32_t)p.b * block_rows + row, i = r / group;
+        const uint32_t r = r0 + row, i = r / group;
         const bool live = r < qrows;
         float v[8] = {};
         if (live)
@@ -435,17 +440,16 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
       int t[RT][2];                            // the row's position; dead rows see nothing
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
-        const int tile = rt * RT + j;
 #pragma unroll
         for (int pl = 0; pl < kQPlanes; ++pl)
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) {
-            const uint4 v = qfrag[((tile * kQPlanes + pl) * kBlocks + b) * 32 + lane];
+            const uint4 v = qfrag[((j * kQPlanes + pl) * kBlocks + b) * 32 + lane];
             qb[j][b][0][pl][0] = v.x, qb[j][b][0][pl][1] = v.y, qb[j][b][1][pl][0] = v.z, qb[j][b][1][pl][1] = v.w;
           }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int row = 8 * tile + 2 * tq + e;
+          const int row = 8 * j + 2 * tq + e;
           rf[j][e] = sm.qfac[row];
           t[j][e] = sm.qpos[row];
 #pragma unroll
@@ -682,14 +686,14 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
         }
       };
 
-      // ---- this warp's half chunks of the part: every `lanes`-th of the CTA's ----
-      for (int x = (int)((sl + lanes - kUnits * it % lanes) % lanes); x < kUnits * p.take; x += lanes) {
+      // ---- this warp's half chunks of the part: every kWarps-th of the CTA's ----
+      for (int x = (int)((warp + kWarps - kUnits * it % kWarps) % kWarps); x < kUnits * p.take; x += kWarps) {
         const uint32_t k = it + x / kUnits;
         const int st = (int)(k % kStages), hh = x % kUnits;
         const bool ok = kv4_wait(&sm.full[st], (k / kStages) & 1, &sm.failed, a.w.err);
         const int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x;
         const bool seen =
-            ok && any && sm.present[st] && p0 <= tmax && (a.window <= 0 || p0 + kUnit - 1 > tmin - a.window);
+            ok && sm.present[st] && p0 <= tmax && (a.window <= 0 || p0 + kUnit - 1 > tmin - a.window);
         if (seen) {
           if (p0 + kUnit - 1 <= tmin && (a.window <= 0 || p0 > tmax - a.window))
             unit(sm.stage[st], hh, p0, std::false_type());
@@ -701,7 +705,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
       }
       it += p.take;
 
-      // ---- the part's warps meet: per row, the warps with that row by their maxima ----
+      // ---- the part's warps meet, by their maxima ----
 #pragma unroll
       for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -728,31 +732,31 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
         }
       named_bar_sync(1, 32 * kWarps);
       const bool whole = p.c0 == 0 && p.take == p.cnt;
-      float* mine = part + (int64_t)(2 * blockIdx.x + (p.c0 == 0 ? 1 : 0)) * block_rows * part_row(D);
-      if (threadIdx.x < block_rows) {   // a thread per row: the weights of its warps' accumulators
-        const int tile = threadIdx.x / warp_rows, from = threadIdx.x % warp_rows;
+      float* mine = part + (int64_t)(2 * blockIdx.x + (p.c0 == 0 ? 1 : 0)) * kRows * part_row(D);
+      if (threadIdx.x < kRows) {   // a thread per row: the weights of the warps' accumulators
         float M = -INFINITY, l = 0.f;
-        for (int v = 0; v < lanes; ++v) M = fmaxf(M, sm.m[v * tiles + tile][from]);
-        for (int v = 0; v < lanes; ++v) {
-          float* mv = &sm.m[v * tiles + tile][from];
-          const float wt = *mv == M ? 1.f : ex2_approx(*mv - M);
-          *mv = wt;
-          l = fmaf(wt, sm.l[v * tiles + tile][from], l);
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) M = fmaxf(M, sm.m[v][threadIdx.x]);
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) {
+          const float mv = sm.m[v][threadIdx.x], wt = mv == M ? 1.f : ex2_approx(mv - M);
+          sm.m[v][threadIdx.x] = wt;
+          l = fmaf(wt, sm.l[v][threadIdx.x], l);
         }
         sm.row_l[threadIdx.x] = whole ? (l == 0.f ? 0.f : 1.f / l) : l;
         sm.row_m[threadIdx.x] = M;
       }
       named_bar_sync(1, 32 * kWarps);
       constexpr int kQuads = D / 4;   // threads per row
-#pragma unroll 2
-      for (int x = threadIdx.x; x < block_rows * kQuads; x += 32 * kWarps) {
-        const int row = x / kQuads, d0 = 4 * (x % kQuads), tile = row / warp_rows, from = row % warp_rows;
-        const uint32_t rr = (uint32_t)p.b * block_rows + row;
+      for (int x = threadIdx.x; x < kRows * kQuads; x += 32 * kWarps) {
+        const int row = x / kQuads, d0 = 4 * (x % kQuads);
+        const uint32_t rr = r0 + row;
         if (rr >= qrows) break;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int v = 0; v < lanes; ++v) {
-          const float wt = sm.m[v * tiles + tile][from];
-          const float4 u = *reinterpret_cast<const float4*>(&sm.acc[v * tiles + tile][from][d0]);
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) {
+          const float wt = sm.m[v][row];
+          const float4 u = *reinterpret_cast<const float4*>(&sm.acc[v][row][d0]);
           y.x = fmaf(wt, u.x, y.x);
           y.y = fmaf(wt, u.y, y.y);
           y.z = fmaf(wt, u.z, y.z);
@@ -880,28 +884,20 @@ __global__ void __launch_bounds__(kCombineThreads)
   }
 }
 
-// A row block: `tiles` warps of rt x 8 rows each, as many as a sequence's rows fill, up to one per warp. 16 rows per warp
-// beyond 8 rows in all (head dim 256 has no registers for them).
-struct RowBlock {
-  int rt, tiles;
-};
-
-RowBlock row_block(int head_dim, int group, int rows_per_seq) {
-  const int64_t rows = (int64_t)group * std::max(1, rows_per_seq);
-  const int rt = head_dim <= 128 && rows > 8 ? 2 : 1;
-  const int64_t need = (rows + 8 * rt - 1) / (8 * rt);
-  return {rt, need >= 5 ? 8 : need >= 3 ? 4 : (int)need};
+// Row blocks of 16 rows where a sequence has more than 8 (head dim 256 has no registers for them).
+int block_rows(int head_dim, int group, int rows_per_seq) {
+  return head_dim <= 128 && (int64_t)group * rows_per_seq > 8 ? 16 : 8;
 }
 
 template <int D, int RT, int TYPE>
-void launch(const Kv4Attn& a, int tiles, int sms, cudaStream_t s) {
-  const int block_rows = 8 * RT * tiles;
+void launch(const Kv4Attn& a, int sms, cudaStream_t s) {
+  using Shape = Kv4Shape<D, RT>;
   float* part = a.part;
-  Kv4Split* splits = reinterpret_cast<Kv4Split*>(part + (int64_t)sms * 2 * block_rows * part_row(D));
+  Kv4Split* splits = reinterpret_cast<Kv4Split*>(part + (int64_t)sms * 2 * Shape::kRows * part_row(D));
   static std::atomic<uint64_t> optin;
   const int smem = (int)sizeof(Kv4Smem<D, RT>);
   ensure_smem_optin((const void*)kv4_attention_kernel<D, RT, TYPE>, smem, optin);
-  kv4_attention_kernel<D, RT, TYPE><<<sms, Kv4Shape<D, RT>::kThreads, smem, s>>>(a, tiles, part, splits);
+  kv4_attention_kernel<D, RT, TYPE><<<sms, Shape::kThreads, smem, s>>>(a, part, splits);
   XTG_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sms * kCombineBlocksPerSm);
@@ -912,36 +908,36 @@ void launch(const Kv4Attn& a, int tiles, int sms, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  XTG_CUDA(cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D>, a, block_rows, sms, (const float*)part,
+  XTG_CUDA(cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D>, a, Shape::kRows, sms, (const float*)part,
                               (const Kv4Split*)splits));
 }
 
 template <int D, int RT>
-void launch_type(const Kv4Attn& a, int tiles, int sms, cudaStream_t s) {
+void launch_type(const Kv4Attn& a, int sms, cudaStream_t s) {
   if (a.dtype == kKv4F32)
-    launch<D, RT, kKv4F32>(a, tiles, sms, s);
+    launch<D, RT, kKv4F32>(a, sms, s);
   else if (a.dtype == kKv4Bf16)
-    launch<D, RT, kKv4Bf16>(a, tiles, sms, s);
+    launch<D, RT, kKv4Bf16>(a, sms, s);
   else
-    launch<D, RT, kKv4F16>(a, tiles, sms, s);
+    launch<D, RT, kKv4F16>(a, sms, s);
 }
 
 }  // namespace
 
 int64_t kv4_workspace_bytes(int head_dim, int group, int rows_per_seq, int sms) {
-  const RowBlock b = row_block(head_dim, group, rows_per_seq);
-  return (int64_t)sms * (2 * 8 * b.rt * b.tiles * part_row(head_dim) * (int64_t)sizeof(float) + (int64_t)sizeof(Kv4Split));
+  return (int64_t)sms * (2 * block_rows(head_dim, group, rows_per_seq) * part_row(head_dim) * (int64_t)sizeof(float) +
+                         (int64_t)sizeof(Kv4Split));
 }
 
 void launch_kv4_attention(const Kv4Attn& a, int sms, cudaStream_t s) {
   XTG_REQUIRE(sms <= kMostSms, "kv4: more SMs than the combine lists");
-  const RowBlock b = row_block(a.w.head_dim, a.group, a.rows_per_seq);
+  const bool wide = block_rows(a.w.head_dim, a.group, a.rows_per_seq) == 16;
   if (a.w.head_dim == 256)
-    launch_type<256, 1>(a, b.tiles, sms, s);
+    launch_type<256, 1>(a, sms, s);
   else if (a.w.head_dim == 128)
-    b.rt == 2 ? launch_type<128, 2>(a, b.tiles, sms, s) : launch_type<128, 1>(a, b.tiles, sms, s);
+    wide ? launch_type<128, 2>(a, sms, s) : launch_type<128, 1>(a, sms, s);
   else
-    b.rt == 2 ? launch_type<64, 2>(a, b.tiles, sms, s) : launch_type<64, 1>(a, b.tiles, sms, s);
+    wide ? launch_type<64, 2>(a, sms, s) : launch_type<64, 1>(a, sms, s);
 }
 
 }  // namespace xtg
