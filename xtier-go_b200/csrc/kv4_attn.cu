@@ -70,9 +70,7 @@ struct Kv4Smem {
   float acc[Shape::kWarps][Shape::kRows][Shape::kMergeStride];
   float qsum[Shape::kRows][D / kKv4Group], qfac[Shape::kRows];   // what belongs to a row's scores
   int qpos[Shape::kRows];
-  // the warps' maxima (then their weights) and sums; per row the joined maximum, sum and factor
   float m[Shape::kWarps][Shape::kRows], l[Shape::kWarps][Shape::kRows];
-  float row_m[Shape::kRows], row_l[Shape::kRows];
   uint64_t full[Shape::kStages], empty[Shape::kStages];
   int present[Shape::kStages];   // 0: no page, nothing was copied
   uint64_t scan[Shape::kThreads / 32];
@@ -482,8 +480,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
       for (int G = 0; G < kGroups; ++G) unit_e[G] = 27;
 
       // half chunk hh of a stage, its first position p0
-      auto unit = [&](const uint8_t* stg, int hh, int p0, auto masked_) {
-        constexpr bool kMasked = decltype(masked_)::value;
+      auto unit = [&](const uint8_t* stg, int hh, int p0, bool masked) {
         const uint32_t* kw = reinterpret_cast<const uint32_t*>(stg) + hh * kUnit * (H / 8);
         const uint32_t* kpar = reinterpret_cast<const uint32_t*>(stg + kv4_k_params(D)) + hh * kUnit;
         const uint32_t* vw = reinterpret_cast<const uint32_t*>(stg + kv4_v_codes(D)) + hh * kUnit * (D / 8);
@@ -542,32 +539,49 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
                 s[j][u][e] = fmaf(sc, c[j][G][e], G == 0 ? of * q1 : fmaf(of, q1, s[j][u][e]));
               }
           }
-          if constexpr (kMasked) {
+        }
+        // ---- V's parameters, slots 8 i + g ----
+        uint32_t w[kGroups][2 * kSteps];
+#pragma unroll
+        for (int G = 0; G < kGroups; ++G)
+#pragma unroll
+          for (int i = 0; i < 2 * kSteps; ++i) w[G][i] = vpar[G * kKv4Page + 8 * i + g];
+        if (masked) {
+          // a row does not see every slot: -inf for its score; what no row sees may hold anything
+#pragma unroll
+          for (int i = 0; i < 2 * kSteps; ++i) {
+            const int pp = p0 + 8 * i + g;
+            const bool none = pp > tmax || (a.window > 0 && pp <= tmin - a.window);
+            bool sees[RT][2];
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int pp = p0 + 16 * u + 8 * (e / 2) + g;
-                if (pp > t[j][e % 2] || (a.window > 0 && pp <= t[j][e % 2] - a.window)) s[j][u][e] = -INFINITY;
+              for (int e = 0; e < 2; ++e) {
+                sees[j][e] = pp <= t[j][e] && (a.window <= 0 || pp > t[j][e] - a.window);
+                if (!sees[j][e]) s[j][i / 2][2 * (i % 2) + e] = -INFINITY;
               }
+#pragma unroll
+            for (int G = 0; G < kGroups; ++G) {
+              if (none) w[G][i] = 0;
+              if ((int)w[G][i] < 0) {   // a NaN scale must not meet a probability of 0: into the sums of those that see it
+                w[G][i] = 0;
+#pragma unroll
+                for (int j = 0; j < RT; ++j)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (sees[j][e]) oz[j][e][G] = __uint_as_float(0x7fc00000u);
+              }
+            }
           }
         }
-        // ---- the scales of V: their largest exponent per group ----
-        uint32_t w[kGroups][2 * kSteps];   // slots 8 i + g
+        // the scales' largest exponent per group: positive f32 order is integer order, NaN's word is negative
         bool move = false;
         int next_e[kGroups];
 #pragma unroll
         for (int G = 0; G < kGroups; ++G) {
-          int top = 0;   // the largest scale's word: positive f32 order is integer order, NaN's word is negative
+          int top = 0;
 #pragma unroll
-          for (int i = 0; i < 2 * kSteps; ++i) {
-            w[G][i] = vpar[G * kKv4Page + 8 * i + g];
-            if constexpr (kMasked) {   // what no row of the warp sees may hold anything
-              const int pp = p0 + 8 * i + g;
-              if (pp > tmax || (a.window > 0 && pp <= tmin - a.window)) w[G][i] = 0;
-            }
-            top = max(top, (int)w[G][i]);
-          }
+          for (int i = 0; i < 2 * kSteps; ++i) top = max(top, (int)w[G][i]);
           next_e[G] = top >> 23;
           move |= next_e[G] > unit_e[G];
         }
@@ -642,11 +656,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
               const float p0_ = s[j][i / 2][2 * (i % 2)], p1_ = s[j][i / 2][2 * (i % 2) + 1];
-              float x0 = p0_ * sc, x1 = p1_ * sc;
-              if constexpr (kMasked) {   // a masked NaN scale gives nothing
-                x0 = p0_ == 0.f ? 0.f : x0;
-                x1 = p1_ == 0.f ? 0.f : x1;
-              }
+              const float x0 = p0_ * sc, x1 = p1_ * sc;
               // hi: the leading 11 bits (cut, so that an AND gives them), lo: the next 11
               const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffffe000u);
               const float h1 = __uint_as_float(__float_as_uint(x1) & 0xffffe000u);
@@ -694,12 +704,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
         const int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x;
         const bool seen =
             ok && sm.present[st] && p0 <= tmax && (a.window <= 0 || p0 + kUnit - 1 > tmin - a.window);
-        if (seen) {
-          if (p0 + kUnit - 1 <= tmin && (a.window <= 0 || p0 > tmax - a.window))
-            unit(sm.stage[st], hh, p0, std::false_type());
-          else
-            unit(sm.stage[st], hh, p0, std::true_type());
-        }
+        if (seen) unit(sm.stage[st], hh, p0, p0 + kUnit - 1 > tmin || (a.window > 0 && p0 <= tmax - a.window));
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[st]);
       }
@@ -733,44 +738,37 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
       named_bar_sync(1, 32 * kWarps);
       const bool whole = p.c0 == 0 && p.take == p.cnt;
       float* mine = part + (int64_t)(2 * blockIdx.x + (p.c0 == 0 ? 1 : 0)) * kRows * part_row(D);
-      if (threadIdx.x < kRows) {   // a thread per row: the weights of the warps' accumulators
-        float M = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int v = 0; v < kWarps; ++v) M = fmaxf(M, sm.m[v][threadIdx.x]);
-#pragma unroll
-        for (int v = 0; v < kWarps; ++v) {
-          const float mv = sm.m[v][threadIdx.x], wt = mv == M ? 1.f : ex2_approx(mv - M);
-          sm.m[v][threadIdx.x] = wt;
-          l = fmaf(wt, sm.l[v][threadIdx.x], l);
-        }
-        sm.row_l[threadIdx.x] = whole ? (l == 0.f ? 0.f : 1.f / l) : l;
-        sm.row_m[threadIdx.x] = M;
-      }
-      named_bar_sync(1, 32 * kWarps);
       constexpr int kQuads = D / 4;   // threads per row
       for (int x = threadIdx.x; x < kRows * kQuads; x += 32 * kWarps) {
         const int row = x / kQuads, d0 = 4 * (x % kQuads);
         const uint32_t rr = r0 + row;
         if (rr >= qrows) break;
+        float mv[kWarps], M = -INFINITY, l = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int v = 0; v < kWarps; ++v) {
-          const float wt = sm.m[v][row];
+          mv[v] = sm.m[v][row];
+          M = fmaxf(M, mv[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) {
+          const float wt = mv[v] == M ? 1.f : ex2_approx(mv[v] - M);
           const float4 u = *reinterpret_cast<const float4*>(&sm.acc[v][row][d0]);
+          l = fmaf(wt, sm.l[v][row], l);
           y.x = fmaf(wt, u.x, y.x);
           y.y = fmaf(wt, u.y, y.y);
           y.z = fmaf(wt, u.z, y.z);
           y.w = fmaf(wt, u.w, y.w);
         }
         if (whole) {
-          const float inv = sm.row_l[row];
+          const float inv = l == 0.f ? 0.f : 1.f / l;
           const uint32_t i = rr / group;
           store_out4(a.out, (((int64_t)p.row0 + i) * a.heads + p.h * group + (rr - i * group)) * D + d0, TYPE,
                      make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
         } else {
           float* to = mine + (int64_t)row * part_row(D);
           *reinterpret_cast<float4*>(to + 4 + d0) = y;
-          if (d0 == 0) *reinterpret_cast<float2*>(to) = make_float2(sm.row_m[row], sm.row_l[row]);
+          if (d0 == 0) *reinterpret_cast<float2*>(to) = make_float2(M, l);
         }
       }
       split_after = p.c0 == 0 && !whole;
