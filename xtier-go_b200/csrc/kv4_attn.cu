@@ -48,11 +48,10 @@ constexpr int kPartCost = 8;
 
 // Consumer warps and registers: a warpgroup of producers beside them, from which setmaxnreg moves registers to the
 // consumers; the sum of both shares must not pass what the CTA started with (threads x kStart).
-template <int D, int RT>
+template <int D, int ROWS>
 struct Kv4Shape {
-  static constexpr int kWarps = RT == 1 && D <= 128 ? 12 : 8;
+  static constexpr int kWarps = ROWS <= 8 && D <= 128 ? 12 : 8;
   static constexpr int kThreads = 32 * (kWarps + 4);
-  static constexpr int kRows = 8 * RT;   // of a row block
   static constexpr int kStart = 65536 / kThreads / 8 * 8;
   static constexpr int kProducerRegs = 40;
   static constexpr int kConsumerRegs = (kThreads * kStart - 128 * kProducerRegs) / (32 * kWarps) / 8 * 8;
@@ -62,15 +61,15 @@ struct Kv4Shape {
   static constexpr int kMergeStride = D + 4;   // floats of a row's accumulator being merged
 };
 
-template <int D, int RT>
+template <int D, int ROWS>
 struct Kv4Smem {
-  using Shape = Kv4Shape<D, RT>;
+  using Shape = Kv4Shape<D, ROWS>;
   uint8_t stage[Shape::kStages][Shape::kBlock];
   // a part's start: the rows' operands [8-row tile][plane][32-dim block][lane], its end: the warps' accumulators
-  float acc[Shape::kWarps][Shape::kRows][Shape::kMergeStride];
-  float qsum[Shape::kRows][D / kKv4Group], qfac[Shape::kRows];   // what belongs to a row's scores
-  int qpos[Shape::kRows];
-  float m[Shape::kWarps][Shape::kRows], l[Shape::kWarps][Shape::kRows];
+  float acc[Shape::kWarps][ROWS][Shape::kMergeStride];
+  float qsum[ROWS][D / kKv4Group], qfac[ROWS];   // what belongs to a row's scores
+  int qpos[ROWS];
+  float m[Shape::kWarps][ROWS], l[Shape::kWarps][ROWS];
   uint64_t full[Shape::kStages], empty[Shape::kStages];
   int present[Shape::kStages];   // 0: no page, nothing was copied
   uint64_t scan[Shape::kThreads / 32];
@@ -262,17 +261,20 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 // floats of a part's row in the workspace: m, l, 2 pads, acc[D]
 __host__ __device__ constexpr int part_row(int D) { return D + 4; }
 
-// RT: 8-row tiles of a row block; TYPE: q's and out's.
-template <int D, int RT, int TYPE>
-__global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
+// ROWS: of a row block, 4, 8 or 16; TYPE: q's and out's.
+template <int D, int ROWS, int TYPE>
+__global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     kv4_attention_kernel(const Kv4Attn a, float* part, Kv4Split* splits) {
-  using Shape = Kv4Shape<D, RT>;
-  constexpr int kStages = Shape::kStages, kWarps = Shape::kWarps, kThreads = Shape::kThreads, kRows = Shape::kRows;
+  using Shape = Kv4Shape<D, ROWS>;
+  constexpr int kStages = Shape::kStages, kWarps = Shape::kWarps, kThreads = Shape::kThreads;
   constexpr int kGroups = D / kKv4Group, kBlocks = D / 32, H = D < 128 ? D : 128;
-  constexpr int kQPlanes = TYPE == kKv4F32 ? 2 : 1;
+  // 8-row tiles; with 4 rows a tile's columns are the two planes of a row (kPair), and a lane has one row of scores, not 2
+  constexpr int RT = ROWS == 16 ? 2 : 1, kE = ROWS == 4 ? 1 : 2;
+  constexpr bool kPair = ROWS == 4;
+  constexpr int kQPlanes = TYPE == kKv4F32 && !kPair ? 2 : 1, kPPlanes = kPair ? 1 : 2;   // operands per tile
   constexpr bool kDirect = TYPE != kKv4F32;   // P V added up in the matrix unit
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  Kv4Smem<D, RT>& sm = *reinterpret_cast<Kv4Smem<D, RT>*>(smem_raw);
+  Kv4Smem<D, ROWS>& sm = *reinterpret_cast<Kv4Smem<D, ROWS>*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, tq = lane & 3;
 
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
     for (int s0 = 0; s0 < a.w.seqs; s0 += kThreads) {
       const int s = s0 + threadIdx.x;
       Part p;
-      const uint64_t mine = s < a.w.seqs ? kv4_items<kRows>(a, s, p) : 0;
+      const uint64_t mine = s < a.w.seqs ? kv4_items<ROWS>(a, s, p) : 0;
       uint64_t x = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
     const int pw = warp - kWarps;
     const uint64_t once = l2_evict_first();
     uint32_t it = 0;
-    while (kv4_next<kRows>(a, walk, p)) {
+    while (kv4_next<ROWS>(a, walk, p)) {
       const uint8_t* head = a.w.pool + (int64_t)p.h * Shape::kBlock;
       int x = (pw - (int)it) & 3;   // this warp's next chunk of the part
       while (x < p.take) {
@@ -377,20 +379,20 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(base_high));
     uint32_t it = 0;            // chunks of the parts before
     bool split_after = false;   // the last part goes on in the next CTA
-    while (kv4_next<kRows>(a, walk, p)) {
+    while (kv4_next<ROWS>(a, walk, p)) {
       // ---- the rows: row r of the sequence and KV head is (row r / group of the sequence, q head r % group) ----
-      const uint32_t qrows = (uint32_t)p.n * group, r0 = (uint32_t)p.b * kRows;
+      const uint32_t qrows = (uint32_t)p.n * group, r0 = (uint32_t)p.b * ROWS;
       // the position of the sequence's row i (past 2^31 - 1 the table holds nothing more to see)
       auto position = [&](uint32_t i) { return (int)min((int64_t)p.pos + i, (int64_t)0x7fffffff); };
       // the block's first and last position
-      const int tmin = position(r0 / group), tmax = position((min(r0 + kRows, qrows) - 1) / group);
+      const int tmin = position(r0 / group), tmax = position((min(r0 + ROWS, qrows) - 1) / group);
 
       // ---- Q as the first product's operand for every row of the block, by all consumer warps: a thread takes 8
       // neighbouring dims, the word of K codes that lane 4 g + (dims / 8) % 4 multiplies: nibble pair i (dims i, i + 4)
       // is a register of step i / 2 ----
       uint4* qfrag = reinterpret_cast<uint4*>(sm.acc);
       constexpr int kPieces = D / 8;   // threads per row
-      for (int x = threadIdx.x; x < kRows * kPieces; x += 32 * kWarps) {   // whole warps: kRows x D / 8 >= 64
+      for (int x = threadIdx.x; x < ROWS * kPieces; x += 32 * kWarps) {   // whole warps: ROWS x D / 8 >= 32
         const int row = x / kPieces, d8 = x % kPieces;
         const uint32_t r = r0 + row, i = r / group;
         const bool live = r < qrows;
@@ -413,18 +415,19 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
         }
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);   // the group's 8 threads
-        uint32_t hi[4], lo[4];
+        uint32_t hi[4], lo[4] = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float f = e % 2 ? 0.0625f : 1.f;   // the codes at bits 4-7 stand for 16 times the others
-          if constexpr (kQPlanes == 2)
+          if constexpr (TYPE == kKv4F32)
             split_f16x2(v[e] * f, v[e + 4] * f, hi[e], lo[e]);
           else
             hi[e] = pack_f16x2(v[e] * f, v[e + 4] * f);
         }
-        const int at = (row / 8 * kQPlanes * kBlocks + d8 / 4) * 32 + 4 * (row % 8) + d8 % 4;
+        const int column = kPair ? 2 * row : row % 8;
+        const int at = (row / 8 * kQPlanes * kBlocks + d8 / 4) * 32 + 4 * column + d8 % 4;
         qfrag[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (kQPlanes == 2) qfrag[at + kBlocks * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if constexpr (kPair || kQPlanes == 2) qfrag[at + (kPair ? 4 : kBlocks * 32)] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         if (d8 % 8 == 0) sm.qsum[row][d8 / 8] = sum * (1.f / 16777216.f);
         if (d8 == 0) {
           sm.qfac[row] = fmaxf(fabsf(a.scale) * kLog2e * (16777216.f / fabsf(up)), 1.1754944e-38f);   // 2^24: the codes' unit
@@ -432,10 +435,10 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
         }
       }
       named_bar_sync(1, 32 * kWarps);
-      // the operands of rows 8 j + g, and what belongs to rows 8 j + 2 tq + {0, 1}, this lane's scores' rows
+      // the operands of column g, and what belongs to the rows of this lane's scores: 8 j + 2 tq + {0, 1}, or tq
       uint32_t qb[RT][kBlocks][2][kQPlanes][2];
-      float qsum[RT][2][kGroups], rf[RT][2];   // (sum q)_G and the factor from the products' unit to base-2 scores
-      int t[RT][2];                            // the row's position; dead rows see nothing
+      float qsum[RT][kE][kGroups], rf[RT][kE];   // (sum q)_G and the factor from the products' unit to base-2 scores
+      int t[RT][kE];                             // the row's position; dead rows see nothing
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
 #pragma unroll
@@ -446,8 +449,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
             qb[j][b][0][pl][0] = v.x, qb[j][b][0][pl][1] = v.y, qb[j][b][1][pl][0] = v.z, qb[j][b][1][pl][1] = v.w;
           }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = 8 * j + 2 * tq + e;
+        for (int e = 0; e < kE; ++e) {
+          const int row = 8 * j + kE * tq + e;
           rf[j][e] = sm.qfac[row];
           t[j][e] = sm.qpos[row];
 #pragma unroll
@@ -456,10 +459,10 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
       }
       named_bar_sync(1, 32 * kWarps);   // before the accumulators take the operands' place
 
-      // the rows' dims 32 c + 16 m + g (+ 8: the last two), rows 8 j + 2 tq + {0, 1}, without the offsets' part
+      // dims 32 c + 16 m + g (+ 8: the last two) of columns 2 tq + {0, 1}, without the offsets' part
       float o[RT][kBlocks][2][4];
-      float oz[RT][2][kGroups];   // sum of P z over this lane's slots
-      float ref[RT][2], run_l[RT][2];
+      float oz[RT][kE][kGroups];   // sum of P z over this lane's slots
+      float ref[RT][kE], run_l[RT][kE];
       int unit_e[kGroups];   // P s 2^(136 - unit_e) is below 2^15
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
@@ -468,7 +471,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
           for (int m = 0; m < 2; ++m) o[j][c][m][0] = o[j][c][m][1] = o[j][c][m][2] = o[j][c][m][3] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < kE; ++e) {
           ref[j][e] = -INFINITY;
           run_l[j][e] = 0.f;
 #pragma unroll
@@ -485,8 +488,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
         const uint32_t* kpar = reinterpret_cast<const uint32_t*>(stg + kv4_k_params(D)) + hh * kUnit;
         const uint32_t* vw = reinterpret_cast<const uint32_t*>(stg + kv4_v_codes(D)) + hh * kUnit * (D / 8);
         const uint32_t* vpar = reinterpret_cast<const uint32_t*>(stg + kv4_v_params(D)) + hh * kUnit;
-        // ---- scores of 16 slots each: [0, 1] slot 16 u + g, [2, 3] slot 16 u + 8 + g; rows 2 tq, 2 tq + 1 ----
-        float s[RT][kSteps][4];
+        // ---- scores of 16 slots each: slot 16 u + g of the lane's kE rows, then slot 16 u + 8 + g ----
+        float s[RT][kSteps][2 * kE];
 #pragma unroll
         for (int u = 0; u < kSteps; ++u) {
           float c[RT][kGroups][4];
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                   if (blk % 2 == 0 && st == 0) {
-                    const float q0 = -8.f * qsum[j][0][G], q1 = -8.f * qsum[j][1][G];
+                    const float q0 = -8.f * qsum[j][0][G], q1 = kPair ? 0.f : -8.f * qsum[j][kE - 1][G];
                     const float start[4] = {q0, q1, q0, q1};
                     mma_f16_from(c[j][G], ka, qb[j][blk][st][0][0], qb[j][blk][st][0][1], start);
                   } else {
@@ -534,9 +537,11 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float sc = e < 2 ? s0 : s1, of = e < 2 ? z0 : z1, q1 = qsum[j][e % 2][G];
-                s[j][u][e] = fmaf(sc, c[j][G][e], G == 0 ? of * q1 : fmaf(of, q1, s[j][u][e]));
+              for (int e = 0; e < 2 * kE; ++e) {
+                const float sc = e < kE ? s0 : s1, of = e < kE ? z0 : z1, q1 = qsum[j][e % kE][G];
+                float dot = c[j][G][kPair ? 2 * e : e];
+                if constexpr (kPair && TYPE == kKv4F32) dot += c[j][G][2 * e + 1];
+                s[j][u][e] = fmaf(sc, dot, G == 0 ? of * q1 : fmaf(of, q1, s[j][u][e]));
               }
           }
         }
@@ -552,13 +557,13 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
           for (int i = 0; i < 2 * kSteps; ++i) {
             const int pp = p0 + 8 * i + g;
             const bool none = pp > tmax || (a.window > 0 && pp <= tmin - a.window);
-            bool sees[RT][2];
+            bool sees[RT][kE];
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
+              for (int e = 0; e < kE; ++e) {
                 sees[j][e] = pp <= t[j][e] && (a.window <= 0 || pp > t[j][e] - a.window);
-                if (!sees[j][e]) s[j][i / 2][2 * (i % 2) + e] = -INFINITY;
+                if (!sees[j][e]) s[j][i / 2][kE * (i % 2) + e] = -INFINITY;
               }
 #pragma unroll
             for (int G = 0; G < kGroups; ++G) {
@@ -568,7 +573,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
                 for (int j = 0; j < RT; ++j)
 #pragma unroll
-                  for (int e = 0; e < 2; ++e)
+                  for (int e = 0; e < kE; ++e)
                     if (sees[j][e]) oz[j][e][G] = __uint_as_float(0x7fc00000u);
               }
             }
@@ -587,14 +592,14 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
         }
         // ---- the rows' references: a row's probabilities are 2^(score - ref), at most 2^kSlack; a reference (and V's
         // exponent) moves up when a maximum passes it by more, and then the sums are scaled ----
-        float mx[RT][2];
+        float mx[RT][kE];
 #pragma unroll
         for (int j = 0; j < RT; ++j)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float m = fmaxf(s[j][0][e], s[j][0][e + 2]);
+          for (int e = 0; e < kE; ++e) {
+            float m = fmaxf(s[j][0][e], s[j][0][e + kE]);
 #pragma unroll
-            for (int u = 1; u < kSteps; ++u) m = fmaxf(m, fmaxf(s[j][u][e], s[j][u][e + 2]));
+            for (int u = 1; u < kSteps; ++u) m = fmaxf(m, fmaxf(s[j][u][e], s[j][u][e + kE]));
             mx[j][e] = m * rf[j][e];
             move |= mx[j][e] > ref[j][e] + kSlack;
           }
@@ -609,7 +614,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
           for (int j = 0; j < RT; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < kE; ++e) {
               float m = fmaxf(mx[j][e], ref[j][e]);
 #pragma unroll
               for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
@@ -623,10 +628,9 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
                 for (int c = 2 * G; c < 2 * G + 2; ++c)
 #pragma unroll
-                  for (int m2 = 0; m2 < 2; ++m2) {
-                    o[j][c][m2][e] *= f;
-                    o[j][c][m2][e + 2] *= f;
-                  }
+                  for (int m2 = 0; m2 < 2; ++m2)
+#pragma unroll
+                    for (int x = kPair ? 0 : e; x < 4; x += kPair ? 1 : 2) o[j][c][m2][x] *= f;
               }
             }
 #pragma unroll
@@ -635,35 +639,41 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
         for (int j = 0; j < RT; ++j)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+          for (int e = 0; e < kE; ++e) {
             const float r = ref[j][e] == -INFINITY ? 0.f : ref[j][e];
 #pragma unroll
             for (int u = 0; u < kSteps; ++u) {
               s[j][u][e] = ex2_approx(fmaf(s[j][u][e], rf[j][e], -r));
-              s[j][u][e + 2] = ex2_approx(fmaf(s[j][u][e + 2], rf[j][e], -r));
-              run_l[j][e] += s[j][u][e] + s[j][u][e + 2];
+              s[j][u][e + kE] = ex2_approx(fmaf(s[j][u][e + kE], rf[j][e], -r));
+              run_l[j][e] += s[j][u][e] + s[j][u][e + kE];
             }
           }
         // ---- P V by group of 64 dims ----
 #pragma unroll
         for (int G = 0; G < kGroups; ++G) {
           const float down = pow2_bits(136 + 127 - unit_e[G]), up = pow2_bits(unit_e[G] - 9) * 16.f;
-          uint32_t pb[RT][2][2 * kSteps];
+          uint32_t pb[RT][kPPlanes][2 * kSteps];
 #pragma unroll
           for (int i = 0; i < 2 * kSteps; ++i) {
             const float sc = __uint_as_float(w[G][i] & 0xffff0000u) * down;
             const float of = __uint_as_float(w[G][i] << 16);
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
-              const float p0_ = s[j][i / 2][2 * (i % 2)], p1_ = s[j][i / 2][2 * (i % 2) + 1];
-              const float x0 = p0_ * sc, x1 = p1_ * sc;
               // hi: the leading 11 bits (cut, so that an AND gives them), lo: the next 11
-              const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffffe000u);
-              const float h1 = __uint_as_float(__float_as_uint(x1) & 0xffffe000u);
-              pb[j][0][i] = transpose8(pack_f16x2(h0, h1));
-              pb[j][1][i] = transpose8(pack_f16x2(x0 - h0, x1 - h1));
-              oz[j][0][G] = fmaf(p0_, of, oz[j][0][G]);
-              oz[j][1][G] = fmaf(p1_, of, oz[j][1][G]);
+              float hi[kE], lo[kE];
+#pragma unroll
+              for (int e = 0; e < kE; ++e) {
+                const float pr = s[j][i / 2][kE * (i % 2) + e], x = pr * sc;
+                hi[e] = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+                lo[e] = x - hi[e];
+                oz[j][e][G] = fmaf(pr, of, oz[j][e][G]);
+              }
+              if constexpr (kPair) {
+                pb[j][0][i] = transpose8(pack_f16x2(hi[0], lo[0]));
+              } else {
+                pb[j][0][i] = transpose8(pack_f16x2(hi[0], hi[kE - 1]));
+                pb[j][kPPlanes - 1][i] = transpose8(pack_f16x2(lo[0], lo[kE - 1]));
+              }
             }
           }
 #pragma unroll
@@ -681,8 +691,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                   float(&to)[4] = kDirect ? o[j][c][m] : d[j][m];
-                  mma_f16_add(to, va, pb[j][0][2 * st], pb[j][0][2 * st + 1]);
-                  mma_f16_add(to, va, pb[j][1][2 * st], pb[j][1][2 * st + 1]);
+#pragma unroll
+                  for (int pl = 0; pl < kPPlanes; ++pl) mma_f16_add(to, va, pb[j][pl][2 * st], pb[j][pl][2 * st + 1]);
                 }
               }
             if constexpr (!kDirect)
@@ -714,8 +724,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
       for (int j = 0; j < RT; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = 8 * j + 2 * tq + e;
+        for (int e = 0; e < kE; ++e) {
+          const int row = 8 * j + kE * tq + e;
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) {
             run_l[j][e] += __shfl_xor_sync(0xffffffffu, run_l[j][e], x);
@@ -731,15 +741,16 @@ __global__ void __launch_bounds__(Kv4Shape<D, RT>::kThreads, 1)
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
               const float up = kDirect ? pow2_bits(unit_e[c / 2] - 9) * 16.f : 1.f;
-              sm.acc[warp][row][32 * c + 16 * m + g] = fmaf(o[j][c][m][e], up, oz[j][e][c / 2]);
-              sm.acc[warp][row][32 * c + 16 * m + 8 + g] = fmaf(o[j][c][m][e + 2], up, oz[j][e][c / 2]);
+              const float(&y)[4] = o[j][c][m];
+              sm.acc[warp][row][32 * c + 16 * m + g] = fmaf(kPair ? y[0] + y[1] : y[e], up, oz[j][e][c / 2]);
+              sm.acc[warp][row][32 * c + 16 * m + 8 + g] = fmaf(kPair ? y[2] + y[3] : y[e + 2], up, oz[j][e][c / 2]);
             }
         }
       named_bar_sync(1, 32 * kWarps);
       const bool whole = p.c0 == 0 && p.take == p.cnt;
-      float* mine = part + (int64_t)(2 * blockIdx.x + (p.c0 == 0 ? 1 : 0)) * kRows * part_row(D);
+      float* mine = part + (int64_t)(2 * blockIdx.x + (p.c0 == 0 ? 1 : 0)) * ROWS * part_row(D);
       constexpr int kQuads = D / 4;   // threads per row
-      for (int x = threadIdx.x; x < kRows * kQuads; x += 32 * kWarps) {
+      for (int x = threadIdx.x; x < ROWS * kQuads; x += 32 * kWarps) {
         const int row = x / kQuads, d0 = 4 * (x % kQuads);
         const uint32_t rr = r0 + row;
         if (rr >= qrows) break;
@@ -882,20 +893,20 @@ __global__ void __launch_bounds__(kCombineThreads)
   }
 }
 
-// Row blocks of 16 rows where a sequence has more than 8 (head dim 256 has no registers for them).
+// Rows of a row block: as many as a sequence has, 4, 8 or 16 (head dim 256 has no registers for 16).
 int block_rows(int head_dim, int group, int rows_per_seq) {
-  return head_dim <= 128 && (int64_t)group * rows_per_seq > 8 ? 16 : 8;
+  const int64_t rows = (int64_t)group * rows_per_seq;
+  return rows <= 4 ? 4 : rows <= 8 || head_dim == 256 ? 8 : 16;
 }
 
-template <int D, int RT, int TYPE>
+template <int D, int ROWS, int TYPE>
 void launch(const Kv4Attn& a, int sms, cudaStream_t s) {
-  using Shape = Kv4Shape<D, RT>;
   float* part = a.part;
-  Kv4Split* splits = reinterpret_cast<Kv4Split*>(part + (int64_t)sms * 2 * Shape::kRows * part_row(D));
+  Kv4Split* splits = reinterpret_cast<Kv4Split*>(part + (int64_t)sms * 2 * ROWS * part_row(D));
   static std::atomic<uint64_t> optin;
-  const int smem = (int)sizeof(Kv4Smem<D, RT>);
-  ensure_smem_optin((const void*)kv4_attention_kernel<D, RT, TYPE>, smem, optin);
-  kv4_attention_kernel<D, RT, TYPE><<<sms, Shape::kThreads, smem, s>>>(a, part, splits);
+  const int smem = (int)sizeof(Kv4Smem<D, ROWS>);
+  ensure_smem_optin((const void*)kv4_attention_kernel<D, ROWS, TYPE>, smem, optin);
+  kv4_attention_kernel<D, ROWS, TYPE><<<sms, Kv4Shape<D, ROWS>::kThreads, smem, s>>>(a, part, splits);
   XTG_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sms * kCombineBlocksPerSm);
@@ -906,18 +917,27 @@ void launch(const Kv4Attn& a, int sms, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  XTG_CUDA(cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D>, a, Shape::kRows, sms, (const float*)part,
-                              (const Kv4Split*)splits));
+  XTG_CUDA(cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D>, a, ROWS, sms, (const float*)part, (const Kv4Split*)splits));
 }
 
-template <int D, int RT>
+template <int D, int ROWS>
 void launch_type(const Kv4Attn& a, int sms, cudaStream_t s) {
   if (a.dtype == kKv4F32)
-    launch<D, RT, kKv4F32>(a, sms, s);
+    launch<D, ROWS, kKv4F32>(a, sms, s);
   else if (a.dtype == kKv4Bf16)
-    launch<D, RT, kKv4Bf16>(a, sms, s);
+    launch<D, ROWS, kKv4Bf16>(a, sms, s);
   else
-    launch<D, RT, kKv4F16>(a, sms, s);
+    launch<D, ROWS, kKv4F16>(a, sms, s);
+}
+
+template <int D>
+void launch_rows(const Kv4Attn& a, int rows, int sms, cudaStream_t s) {
+  if (rows == 4)
+    launch_type<D, 4>(a, sms, s);
+  else if (D == 256 || rows == 8)
+    launch_type<D, 8>(a, sms, s);
+  else
+    launch_type<D, D == 256 ? 8 : 16>(a, sms, s);
 }
 
 }  // namespace
@@ -929,13 +949,13 @@ int64_t kv4_workspace_bytes(int head_dim, int group, int rows_per_seq, int sms) 
 
 void launch_kv4_attention(const Kv4Attn& a, int sms, cudaStream_t s) {
   XTG_REQUIRE(sms <= kMostSms, "kv4: more SMs than the combine lists");
-  const bool wide = block_rows(a.w.head_dim, a.group, a.rows_per_seq) == 16;
+  const int rows = block_rows(a.w.head_dim, a.group, a.rows_per_seq);
   if (a.w.head_dim == 256)
-    launch_type<256, 1>(a, sms, s);
+    launch_rows<256>(a, rows, sms, s);
   else if (a.w.head_dim == 128)
-    wide ? launch_type<128, 2>(a, sms, s) : launch_type<128, 1>(a, sms, s);
+    launch_rows<128>(a, rows, sms, s);
   else
-    wide ? launch_type<64, 2>(a, sms, s) : launch_type<64, 1>(a, sms, s);
+    launch_rows<64>(a, rows, sms, s);
 }
 
 }  // namespace xtg
