@@ -57,7 +57,12 @@ struct Kv4Shape {
   static constexpr int kConsumerRegs = (kThreads * kStart - 128 * kProducerRegs) / (32 * kWarps) / 8 * 8;
   static_assert(32 * kWarps * kConsumerRegs + 128 * kProducerRegs <= kThreads * kStart, "more registers than launched");
   static constexpr int kBlock = kv4_block_bytes(D);
-  static constexpr int kStages = D == 256 ? 8 : D == 128 ? 16 : 24;   // a multiple of 4; 110 or 147 KB
+  // The ring: 110 to 166 KB. A stage's chunks are always brought by the same producer and its halves taken by the same
+  // consumer warps. A wait tells the phases of a barrier apart by their parity only, so it must not start while the
+  // phase before is open: a warp that waits for a stage's next chunk has itself seen the last one arrive.
+  static constexpr int kStages = D == 256 ? 8 : D == 128 ? (kWarps == 12 ? 18 : 16) : 24;
+  static constexpr int kProducers = kStages % 4 ? 3 : 4;
+  static_assert(kUnits * kStages % kWarps == 0 && kStages % kProducers == 0, "a stage with several owners");
   static constexpr int kMergeStride = D + 4;   // floats of a row's accumulator being merged
 };
 
@@ -339,18 +344,20 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
 
   if (warp >= kWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kProducerRegs));
-    // ---- producers: chunk k of the parts in order is warp k % 4's, a page's block of the head into stage k % kStages;
-    // 32 chunks' pages are looked up at once ----
+    // ---- producers: chunk k of the parts in order is warp k % kProducers', a page's block of the head into stage
+    // k % kStages; 32 chunks' pages are looked up at once ----
+    constexpr int kProducers = Shape::kProducers;
     const int pw = warp - kWarps;
+    if (pw >= kProducers) return;
     const uint64_t once = l2_evict_first();
     uint32_t it = 0;
     while (kv4_next<ROWS>(a, walk, p)) {
       const uint8_t* head = a.w.pool + (int64_t)p.h * Shape::kBlock;
-      int x = (pw - (int)it) & 3;   // this warp's next chunk of the part
+      int x = (int)((pw + kProducers - it % kProducers) % kProducers);   // this warp's next chunk of the part
       while (x < p.take) {
-        const int count = min((p.take - x + 3) / 4, 32);
-        const int64_t mine = lane < count ? kv4_page(a.w, p.seq, p.lo + p.c0 + x + 4 * lane) : -1;
-        for (int j = 0; j < count; ++j, x += 4) {
+        const int count = min((p.take - x + kProducers - 1) / kProducers, 32);
+        const int64_t mine = lane < count ? kv4_page(a.w, p.seq, p.lo + p.c0 + x + kProducers * lane) : -1;
+        for (int j = 0; j < count; ++j, x += kProducers) {
           const int64_t page = __shfl_sync(0xffffffffu, mine, j);
           const uint32_t k = it + x, st = k % kStages, turn = k / kStages;
           if (lane == 0 && (turn == 0 || kv4_wait(&sm.empty[st], (turn - 1) & 1, &sm.failed, a.w.err))) {
