@@ -8,7 +8,7 @@
 // idle: S^T = K Q^T takes 16 slots x 16 dims of K, o^T = V^T P^T 16 dims x 16 slots of V. A lane then holds the scores
 // of slots g, g + 8 and rows 2 a, 2 a + 1 (lane = 4 g + a); movmatrix turns the probabilities into the second
 // product's operand. The scales and offsets enter in f32:
-//   q . K[p] = sum_G s[p][G] (q . code - 8 sum q)_G + z[p][G] (sum q)_G        (-8 sum q: the accumulator's start)
+//   q . K[p] = sum_G s[p][G] (q . code)_G + (z[p][G] - 8 s[p][G]) (sum q)_G
 //   o[r]     = sum_p (P[r][p] s[p][G]) (code - 8) + P[r][p] z[p][G]            (P s: the operand, by group G)
 // K's codes enter as f16 subnormals, the nibble itself: code 2^-24 (bits 0-3) or code 2^-20 (bits 4-7), exact; q
 // carries 1/16 where they lie at bits 4-7. V's are centred first (64 + c / 16 less 64.5): a sum of uncentred codes over
@@ -55,6 +55,7 @@ struct Kv4Shape {
   static constexpr int kStart = 65536 / kThreads / 8 * 8;
   static constexpr int kProducerRegs = 40;
   static constexpr int kConsumerRegs = (kThreads * kStart - 128 * kProducerRegs) / (32 * kWarps) / 8 * 8;
+  static_assert(kWarps % 4 == 0, "setmaxnreg takes whole warpgroups");
   static_assert(32 * kWarps * kConsumerRegs + 128 * kProducerRegs <= kThreads * kStart, "more registers than launched");
   static constexpr int kBlock = kv4_block_bytes(D);
   // The ring: 110 to 166 KB. A stage's chunks are always brought by the same producer and its halves taken by the same
@@ -224,13 +225,12 @@ __device__ __forceinline__ uint32_t v_codes_high(uint32_t w, uint32_t base) {
   return hfma2_u32(and_or<0x00f000f0u>(w, base), 0x1c001c00u, 0xc480c480u);
 }
 
-// D = A B + C with C apart from D
-__device__ __forceinline__ void mma_f16_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
-                                             const float (&c)[4]) {
+// D = A B
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_f16_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   mma_f16(d, a[0], a[1], a[2], a[3], b0, b1);
@@ -523,13 +523,10 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
                 const uint32_t ka[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
-                  if (blk % 2 == 0 && st == 0) {
-                    const float q0 = -8.f * qsum[j][0][G], q1 = kPair ? 0.f : -8.f * qsum[j][kE - 1][G];
-                    const float start[4] = {q0, q1, q0, q1};
-                    mma_f16_from(c[j][G], ka, qb[j][blk][st][0][0], qb[j][blk][st][0][1], start);
-                  } else {
+                  if (blk % 2 == 0 && st == 0)
+                    mma_f16_new(c[j][G], ka, qb[j][blk][st][0][0], qb[j][blk][st][0][1]);
+                  else
                     mma_f16_add(c[j][G], ka, qb[j][blk][st][0][0], qb[j][blk][st][0][1]);
-                  }
                   if constexpr (kQPlanes == 2)
                     mma_f16_add(c[j][G], ka, qb[j][blk][st][kQPlanes - 1][0], qb[j][blk][st][kQPlanes - 1][1]);
                 }
@@ -540,7 +537,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
           for (int G = 0; G < kGroups; ++G) {
             const uint32_t w0 = kpar[G * kKv4Page + 16 * u + g], w1 = kpar[G * kKv4Page + 16 * u + 8 + g];
             const float s0 = __uint_as_float(w0 & 0xffff0000u), s1 = __uint_as_float(w1 & 0xffff0000u);
-            const float z0 = __uint_as_float(w0 << 16), z1 = __uint_as_float(w1 << 16);
+            const float z0 = fmaf(-8.f, s0, __uint_as_float(w0 << 16)), z1 = fmaf(-8.f, s1, __uint_as_float(w1 << 16));
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -685,7 +682,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
           }
 #pragma unroll
           for (int c = 2 * G; c < 2 * G + 2; ++c) {
-            float d[RT][2][4] = {};
+            float d[RT][2][4];
             const uint4 v = *reinterpret_cast<const uint4*>(vw + ((c * 8 + g) * 4 + tq) * 4);
             const uint32_t word[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -699,7 +696,12 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
                 for (int j = 0; j < RT; ++j) {
                   float(&to)[4] = kDirect ? o[j][c][m] : d[j][m];
 #pragma unroll
-                  for (int pl = 0; pl < kPPlanes; ++pl) mma_f16_add(to, va, pb[j][pl][2 * st], pb[j][pl][2 * st + 1]);
+                  for (int pl = 0; pl < kPPlanes; ++pl) {
+                    if (!kDirect && st == 0 && pl == 0)
+                      mma_f16_new(to, va, pb[j][pl][0], pb[j][pl][1]);
+                    else
+                      mma_f16_add(to, va, pb[j][pl][2 * st], pb[j][pl][2 * st + 1]);
+                  }
                 }
               }
             if constexpr (!kDirect)
