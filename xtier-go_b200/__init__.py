@@ -10,7 +10,6 @@ import ctypes as C
 import json
 import os
 import subprocess
-import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libxtg_cuda.so")
@@ -603,17 +602,29 @@ KV4_PAGE = 64
 
 _KV4_ERRORS = {1: "a device wait timed out", 6: "a position lies past its sequence's page table",
                7: "a page table entry lies past the pool"}
-_kv4_dtypes = {}            # torch dtype -> the C ABI's code
-_kv4_workspace_bytes = {}   # by shape and device
-_kv4_local = threading.local()
+_kv4_module = None
+_kv4_dtypes = {}   # torch dtype -> the C ABI's code
 
 
-def _kv4_dtype(t):
-    """The C ABI's code of a torch dtype, None for one it does not take."""
-    if not _kv4_dtypes:
+def _kv4():
+    """csrc/kv4_torch.cpp, which checks the tensors and calls the C ABI; raises if it was not built."""
+    global _kv4_module
+    if _kv4_module is None:
+        import importlib.util
         import torch
+        path = os.path.join(HERE, "_kv4_torch.so")
+        if not os.path.exists(path):
+            raise XtgError(f"{path} is missing: build it with xtier-go_b200's Makefile (__graft_entry__.build())")
+        spec = importlib.util.spec_from_file_location("_kv4_torch", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        L = lib()
+        mod.bind(XtgError, *[C.cast(f, C.c_void_p).value for f in (L.xtg_cuda_kv4_store, L.xtg_cuda_kv4_load,
+                                                                   L.xtg_cuda_kv4_workspace,
+                                                                   L.xtg_cuda_kv4_attention)])
         _kv4_dtypes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
-    return _kv4_dtypes.get(t)
+        _kv4_module = mod
+    return _kv4_module
 
 
 def kv4_pool(pages, kv_heads, head_dim, device="cuda"):
@@ -630,112 +641,21 @@ def kv4_check(err):
         raise XtgError("kv4: " + _KV4_ERRORS.get(code, f"error {code}"))
 
 
-def _kv4_index(name, t, dims, dev):
-    """The shape of an index tensor (contiguous int32 on device dev)."""
-    import torch
-    shape = t.shape
-    if t.dtype is not torch.int32 or len(shape) != dims or t.get_device() != dev or not t.is_contiguous():
-        raise XtgError(f"kv4: {name} is a contiguous int32 tensor of {dims} dimension(s) on the pool's device")
-    return shape
-
-
-def _kv4_where(pool, table, pos, cu_rows, rows, err):
-    """(xtg_cuda_kv4, the pool's device) after the checks that need no device work."""
-    import torch
-    dev = pool.get_device()
-    shape = pool.shape
-    if pool.dtype is not torch.uint8 or len(shape) != 3 or not pool.is_contiguous() or dev < 0:
-        raise XtgError("kv4: pool is a contiguous uint8 CUDA tensor [pages][kv_heads][72 head_dim]")
-    pages, kvh, block = shape
-    if block not in (72 * 64, 72 * 128, 72 * 256):
-        raise XtgError("kv4: head_dim 64, 128 or 256 (pool.shape[2] / 72)")
-    seqs, max_pages = _kv4_index("table", table, 2, dev)
-    if _kv4_index("pos", pos, 1, dev)[0] != seqs or _kv4_index("cu_rows", cu_rows, 1, dev)[0] != seqs + 1:
-        raise XtgError("kv4: table [seqs][max_pages], pos [seqs], cu_rows [seqs + 1]")
-    if err is not None and (err.dtype is not torch.int32 or err.numel() != 1 or err.get_device() != dev):
-        raise XtgError("kv4: err is one int32 on the pool's device")
-    return Kv4(pool.data_ptr(), pages, kvh, block // 72, table.data_ptr(), max_pages, seqs, pos.data_ptr(),
-               cu_rows.data_ptr(), rows, None if err is None else err.data_ptr()), dev
-
-
-def _kv4_rows(name, t, heads, c, dev):
-    """(dtype code, strides) of rows t [rows][heads][head_dim] with contiguous head dims on device dev; heads 0: any."""
-    dtype = _kv4_dtype(t.dtype)
-    if dtype is None:
-        raise XtgError(f"kv4: {name} is float32, bfloat16 or float16")
-    shape, strides = t.shape, t.stride()
-    if len(shape) != 3 or shape[2] != c.head_dim or (heads and shape[1] != heads) or t.get_device() != dev:
-        raise XtgError(f"kv4: {name} is [rows][heads][head_dim] of the pool's head_dim on the pool's device")
-    if strides[2] != 1:
-        raise XtgError(f"kv4: {name}'s head dims must be contiguous")
-    return dtype, strides
-
-
-def _kv4_call(dev, f, *args):
-    """Call entry point f with device dev current, on its current stream."""
-    import torch
-    err = getattr(_kv4_local, "err", None)
-    if err is None:
-        err = _kv4_local.err = _err()
-    if torch.cuda.current_device() != dev:
-        with torch.cuda.device(dev):
-            return _kv4_call(dev, f, *args)
-    # torch.cuda.current_stream() builds a Stream object for the same handle: 3 us a call
-    if f(*args, torch._C._cuda_getCurrentRawStream(dev), err, 1024):
-        raise XtgError(err.value.decode(errors="replace"))
-
-
 def kv4_store(pool, k, v, table, pos, cu_rows, err=None):
     """Quantise rows k, v [rows][kv_heads][head_dim] (float32, bfloat16 or float16; row and head strides of 16-byte
     multiples) into the pool. Two sequences of a call must not write the same page."""
-    rows = k.shape[0]
-    c, dev = _kv4_where(pool, table, pos, cu_rows, rows, err)
-    dtype, ks = _kv4_rows("k", k, c.kv_heads, c, dev)
-    other, vs = _kv4_rows("v", v, c.kv_heads, c, dev)
-    if other != dtype or v.shape[0] != rows:
-        raise XtgError("kv4: k and v have the same type and rows")
-    _kv4_call(dev, lib().xtg_cuda_kv4_store, c, k.data_ptr(), v.data_ptr(), dtype, ks[0], ks[1], vs[0], vs[1])
+    _kv4().store(pool, table, pos, cu_rows, err, k, v)
 
 
 def kv4_load(pool, table, pos, cu_rows, rows, dtype=None, err=None):
     """The cached keys and values of `rows` rows (cu_rows' last entry): (k, v) [rows][kv_heads][head_dim] of dtype
     (default bfloat16)."""
-    import torch
-    dtype = dtype or torch.bfloat16
-    code = _kv4_dtype(dtype)
-    if code is None:
-        raise XtgError("kv4: dtype is float32, bfloat16 or float16")
-    c, dev = _kv4_where(pool, table, pos, cu_rows, rows, err)
-    k = torch.empty((rows, c.kv_heads, c.head_dim), dtype=dtype, device=pool.device)
-    v = torch.empty_like(k)
-    _kv4_call(dev, lib().xtg_cuda_kv4_load, c, k.data_ptr(), v.data_ptr(), code)
-    return k, v
+    m = _kv4()
+    return m.load(pool, table, pos, cu_rows, err, rows, 1 if dtype is None else _kv4_dtypes.get(dtype, -1))
 
 
 def kv4_attention(q, pool, table, pos, cu_rows, scale, window=0, rows_per_seq=None, out=None, err=None):
     """Attention of rows q [rows][heads][head_dim] over the cached positions up to each row's own (window > 0: the last
     `window` of these), after the call's rows were stored: [rows][heads][head_dim] in q's type. rows_per_seq: about how
     many rows a sequence has (default rows / seqs); it chooses the tiling only."""
-    import torch
-    rows = q.shape[0]
-    c, dev = _kv4_where(pool, table, pos, cu_rows, rows, err)
-    dtype, qs = _kv4_rows("q", q, 0, c, dev)
-    heads = q.shape[1]
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise XtgError("kv4: out is contiguous, of q's shape and type")
-    if rows_per_seq is None:
-        rows_per_seq = max(1, -(-rows // max(1, c.seqs)))
-    key = (dev, heads, c.kv_heads, c.head_dim, rows_per_seq)
-    size = _kv4_workspace_bytes.get(key)
-    if size is None:
-        with torch.cuda.device(dev):
-            size = lib().xtg_cuda_kv4_workspace(heads, c.kv_heads, c.head_dim, rows_per_seq)
-        if size < 0:
-            raise XtgError("kv4: q heads a multiple of KV heads, rows_per_seq at least 1")
-        _kv4_workspace_bytes[key] = size
-    work = torch.empty(size, dtype=torch.uint8, device=q.device)
-    _kv4_call(dev, lib().xtg_cuda_kv4_attention, c, q.data_ptr(), out.data_ptr(), dtype, heads, qs[0], qs[1], scale,
-              window, rows_per_seq, work.data_ptr(), size)
-    return out
+    return _kv4().attention(pool, table, pos, cu_rows, err, q, scale, window, rows_per_seq, out)
