@@ -347,3 +347,20 @@ def test_python_refusals(cuda, xtg, torch):
     for call in bad:
         with pytest.raises(xtg.XtgError):
             call()
+
+
+def test_the_serving_example(cuda, xtg, torch):
+    """examples/kv4_serving.py: prompts in chunks, one token steps, pages given back and taken again. 4-bit values are
+    off by a uniform error of at most half a step: a step is a 15th of the range of 64 normal values, about 4.8 sigma, so
+    0.32 sigma and 0.093 sigma rms; values' errors average as the values themselves do (9 %), and keys' errors move a
+    score of sigma 1 by 0.09, whose effect on the weights adds about as much. 0.25 leaves room for the single rows."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "kv4_serving.py")
+    spec = importlib.util.spec_from_file_location("kv4_serving", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    worst, pages = mod.serve(prompts=(200, 65, 1, 130), steps=10)
+    assert worst < 0.25 and pages == 4 + 2 + 1 + 3
+    worst, pages = mod.serve(prompts=(400, 1), steps=12, window=100, heads=8, kv_heads=2)
+    assert worst < 0.25 and pages <= 3 + 1

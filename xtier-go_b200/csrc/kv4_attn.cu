@@ -8,11 +8,12 @@
 // idle: S^T = K Q^T takes 16 slots x 16 dims of K, o^T = V^T P^T 16 dims x 16 slots of V. A lane then holds the scores
 // of slots g, g + 8 and rows 2 a, 2 a + 1 (lane = 4 g + a); movmatrix turns the probabilities into the second
 // product's operand. The scales and offsets enter in f32:
-//   q . K[p] = sum_G s[p][G] (q . code)_G + (z[p][G] - 8 s[p][G]) (sum q)_G
+//   q . K[p] = sum_G s[p][G] (q . code)_G + (z[p][G] - 8 s[p][G]) (sum q)_G    (f32 rows: code - 8, and z alone)
 //   o[r]     = sum_p (P[r][p] s[p][G]) (code - 8) + P[r][p] z[p][G]            (P s: the operand, by group G)
 // K's codes enter as f16 subnormals, the nibble itself: code 2^-24 (bits 0-3) or code 2^-20 (bits 4-7), exact; q
 // carries 1/16 where they lie at bits 4-7. V's are centred first (64 + c / 16 less 64.5): a sum of uncentred codes over
-// positions would put an error of about 2^-20 of the group's range into components far smaller than it.
+// positions would put an error of about 2^-20 of the group's range into components far smaller than it. So are K's for
+// f32 rows, whose scores would lose about two bits to the part that cancels.
 // Precision of the f16 operands: q of 16-bit rows is exact in one plane (a power of two brings the row's largest value
 // to 2^14 .. 2^15); of f32 rows it is hi + lo, 22 bits. P s is brought below 2^15 by a power of two per chunk and
 // group (its largest scale) and always has two planes: one would put 2^-12 of the largest value into the result, which
@@ -101,6 +102,10 @@ __device__ __forceinline__ uint64_t divide(uint64_t a, uint32_t b) {
   return a >> 32 ? a / b : (uint32_t)a / b;
 }
 
+__device__ __forceinline__ uint64_t item_count(const Kv4Attn& a, const Part& p) {
+  return (uint64_t)p.blocks * (uint32_t)a.w.kv_heads * (uint32_t)(p.cnt + kPartCost);
+}
+
 // The items of sequence s: KV heads x row blocks x (kPartCost + chunks). Sequences with rows have at least one chunk (it may hold
 // nothing), so that every row is written.
 template <int ROWS>
@@ -120,19 +125,21 @@ __device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, Part& p) 
   p.lo = first / kKv4Page;
   p.cnt = max((int)((end + kKv4Page - 1) >> 6) - p.lo, 1);
   p.blocks = ((uint32_t)p.n * (uint32_t)a.group + ROWS - 1) / ROWS;
-  return (uint64_t)p.blocks * (uint32_t)a.w.kv_heads * (uint32_t)(p.cnt + kPartCost);
+  return item_count(a, p);
 }
 
 // Walks a CTA's share of the items part by part.
 struct Walk {
   int s;
+  bool known;           // the Part given to the next step has sequence s's fields already
   uint64_t off, left;   // from sequence s's first item
 };
 
 template <int ROWS>
 __device__ __forceinline__ bool kv4_next(const Kv4Attn& a, Walk& k, Part& p) {
   while (k.left > 0 && k.s < a.w.seqs) {
-    const uint64_t items = kv4_items<ROWS>(a, k.s, p);
+    const uint64_t items = k.known ? item_count(a, p) : kv4_items<ROWS>(a, k.s, p);
+    k.known = false;
     if (k.off >= items) {
       k.off -= items;
       ++k.s;
@@ -216,12 +223,12 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t c) {
   return r;
 }
 
-// The V codes at bits 0-3 (low) or 4-7 (high) of a word's halves as (code - 8) 2^-4 in f16: 64 + c / 16 less 64.5, and
+// The codes at bits 0-3 (low) or 4-7 (high) of a word's halves as (code - 8) 2^-4 in f16: 64 + c / 16 less 64.5, and
 // (1024 + 16 c) / 256 less 4.5; exact. base: 64 (low) and 1024 (high) in both halves.
-__device__ __forceinline__ uint32_t v_codes_low(uint32_t w, uint32_t base) {
+__device__ __forceinline__ uint32_t codes_low(uint32_t w, uint32_t base) {
   return hadd2_u32(and_or<0x000f000fu>(w, base), 0xd408d408u);
 }
-__device__ __forceinline__ uint32_t v_codes_high(uint32_t w, uint32_t base) {
+__device__ __forceinline__ uint32_t codes_high(uint32_t w, uint32_t base) {
   return hfma2_u32(and_or<0x00f000f0u>(w, base), 0x1c001c00u, 0xc480c480u);
 }
 
@@ -277,70 +284,88 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
   constexpr int RT = ROWS == 16 ? 2 : 1, kE = ROWS == 4 ? 1 : 2;
   constexpr bool kPair = ROWS == 4;
   constexpr int kQPlanes = TYPE == kKv4F32 && !kPair ? 2 : 1, kPPlanes = kPair ? 1 : 2;   // operands per tile
-  constexpr bool kDirect = TYPE != kKv4F32;   // P V added up in the matrix unit
+  constexpr bool kDirect = TYPE != kKv4F32;    // P V added up in the matrix unit
+  constexpr bool kCentred = TYPE == kKv4F32;   // K's codes less 8 before the product
+  constexpr float kCode = kCentred ? 1.f / 16.f : 1.f / 16777216.f;   // the unit in which K's codes enter
   extern __shared__ __align__(128) unsigned char smem_raw[];
   Kv4Smem<D, ROWS>& sm = *reinterpret_cast<Kv4Smem<D, ROWS>*>(smem_raw);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, tq = lane & 3;
 
-  // ---- this CTA's share of the items: an equal part of their sum over the sequences ----
-  uint64_t total = 0, share = 0;
-  uint32_t share_items = 0, most = 0, extra = 0;   // CTAs below `extra` have `most` + 1 items, the others `most`
-  const bool one_pass = a.w.seqs <= kThreads;
-  for (int pass = 0; pass < 2; ++pass) {   // the sum, then where the share starts
-    uint64_t base = 0;
-    for (int s0 = 0; s0 < a.w.seqs; s0 += kThreads) {
-      const int s = s0 + threadIdx.x;
-      Part p;
-      const uint64_t mine = s < a.w.seqs ? kv4_items<ROWS>(a, s, p) : 0;
-      uint64_t x = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (lane == 31) sm.scan[warp] = x;
-      if (threadIdx.x == 0 && pass == 0 && s0 == 0) {
-        for (int st = 0; st < kStages; ++st) {
-          mbar_init(&sm.full[st], 1);
-          mbar_init(&sm.empty[st], kUnits);
-        }
-        mbar_init_fence();
-        sm.failed = 0;
-        sm.start_seq = a.w.seqs;
-        sm.start_base = 0;
-      }
-      __syncthreads();
-      uint64_t sum = 0;
-#pragma unroll
-      for (int v = 0; v < kThreads / 32; ++v) {
-        if (v < warp) x += sm.scan[v];
-        sum += sm.scan[v];
-      }
-      if (one_pass || pass == 0) {
-        total = base + sum;
-        if (s0 + kThreads >= a.w.seqs) {
-          // with fewer items than CTAs one each, so that no share between two others is empty
-          const uint32_t ctas = total < gridDim.x ? (uint32_t)total : gridDim.x;
-          if (blockIdx.x < ctas) {
-            most = (uint32_t)divide(total, ctas);
-            extra = (uint32_t)(total - (uint64_t)most * ctas);
-            share = (uint64_t)most * blockIdx.x + min(blockIdx.x, extra);
-            share_items = most + (blockIdx.x < extra);
-          }
-        }
-      }
-      if ((one_pass || pass == 1) && base + x - mine <= share && share < base + x) {
-        sm.start_seq = s;
-        sm.start_base = base + x - mine;
-      }
-      base += sum;
-      __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int st = 0; st < kStages; ++st) {
+      mbar_init(&sm.full[st], 1);
+      mbar_init(&sm.empty[st], kUnits);
     }
-    if (one_pass) break;
+    mbar_init_fence();
+    sm.failed = 0;
+    sm.start_seq = a.w.seqs;
+    sm.start_base = 0;
   }
-  Walk walk = {sm.start_seq, share - sm.start_base, share_items};
+  // ---- this CTA's share of the items: an equal part of their sum over the sequences ----
+  uint64_t share = 0;
+  uint32_t share_items = 0, most = 0, extra = 0;   // CTAs below `extra` have `most` + 1 items, the others `most`
+  auto take_share = [&](uint64_t total) {
+    // with fewer items than CTAs one each, so that no share between two others is empty
+    const uint32_t ctas = total < gridDim.x ? (uint32_t)total : gridDim.x;
+    if (blockIdx.x >= ctas) return;
+    most = (uint32_t)divide(total, ctas);
+    extra = (uint32_t)(total - (uint64_t)most * ctas);
+    share = (uint64_t)most * blockIdx.x + min(blockIdx.x, extra);
+    share_items = most + (blockIdx.x < extra);
+  };
+  auto warp_sum_to = [&](uint64_t x) {   // inclusive, over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  Walk walk = {};
   Part p;
+  if (a.w.seqs <= 32) {   // every warp by itself, a sequence per lane
+    const uint64_t mine = lane < a.w.seqs ? kv4_items<ROWS>(a, lane, p) : 0, x = warp_sum_to(mine);
+    take_share(__shfl_sync(0xffffffffu, x, 31));
+    // the lane whose sequence the share starts in (CTAs without items: any)
+    const uint32_t at = __ballot_sync(0xffffffffu, x - mine <= share && share < x);
+    const int from = at ? __ffs(at) - 1 : 0;
+    walk = {from, true, share - __shfl_sync(0xffffffffu, x - mine, from), share_items};
+    p.seq = from;
+    p.row0 = __shfl_sync(0xffffffffu, p.row0, from);
+    p.n = __shfl_sync(0xffffffffu, p.n, from);
+    p.pos = __shfl_sync(0xffffffffu, p.pos, from);
+    p.lo = __shfl_sync(0xffffffffu, p.lo, from);
+    p.cnt = __shfl_sync(0xffffffffu, p.cnt, from);
+    p.blocks = __shfl_sync(0xffffffffu, p.blocks, from);
+    __syncthreads();
+  } else {
+    const bool one_pass = a.w.seqs <= kThreads;
+    for (int pass = 0; pass < 2; ++pass) {   // the sum, then where the share starts
+      uint64_t base = 0;
+      for (int s0 = 0; s0 < a.w.seqs; s0 += kThreads) {
+        const int s = s0 + threadIdx.x;
+        const uint64_t mine = s < a.w.seqs ? kv4_items<ROWS>(a, s, p) : 0;
+        uint64_t x = warp_sum_to(mine), sum = 0;
+        if (lane == 31) sm.scan[warp] = x;
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < kThreads / 32; ++v) {
+          if (v < warp) x += sm.scan[v];
+          sum += sm.scan[v];
+        }
+        if ((one_pass || pass == 0) && s0 + kThreads >= a.w.seqs) take_share(base + sum);
+        if ((one_pass || pass == 1) && base + x - mine <= share && share < base + x) {
+          sm.start_seq = s;
+          sm.start_base = base + x - mine;
+        }
+        base += sum;
+        __syncthreads();
+      }
+      if (one_pass) break;
+    }
+    walk = {sm.start_seq, false, share - sm.start_base, share_items};
+  }
 
   if (warp >= kWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kProducerRegs));
@@ -381,7 +406,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kConsumerRegs));
     const uint32_t group = a.group;
-    uint32_t base_low, base_high;   // kept in registers (v_codes_low)
+    uint32_t base_low, base_high;   // kept in registers (codes_low)
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(base_low));
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(base_high));
     uint32_t it = 0;            // chunks of the parts before
@@ -425,7 +450,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
         uint32_t hi[4], lo[4] = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float f = e % 2 ? 0.0625f : 1.f;   // the codes at bits 4-7 stand for 16 times the others
+          const float f = e % 2 && !kCentred ? 0.0625f : 1.f;   // codes at bits 4-7 stand for 16 times the others
           if constexpr (TYPE == kKv4F32)
             split_f16x2(v[e] * f, v[e + 4] * f, hi[e], lo[e]);
           else
@@ -435,9 +460,9 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
         const int at = (row / 8 * kQPlanes * kBlocks + d8 / 4) * 32 + 4 * column + d8 % 4;
         qfrag[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         if constexpr (kPair || kQPlanes == 2) qfrag[at + (kPair ? 4 : kBlocks * 32)] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if (d8 % 8 == 0) sm.qsum[row][d8 / 8] = sum * (1.f / 16777216.f);
+        if (d8 % 8 == 0) sm.qsum[row][d8 / 8] = sum * kCode;
         if (d8 == 0) {
-          sm.qfac[row] = fmaxf(fabsf(a.scale) * kLog2e * (16777216.f / fabsf(up)), 1.1754944e-38f);   // 2^24: the codes' unit
+          sm.qfac[row] = fmaxf(fabsf(a.scale) * kLog2e * (1.f / kCode / fabsf(up)), 1.1754944e-38f);
           sm.qpos[row] = live ? position(i) : -1;
         }
       }
@@ -520,7 +545,11 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
 #pragma unroll
               for (int st = 0; st < 2; ++st) {
                 const uint32_t w0 = st ? w[0][b] >> 8 : w[0][b], w1 = st ? w[1][b] >> 8 : w[1][b];
-                const uint32_t ka[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+                uint32_t ka[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+                if constexpr (kCentred) {
+                  ka[0] = codes_low(w0, base_low), ka[1] = codes_low(w1, base_low);
+                  ka[2] = codes_high(w0, base_high), ka[3] = codes_high(w1, base_high);
+                }
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                   if (blk % 2 == 0 && st == 0)
@@ -537,7 +566,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
           for (int G = 0; G < kGroups; ++G) {
             const uint32_t w0 = kpar[G * kKv4Page + 16 * u + g], w1 = kpar[G * kKv4Page + 16 * u + 8 + g];
             const float s0 = __uint_as_float(w0 & 0xffff0000u), s1 = __uint_as_float(w1 & 0xffff0000u);
-            const float z0 = fmaf(-8.f, s0, __uint_as_float(w0 << 16)), z1 = fmaf(-8.f, s1, __uint_as_float(w1 << 16));
+            constexpr float kLess = kCentred ? 0.f : -8.f;
+            const float z0 = fmaf(kLess, s0, __uint_as_float(w0 << 16)), z1 = fmaf(kLess, s1, __uint_as_float(w1 << 16));
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -690,8 +720,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
 #pragma unroll
               for (int st = 0; st < 2; ++st) {
                 const uint32_t w0 = st ? word[2 * m] >> 8 : word[2 * m], w1 = st ? word[2 * m + 1] >> 8 : word[2 * m + 1];
-                const uint32_t va[4] = {v_codes_low(w0, base_low), v_codes_low(w1, base_low), v_codes_high(w0, base_high),
-                                        v_codes_high(w1, base_high)};
+                const uint32_t va[4] = {codes_low(w0, base_low), codes_low(w1, base_low), codes_high(w0, base_high),
+                                        codes_high(w1, base_high)};
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                   float(&to)[4] = kDirect ? o[j][c][m] : d[j][m];
@@ -805,101 +835,54 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
   pdl_launch_next();
 }
 
-// The splits (sequence, row block, KV head) that a CTA's share ended in: the last part of that CTA and the first parts
-// of the CTAs after it, joined by their maxima. A set of D / 4 threads takes 4 dims each of a part's row. With few rows
-// (the parts' latency counts) a block's sets share a row and take every kSets-th part, else a set has a row of its own.
-constexpr int kCombineThreads = 256, kCombineBlocksPerSm = 4, kMostSms = 256;
+// Row blockIdx.x % ROWS of the split (sequence, row block, KV head), if any, that CTA blockIdx.x / ROWS's share ended
+// in: the last part of that CTA and the first parts of the CTAs after it, joined by their maxima. D / 4 threads take 4
+// dims each of every kSets-th part; the sets' results are joined in their order.
+constexpr int kCombineThreads = 256;
 
-template <int D>
+template <int D, int ROWS>
 __global__ void __launch_bounds__(kCombineThreads)
-    kv4_combine_kernel(const Kv4Attn a, const int block_rows, const int ctas, const float* part, const Kv4Split* splits) {
+    kv4_combine_kernel(const Kv4Attn a, const float* part, const Kv4Split* splits) {
   constexpr int kQuads = D / 4, kSets = kCombineThreads / kQuads;   // 4, 8 or 16 sets of threads
-  __shared__ Kv4Split found[kMostSms];
-  __shared__ short cta[kMostSms];
-  __shared__ int before[kMostSms / 32 + 1];
   __shared__ __align__(16) float acc[kSets][D];
   __shared__ float sm_m[kSets], sm_l[kSets];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
-  // the CTAs with a split, in order
-  Kv4Split mine;
-  mine.last = -1;
-  if (threadIdx.x < ctas) mine = splits[threadIdx.x];
-  const uint32_t has = __ballot_sync(0xffffffffu, mine.last >= 0);
-  if (lane == 0) before[warp + 1] = __popc(has);
-  if (threadIdx.x == 0) before[0] = 0;
-  __syncthreads();
-  int n = 0, count = 0;
-  for (int v = 1; v <= kMostSms / 32; ++v) {
-    if (v <= warp) n += before[v];
-    count += before[v];
-  }
-  if (mine.last >= 0) {
-    n += __popc(has & ((1u << lane) - 1));
-    found[n] = mine;
-    cta[n] = (short)threadIdx.x;
-  }
-  __syncthreads();
-  const uint32_t group = a.group;
-  const int rows = count * block_rows, set = threadIdx.x / kQuads, d0 = 4 * (threadIdx.x % kQuads);
-  const bool together = rows <= (int)gridDim.x;   // a block per row
-  const int step = together ? 1 : kSets;
-  for (int r0 = blockIdx.x * step; r0 < rows; r0 += gridDim.x * step) {
-    const int r = together ? r0 : r0 + set;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    float M = -INFINITY, l = 0.f;
-    int64_t to = -1;
-    if (r < rows) {
-      const Kv4Split sp = found[r / block_rows];
-      const int first = cta[r / block_rows], row = r % block_rows;
-      const uint32_t rr = (uint32_t)sp.b * block_rows + row;
-      if (rr < (uint32_t)sp.n * group) {
-        const uint32_t i = rr / group;
-        to = (((int64_t)sp.row0 + i) * a.heads + sp.h * group + (rr - i * group)) * D + d0;
-        const int parts = sp.last - first + 1;
+  const int first = blockIdx.x / ROWS, row = blockIdx.x % ROWS;
+  const Kv4Split sp = splits[first];
+  const uint32_t group = a.group, rr = (uint32_t)sp.b * ROWS + row;
+  if (sp.last < 0 || rr >= (uint32_t)sp.n * group) return;
+  const int set = threadIdx.x / kQuads, d0 = 4 * (threadIdx.x % kQuads), parts = sp.last - first + 1;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  float M = -INFINITY, l = 0.f;
+  auto join = [&](float m, float add_l, const float4& u) {
+    const float top = fmaxf(M, m);
+    const float old = M == top ? 1.f : ex2_approx(M - top), add = m == top ? 1.f : ex2_approx(m - top);
+    M = top;
+    l = fmaf(add, add_l, l * old);
+    y.x = fmaf(add, u.x, y.x * old);
+    y.y = fmaf(add, u.y, y.y * old);
+    y.z = fmaf(add, u.z, y.z * old);
+    y.w = fmaf(add, u.w, y.w * old);
+  };
 #pragma unroll 4
-        for (int k = together ? set : 0; k < parts; k += together ? kSets : 1) {
-          const float* from = part + ((int64_t)(2 * (first + k) + (k == 0 ? 1 : 0)) * block_rows + row) * part_row(D);
-          const float2 ml = *reinterpret_cast<const float2*>(from);
-          const float4 u = *reinterpret_cast<const float4*>(from + 4 + d0);
-          const float top = fmaxf(M, ml.x);
-          const float old = M == top ? 1.f : ex2_approx(M - top), add = ml.x == top ? 1.f : ex2_approx(ml.x - top);
-          M = top;
-          l = fmaf(add, ml.y, l * old);
-          y.x = fmaf(add, u.x, y.x * old);
-          y.y = fmaf(add, u.y, y.y * old);
-          y.z = fmaf(add, u.z, y.z * old);
-          y.w = fmaf(add, u.w, y.w * old);
-        }
-      }
-    }
-    if (together) {
-      __syncthreads();
-      *reinterpret_cast<float4*>(&acc[set][d0]) = y;
-      if (d0 == 0) {
-        sm_m[set] = M;
-        sm_l[set] = l;
-      }
-      __syncthreads();
-      if (set != 0) continue;
-      float top = M;
-      for (int v = 1; v < kSets; ++v) top = fmaxf(top, sm_m[v]);
-      y = make_float4(0.f, 0.f, 0.f, 0.f);
-      l = 0.f;
-      for (int v = 0; v < kSets; ++v) {
-        const float wt = sm_m[v] == top ? 1.f : ex2_approx(sm_m[v] - top);
-        const float4 u = *reinterpret_cast<const float4*>(&acc[v][d0]);
-        l = fmaf(wt, sm_l[v], l);
-        y.x = fmaf(wt, u.x, y.x);
-        y.y = fmaf(wt, u.y, y.y);
-        y.z = fmaf(wt, u.z, y.z);
-        y.w = fmaf(wt, u.w, y.w);
-      }
-    }
-    if (to < 0) continue;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    store_out4(a.out, to, a.dtype, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+  for (int k = set; k < parts; k += kSets) {
+    const float* from = part + ((int64_t)(2 * (first + k) + (k == 0 ? 1 : 0)) * ROWS + row) * part_row(D);
+    const float2 ml = *reinterpret_cast<const float2*>(from);
+    join(ml.x, ml.y, *reinterpret_cast<const float4*>(from + 4 + d0));
   }
+  *reinterpret_cast<float4*>(&acc[set][d0]) = y;
+  if (d0 == 0) {
+    sm_m[set] = M;
+    sm_l[set] = l;
+  }
+  __syncthreads();
+  if (set != 0) return;
+#pragma unroll
+  for (int v = 1; v < kSets; ++v) join(sm_m[v], sm_l[v], *reinterpret_cast<const float4*>(&acc[v][d0]));
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const uint32_t i = rr / group;
+  store_out4(a.out, (((int64_t)sp.row0 + i) * a.heads + sp.h * group + (rr - i * group)) * D + d0, a.dtype,
+             make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
 }
 
 // Rows of a row block: as many as a sequence has, 4, 8 or 16 (head dim 256 has no registers for 16).
@@ -918,7 +901,7 @@ void launch(const Kv4Attn& a, int sms, cudaStream_t s) {
   kv4_attention_kernel<D, ROWS, TYPE><<<sms, Kv4Shape<D, ROWS>::kThreads, smem, s>>>(a, part, splits);
   XTG_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sms * kCombineBlocksPerSm);
+  cfg.gridDim = dim3(sms * ROWS);
   cfg.blockDim = dim3(kCombineThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -926,7 +909,7 @@ void launch(const Kv4Attn& a, int sms, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  XTG_CUDA(cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D>, a, ROWS, sms, (const float*)part, (const Kv4Split*)splits));
+  XTG_CUDA(cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D, ROWS>, a, (const float*)part, (const Kv4Split*)splits));
 }
 
 template <int D, int ROWS>
@@ -957,7 +940,6 @@ int64_t kv4_workspace_bytes(int head_dim, int group, int rows_per_seq, int sms) 
 }
 
 void launch_kv4_attention(const Kv4Attn& a, int sms, cudaStream_t s) {
-  XTG_REQUIRE(sms <= kMostSms, "kv4: more SMs than the combine lists");
   const int rows = block_rows(a.w.head_dim, a.group, a.rows_per_seq);
   if (a.w.head_dim == 256)
     launch_rows<256>(a, rows, sms, s);
