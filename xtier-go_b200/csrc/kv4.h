@@ -63,6 +63,7 @@ struct Kv4Attn {
   float scale;
   int rows_per_seq;   // about how many rows a sequence has: chooses the tiling, not the result
   float* part;        // workspace, kv4_workspace_bytes
+  int part_cost;      // set at the launch
 };
 
 void launch_kv4_store(const Kv4Where& w, const Kv4Rows& r, cudaStream_t s);

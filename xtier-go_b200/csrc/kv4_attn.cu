@@ -43,15 +43,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 6.f;   // how far, in powers of two, a row's probabilities may pass 1 before its sums are scaled
 constexpr int kUnit = 32;                        // positions a warp takes at once: half a chunk
 constexpr int kUnits = kKv4Page / kUnit, kSteps = kUnit / 16;
-// What the start of another part costs a CTA (its rows, its sums), in chunks: counted as items before the part's first,
-// so that a CTA with several parts gets fewer chunks, and few sequences' parts go to CTAs of their own.
-constexpr int kPartCost = 8;
-
 // Consumer warps and registers: a warpgroup of producers beside them, from which setmaxnreg moves registers to the
 // consumers; the sum of both shares must not pass what the CTA started with (threads x kStart).
 template <int D, int ROWS>
 struct Kv4Shape {
   static constexpr int kWarps = ROWS <= 8 && D <= 128 ? 12 : 8;
+  static constexpr bool kQShared = ROWS == 16;   // the rows' operands stay in shared memory
   static constexpr int kThreads = 32 * (kWarps + 4);
   static constexpr int kStart = 65536 / kThreads / 8 * 8;
   static constexpr int kProducerRegs = 40;
@@ -62,7 +59,7 @@ struct Kv4Shape {
   // The ring: 110 to 166 KB. A stage's chunks are always brought by the same producer and its halves taken by the same
   // consumer warps. A wait tells the phases of a barrier apart by their parity only, so it must not start while the
   // phase before is open: a warp that waits for a stage's next chunk has itself seen the last one arrive.
-  static constexpr int kStages = D == 256 ? 8 : D == 128 ? (kWarps == 12 ? 18 : 16) : 24;
+  static constexpr int kStages = D == 256 ? 8 : D == 128 ? (ROWS == 16 ? 12 : 18) : 24;
   static constexpr int kProducers = kStages % 4 ? 3 : 4;
   static_assert(kUnits * kStages % kWarps == 0 && kStages % kProducers == 0, "a stage with several owners");
   static constexpr int kMergeStride = D + 4;   // floats of a row's accumulator being merged
@@ -74,6 +71,7 @@ struct Kv4Smem {
   uint8_t stage[Shape::kStages][Shape::kBlock];
   // a part's start: the rows' operands [8-row tile][plane][32-dim block][lane], its end: the warps' accumulators
   float acc[Shape::kWarps][ROWS][Shape::kMergeStride];
+  uint4 q[Shape::kQShared ? 2 * 2 * (D / 32) * 32 : 1];
   float qsum[ROWS][D / kKv4Group], qfac[ROWS];   // what belongs to a row's scores
   int qpos[ROWS];
   float m[Shape::kWarps][ROWS], l[Shape::kWarps][ROWS];
@@ -103,10 +101,10 @@ __device__ __forceinline__ uint64_t divide(uint64_t a, uint32_t b) {
 }
 
 __device__ __forceinline__ uint64_t item_count(const Kv4Attn& a, const Part& p) {
-  return (uint64_t)p.blocks * (uint32_t)a.w.kv_heads * (uint32_t)(p.cnt + kPartCost);
+  return (uint64_t)p.blocks * (uint32_t)a.w.kv_heads * (uint32_t)(p.cnt + a.part_cost);
 }
 
-// The items of sequence s: KV heads x row blocks x (kPartCost + chunks). Sequences with rows have at least one chunk (it may hold
+// The items of sequence s: KV heads x row blocks x (part_cost + chunks). Sequences with rows have at least one chunk (it may hold
 // nothing), so that every row is written.
 template <int ROWS>
 __device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, Part& p) {
@@ -145,11 +143,11 @@ __device__ __forceinline__ bool kv4_next(const Kv4Attn& a, Walk& k, Part& p) {
       ++k.s;
       continue;
     }
-    const uint64_t seg = divide(k.off, p.cnt + kPartCost);
-    const int at = (int)(k.off - seg * (uint32_t)(p.cnt + kPartCost));
-    const int skip = max(kPartCost - at, 0);
+    const uint64_t seg = divide(k.off, p.cnt + a.part_cost);
+    const int at = (int)(k.off - seg * (uint32_t)(p.cnt + a.part_cost));
+    const int skip = max(a.part_cost - at, 0);
     if (skip >= k.left) break;
-    p.c0 = at + skip - kPartCost;
+    p.c0 = at + skip - a.part_cost;
     p.h = (int)divide(seg, p.blocks);
     p.b = (int)(seg - (uint64_t)p.h * p.blocks);
     k.left -= skip;
@@ -279,6 +277,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     kv4_attention_kernel(const Kv4Attn a, float* part, Kv4Split* splits) {
   using Shape = Kv4Shape<D, ROWS>;
   constexpr int kStages = Shape::kStages, kWarps = Shape::kWarps, kThreads = Shape::kThreads;
+  constexpr bool kQShared = Shape::kQShared;
   constexpr int kGroups = D / kKv4Group, kBlocks = D / 32, H = D < 128 ? D : 128;
   // 8-row tiles; with 4 rows a tile's columns are the two planes of a row (kPair), and a lane has one row of scores, not 2
   constexpr int RT = ROWS == 16 ? 2 : 1, kE = ROWS == 4 ? 1 : 2;
@@ -422,7 +421,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // ---- Q as the first product's operand for every row of the block, by all consumer warps: a thread takes 8
       // neighbouring dims, the word of K codes that lane 4 g + (dims / 8) % 4 multiplies: nibble pair i (dims i, i + 4)
       // is a register of step i / 2 ----
-      uint4* qfrag = reinterpret_cast<uint4*>(sm.acc);
+      uint4* qfrag = kQShared ? sm.q : reinterpret_cast<uint4*>(sm.acc);
       constexpr int kPieces = D / 8;   // threads per row
       for (int x = threadIdx.x; x < ROWS * kPieces; x += 32 * kWarps) {   // whole warps: ROWS x D / 8 >= 32
         const int row = x / kPieces, d8 = x % kPieces;
@@ -468,18 +467,17 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       }
       named_bar_sync(1, 32 * kWarps);
       // the operands of column g, and what belongs to the rows of this lane's scores: 8 j + 2 tq + {0, 1}, or tq
-      uint32_t qb[RT][kBlocks][2][kQPlanes][2];
+      uint4 qb[kQShared ? 1 : RT][kQPlanes][kQShared ? 1 : kBlocks];
+      auto q_of = [&](int j, int pl, int b) { return qfrag[((j * kQPlanes + pl) * kBlocks + b) * 32 + lane]; };
       float qsum[RT][kE][kGroups], rf[RT][kE];   // (sum q)_G and the factor from the products' unit to base-2 scores
       int t[RT][kE];                             // the row's position; dead rows see nothing
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
+        if constexpr (!kQShared)
 #pragma unroll
-        for (int pl = 0; pl < kQPlanes; ++pl)
+          for (int pl = 0; pl < kQPlanes; ++pl)
 #pragma unroll
-          for (int b = 0; b < kBlocks; ++b) {
-            const uint4 v = qfrag[((j * kQPlanes + pl) * kBlocks + b) * 32 + lane];
-            qb[j][b][0][pl][0] = v.x, qb[j][b][0][pl][1] = v.y, qb[j][b][1][pl][0] = v.z, qb[j][b][1][pl][1] = v.w;
-          }
+            for (int b = 0; b < kBlocks; ++b) qb[j][pl][b] = q_of(j, pl, b);
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
           const int row = 8 * j + kE * tq + e;
@@ -489,7 +487,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
           for (int G = 0; G < kGroups; ++G) qsum[j][e][G] = sm.qsum[row][G];
         }
       }
-      named_bar_sync(1, 32 * kWarps);   // before the accumulators take the operands' place
+      if (!kQShared) named_bar_sync(1, 32 * kWarps);   // before the accumulators take the operands' place
 
       // dims 32 c + 16 m + g (+ 8: the last two) of columns 2 tq + {0, 1}, without the offsets' part
       float o[RT][kBlocks][2][4];
@@ -542,6 +540,16 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
 #pragma unroll
             for (int b = 0; b < H / 32; ++b) {
               const int blk = hf * (H / 32) + b, G = blk / 2;
+              uint4 q[RT][kQPlanes];
+#pragma unroll
+              for (int j = 0; j < RT; ++j)
+#pragma unroll
+                for (int pl = 0; pl < kQPlanes; ++pl) {
+                  if constexpr (kQShared)
+                    q[j][pl] = q_of(j, pl, blk);
+                  else
+                    q[j][pl] = qb[j][pl][blk];
+                }
 #pragma unroll
               for (int st = 0; st < 2; ++st) {
                 const uint32_t w0 = st ? w[0][b] >> 8 : w[0][b], w1 = st ? w[1][b] >> 8 : w[1][b];
@@ -552,12 +560,14 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
                 }
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
-                  if (blk % 2 == 0 && st == 0)
-                    mma_f16_new(c[j][G], ka, qb[j][blk][st][0][0], qb[j][blk][st][0][1]);
-                  else
-                    mma_f16_add(c[j][G], ka, qb[j][blk][st][0][0], qb[j][blk][st][0][1]);
-                  if constexpr (kQPlanes == 2)
-                    mma_f16_add(c[j][G], ka, qb[j][blk][st][kQPlanes - 1][0], qb[j][blk][st][kQPlanes - 1][1]);
+#pragma unroll
+                  for (int pl = 0; pl < kQPlanes; ++pl) {
+                    const uint32_t b0 = st ? q[j][pl].z : q[j][pl].x, b1 = st ? q[j][pl].w : q[j][pl].y;
+                    if (blk % 2 == 0 && st == 0 && pl == 0)
+                      mma_f16_new(c[j][G], ka, b0, b1);
+                    else
+                      mma_f16_add(c[j][G], ka, b0, b1);
+                  }
                 }
               }
             }
@@ -939,8 +949,14 @@ int64_t kv4_workspace_bytes(int head_dim, int group, int rows_per_seq, int sms) 
                          (int64_t)sizeof(Kv4Split));
 }
 
-void launch_kv4_attention(const Kv4Attn& a, int sms, cudaStream_t s) {
+void launch_kv4_attention(const Kv4Attn& args, int sms, cudaStream_t s) {
+  Kv4Attn a = args;
   const int rows = block_rows(a.w.head_dim, a.group, a.rows_per_seq);
+  // What the start of another part costs a CTA (its rows, its sums), in chunks: counted as items before the part's first,
+  // so that a CTA with several parts gets fewer chunks, and few sequences' parts go to CTAs of their own. Measured at 4,
+  // 8, 12, 16: 1 x 131072 (4 rows, head dim 128) 29.6, 28.7, 27.9, 27.9 us; 64 rows x 8192 50.9, 50.4, 51.3, 52.4 us;
+  // 16 x 8191 at head dim 256 35.7, 35.0, 35.9, 36.4 us.
+  a.part_cost = rows == 4 && a.w.head_dim <= 128 ? 12 : 8;
   if (a.w.head_dim == 256)
     launch_rows<256>(a, rows, sms, s);
   else if (a.w.head_dim == 128)
