@@ -48,7 +48,6 @@ constexpr int kUnits = kKv4Page / kUnit, kSteps = kUnit / 16;
 template <int D, int ROWS>
 struct Kv4Shape {
   static constexpr int kWarps = ROWS <= 8 && D <= 128 ? 12 : 8;
-  static constexpr bool kQShared = ROWS == 16;   // the rows' operands stay in shared memory
   static constexpr int kThreads = 32 * (kWarps + 4);
   static constexpr int kStart = 65536 / kThreads / 8 * 8;
   static constexpr int kProducerRegs = 40;
@@ -69,9 +68,10 @@ template <int D, int ROWS>
 struct Kv4Smem {
   using Shape = Kv4Shape<D, ROWS>;
   uint8_t stage[Shape::kStages][Shape::kBlock];
-  // a part's start: the rows' operands [8-row tile][plane][32-dim block][lane], its end: the warps' accumulators
-  float acc[Shape::kWarps][ROWS][Shape::kMergeStride];
-  uint4 q[Shape::kQShared ? 2 * 2 * (D / 32) * 32 : 1];
+  float acc[Shape::kWarps][ROWS][Shape::kMergeStride];   // a part's end: the warps' accumulators
+  // the part's rows as operands, [8-row tile][plane][32-dim block][lane] (held in registers they cost more in spills than
+  // their loads do here: 1 x 8 f32 rows at 32768 37.0 -> 34.5 us, 16 x 8 f32 rows of head dim 256 148 -> 130 us)
+  uint4 q[(ROWS == 16 ? 2 : 1) * 2 * (D / 32) * 32];
   float qsum[ROWS][D / kKv4Group], qfac[ROWS];   // what belongs to a row's scores
   int qpos[ROWS];
   float m[Shape::kWarps][ROWS], l[Shape::kWarps][ROWS];
@@ -277,7 +277,6 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     kv4_attention_kernel(const Kv4Attn a, float* part, Kv4Split* splits) {
   using Shape = Kv4Shape<D, ROWS>;
   constexpr int kStages = Shape::kStages, kWarps = Shape::kWarps, kThreads = Shape::kThreads;
-  constexpr bool kQShared = Shape::kQShared;
   constexpr int kGroups = D / kKv4Group, kBlocks = D / 32, H = D < 128 ? D : 128;
   // 8-row tiles; with 4 rows a tile's columns are the two planes of a row (kPair), and a lane has one row of scores, not 2
   constexpr int RT = ROWS == 16 ? 2 : 1, kE = ROWS == 4 ? 1 : 2;
@@ -421,7 +420,6 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // ---- Q as the first product's operand for every row of the block, by all consumer warps: a thread takes 8
       // neighbouring dims, the word of K codes that lane 4 g + (dims / 8) % 4 multiplies: nibble pair i (dims i, i + 4)
       // is a register of step i / 2 ----
-      uint4* qfrag = kQShared ? sm.q : reinterpret_cast<uint4*>(sm.acc);
       constexpr int kPieces = D / 8;   // threads per row
       for (int x = threadIdx.x; x < ROWS * kPieces; x += 32 * kWarps) {   // whole warps: ROWS x D / 8 >= 32
         const int row = x / kPieces, d8 = x % kPieces;
@@ -457,8 +455,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
         }
         const int column = kPair ? 2 * row : row % 8;
         const int at = (row / 8 * kQPlanes * kBlocks + d8 / 4) * 32 + 4 * column + d8 % 4;
-        qfrag[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (kPair || kQPlanes == 2) qfrag[at + (kPair ? 4 : kBlocks * 32)] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        sm.q[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (kPair || kQPlanes == 2) sm.q[at + (kPair ? 4 : kBlocks * 32)] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         if (d8 % 8 == 0) sm.qsum[row][d8 / 8] = sum * kCode;
         if (d8 == 0) {
           sm.qfac[row] = fmaxf(fabsf(a.scale) * kLog2e * (1.f / kCode / fabsf(up)), 1.1754944e-38f);
@@ -466,18 +464,11 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
         }
       }
       named_bar_sync(1, 32 * kWarps);
-      // the operands of column g, and what belongs to the rows of this lane's scores: 8 j + 2 tq + {0, 1}, or tq
-      uint4 qb[kQShared ? 1 : RT][kQPlanes][kQShared ? 1 : kBlocks];
-      auto q_of = [&](int j, int pl, int b) { return qfrag[((j * kQPlanes + pl) * kBlocks + b) * 32 + lane]; };
+      // what belongs to the rows of this lane's scores: 8 j + 2 tq + {0, 1}, or tq
       float qsum[RT][kE][kGroups], rf[RT][kE];   // (sum q)_G and the factor from the products' unit to base-2 scores
       int t[RT][kE];                             // the row's position; dead rows see nothing
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
-        if constexpr (!kQShared)
-#pragma unroll
-          for (int pl = 0; pl < kQPlanes; ++pl)
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) qb[j][pl][b] = q_of(j, pl, b);
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
           const int row = 8 * j + kE * tq + e;
@@ -487,7 +478,6 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
           for (int G = 0; G < kGroups; ++G) qsum[j][e][G] = sm.qsum[row][G];
         }
       }
-      if (!kQShared) named_bar_sync(1, 32 * kWarps);   // before the accumulators take the operands' place
 
       // dims 32 c + 16 m + g (+ 8: the last two) of columns 2 tq + {0, 1}, without the offsets' part
       float o[RT][kBlocks][2][4];
@@ -544,12 +534,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
 #pragma unroll
               for (int j = 0; j < RT; ++j)
 #pragma unroll
-                for (int pl = 0; pl < kQPlanes; ++pl) {
-                  if constexpr (kQShared)
-                    q[j][pl] = q_of(j, pl, blk);
-                  else
-                    q[j][pl] = qb[j][pl][blk];
-                }
+                for (int pl = 0; pl < kQPlanes; ++pl) q[j][pl] = sm.q[((j * kQPlanes + pl) * kBlocks + blk) * 32 + lane];
 #pragma unroll
               for (int st = 0; st < 2; ++st) {
                 const uint32_t w0 = st ? w[0][b] >> 8 : w[0][b], w1 = st ? w[1][b] >> 8 : w[1][b];
@@ -795,6 +780,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
               sm.acc[warp][row][32 * c + 16 * m + 8 + g] = fmaf(kPair ? y[2] + y[3] : y[e + 2], up, oz[j][e][c / 2]);
             }
         }
+      // the next part's rows may now be staged; its accumulators are written after the barrier that follows them
       named_bar_sync(1, 32 * kWarps);
       const bool whole = p.c0 == 0 && p.take == p.cnt;
       float* mine = part + (int64_t)(2 * blockIdx.x + (p.c0 == 0 ? 1 : 0)) * ROWS * part_row(D);
@@ -838,7 +824,6 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
         splits[blockIdx.x] = {p.row0, p.n, p.h, p.b,
                               (int)(end < longer ? divide(end, most + 1) : extra + divide(end - longer, most))};
       }
-      named_bar_sync(1, 32 * kWarps);   // before the next part's sums
     }
     if (threadIdx.x == 0 && !split_after) splits[blockIdx.x].last = -1;
   }
