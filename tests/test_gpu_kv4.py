@@ -185,6 +185,17 @@ def test_attention(cuda, xtg, torch, rows, pos, heads, kvh, d, dtype, window):
     xtg.kv4_check(s.err)
 
 
+@pytest.mark.parametrize("window", [0, 1, 3, 70, 2 ** 31 - 1])
+def test_rows_before_the_first_position(cuda, xtg, torch, window):
+    """Rows at negative positions, some beside rows that see something in the same block, with windows of every size."""
+    rows, pos = [9, 3, 70, 2], [-4, -3, -6, -2 ** 31]
+    s = Setup(torch, xtg, 16, rows, pos, 2, 128, max_pages=2)
+    s.fill([5, 0, 64, 0])
+    out = s.check_attention(8, "f32", window)
+    assert not out[:4].any() and not out[9:12].any() and not out[12:18].any() and out[4:9].any()
+    xtg.kv4_check(s.err)
+
+
 def test_attention_over_more_sequences_than_threads(cuda, xtg, torch):
     rows = [1 + i % 3 if i % 7 else 0 for i in range(700)]
     pos = [(37 * i) % 150 for i in range(700)]

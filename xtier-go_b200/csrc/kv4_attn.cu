@@ -414,8 +414,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       const uint32_t qrows = (uint32_t)p.n * group, r0 = (uint32_t)p.b * ROWS;
       // the position of the sequence's row i (past 2^31 - 1 the table holds nothing more to see)
       auto position = [&](uint32_t i) { return (int)min((int64_t)p.pos + i, (int64_t)0x7fffffff); };
-      // the block's first and last position
-      const int tmin = position(r0 / group), tmax = position((min(r0 + ROWS, qrows) - 1) / group);
+      // the block's first position (below 0 nothing is seen) and last
+      const int tmin = max(position(r0 / group), -1), tmax = position((min(r0 + ROWS, qrows) - 1) / group);
 
       // ---- Q as the first product's operand for every row of the block, by all consumer warps: a thread takes 8
       // neighbouring dims, the word of K codes that lane 4 g + (dims / 8) % 4 multiplies: nibble pair i (dims i, i + 4)
@@ -741,16 +741,27 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       };
 
       // ---- this warp's half chunks of the part: every kWarps-th of the CTA's ----
-      for (int x = (int)((warp + kWarps - kUnits * it % kWarps) % kWarps); x < kUnits * p.take; x += kWarps) {
-        const uint32_t k = it + x / kUnits;
-        const int st = (int)(k % kStages), hh = x % kUnits;
-        const bool ok = kv4_wait(&sm.full[st], (k / kStages) & 1, &sm.failed, a.w.err);
-        const int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x;
-        const bool seen =
-            ok && sm.present[st] && p0 <= tmax && (a.window <= 0 || p0 + kUnit - 1 > tmin - a.window);
-        if (seen) unit(sm.stage[st], hh, p0, p0 + kUnit - 1 > tmin || (a.window > 0 && p0 <= tmax - a.window));
+      // Half chunk x is chunk x / kUnits, in the ring's stage and turn after `it` chunks; kWarps is a multiple of kUnits, so
+      // a warp's half of the chunks stays the same.
+      static_assert(kWarps % kUnits == 0 && kWarps / kUnits <= kStages, "the ring goes round once between a warp's chunks at most");
+      int x = (int)((warp + kWarps - kUnits * it % kWarps) % kWarps);
+      const int hh = x % kUnits;
+      const uint32_t k0 = it + x / kUnits;
+      uint32_t st = k0 % kStages, turn = k0 / kStages;
+      // units from seen_from + 1 to tmax hold a position that some row sees, those from full_from + 1 to full_to only such
+      // that every row sees
+      const int seen_from = a.window > 0 ? tmin - a.window - (kUnit - 1) : -kUnit;
+      const int full_from = a.window > 0 ? tmax - a.window : -kUnit, full_to = tmin - (kUnit - 1);
+      for (int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x; x < kUnits * p.take; x += kWarps, p0 += kUnit * kWarps) {
+        const bool ok = kv4_wait(&sm.full[st], turn & 1, &sm.failed, a.w.err);
+        if (ok && sm.present[st] && p0 <= tmax && p0 > seen_from) unit(sm.stage[st], hh, p0, p0 > full_to || p0 <= full_from);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[st]);
+        st += kWarps / kUnits;
+        if (st >= kStages) {
+          st -= kStages;
+          ++turn;
+        }
       }
       it += p.take;
 
@@ -941,6 +952,7 @@ void launch_kv4_attention(const Kv4Attn& args, int sms, cudaStream_t s) {
   // so that a CTA with several parts gets fewer chunks, and few sequences' parts go to CTAs of their own. Measured at 4,
   // 8, 12, 16: 1 x 131072 (4 rows, head dim 128) 29.6, 28.7, 27.9, 27.9 us; 64 rows x 8192 50.9, 50.4, 51.3, 52.4 us;
   // 16 x 8191 at head dim 256 35.7, 35.0, 35.9, 36.4 us.
+  a.window = std::min(a.window, 0x7fffffff - 63);   // all positions, and no overflow of -1 - window - 31
   a.part_cost = rows == 4 && a.w.head_dim <= 128 ? 12 : 8;
   if (a.w.head_dim == 256)
     launch_rows<256>(a, rows, sms, s);
