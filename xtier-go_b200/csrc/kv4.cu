@@ -11,10 +11,10 @@
 // which share the rows' DRAM pages. The page is the unit because neighbouring positions share the bytes of V: a CTA that
 // owns the page merges all the call's rows into it without atomics, whatever their number.
 //
-// Measured (B200; bytes moved / time against a copy's 6545 GB/s): 64 x 4096 rows of 6 x 128 read back as bf16 in 116 us,
-// 5.8 TB/s, 89 %. 8 x 4096 rows of 4 x 256 f16 written and read back in 72 us, 4.8 TB/s, 73 %: the store is bound by its
-// instructions (issue slots 75 % busy; about 10 per value, 4 of them the quantiser's), which a thread's 16 values share
-// (8 values a thread: 75 us).
+// Measured (B200; algorithmic bytes / time against a copy's 6545 GB/s): 64 x 4096 rows of 6 x 128 read back as bf16 in
+// 113 us, 6.0 TB/s, 92 %. 8 x 4096 rows of 4 x 256 f16 written and read back in 72 us, 4.8 TB/s, 73 %: the store is bound
+// by its instructions (issue slots 75 % busy), which a thread's 16 values share (8 values a thread: 75 us). Small calls
+// are a chain of dependent loads (row offsets and position, page table, rows): 2.7 us for one row.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -176,33 +176,28 @@ __device__ __forceinline__ void transpose_nibbles(uint32_t (&w)[8]) {
 // start at cu_rows[s] / 64 + 2 s for sequence s: found without a prefix sum over the sequences' positions.
 struct Task {
   int64_t row0;   // the call's row at the page's first touched slot
+  int64_t page;   // -1: nothing there
   int slot0, count;
-  int64_t page;
 };
 
-__device__ __forceinline__ bool find_task(const Kv4Where& w, int* shared_seq, Task& t) {
+// The thread that finds the task's sequence works the rest out (its position is loaded with the search: these loads one
+// after another are most of a small call's time). False: nothing to do.
+__device__ __forceinline__ bool find_task(const Kv4Where& w, Task& shared, Task& t) {
   const int64_t task = blockIdx.x / (uint32_t)w.kv_heads;
-  if (threadIdx.x == 0) *shared_seq = -1;
+  if (threadIdx.x == 0) shared.count = 0;
   __syncthreads();
   for (int s = threadIdx.x; s < w.seqs; s += kThreads) {
-    const int64_t lo = kv4_row_bound(w, s) / kKv4Page + 2 * (int64_t)s;
-    const int64_t hi = kv4_row_bound(w, s + 1) / kKv4Page + 2 * (int64_t)(s + 1);
-    if (lo <= task && task < hi) *shared_seq = s;
+    const int64_t a = kv4_row_bound(w, s), b = kv4_row_bound(w, s + 1), pos = w.pos[s];
+    const int64_t from = task - (a / kKv4Page + 2 * (int64_t)s);
+    if (from < 0 || task >= b / kKv4Page + 2 * (int64_t)(s + 1)) continue;
+    const int64_t index = (pos >> 6) + from;   // floor: positions may be negative
+    const int64_t p = index * kKv4Page;        // the page's first position
+    const int64_t i0 = p > pos ? p - pos : 0, i1 = p + kKv4Page - pos < b - a ? p + kKv4Page - pos : b - a;
+    if (i0 < i1) shared = {a + i0, kv4_page(w, s, index), (int)(pos + i0 - p), (int)(i1 - i0)};
   }
   __syncthreads();
-  const int s = *shared_seq;
-  if (s < 0) return false;
-  const int64_t a = kv4_row_bound(w, s), n = kv4_row_bound(w, s + 1) - a;
-  const int64_t pos = w.pos[s];
-  const int64_t index = (pos >> 6) + task - (a / kKv4Page + 2 * (int64_t)s);   // floor: positions may be negative
-  const int64_t p = index * kKv4Page;                                          // the page's first position
-  const int64_t i0 = p > pos ? p - pos : 0, i1 = p + kKv4Page - pos < n ? p + kKv4Page - pos : n;
-  if (i0 >= i1) return false;
-  t.row0 = a + i0;
-  t.slot0 = (int)(pos + i0 - p);
-  t.count = (int)(i1 - i0);
-  t.page = kv4_page(w, s, index);
-  return true;
+  t = shared;
+  return t.count > 0;
 }
 
 // Quantises the 16 values that this lane has of a group: their codes as nibbles, the group's parameters.
@@ -241,15 +236,32 @@ __global__ void __launch_bounds__(kThreads) kv4_store_kernel(const Kv4Where w, c
   constexpr int H = D < 128 ? D : 128, kPerRow = D / 16, kRowsAtOnce = kThreads / kPerRow;
   constexpr int kStride = D / 8 + 4;   // of a slot's words in shared memory: 4 slots x 8 words without bank conflicts
   __shared__ __align__(8) uint32_t codes[kKv4Page * kStride];
-  __shared__ int seq;
+  __shared__ Task task;
   Task t;
-  if (!find_task(w, &seq, t) || t.page < 0) return;
+  if (!find_task(w, task, t) || t.page < 0) return;
   const int h = blockIdx.x % (uint32_t)w.kv_heads;
   uint8_t* block = w.pool + (t.page * w.kv_heads + h) * (int64_t)kv4_block_bytes(D);
   uint32_t* kcodes = reinterpret_cast<uint32_t*>(block);
   uint32_t* kpar = reinterpret_cast<uint32_t*>(block + kv4_k_params(D));
   uint32_t* vcodes = reinterpret_cast<uint32_t*>(block + kv4_v_codes(D));
   uint32_t* vpar = reinterpret_cast<uint32_t*>(block + kv4_v_params(D));
+
+  // V's words, of a head dim each and 8 slots: item i < D is 8 neighbouring dims'. The slots that this call does not write
+  // keep their codes, requested before the rows.
+  static_assert(D <= kThreads, "an item per thread");
+  const int tt = threadIdx.x & 3, a = (threadIdx.x >> 2) & 3, c = (threadIdx.x >> 4) % (D / 32), hh = threadIdx.x / (D / 2);
+  uint32_t* vto = vcodes + ((hh * (D / 32) + c) * 8 * 4 + a) * 4 + tt;
+  uint32_t mask = 0, old[8] = {};
+  if (threadIdx.x < D) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int slot = 32 * hh + 2 * a + 8 * (n % 4) + n / 4;
+      if (slot >= t.slot0 && slot < t.slot0 + t.count) mask |= 15u << (4 * n);
+    }
+    if (mask != 0 && mask != 0xffffffffu)
+#pragma unroll
+      for (int g = 0; g < 8; ++g) old[g] = vto[16 * g];
+  }
 
   // a thread has dims d0 .. d0 + 15 of every kRowsAtOnce-th row, 4 threads a group
   const int d0 = 16 * (threadIdx.x % kPerRow), first = threadIdx.x / kPerRow;
@@ -277,40 +289,23 @@ __global__ void __launch_bounds__(kThreads) kv4_store_kernel(const Kv4Where w, c
     }
   }
   __syncthreads();
-  // V's words, of a head dim each, from 8 slots' words of 8 dims. The slots that this call does not write keep their
-  // codes.
-  for (int i = threadIdx.x; i < D; i += kThreads) {
-    const int tt = i & 3, a = (i >> 2) & 3, c = (i >> 4) % (D / 32), hh = i / (D / 2);
-    uint32_t words[8], mask = 0;
+  if (mask != 0) {
+    uint32_t words[8];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const int slot = 32 * hh + 2 * a + 8 * (n % 4) + n / 4;
-      if (slot >= t.slot0 && slot < t.slot0 + t.count) mask |= 15u << (4 * n);
-      words[n] = codes[slot * kStride + 4 * c + tt];
-    }
-    if (mask == 0) continue;
+    for (int n = 0; n < 8; ++n) words[n] = codes[(32 * hh + 2 * a + 8 * (n % 4) + n / 4) * kStride + 4 * c + tt];
     transpose_nibbles(words);
-    uint32_t* to = vcodes + ((hh * (D / 32) + c) * 8 * 4 + a) * 4 + tt;
-    if (mask == 0xffffffffu) {
 #pragma unroll
-      for (int g = 0; g < 8; ++g) to[16 * g] = words[g];
-    } else {
-      uint32_t old[8];
-#pragma unroll
-      for (int g = 0; g < 8; ++g) old[g] = to[16 * g];
-#pragma unroll
-      for (int g = 0; g < 8; ++g) to[16 * g] = (old[g] & ~mask) | (words[g] & mask);
-    }
+    for (int g = 0; g < 8; ++g) vto[16 * g] = (old[g] & ~mask) | (words[g] & mask);
   }
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kThreads) kv4_load_kernel(const Kv4Where w, const Kv4Rows r) {
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 8 : 6) kv4_load_kernel(const Kv4Where w, const Kv4Rows r) {
   constexpr int H = D < 128 ? D : 128, kPerRow = D / 8;
   __shared__ __align__(16) uint32_t par[2][D / 64][kKv4Page];   // K's, V's
-  __shared__ int seq;
+  __shared__ Task task;
   Task t;
-  if (!find_task(w, &seq, t)) return;
+  if (!find_task(w, task, t)) return;
   const int h = blockIdx.x % (uint32_t)w.kv_heads;
   T* kout = static_cast<T*>(r.k) + t.row0 * r.k_row + h * r.k_head;
   T* vout = static_cast<T*>(r.v) + t.row0 * r.v_row + h * r.v_head;
