@@ -238,6 +238,24 @@ def test_attention_of_loud_values(cuda, xtg, torch, dtype):
     s.check_attention(8, dtype, scale=1e-3)
 
 
+@pytest.mark.parametrize("dtype,factor,scale", [
+    ("f32", 1.0, -0.2), ("bf16", 1.0, -0.2), ("f32", 1.0, 0.0), ("f16", 1.0, 0.0), ("f32", 1e-30, 2e29),
+    ("f32", 1e30, 2e-31), ("bf16", 1e-30, 2e29), ("f16", 1e-4, 2e3), ("f32", 0.0, 1.0),
+])
+def test_attention_of_queries_of_any_size(cuda, xtg, torch, dtype, factor, scale):
+    """Negative and zero scales, queries near the ends of their type beside a scale that undoes it, rows of zeros, and
+    rows whose values differ by a factor of 2^20 within the row."""
+    s = Setup(torch, xtg, 17, [3], [150], 2, 128)
+    s.fill([153])
+    rows = s.rows_of(8)
+    rows[1, :, ::3] *= 2.0 ** -20
+    rows[2, 3] = 0
+    q = torch.from_numpy(rows * np.float32(factor)).cuda().to(dtype_of(torch, dtype))
+    got = xtg.kv4_attention(q, s.pool, *s.where, scale=scale).double().cpu().numpy()
+    want, reach, top = s.ref.attention(q.double().cpu().numpy(), s.table, s.pos, s.cu, scale)
+    assert (np.abs(got - want) <= R.attention_bound(want, reach, top, MANTISSA[dtype])).all()
+
+
 def test_nan_stays_with_the_rows_that_see_it(cuda, xtg, torch):
     """A NaN key at position 102 and a NaN value group at 104: rows up to 101 are clean, rows to 103 all NaN from the
     key; a query with a NaN spoils its own row."""

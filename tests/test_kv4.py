@@ -104,7 +104,8 @@ def test_cache_refusals(xtg, entry, cache, needle):
     ("attention", dict(q=None), "null"), ("attention", dict(out=4096 + 8), "16-byte"),
     ("attention", dict(dtype=7), "f32"), ("attention", dict(heads=3), "multiple"), ("attention", dict(heads=0), "heads"),
     ("attention", dict(q_row=516), "strides"), ("attention", dict(window=-1), "window"),
-    ("attention", dict(rows_per_seq=0), "rows_per_seq"),
+    ("attention", dict(rows_per_seq=0), "rows_per_seq"), ("attention", dict(scale=float("nan")), "scale"),
+    ("attention", dict(scale=float("inf")), "scale"), ("attention", dict(heads=1 << 30), "2^31"),
 ])
 def test_row_refusals(xtg, entry, kw, needle):
     rc, why = call(xtg, entry, **kw)

@@ -1,6 +1,7 @@
 // Kernel-level entry points of include/xtg_cuda.h: the device forms of the reference's CPU kernels on caller-owned
 // device memory (matmul_nvfp4, attention, KvCache::store, the quantizer, the generators).
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <mutex>
@@ -450,6 +451,7 @@ int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, void* out, int 
     const Kv4Where w = kv4_where(c);
     kv4_require_heads(heads, w.kv_heads, rows_per_seq);
     XTG_REQUIRE(window >= 0, "kv4: window 0 (none) or more");
+    XTG_REQUIRE(std::isfinite(scale), "kv4: a finite scale");
     XTG_REQUIRE(w.rows * heads < (1ll << 31), "kv4: rows x heads below 2^31");
     if (w.rows == 0 || w.seqs == 0) return;
     kv4_require_rows(dtype, {q, out}, {q_row, q_head});

@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
         if constexpr (kPair || kQPlanes == 2) sm.q[at + (kPair ? 4 : kBlocks * 32)] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         if (d8 % 8 == 0) sm.qsum[row][d8 / 8] = sum * kCode;
         if (d8 == 0) {
-          sm.qfac[row] = fmaxf(fabsf(a.scale) * kLog2e * (1.f / kCode / fabsf(up)), 1.1754944e-38f);
+          sm.qfac[row] = fmaxf(fabsf(a.scale) / fabsf(up) * (kLog2e / kCode), 1.1754944e-38f);
           sm.qpos[row] = live ? position(i) : -1;
         }
       }
