@@ -293,6 +293,12 @@ def test_errors_are_recorded(cuda, xtg, torch):
     xtg.kv4_attention(k, s.pool, *s.where, scale=0.1, err=s.err)
     with pytest.raises(xtg.XtgError, match="page table"):
         xtg.kv4_check(s.err)
+    for seqs in (2, 20, 50):   # the last sequence's row past its table, whichever way the work is shared out
+        t = Setup(torch, xtg, 18, [1] * seqs, [5] * (seqs - 1) + [64], 1, 64, max_pages=1)
+        t.fill([6] * (seqs - 1) + [64])
+        t.check_attention(2, "f32")
+        with pytest.raises(xtg.XtgError, match="page table"):
+            xtg.kv4_check(t.err)
     s.table[1, 0] = len(s.ref.words)
     s.upload()
     for call in (lambda: xtg.kv4_store(s.pool, k, k, *s.where, err=s.err),

@@ -15,19 +15,28 @@
 // positions would put an error of about 2^-20 of the group's range into components far smaller than it. So are K's for
 // f32 rows, whose scores would lose about two bits to the part that cancels.
 // Precision of the f16 operands: q of 16-bit rows is exact in one plane (a power of two brings the row's largest value
-// to 2^14 .. 2^15); of f32 rows it is hi + lo, 22 bits. P s is brought below 2^15 by a power of two per chunk and
-// group (its largest scale) and always has two planes: one would put 2^-12 of the largest value into the result, which
-// a small component beside large values of other positions shows even after bf16's rounding. A chunk's product starts from zero and is added to the row's f32
-// accumulator, so the matrix unit itself sums at most 64 positions.
+// to 2^14 .. 2^15); of f32 rows it is hi + lo, 22 bits. P s is brought below 2^16 by a power of two per group (the largest
+// scale met) and always has two planes: one would put 2^-12 of the largest value into the result, which a small component
+// beside large values of other positions shows even after bf16's rounding. 16-bit rows' P V is added up in the matrix
+// unit; f32 rows' is taken from zero for every half chunk and added to an f32 accumulator, because the unit's own sum
+// loses about 2^-24 per step to truncation. A row's maximum is followed loosely (kSlack): scaling the sums at every new
+// maximum cost 10 % more instructions.
 //
-// What bounds it: the cache's bytes with few rows, the instructions around the matrix products with many. One CTA per
-// SM takes an equal share of all (sequence, row block, KV head, 64-position chunk) items in that order, whatever the
-// sequences' lengths: shares start and end inside a sequence, whose parts a second kernel joins. Producer warps
-// bring chunks (one bulk copy of a page's block of the head) into a ring of shared memory; the consumer warps take
+// One CTA per SM takes an equal share of all (sequence, KV head, row block, 64-position chunk) items in that order,
+// whatever the sequences' lengths: shares start and end inside a sequence, whose parts a second kernel joins. Producer
+// warps bring chunks (one bulk copy of a page's block of the head) into a ring of shared memory; the consumer warps take
 // half chunks (32 positions) in turn, each with a running maximum of its own, so that no warp waits for another before
-// the end of a sequence's part. A row block is 8 rows, or 16 (the codes unpacked once for both), all held by every
-// warp: more rows read the chunks again, from L2 when the row blocks of a head run at the same time, which costs less
-// than the products of 16 rows take, and larger blocks would cost more at every part's start and end.
+// the end of a sequence's part. A row block is 4, 8 or 16 rows held by every warp. 4 rows are 8 columns, the two planes
+// of P s side by side, and half the work per lane; 16 rows share the unpacked codes. More rows read the chunks again,
+// from L2 when the row blocks of a head run at the same time, which costs less than the products of 16 rows take, and
+// larger blocks would cost more at every part's start and end (64 rows over 8192 positions: blocks of 128 rows 66 us,
+// of 16 rows 52 us).
+//
+// What bounds it (B200, head dim 128, bf16): with 4 rows the cache's bytes, 64 sequences of 16384 .. 32768 positions in
+// 250 us, 5.4 TB/s, 83 % of a copy's rate (without any computation the copies take 240 us); one sequence of 131072
+// positions in 28 us, 4.0 TB/s, of which 10 us are the start, the end of the parts and the join. With 16 rows the
+// instructions around the products: 64 rows over 8192 positions in 49 us, 132 TFLOP/s, tensor pipe 36 % and issue slots
+// 54 % busy.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -104,8 +113,8 @@ __device__ __forceinline__ uint64_t item_count(const Kv4Attn& a, const Part& p) 
   return (uint64_t)p.blocks * (uint32_t)a.w.kv_heads * (uint32_t)(p.cnt + a.part_cost);
 }
 
-// The items of sequence s: KV heads x row blocks x (part_cost + chunks). Sequences with rows have at least one chunk (it may hold
-// nothing), so that every row is written.
+// The items of sequence s: KV heads x row blocks x (part_cost + chunks). Sequences with rows have at least one chunk (it
+// may hold nothing), so that every row is written.
 template <int ROWS>
 __device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, Part& p) {
   p.pos = a.w.pos[s];
@@ -116,7 +125,7 @@ __device__ __forceinline__ uint64_t kv4_items(const Kv4Attn& a, int s, Part& p) 
   const int64_t held = (int64_t)a.w.max_pages * kKv4Page;
   int64_t end = (int64_t)p.pos + p.n;
   if (end > held) {   // rows past the table see what the table holds
-    if (a.w.err && threadIdx.x == 0) atomicExch(a.w.err, 6);
+    if (a.w.err) atomicExch(a.w.err, 6);
     end = held;
   }
   const int first = a.window > 0 && p.pos >= a.window ? p.pos - a.window + 1 : 0;
@@ -301,6 +310,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     sm.start_base = 0;
   }
   // ---- this CTA's share of the items: an equal part of their sum over the sequences ----
+  // (a CTA's items fit 32 bits: 2^32 chunks would take it a quarter of an hour)
   uint64_t share = 0;
   uint32_t share_items = 0, most = 0, extra = 0;   // CTAs below `extra` have `most` + 1 items, the others `most`
   auto take_share = [&](uint64_t total) {
@@ -483,7 +493,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       float o[RT][kBlocks][2][4];
       float oz[RT][kE][kGroups];   // sum of P z over this lane's slots
       float ref[RT][kE], run_l[RT][kE];
-      int unit_e[kGroups];   // P s 2^(136 - unit_e) is below 2^15
+      int unit_e[kGroups];   // P s 2^(136 - unit_e) is below 2^16
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
 #pragma unroll
