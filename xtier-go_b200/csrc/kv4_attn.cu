@@ -383,33 +383,39 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     const int pw = warp - kWarps;
     if (pw >= kProducers) return;
     const uint64_t once = l2_evict_first();
-    uint32_t it = 0;
+    const int64_t page_bytes = (int64_t)a.w.kv_heads * Shape::kBlock;
+    int st = pw, next = pw;   // this warp's next stage, and its next chunk of the part
+    uint32_t turn = 0;
     while (kv4_next<ROWS>(a, walk, p)) {
       const uint8_t* head = a.w.pool + (int64_t)p.h * Shape::kBlock;
-      int x = (int)((pw + kProducers - it % kProducers) % kProducers);   // this warp's next chunk of the part
-      while (x < p.take) {
-        const int count = min((p.take - x + kProducers - 1) / kProducers, 32);
-        const int64_t mine = lane < count ? kv4_page(a.w, p.seq, p.lo + p.c0 + x + kProducers * lane) : -1;
-        for (int j = 0; j < count; ++j, x += kProducers) {
-          const int64_t page = __shfl_sync(0xffffffffu, mine, j);
-          const uint32_t k = it + x, st = k % kStages, turn = k / kStages;
+      while (next < p.take) {
+        const int count = min((p.take - next + kProducers - 1) / kProducers, 32);
+        const int64_t page = lane < count ? kv4_page(a.w, p.seq, p.lo + p.c0 + next + kProducers * lane) : -1;
+        const uint64_t mine = page >= 0 ? reinterpret_cast<uint64_t>(head + page * page_bytes) : 0;
+        for (int j = 0; j < count; ++j) {
+          const void* from = reinterpret_cast<const void*>(__shfl_sync(0xffffffffu, mine, j));
           if (lane == 0 && (turn == 0 || kv4_wait(&sm.empty[st], (turn - 1) & 1, &sm.failed, a.w.err))) {
-            sm.present[st] = page >= 0;
-            if (page >= 0) {
+            sm.present[st] = from != nullptr;
+            if (!from) {
+              mbar_arrive(&sm.full[st]);
+            } else {
               mbar_expect_tx(&sm.full[st], Shape::kBlock);
-              const uint8_t* from = head + page * a.w.kv_heads * (int64_t)Shape::kBlock;
               if (p.blocks == 1)   // read once: the first to leave L2
                 bulk_g2s_hint(sm.stage[st], from, Shape::kBlock, &sm.full[st], once);
               else
                 bulk_g2s(sm.stage[st], from, Shape::kBlock, &sm.full[st]);
-            } else {
-              mbar_arrive(&sm.full[st]);
             }
           }
           __syncwarp();
+          st += kProducers;
+          if (st >= kStages) {
+            st -= kStages;
+            ++turn;
+          }
         }
+        next += count * kProducers;
       }
-      it += p.take;
+      next -= p.take;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kConsumerRegs));
