@@ -32,11 +32,11 @@
 // larger blocks would cost more at every part's start and end (64 rows over 8192 positions: blocks of 128 rows 66 us,
 // of 16 rows 52 us).
 //
-// What bounds it (B200, head dim 128, bf16): with 4 rows the cache's bytes, 64 sequences of 16384 .. 32768 positions in
-// 250 us, 5.4 TB/s, 83 % of a copy's rate (without any computation the copies take 240 us); one sequence of 131072
-// positions in 28 us, 4.0 TB/s, of which 10 us are the start, the end of the parts and the join. With 16 rows the
-// instructions around the products: 64 rows over 8192 positions in 49 us, 132 TFLOP/s, tensor pipe 36 % and issue slots
-// 54 % busy.
+// What bounds it (B200, head dim 128, bf16): with 4 rows about equally the cache's bytes and the instructions, 64
+// sequences of 16384 .. 32768 positions in 250 us, 5.4 TB/s, 83 % of a copy's rate (204 us without any computation, 1190
+// instructions per chunk and head); one sequence of 131072 positions in 28 us, 4.0 TB/s, of which 10 us are the start, the
+// end of the parts and the join. With 16 rows the instructions around the products: 64 rows over 8192 positions in 49 us,
+// 131 TFLOP/s, tensor pipe 36 % and issue slots 54 % busy.
 #include <cuda_bf16.h>
 
 #include <algorithm>
