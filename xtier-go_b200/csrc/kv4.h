@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "common.cuh"
+
 namespace xtg {
 
 // ---- the cache's layout: pool [pages][kv_heads][72 D] bytes, head dim D 64, 128 or 256; every word 32 bits ----
@@ -72,6 +74,23 @@ int64_t kv4_workspace_bytes(int head_dim, int group, int rows_per_seq, int sms);
 void launch_kv4_attention(const Kv4Attn& a, int sms, cudaStream_t s);
 
 #ifdef __CUDACC__
+// A launch that may overlap the end of the kernel before it on the stream: the kernel waits (pdl_wait) before it reads or
+// writes memory. Each of these kernels lets the next one launch once its own wait is over.
+template <class... P, class... A>
+void launch_kv4(void (*f)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  XTG_CUDA(cudaLaunchKernelEx(&cfg, f, static_cast<P>(args)...));
+}
+
 // Sequence s's rows within the call's `rows` (a bad cu_rows shortens them, never reaches outside).
 __device__ __forceinline__ int64_t kv4_row_bound(const Kv4Where& w, int s) {
   const int64_t c = w.cu_rows[s];

@@ -309,6 +309,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     sm.start_seq = a.w.seqs;
     sm.start_base = 0;
   }
+  pdl_wait();   // everything the call reads may come from the kernel before
   // ---- this CTA's share of the items: an equal part of their sum over the sequences ----
   // (a CTA's items fit 32 bits: 2^32 chunks would take it a quarter of an hour)
   uint64_t share = 0;
@@ -869,6 +870,7 @@ __global__ void __launch_bounds__(kCombineThreads)
   __shared__ __align__(16) float acc[kSets][D];
   __shared__ float sm_m[kSets], sm_l[kSets];
   pdl_wait();
+  pdl_launch_next();
   const int first = blockIdx.x / ROWS, row = blockIdx.x % ROWS;
   const Kv4Split sp = splits[first];
   const uint32_t group = a.group, rr = (uint32_t)sp.b * ROWS + row;
@@ -920,18 +922,9 @@ void launch(const Kv4Attn& a, int sms, cudaStream_t s) {
   static std::atomic<uint64_t> optin;
   const int smem = (int)sizeof(Kv4Smem<D, ROWS>);
   ensure_smem_optin((const void*)kv4_attention_kernel<D, ROWS, TYPE>, smem, optin);
-  kv4_attention_kernel<D, ROWS, TYPE><<<sms, Kv4Shape<D, ROWS>::kThreads, smem, s>>>(a, part, splits);
-  XTG_CUDA(cudaGetLastError());
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sms * ROWS);
-  cfg.blockDim = dim3(kCombineThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  XTG_CUDA(cudaLaunchKernelEx(&cfg, kv4_combine_kernel<D, ROWS>, a, (const float*)part, (const Kv4Split*)splits));
+  launch_kv4(kv4_attention_kernel<D, ROWS, TYPE>, sms, Kv4Shape<D, ROWS>::kThreads, smem, s, a, part, splits);
+  launch_kv4(kv4_combine_kernel<D, ROWS>, sms * ROWS, kCombineThreads, 0, s, a, (const float*)part,
+             (const Kv4Split*)splits);
 }
 
 template <int D, int ROWS>
