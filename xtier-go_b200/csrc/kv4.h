@@ -17,8 +17,8 @@ namespace xtg {
 //   V codes   [2][D / 32][8][4][4] words: nibble n of word [h][c][g][a][t] is the code of head dim 32 c + 8 t + g at
 //             slot 32 h + 8 (n % 4) + 2 a + n / 4
 //   V params  as K's
-// A code c stands for s (c - 8) + z. The orders are the fragment orders of mma.m16n8k16's B operand: lane (g, a) of
-// the attention kernel reads its K codes of a slot and its V codes of 32 slots with 16-byte shared-memory loads, and
+// A code c stands for s (c - 8) + z. The orders are those of mma.m16n8k16's operand fragments: lane 4 g + a of the
+// attention kernel reads its K codes of a slot and its V codes of 32 slots with 16-byte shared-memory loads, and
 // the nibbles n and n + 4 of a word become the two halves of one operand register.
 constexpr int kKv4Page = 64;    // positions per page
 constexpr int kKv4Group = 64;   // head dims sharing a scale and an offset
