@@ -121,7 +121,7 @@ class Cache:
             v = np.stack([self.value(*at, 1) for _, at in held])
             p = np.array([p for p, _ in held])
             for r in range(cu[s], cu[s + 1]):
-                t = int(pos[s]) + r - cu[s]
+                t = int(pos[s]) + r - int(cu[s])
                 see = (p <= t) & ((p > t - window) if window else True)
                 if not see.any():
                     continue

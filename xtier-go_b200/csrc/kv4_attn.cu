@@ -922,6 +922,13 @@ void launch(const Kv4Attn& a, int sms, cudaStream_t s) {
   static std::atomic<uint64_t> optin;
   const int smem = (int)sizeof(Kv4Smem<D, ROWS>);
   ensure_smem_optin((const void*)kv4_attention_kernel<D, ROWS, TYPE>, smem, optin);
+  // setmaxnreg would wait forever in a kernel that starts with fewer registers than its shares were worked out for
+  static const bool enough = [] {
+    cudaFuncAttributes f;
+    XTG_CUDA(cudaFuncGetAttributes(&f, (const void*)kv4_attention_kernel<D, ROWS, TYPE>));
+    return f.numRegs >= Kv4Shape<D, ROWS>::kStart;
+  }();
+  XTG_REQUIRE(enough, "kv4: the attention kernel was compiled to fewer registers than it shares out");
   launch_kv4(kv4_attention_kernel<D, ROWS, TYPE>, sms, Kv4Shape<D, ROWS>::kThreads, smem, s, a, part, splits);
   launch_kv4(kv4_combine_kernel<D, ROWS>, sms * ROWS, kCombineThreads, 0, s, a, (const float*)part,
              (const Kv4Split*)splits);
