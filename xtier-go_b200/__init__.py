@@ -141,6 +141,8 @@ def lib():
         L.xtg_cuda_kv4_attention.argtypes = [C.POINTER(Kv4), C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int64,
                                              C.c_int64, C.c_float, C.c_int, C.c_int, C.c_void_p, C.c_int64,
                                              C.c_void_p, E, C.c_int]
+        L.xtg_cuda_kv4_wait_polls.restype = C.c_int
+        L.xtg_cuda_kv4_wait_polls.argtypes = [C.c_int]
         L.xtg_cuda_gen.restype = C.c_int
         L.xtg_cuda_gen.argtypes = [C.c_int, C.c_uint64, C.c_uint64, C.c_float, C.c_float, C.c_void_p, C.c_int64,
                                    C.c_void_p, E, C.c_int]

@@ -444,6 +444,8 @@ int64_t xtg_cuda_kv4_workspace(int heads, int kv_heads, int head_dim, int rows_p
   return bytes;
 }
 
+int xtg_cuda_kv4_wait_polls(int polls) { return kv4_wait_polls(polls); }
+
 int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, void* out, int dtype, int heads, int64_t q_row,
                            int64_t q_head, float scale, int window, int rows_per_seq, void* workspace,
                            int64_t workspace_bytes, void* stream, char* err, int err_len) {

@@ -65,12 +65,14 @@ struct Kv4Attn {
   float scale;
   int rows_per_seq;   // about how many rows a sequence has: chooses the tiling, not the result
   float* part;        // workspace, kv4_workspace_bytes
-  int part_cost;      // set at the launch
+  int part_cost;      // set at the launch, as
+  uint32_t polls;     // of a barrier before a wait gives up
 };
 
 void launch_kv4_store(const Kv4Where& w, const Kv4Rows& r, cudaStream_t s);
 void launch_kv4_load(const Kv4Where& w, const Kv4Rows& r, cudaStream_t s);
 int64_t kv4_workspace_bytes(int head_dim, int group, int rows_per_seq, int sms);
+int kv4_wait_polls(int polls);   // sets the attention's polls (below 0: leaves them); the former value
 void launch_kv4_attention(const Kv4Attn& a, int sms, cudaStream_t s);
 
 #ifdef __CUDACC__

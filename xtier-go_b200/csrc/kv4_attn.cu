@@ -40,6 +40,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "kv4.h"
@@ -89,7 +90,9 @@ struct Kv4Smem {
   uint64_t scan[Shape::kThreads / 32];
   uint64_t start_base;   // items before the sequence that the CTA's share starts in
   int start_seq;
-  int failed;            // a wait ran out: the rest of the call waits only briefly and computes nothing
+  // A wait ran out. Its warp leaves the stage as it is (a copy may be on its way there) and takes no more; the producers,
+  // who get no free stage, stop, and wait for the copies that they have issued before they end. The CTA's rows become NaN.
+  int failed;
 };
 
 // A part of a sequence's items: row block b of KV head h, chunks c0 .. c0 + take - 1 of the sequence's cnt from page lo.
@@ -259,18 +262,16 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 
 __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)biased << 23); }
 
-// mbarrier wait that gives up: after the bound, or soon once another wait of the CTA has.
-__device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, int* failed, int32_t* err) {
-  uint32_t spins = 0;
-  while (!mbar_try_wait(bar, parity)) {
-    ++spins;
-    if (spins > kMaxSpins || (spins > 4096 && *reinterpret_cast<volatile int*>(failed))) {
-      atomicExch(failed, 1);
-      if (err) atomicExch(err, 1);
-      return false;
-    }
+// mbarrier wait that gives up: after `polls` looks, or soon once another wait of the CTA has. The lanes of a warp that
+// wait together may come to different ends: a vote decides for all.
+__device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, uint32_t polls, int* failed, int32_t* err) {
+  for (uint32_t i = 0; i < polls; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (i > 4096 && *reinterpret_cast<volatile int*>(failed)) break;
   }
-  return true;
+  atomicExch(failed, 1);
+  if (err) atomicExch(err, 1);
+  return false;
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -387,15 +388,19 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     const int64_t page_bytes = (int64_t)a.w.kv_heads * Shape::kBlock;
     int st = pw, next = pw;   // this warp's next stage, and its next chunk of the part
     uint32_t turn = 0;
-    while (kv4_next<ROWS>(a, walk, p)) {
+    bool ok = true;
+    while (ok && kv4_next<ROWS>(a, walk, p)) {
       const uint8_t* head = a.w.pool + (int64_t)p.h * Shape::kBlock;
-      while (next < p.take) {
+      while (ok && next < p.take) {
         const int count = min((p.take - next + kProducers - 1) / kProducers, 32);
         const int64_t page = lane < count ? kv4_page(a.w, p.seq, p.lo + p.c0 + next + kProducers * lane) : -1;
         const uint64_t mine = page >= 0 ? reinterpret_cast<uint64_t>(head + page * page_bytes) : 0;
         for (int j = 0; j < count; ++j) {
           const void* from = reinterpret_cast<const void*>(__shfl_sync(0xffffffffu, mine, j));
-          if (lane == 0 && (turn == 0 || kv4_wait(&sm.empty[st], (turn - 1) & 1, &sm.failed, a.w.err))) {
+          if (lane == 0 && turn > 0) ok = kv4_wait(&sm.empty[st], (turn - 1) & 1, a.polls, &sm.failed, a.w.err);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) break;
+          if (lane == 0) {
             sm.present[st] = from != nullptr;
             if (!from) {
               mbar_arrive(&sm.full[st]);
@@ -407,7 +412,6 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
                 bulk_g2s(sm.stage[st], from, Shape::kBlock, &sm.full[st]);
             }
           }
-          __syncwarp();
           st += kProducers;
           if (st >= kStages) {
             st -= kStages;
@@ -418,6 +422,13 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       }
       next -= p.take;
     }
+    pdl_launch_next();
+    // no copy may outlive the CTA: the consumers have seen all of them arrive, unless a wait ran out
+    if (lane == 0)
+      for (int s = pw; s < kStages; s += kProducers) {
+        const uint32_t issued = turn + (s < st);   // into this stage
+        if (issued > 0) mbar_wait_bounded(&sm.full[s], (issued - 1) & 1, a.w.err);
+      }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kConsumerRegs));
     const uint32_t group = a.group;
@@ -762,6 +773,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // a warp's half of the chunks stays the same.
       static_assert(kWarps % kUnits == 0 && kWarps / kUnits <= kStages, "the ring goes round once between a warp's chunks at most");
       int x = (int)((warp + kWarps - kUnits * it % kWarps) % kWarps);
+      const bool given_up = __any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&sm.failed) != 0);
       const int hh = x % kUnits;
       const uint32_t k0 = it + x / kUnits;
       uint32_t st = k0 % kStages, turn = k0 / kStages;
@@ -769,9 +781,10 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // that every row sees
       const int seen_from = a.window > 0 ? tmin - a.window - (kUnit - 1) : -kUnit;
       const int full_from = a.window > 0 ? tmax - a.window : -kUnit, full_to = tmin - (kUnit - 1);
-      for (int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x; x < kUnits * p.take; x += kWarps, p0 += kUnit * kWarps) {
-        const bool ok = kv4_wait(&sm.full[st], turn & 1, &sm.failed, a.w.err);
-        if (ok && sm.present[st] && p0 <= tmax && p0 > seen_from) unit(sm.stage[st], hh, p0, p0 > full_to || p0 <= full_from);
+      const int units = given_up ? 0 : kUnits * p.take;
+      for (int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x; x < units; x += kWarps, p0 += kUnit * kWarps) {
+        if (!__all_sync(0xffffffffu, kv4_wait(&sm.full[st], turn & 1, a.polls, &sm.failed, a.w.err))) break;
+        if (sm.present[st] && p0 <= tmax && p0 > seen_from) unit(sm.stage[st], hh, p0, p0 > full_to || p0 <= full_from);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[st]);
         st += kWarps / kUnits;
@@ -811,13 +824,14 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // the next part's rows may now be staged; its accumulators are written after the barrier that follows them
       named_bar_sync(1, 32 * kWarps);
       const bool whole = p.c0 == 0 && p.take == p.cnt;
+      const float none = *reinterpret_cast<volatile int*>(&sm.failed) ? __uint_as_float(0x7fc00000u) : 0.f;
       float* mine = part + (int64_t)(2 * blockIdx.x + (p.c0 == 0 ? 1 : 0)) * ROWS * part_row(D);
       constexpr int kQuads = D / 4;   // threads per row
       for (int x = threadIdx.x; x < ROWS * kQuads; x += 32 * kWarps) {
         const int row = x / kQuads, d0 = 4 * (x % kQuads);
         const uint32_t rr = r0 + row;
         if (rr >= qrows) break;
-        float mv[kWarps], M = -INFINITY, l = 0.f;
+        float mv[kWarps], M = -INFINITY, l = none;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int v = 0; v < kWarps; ++v) {
@@ -956,6 +970,14 @@ void launch_rows(const Kv4Attn& a, int rows, int sms, cudaStream_t s) {
 
 }  // namespace
 
+namespace {
+std::atomic<uint32_t> wait_polls{kMaxSpins};
+}
+
+int kv4_wait_polls(int polls) {
+  return (int)(polls < 0 ? wait_polls.load() : wait_polls.exchange(std::min((uint32_t)polls, kMaxSpins)));
+}
+
 int64_t kv4_workspace_bytes(int head_dim, int group, int rows_per_seq, int sms) {
   return (int64_t)sms * (2 * block_rows(head_dim, group, rows_per_seq) * part_row(head_dim) * (int64_t)sizeof(float) +
                          (int64_t)sizeof(Kv4Split));
@@ -968,6 +990,7 @@ void launch_kv4_attention(const Kv4Attn& args, int sms, cudaStream_t s) {
   // so that a CTA with several parts gets fewer chunks, and few sequences' parts go to CTAs of their own. Measured at 4,
   // 8, 12, 16: 1 x 131072 (4 rows, head dim 128) 29.6, 28.7, 27.9, 27.9 us; 64 rows x 8192 50.9, 50.4, 51.3, 52.4 us;
   // 16 x 8191 at head dim 256 35.7, 35.0, 35.9, 36.4 us.
+  a.polls = wait_polls.load(std::memory_order_relaxed);
   a.window = std::min(a.window, 0x7fffffff - 63);   // all positions, and no overflow of -1 - window - 31
   a.part_cost = rows == 4 && a.w.head_dim <= 128 ? 12 : 8;
   if (a.w.head_dim == 256)
