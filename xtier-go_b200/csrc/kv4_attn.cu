@@ -17,10 +17,11 @@
 // Precision of the f16 operands: q of 16-bit rows is exact in one plane (a power of two brings the row's largest value
 // to 2^14 .. 2^15); of f32 rows it is hi + lo, 22 bits. P s is brought below 2^16 by a power of two per group (the largest
 // scale met) and always has two planes: one would put 2^-12 of the largest value into the result, which a small component
-// beside large values of other positions shows even after bf16's rounding. 16-bit rows' P V is added up in the matrix
-// unit; f32 rows' is taken from zero for every half chunk and added to an f32 accumulator, because the unit's own sum
-// loses about 2^-24 per step to truncation. A row's maximum is followed loosely (kSlack): scaling the sums at every new
-// maximum cost 10 % more instructions.
+// beside large values of other positions shows even after bf16's rounding. The matrix unit's own sum loses about 2^-24 of
+// itself per step to truncation, always towards zero. So f32 rows' P V is taken from zero for every half chunk and added
+// to an f32 accumulator, and 16-bit rows' is added up in the unit for 128 steps at most (2^-18), then to f32 sums in
+// shared memory. A row's maximum is followed loosely (kSlack): scaling the sums at every new maximum cost 10 % more
+// instructions.
 //
 // One CTA per SM takes an equal share of all (sequence, KV head, row block, 64-position chunk) items in that order,
 // whatever the sequences' lengths: shares start and end inside a sequence, whose parts a second kernel joins. Producer
@@ -292,7 +293,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
   constexpr int RT = ROWS == 16 ? 2 : 1, kE = ROWS == 4 ? 1 : 2;
   constexpr bool kPair = ROWS == 4;
   constexpr int kQPlanes = TYPE == kKv4F32 && !kPair ? 2 : 1, kPPlanes = kPair ? 1 : 2;   // operands per tile
-  constexpr bool kDirect = TYPE != kKv4F32;    // P V added up in the matrix unit
+  constexpr bool kDirect = TYPE != kKv4F32;    // P V added up in the matrix unit, kFold half chunks at most
+  constexpr int kFold = kPair ? 64 : 32;       // 128 products into a sum
   constexpr bool kCentred = TYPE == kKv4F32;   // K's codes less 8 before the product
   constexpr float kCode = kCentred ? 1.f / 16.f : 1.f / 16777216.f;   // the unit in which K's codes enter
   extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -437,7 +439,9 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(base_high));
     uint32_t it = 0;            // chunks of the parts before
     bool split_after = false;   // the last part goes on in the next CTA
-    while (kv4_next<ROWS>(a, walk, p)) {
+    int x = 0;                  // this warp's next half chunk of the part
+    bool more = false;          // the part goes on, its sums so far are in shared memory
+    while (more || kv4_next<ROWS>(a, walk, p)) {
       // ---- the rows: row r of the sequence and KV head is (row r / group of the sequence, q head r % group) ----
       const uint32_t qrows = (uint32_t)p.n * group, r0 = (uint32_t)p.b * ROWS;
       // the position of the sequence's row i (past 2^31 - 1 the table holds nothing more to see)
@@ -449,7 +453,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // neighbouring dims, the word of K codes that lane 4 g + (dims / 8) % 4 multiplies: nibble pair i (dims i, i + 4)
       // is a register of step i / 2 ----
       constexpr int kPieces = D / 8;   // threads per row
-      for (int x = threadIdx.x; x < ROWS * kPieces; x += 32 * kWarps) {   // whole warps: ROWS x D / 8 >= 32
+      const int pieces = more ? 0 : ROWS * kPieces;
+      for (int x = threadIdx.x; x < pieces; x += 32 * kWarps) {   // whole warps: ROWS x D / 8 >= 32
         const int row = x / kPieces, d8 = x % kPieces;
         const uint32_t r = r0 + row, i = r / group;
         const bool live = r < qrows;
@@ -491,7 +496,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
           sm.qpos[row] = live ? position(i) : -1;
         }
       }
-      named_bar_sync(1, 32 * kWarps);
+      if (!more) named_bar_sync(1, 32 * kWarps);
       // what belongs to the rows of this lane's scores: 8 j + 2 tq + {0, 1}, or tq
       float qsum[RT][kE][kGroups], rf[RT][kE];   // (sum q)_G and the factor from the products' unit to base-2 scores
       int t[RT][kE];                             // the row's position; dead rows see nothing
@@ -520,13 +525,12 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
           for (int m = 0; m < 2; ++m) o[j][c][m][0] = o[j][c][m][1] = o[j][c][m][2] = o[j][c][m][3] = 0.f;
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
-          ref[j][e] = -INFINITY;
+          ref[j][e] = more ? sm.m[warp][8 * j + kE * tq + e] : -INFINITY;
           run_l[j][e] = 0.f;
 #pragma unroll
           for (int G = 0; G < kGroups; ++G) oz[j][e][G] = 0.f;
         }
       }
-
 #pragma unroll
       for (int G = 0; G < kGroups; ++G) unit_e[G] = 27;
 
@@ -772,7 +776,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // Half chunk x is chunk x / kUnits, in the ring's stage and turn after `it` chunks; kWarps is a multiple of kUnits, so
       // a warp's half of the chunks stays the same.
       static_assert(kWarps % kUnits == 0 && kWarps / kUnits <= kStages, "the ring goes round once between a warp's chunks at most");
-      int x = (int)((warp + kWarps - kUnits * it % kWarps) % kWarps);
+      if (!more) x = (int)((warp + kWarps - kUnits * it % kWarps) % kWarps);
       const bool given_up = __any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&sm.failed) != 0);
       const int hh = x % kUnits;
       const uint32_t k0 = it + x / kUnits;
@@ -782,8 +786,11 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       const int seen_from = a.window > 0 ? tmin - a.window - (kUnit - 1) : -kUnit;
       const int full_from = a.window > 0 ? tmax - a.window : -kUnit, full_to = tmin - (kUnit - 1);
       const int units = given_up ? 0 : kUnits * p.take;
-      for (int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x; x < units; x += kWarps, p0 += kUnit * kWarps) {
-        if (!__all_sync(0xffffffffu, kv4_wait(&sm.full[st], turn & 1, a.polls, &sm.failed, a.w.err))) break;
+      const int stop = kDirect ? min(units, x + kFold * kWarps) : units;
+      bool ok = true;
+      for (int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x; x < stop; x += kWarps, p0 += kUnit * kWarps) {
+        ok = __all_sync(0xffffffffu, kv4_wait(&sm.full[st], turn & 1, a.polls, &sm.failed, a.w.err));
+        if (!ok) break;
         if (sm.present[st] && p0 <= tmax && p0 > seen_from) unit(sm.stage[st], hh, p0, p0 > full_to || p0 <= full_from);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[st]);
@@ -793,9 +800,34 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
           ++turn;
         }
       }
-      it += p.take;
 
-      // ---- the part's warps meet, by their maxima ----
+      // ---- the warp's sums into shared memory, with those of its half chunks before, which a lane finds in its own places
+      // (added apart from the last lines: there, even where it does not happen, it cost 3 %) ----
+      float up[kGroups];
+#pragma unroll
+      for (int G = 0; G < kGroups; ++G) up[G] = kDirect ? pow2_bits(unit_e[G] - 9) * 16.f : 1.f;
+      if (kDirect && more) {
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+          for (int e = 0; e < kE; ++e) {
+            const int row = 8 * j + kE * tq + e;
+            const float m = sm.m[warp][row], old = m == ref[j][e] ? 1.f : ex2_approx(m - ref[j][e]);
+            if (g == 0) run_l[j][e] = fmaf(old, sm.l[warp][row], run_l[j][e]);
+#pragma unroll
+            for (int c = 0; c < kBlocks; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {   // dims 8 i + g of the block
+                float* y = &o[j][c][i / 2][2 * (i % 2)];
+                y[kPair ? 0 : e] =
+                    fmaf(old, sm.acc[warp][row][32 * c + 8 * i + g], (kPair ? y[0] + y[1] : y[e]) * up[c / 2]);
+                if (kPair) y[1] = 0.f;
+              }
+          }
+#pragma unroll
+        for (int G = 0; G < kGroups; ++G) up[G] = 1.f;
+        __syncwarp();
+      }
 #pragma unroll
       for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -815,12 +847,20 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
           for (int c = 0; c < kBlocks; ++c)
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-              const float up = kDirect ? pow2_bits(unit_e[c / 2] - 9) * 16.f : 1.f;
               const float(&y)[4] = o[j][c][m];
-              sm.acc[warp][row][32 * c + 16 * m + g] = fmaf(kPair ? y[0] + y[1] : y[e], up, oz[j][e][c / 2]);
-              sm.acc[warp][row][32 * c + 16 * m + 8 + g] = fmaf(kPair ? y[2] + y[3] : y[e + 2], up, oz[j][e][c / 2]);
+              float* to = &sm.acc[warp][row][32 * c + 16 * m + g];
+              to[0] = fmaf(kPair ? y[0] + y[1] : y[e], up[c / 2], oz[j][e][c / 2]);
+              to[8] = fmaf(kPair ? y[2] + y[3] : y[e + 2], up[c / 2], oz[j][e][c / 2]);
             }
         }
+      more = kDirect && ok && x < units;
+      if (more) {   // the same part and rows: no other warp is waited for
+        __syncwarp();
+        continue;
+      }
+      it += p.take;
+
+      // ---- the part's warps meet, by their maxima ----
       // the next part's rows may now be staged; its accumulators are written after the barrier that follows them
       named_bar_sync(1, 32 * kWarps);
       const bool whole = p.c0 == 0 && p.take == p.cnt;
