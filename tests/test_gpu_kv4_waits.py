@@ -42,6 +42,6 @@ def test_waits_that_give_up(cuda, xtg, torch, polls, rows, pos, heads, kvh, d, d
             recorded = int(s.err.item())
             assert same and (recorded == 1 or not torch.isnan(out).any())
             s.err.zero_()
-    polls(1 << 24)
+    polls(1 << 18)
     assert torch.equal(attend(err=s.err), right)
     xtg.kv4_check(s.err)

@@ -51,6 +51,9 @@ namespace xtg {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// Looks at a barrier before a wait gives up. One that finds nothing takes 4 us (mbarrier.try_wait suspends the thread), so
+// this is a second; no wait of the kernel begins before the kernels it depends on have ended.
+constexpr uint32_t kKv4Polls = 1u << 18;
 constexpr float kSlack = 6.f;   // how far, in powers of two, a row's probabilities may pass 1 before its sums are scaled
 constexpr int kUnit = 32;                        // positions a warp takes at once: half a chunk
 constexpr int kUnits = kKv4Page / kUnit, kSteps = kUnit / 16;
@@ -268,7 +271,7 @@ __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float(
 __device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, uint32_t polls, int* failed, int32_t* err) {
   for (uint32_t i = 0; i < polls; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
-    if (i > 4096 && *reinterpret_cast<volatile int*>(failed)) break;
+    if (i > 64 && *reinterpret_cast<volatile int*>(failed)) break;
   }
   atomicExch(failed, 1);
   if (err) atomicExch(err, 1);
@@ -429,7 +432,9 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     if (lane == 0)
       for (int s = pw; s < kStages; s += kProducers) {
         const uint32_t issued = turn + (s < st);   // into this stage
-        if (issued > 0) mbar_wait_bounded(&sm.full[s], (issued - 1) & 1, a.w.err);
+        uint32_t i = 0;
+        while (issued > 0 && !mbar_try_wait(&sm.full[s], (issued - 1) & 1) && ++i < kKv4Polls) continue;
+        if (i == kKv4Polls && a.w.err) atomicExch(a.w.err, 1);
       }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kConsumerRegs));
@@ -1011,11 +1016,11 @@ void launch_rows(const Kv4Attn& a, int rows, int sms, cudaStream_t s) {
 }  // namespace
 
 namespace {
-std::atomic<uint32_t> wait_polls{kMaxSpins};
+std::atomic<uint32_t> wait_polls{kKv4Polls};
 }
 
 int kv4_wait_polls(int polls) {
-  return (int)(polls < 0 ? wait_polls.load() : wait_polls.exchange(std::min((uint32_t)polls, kMaxSpins)));
+  return (int)(polls < 0 ? wait_polls.load() : wait_polls.exchange(std::min((uint32_t)polls, 1u << 24)));
 }
 
 int64_t kv4_workspace_bytes(int head_dim, int group, int rows_per_seq, int sms) {
