@@ -217,7 +217,8 @@ __device__ __forceinline__ void quantise(const Piece<T>& p, uint32_t (&word)[2],
   // from z's rounding where |z| passes 2^8 s: the least and the greatest value, which bound the others, tell.
   constexpr float kRound = 12582920.f;
   constexpr uint32_t kBits = 0x4b400000u;   // of code 0
-  auto code = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(__fsub_rn(v, z), inv), kRound)); };
+  auto level = [&](float v) { return __fmul_rn(__fsub_rn(v, z), inv); };
+  auto code = [&](float v) { return __float_as_uint(__fadd_rn(level(v), kRound)); };
   word[0] = word[1] = 0;
   if (code(lo) >= kBits && code(hi) <= kBits + 15) {
     // sum of 16^e bits(e) less that of code 0's bits
@@ -227,7 +228,10 @@ __device__ __forceinline__ void quantise(const Piece<T>& p, uint32_t (&word)[2],
     word[1] -= kBits * 0x11111111u;
   } else {
 #pragma unroll
-    for (int e = 15; e >= 0; --e) word[e / 8] = 16u * word[e / 8] + min(max((int)(code(x[e]) - kBits), 0), 15);
+    for (int e = 15; e >= 0; --e) {   // clamped first: a level may lie past what the addition rounds
+      const float t = fminf(fmaxf(level(x[e]), -8.f), 7.f);
+      word[e / 8] = 16u * word[e / 8] + (__float_as_uint(__fadd_rn(t, kRound)) - kBits);
+    }
   }
   if (!fine) word[0] = word[1] = 0;
   par = fine ? (__float_as_uint(s) & 0xffff0000u) | (__float_as_uint(z) >> 16) : kKv4NanParam;
