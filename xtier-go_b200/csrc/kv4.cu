@@ -3,7 +3,7 @@
 // Quantiser, per group of 64 head dims, each step in f32 rounded to nearest:
 //   lo, hi = min, max;  s = up_bf16(max(2^-100, (hi - lo) (1 / 15)));  z = bf16(lo + 8 s)
 //   code = clamp(rint((x - z) (1 / s)), -8, 7) + 8
-// The 16 levels z - 8 s .. z + 7 s reach from lo to hi (s is rounded up); only z's own rounding, at most 2^-9 |z|, can
+// The 16 levels z - 8 s .. z + 7 s reach from lo to hi (s is rounded up); only z's own rounding, at most 2^-8 |z|, can
 // cut an end. The offset sits at the middle of the levels and not at lo, so that sums of s (code - 8) over many
 // positions stay as small as the values' own sums.
 //
@@ -214,7 +214,7 @@ __device__ __forceinline__ void quantise(const Piece<T>& p, uint32_t (&word)[2],
   const bool fine = raw < INFINITY && fabsf(z) < INFINITY;   // false for NaN too
   const float inv = __frcp_rn(s);
   // adding 1.5 2^23 + 8 rounds to an integer, ties to even, in the low bits: the code. Codes outside 0 .. 15 come only
-  // from z's rounding where |z| passes 2^8 s: the least and the greatest value, which bound the others, tell.
+  // from z's rounding where |z| passes 2^7 s: the least and the greatest value, which bound the others, tell.
   constexpr float kRound = 12582920.f;
   constexpr uint32_t kBits = 0x4b400000u;   // of code 0
   auto level = [&](float v) { return __fmul_rn(__fsub_rn(v, z), inv); };
