@@ -236,7 +236,8 @@ XTG_CUDA_API int xtg_cuda_kv_store(const float* k, const float* v, int64_t pos, 
 // positions pos[i], pos[i] + 1, ... Position p of sequence i is slot p % 64 of page table[i][p / 64]. A negative table
 // entry or position holds nothing: a store skips it, a load gives zeros, attention does not see it. table, pos, cu_rows
 // and err are device memory, read when the call runs on `stream` (a captured call follows their later contents); the
-// calls allocate nothing and do not wait. Rows past cu_rows[seqs] are left alone. A position past the table or a page
+// calls allocate nothing and do not wait. Rows that are no sequence's (past cu_rows[seqs]) are left alone, or, with
+// XTG_CUDA_KV4_ZERO_REST added to dtype, zeros in the outputs of a load or an attention. A position past the table or a page
 // past the pool is treated as nothing there and recorded in *err (6, 7; 1 when a device wait timed out).
 // Two sequences of one store must not write the same page. Sequences may share pages that are only read.
 typedef struct {
@@ -250,6 +251,8 @@ typedef struct {
   int64_t rows;             // rows of this call's arrays, below 2^31
   int32_t* err;             // one word, or NULL
 } xtg_cuda_kv4;
+
+#define XTG_CUDA_KV4_ZERO_REST 256
 
 // dtype of rows: 0 f32, 1 bf16, 2 f16. Pointers start on 16-byte boundaries and strides (in elements) are multiples of
 // 16 bytes; the head_dim values of a row's head are contiguous.

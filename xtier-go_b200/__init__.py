@@ -651,7 +651,7 @@ def kv4_store(pool, k, v, table, pos, cu_rows, err=None):
 
 def kv4_load(pool, table, pos, cu_rows, rows, dtype=None, err=None):
     """The cached keys and values of `rows` rows (cu_rows' last entry): (k, v) [rows][kv_heads][head_dim] of dtype
-    (default bfloat16)."""
+    (default bfloat16). Rows past cu_rows' last entry are zeros."""
     m = _kv4()
     return m.load(pool, table, pos, cu_rows, err, rows, 1 if dtype is None else _kv4_dtypes.get(dtype, -1))
 
@@ -659,5 +659,6 @@ def kv4_load(pool, table, pos, cu_rows, rows, dtype=None, err=None):
 def kv4_attention(q, pool, table, pos, cu_rows, scale, window=0, rows_per_seq=None, out=None, err=None):
     """Attention of rows q [rows][heads][head_dim] over the cached positions up to each row's own (window > 0: the last
     `window` of these), after the call's rows were stored: [rows][heads][head_dim] in q's type. rows_per_seq: about how
-    many rows a sequence has (default rows / seqs); it chooses the tiling only."""
+    many rows a sequence has (default rows / seqs); it chooses the tiling only. Rows past cu_rows' last entry are zeros, or
+    left as they are in a given out."""
     return _kv4().attention(pool, table, pos, cu_rows, err, q, scale, window, rows_per_seq, out)

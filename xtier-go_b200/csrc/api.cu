@@ -386,7 +386,7 @@ Kv4Where kv4_where(const xtg_cuda_kv4* c) {
   XTG_REQUIRE(c->pool && (c->seqs == 0 || (c->table && c->pos && c->cu_rows)), "kv4: null pointer");
   XTG_REQUIRE(aligned16(c->pool), "kv4: the pool must start on a 16-byte boundary");
   return {c->pool, c->pages, c->kv_heads, c->head_dim, c->table, c->max_pages, c->seqs, c->pos, c->cu_rows, c->rows,
-          c->err};
+          c->err, false};
 }
 
 void kv4_require_rows(int dtype, std::initializer_list<const void*> pointers, std::initializer_list<int64_t> strides) {
@@ -397,6 +397,18 @@ void kv4_require_rows(int dtype, std::initializer_list<const void*> pointers, st
   }
   for (int64_t s : strides)
     XTG_REQUIRE(s >= 0 && s % (dtype == kKv4F32 ? 4 : 8) == 0, "kv4: row and head strides must be multiples of 16 bytes");
+}
+
+// An output's dtype and whether rows that are no sequence's become zeros. Without sequences these are all of them.
+bool kv4_zero_rest(int& dtype) {
+  const bool zero = dtype >= 0 && (dtype & XTG_CUDA_KV4_ZERO_REST);
+  if (zero) dtype -= XTG_CUDA_KV4_ZERO_REST;
+  return zero;
+}
+
+void kv4_zero_rows(std::initializer_list<void*> outs, int64_t values, int dtype, void* stream) {
+  for (void* out : outs)
+    XTG_CUDA(cudaMemsetAsync(out, 0, values * (dtype == kKv4F32 ? 4 : 2), static_cast<cudaStream_t>(stream)));
 }
 
 int device_sms() {
@@ -426,10 +438,12 @@ int xtg_cuda_kv4_store(const xtg_cuda_kv4* c, const void* k, const void* v, int 
 
 int xtg_cuda_kv4_load(const xtg_cuda_kv4* c, void* k, void* v, int dtype, void* stream, char* err, int err_len) {
   return guarded(err, err_len, [&] {
-    const Kv4Where w = kv4_where(c);
-    if (w.rows == 0 || w.seqs == 0) return;
+    Kv4Where w = kv4_where(c);
+    w.zero_rest = kv4_zero_rest(dtype);
+    if (w.rows == 0 || (w.seqs == 0 && !w.zero_rest)) return;
     kv4_require_rows(dtype, {k, v}, {});
     const int64_t head = w.head_dim, row = head * w.kv_heads;
+    if (w.seqs == 0) return kv4_zero_rows({k, v}, w.rows * row, dtype, stream);
     launch_kv4_load(w, {k, v, dtype, row, head, row, head}, static_cast<cudaStream_t>(stream));
   });
 }
@@ -450,13 +464,15 @@ int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, void* out, int 
                            int64_t q_head, float scale, int window, int rows_per_seq, void* workspace,
                            int64_t workspace_bytes, void* stream, char* err, int err_len) {
   return guarded(err, err_len, [&] {
-    const Kv4Where w = kv4_where(c);
+    Kv4Where w = kv4_where(c);
+    w.zero_rest = kv4_zero_rest(dtype);
     kv4_require_heads(heads, w.kv_heads, rows_per_seq);
     XTG_REQUIRE(window >= 0, "kv4: window 0 (none) or more");
     XTG_REQUIRE(std::isfinite(scale), "kv4: a finite scale");
     XTG_REQUIRE(w.rows * heads < (1ll << 31), "kv4: rows x heads below 2^31");
-    if (w.rows == 0 || w.seqs == 0) return;
+    if (w.rows == 0 || (w.seqs == 0 && !w.zero_rest)) return;
     kv4_require_rows(dtype, {q, out}, {q_row, q_head});
+    if (w.seqs == 0) return kv4_zero_rows({out}, w.rows * heads * w.head_dim, dtype, stream);
     const int sms = device_sms();
     XTG_REQUIRE(workspace && aligned16(workspace) &&
                     workspace_bytes >= kv4_workspace_bytes(w.head_dim, heads / w.kv_heads, rows_per_seq, sms),

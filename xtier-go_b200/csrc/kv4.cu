@@ -306,11 +306,17 @@ __global__ void __launch_bounds__(kThreads) kv4_store_kernel(const Kv4Where w, c
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kThreads, D <= 128 ? 8 : 6) kv4_load_kernel(const Kv4Where w, const Kv4Rows r) {
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 8 : 6) kv4_load_kernel(const Kv4Where w, const Kv4Rows r, unsigned tasks) {
   constexpr int H = D < 128 ? D : 128, kPerRow = D / 8;
   __shared__ __align__(16) uint32_t par[2][D / 64][kKv4Page];   // K's, V's
   __shared__ Task task;
   Task t;
+  if (blockIdx.x >= tasks) {
+    pdl_wait();
+    pdl_launch_next();
+    kv4_zero_rest(w, r.k, r.v, r.k_row * sizeof(T), tasks);
+    return;
+  }
   if (!find_task(w, task, t)) return;
   const int h = blockIdx.x % (uint32_t)w.kv_heads;
   T* kout = static_cast<T*>(r.k) + t.row0 * r.k_row + h * r.k_head;
@@ -401,7 +407,7 @@ void by_type_and_dim(int dtype, int head_dim, F&& f) {
 
 unsigned task_grid(const Kv4Where& w) {
   const int64_t ctas = (w.rows / kKv4Page + 2 * (int64_t)w.seqs) * w.kv_heads;
-  XTG_REQUIRE(ctas < (1ll << 31), "kv4: too many pages x KV heads in one call");
+  XTG_REQUIRE(ctas < (1ll << 31) - 4, "kv4: too many pages x KV heads in one call");
   return (unsigned)ctas;
 }
 
@@ -415,7 +421,8 @@ void launch_kv4_store(const Kv4Where& w, const Kv4Rows& r, cudaStream_t s) {
 
 void launch_kv4_load(const Kv4Where& w, const Kv4Rows& r, cudaStream_t s) {
   by_type_and_dim(r.dtype, w.head_dim, [&](auto t, auto d) {
-    launch_kv4(kv4_load_kernel<decltype(t), decltype(d)::value>, task_grid(w), kThreads, 0, s, w, r);
+    const unsigned tasks = task_grid(w);
+    launch_kv4(kv4_load_kernel<decltype(t), decltype(d)::value>, tasks + kv4_rest_blocks(w), kThreads, 0, s, w, r, tasks);
   });
 }
 

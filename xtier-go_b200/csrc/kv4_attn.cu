@@ -923,18 +923,23 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
 
 // Row blockIdx.x % ROWS of the split (sequence, row block, KV head), if any, that CTA blockIdx.x / ROWS's share ended
 // in: the last part of that CTA and the first parts of the CTAs after it, joined by their maxima. D / 4 threads take 4
-// dims each of every kSets-th part; the sets' results are joined in their order.
+// dims each of every kSets-th part; the sets' results are joined in their order. Blocks from sms x ROWS on write the zeros
+// of rows that are no sequence's.
 constexpr int kCombineThreads = 256;
 
 template <int D, int ROWS>
 __global__ void __launch_bounds__(kCombineThreads)
-    kv4_combine_kernel(const Kv4Attn a, const float* part, const Kv4Split* splits) {
+    kv4_combine_kernel(const Kv4Attn a, const float* part, const Kv4Split* splits, int sms) {
   constexpr int kQuads = D / 4, kSets = kCombineThreads / kQuads;   // 4, 8 or 16 sets of threads
   __shared__ __align__(16) float acc[kSets][D];
   __shared__ float sm_m[kSets], sm_l[kSets];
   pdl_wait();
   pdl_launch_next();
   const int first = blockIdx.x / ROWS, row = blockIdx.x % ROWS;
+  if (first >= sms) {
+    kv4_zero_rest(a.w, a.out, nullptr, (int64_t)a.heads * D * (a.dtype == kKv4F32 ? 4 : 2), sms * ROWS);
+    return;
+  }
   const Kv4Split sp = splits[first];
   const uint32_t group = a.group, rr = (uint32_t)sp.b * ROWS + row;
   if (sp.last < 0 || rr >= (uint32_t)sp.n * group) return;
@@ -993,8 +998,8 @@ void launch(const Kv4Attn& a, int sms, cudaStream_t s) {
   }();
   XTG_REQUIRE(enough, "kv4: the attention kernel was compiled to fewer registers than it shares out");
   launch_kv4(kv4_attention_kernel<D, ROWS, TYPE>, sms, Kv4Shape<D, ROWS>::kThreads, smem, s, a, part, splits);
-  launch_kv4(kv4_combine_kernel<D, ROWS>, sms * ROWS, kCombineThreads, 0, s, a, (const float*)part,
-             (const Kv4Split*)splits);
+  launch_kv4(kv4_combine_kernel<D, ROWS>, sms * ROWS + kv4_rest_blocks(a.w), kCombineThreads, 0, s, a, (const float*)part,
+             (const Kv4Split*)splits, sms);
 }
 
 template <int D, int ROWS>

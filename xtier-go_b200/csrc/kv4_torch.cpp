@@ -166,7 +166,7 @@ PyObject* load(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const auto options = at::TensorOptions().dtype(types[type]).device(dev);
     at::Tensor k = at::empty({rows, c.kv_heads, c.head_dim}, options), v = at::empty({rows, c.kv_heads, c.head_dim}, options);
     call(dev, [&](void* stream, char* why, int len) {
-      return load_fn(&c, k.data_ptr(), v.data_ptr(), type, stream, why, len);
+      return load_fn(&c, k.data_ptr(), v.data_ptr(), type + XTG_CUDA_KV4_ZERO_REST, stream, why, len);
     });
     PyObject* both = PyTuple_New(2);
     if (!both) return nullptr;
@@ -195,7 +195,9 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int per_seq = args[8] == Py_None ? (int)std::min<int64_t>(std::max<int64_t>(mean, 1), INT32_MAX)
                                            : small(args[8], "rows_per_seq");
     at::Tensor out;
-    if (args[9] == Py_None) {
+    int out_type = type;
+    if (args[9] == Py_None) {   // nothing unwritten is returned
+      out_type += XTG_CUDA_KV4_ZERO_REST;
       out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     } else {
       out = tensor(args[9], "out");
@@ -206,7 +208,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       const int64_t bytes = workspace_fn((int)q.size(1), c.kv_heads, c.head_dim, per_seq);
       require(bytes >= 0, "q heads a multiple of KV heads, rows_per_seq at least 1");
       const at::Tensor work = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
-      return attention_fn(&c, q.data_ptr(), out.data_ptr(), type, (int)q.size(1), q.stride(0), q.stride(1), (float)scale,
+      return attention_fn(&c, q.data_ptr(), out.data_ptr(), out_type, (int)q.size(1), q.stride(0), q.stride(1), (float)scale,
                           window, per_seq, work.data_ptr(), bytes, stream, why, len);
     });
     return THPVariable_Wrap(std::move(out));
