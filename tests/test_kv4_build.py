@@ -1,8 +1,10 @@
-"""CPU: the library is built without torch."""
+"""CPU: the library is built without torch, and a binding that is missing or does not load raises the package's error."""
 import os
 import shutil
 import subprocess
 import sys
+
+import pytest
 
 PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xtier-go_b200")
 
@@ -32,3 +34,13 @@ def test_make_builds_the_library_alone_without_torch(tmp_path):
 def test_make_builds_the_binding_with_torch(tmp_path):
     out = plan(tmp_path, sys.executable)
     assert "libxtg_cuda.so" in out and "kv4_torch.cpp" in out
+
+
+def test_a_binding_that_does_not_load(xtg, monkeypatch, tmp_path):
+    monkeypatch.setattr(xtg, "HERE", str(tmp_path))
+    monkeypatch.setattr(xtg, "_kv4_module", None)
+    with pytest.raises(xtg.XtgError, match="is missing"):
+        xtg.kv4_load(*[None] * 5)
+    (tmp_path / "_kv4_torch.so").write_bytes(b"not a library")
+    with pytest.raises(xtg.XtgError, match="does not load"):
+        xtg.kv4_load(*[None] * 5)

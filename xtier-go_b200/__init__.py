@@ -618,8 +618,11 @@ def _kv4():
         if not os.path.exists(path):
             raise XtgError(f"{path} is missing: build it with xtier-go_b200's Makefile (__graft_entry__.build())")
         spec = importlib.util.spec_from_file_location("_kv4_torch", path)
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
+        try:
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+        except ImportError as e:   # built for another torch or Python
+            raise XtgError(f"{path} does not load, build it again with xtier-go_b200's Makefile: {e}") from e
         L = lib()
         mod.bind(XtgError, *[C.cast(f, C.c_void_p).value for f in (L.xtg_cuda_kv4_store, L.xtg_cuda_kv4_load,
                                                                    L.xtg_cuda_kv4_workspace,
