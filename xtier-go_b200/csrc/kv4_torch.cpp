@@ -98,6 +98,9 @@ int rows_type(const char* name, const at::Tensor& t, int64_t heads, const xtg_cu
   return code;
 }
 
+// The stride of dimension d; that of a single row or head, which nothing steps by, may be any number.
+int64_t stride(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
 // Runs f (which gets the current stream and a message buffer) with device dev current.
 template <class F>
 void call(c10::Device dev, F&& f) {
@@ -146,8 +149,8 @@ PyObject* store(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int type = rows_type("k", k, c.kv_heads, c, dev);
     require(rows_type("v", v, c.kv_heads, c, dev) == type, "k and v have the same type and rows");
     call(dev, [&](void* stream, char* why, int len) {
-      return store_fn(&c, k.data_ptr(), v.data_ptr(), type, k.stride(0), k.stride(1), v.stride(0), v.stride(1), stream,
-                      why, len);
+      return store_fn(&c, k.data_ptr(), v.data_ptr(), type, stride(k, 0), stride(k, 1), stride(v, 0), stride(v, 1),
+                      stream, why, len);
     });
     Py_RETURN_NONE;
   });
@@ -208,7 +211,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       const int64_t bytes = workspace_fn((int)q.size(1), c.kv_heads, c.head_dim, per_seq);
       require(bytes >= 0, "q heads a multiple of KV heads, rows_per_seq at least 1");
       const at::Tensor work = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
-      return attention_fn(&c, q.data_ptr(), out.data_ptr(), out_type, (int)q.size(1), q.stride(0), q.stride(1), (float)scale,
+      return attention_fn(&c, q.data_ptr(), out.data_ptr(), out_type, (int)q.size(1), stride(q, 0), stride(q, 1), (float)scale,
                           window, per_seq, work.data_ptr(), bytes, stream, why, len);
     });
     return THPVariable_Wrap(std::move(out));
