@@ -266,12 +266,12 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 
 __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)biased << 23); }
 
-// mbarrier wait that gives up: after `polls` looks, or soon once another wait of the CTA has. The lanes of a warp that
+// mbarrier wait that gives up: after `polls` looks, or after the first once another wait of the CTA has. The lanes of a warp that
 // wait together may come to different ends: a vote decides for all.
 __device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, uint32_t polls, int* failed, int32_t* err) {
   for (uint32_t i = 0; i < polls; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
-    if (i > 64 && *reinterpret_cast<volatile int*>(failed)) break;
+    if (*reinterpret_cast<volatile int*>(failed)) break;
   }
   atomicExch(failed, 1);
   if (err) atomicExch(err, 1);
@@ -782,8 +782,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // a warp's half of the chunks stays the same.
       static_assert(kWarps % kUnits == 0 && kWarps / kUnits <= kStages, "the ring goes round once between a warp's chunks at most");
       if (!more) x = (int)((warp + kWarps - kUnits * it % kWarps) % kWarps);
-      if (a.polls == 0) kv4_wait(&sm.full[0], 0, 0, &sm.failed, a.w.err);   // the first wait gives up before its first look
-      const bool given_up = __any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&sm.failed) != 0);
+      if (a.polls == 0) kv4_wait(&sm.full[0], 0, 0, &sm.failed, a.w.err);   // a wait that gives up before its first look
       const int hh = x % kUnits;
       const uint32_t k0 = it + x / kUnits;
       uint32_t st = k0 % kStages, turn = k0 / kStages;
@@ -791,7 +790,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // that every row sees
       const int seen_from = a.window > 0 ? tmin - a.window - (kUnit - 1) : -kUnit;
       const int full_from = a.window > 0 ? tmax - a.window : -kUnit, full_to = tmin - (kUnit - 1);
-      const int units = given_up ? 0 : kUnits * p.take;
+      const int units = kUnits * p.take;
       const int stop = kDirect ? min(units, x + kFold * kWarps) : units;
       bool ok = true;
       for (int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x; x < stop; x += kWarps, p0 += kUnit * kWarps) {
