@@ -238,7 +238,8 @@ XTG_CUDA_API int xtg_cuda_kv_store(const float* k, const float* v, int64_t pos, 
 // and err are device memory, read when the call runs on `stream` (a captured call follows their later contents); the
 // calls allocate nothing and do not wait. Rows that are no sequence's (past cu_rows[seqs]) are left alone, or, with
 // XTG_CUDA_KV4_ZERO_REST added to dtype, zeros in the outputs of a load or an attention. A position past the table or a page
-// past the pool is treated as nothing there and recorded in *err (6, 7; 1 when a device wait timed out).
+// past the pool is treated as nothing there and recorded in *err (6, 7; 1 when a device wait timed out); without err
+// nobody learns of rows that a store could not place.
 // Two sequences of one store must not write the same page. Sequences may share pages that are only read.
 typedef struct {
   uint8_t* pool;
@@ -272,7 +273,9 @@ XTG_CUDA_API int64_t xtg_cuda_kv4_workspace(int heads, int kv_heads, int head_di
 // sees nothing gives zeros. rows_per_seq >= 1: about how many rows a sequence has; it chooses the tiling, the result
 // holds for any. workspace: device memory of at least xtg_cuda_kv4_workspace bytes, 16-byte aligned, not shared by
 // calls that may overlap. Sums, softmax and outputs before their last rounding are f32; a call's result does not
-// depend on timing (no atomics).
+// depend on timing (no atomics). Every 16 q rows of a KV head go through all the pages that the call's rows of the
+// sequence see between them: a prompt longer than its window is faster in calls of 512 to 1024 rows (8192 rows, window
+// 1024, 24 q / 6 KV heads of 128: 1.83 ms in one call, at most 1.16 ms in eight).
 XTG_CUDA_API int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, void* out, int dtype, int heads,
                                         int64_t q_row, int64_t q_head, float scale, int window, int rows_per_seq,
                                         void* workspace, int64_t workspace_bytes, void* stream, char* err,

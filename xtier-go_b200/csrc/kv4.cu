@@ -12,9 +12,11 @@
 // owns the page merges all the call's rows into it without atomics, whatever their number.
 //
 // Measured (B200; algorithmic bytes / time against a copy's 6545 GB/s): 64 x 4096 rows of 6 x 128 read back as bf16 in
-// 113 us, 6.0 TB/s, 92 %. 8 x 4096 rows of 4 x 256 f16 written and read back in 72 us, 4.8 TB/s, 73 %: the store is bound
-// by its instructions (issue slots 75 % busy), which a thread's 16 values share (8 values a thread: 75 us). Small calls
-// are a chain of dependent loads (row offsets and position, page table, rows): 2.5 us for one row.
+// 113 us, 6.0 TB/s, 91 % (123 us, 84 %, in runs of seconds on changing data). 8 x 4096 rows of 4 x 256 f16 written and read
+// back in 73 us, 4.7 TB/s, 72 %: the store is bound by its instructions (issue slots 75 % busy), which a thread's 16 values
+// share (8 values a thread: 75 us). Small calls are a chain of dependent loads (row offsets and position, page table,
+// rows): 2.5 us for one row. Every CTA looks through all sequences, so that calls of very many take long: one row of each
+// of 512 written and read back 40 us, of 4096 840 us.
 #include <cuda_bf16.h>
 
 #include "common.cuh"

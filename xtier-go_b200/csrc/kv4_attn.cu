@@ -31,13 +31,17 @@
 // of P s side by side, and half the work per lane; 16 rows share the unpacked codes. More rows read the chunks again,
 // from L2 when the row blocks of a head run at the same time, which costs less than the products of 16 rows take, and
 // larger blocks would cost more at every part's start and end (64 rows over 8192 positions: blocks of 128 rows 66 us,
-// of 16 rows 52 us).
+// of 16 rows 52 us). A block's chunks are those that the sequence's rows see between them; those that its own rows do not
+// see are brought and passed over. That is nothing for the rows of a step, half the chunks of a prompt from position 0
+// (4096 rows 1.29 ms), and most of them for a prompt longer than its window (8192 rows, window 1024: 1.83 ms; in eight calls
+// at most 1.16 ms).
 //
-// What bounds it (B200, head dim 128, bf16): with 4 rows about equally the cache's bytes and the instructions, 64
-// sequences of 16384 .. 32768 positions in 250 us, 5.4 TB/s, 83 % of a copy's rate (204 us without any computation, 1190
-// instructions per chunk and head); one sequence of 131072 positions in 28 us, 4.0 TB/s, of which 10 us are the start, the
-// end of the parts and the join. With 16 rows the instructions around the products: 64 rows over 8192 positions in 49 us,
-// 131 TFLOP/s, tensor pipe 36 % and issue slots 54 % busy.
+// What bounds it (B200, head dim 128, bf16): with 4 rows about equally the cache's bytes and the instructions (1180 per
+// chunk and head), 64 sequences of 16384 .. 32768 positions in 240 us, 5.6 TB/s, 86 % of a copy's rate (204 us without any
+// computation), and in 278 us, 74 %, in runs of seconds, where the power limit lowers the clock; one sequence of 131072
+// positions in 28 us, 4.1 TB/s, of which 10 us are the start, the end of the parts and the join. With 16 rows the
+// instructions around the products: 64 rows over 8192 positions in 49 us, 131 TFLOP/s, tensor pipe 35 % and issue slots
+// 55 % busy.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -1041,8 +1045,9 @@ void launch_kv4_attention(const Kv4Attn& args, int sms, cudaStream_t s) {
   const int rows = block_rows(a.w.head_dim, a.group, a.rows_per_seq);
   // What the start of another part costs a CTA (its rows, its sums), in chunks: counted as items before the part's first,
   // so that a CTA with several parts gets fewer chunks, and few sequences' parts go to CTAs of their own. Measured at 4,
-  // 8, 12, 16: 1 x 131072 (4 rows, head dim 128) 29.6, 28.7, 27.9, 27.9 us; 64 rows x 8192 50.9, 50.4, 51.3, 52.4 us;
-  // 16 x 8191 at head dim 256 35.7, 35.0, 35.9, 36.4 us.
+  // 8, 12, 16: 4 rows: 1 x 131072 29.2, 28.5, 27.7, 27.9 us, 512 x 2048 188, 184, 182, 182, 64 x 4096 of head dim 64, 8 q
+  // on 8 KV heads 42.8, 42.5, 41.1, 40.4; others: 64 rows x 8192 49.5, 49.2, 49.4, 50.5, 12 rows x 8192 of 64 sequences
+  // 31.8, 30.9, 30.7, 31.6, 16 x 8191 at head dim 256 35.6, 34.9, 35.8, 36.3 us.
   a.polls = wait_polls.load(std::memory_order_relaxed);
   a.window = std::min(a.window, 0x7fffffff - 63);   // all positions, and no overflow of -1 - window - 31
   a.part_cost = rows == 4 && a.w.head_dim <= 128 ? 12 : 8;
