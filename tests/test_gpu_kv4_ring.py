@@ -31,17 +31,21 @@ class Shared:
         self.cu = np.arange(self.kinds + 1, dtype=np.int32) * rows
         self.pool = torch.from_numpy(self.ref.bytes).cuda().view(len(self.ref.words), kvh, 72 * d)
 
-    def run(self, seqs, scale, window=0, **kw):
+    def run(self, seqs, scale, window=0):
         """The call's rows [seqs][rows][heads][d]."""
+        out, err = self.attend(seqs, scale, window)
+        self.xtg.kv4_check(err)
+        return out
+
+    def attend(self, seqs, scale, window=0):
         torch = self.torch  # noqa: F811
         kind = torch.arange(seqs) % self.kinds
         q = self.q.view(self.kinds, self.rows, *self.q.shape[1:])[kind].flatten(0, 1).cuda()
         cu = torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * self.rows
         err = torch.zeros(1, dtype=torch.int32, device="cuda")
         out = self.xtg.kv4_attention(q, self.pool, torch.from_numpy(self.table)[kind].cuda(),
-                                     torch.from_numpy(self.pos)[kind].cuda(), cu, scale, window, err=err, **kw)
-        self.xtg.kv4_check(err)
-        return out.view(seqs, self.rows, *q.shape[1:])
+                                     torch.from_numpy(self.pos)[kind].cuda(), cu, scale, window, err=err)
+        return out.view(seqs, self.rows, *q.shape[1:]), err
 
     def check(self, out, scale, window=0):
         q = self.q.double().numpy()

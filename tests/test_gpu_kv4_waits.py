@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from test_gpu_kv4 import Setup, torch  # noqa: F401 (a fixture)
+from test_gpu_kv4_ring import Shared
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +46,20 @@ def test_waits_that_give_up(cuda, xtg, torch, polls, rows, pos, heads, kvh, d, d
     polls(1 << 18)
     assert torch.equal(attend(err=s.err), right)
     xtg.kv4_check(s.err)
+
+
+@pytest.mark.parametrize("d,rows,dtype", [(128, 1, "bf16"), (128, 2, "f16"), (64, 5, "f32"), (256, 2, "bf16")])
+def test_waits_that_give_up_over_many_parts(cuda, xtg, torch, polls, d, rows, dtype):  # noqa: F811
+    """A warp that gave up goes through the CTA's other parts, several turns of the ring, without its waits."""
+    table = np.arange(22)[None].repeat(4, 0)
+    s = Shared(torch, xtg, 23, rows, [1290, 70, 0, 639], table, 8, 2, d, dtype)
+    right = s.run(600, 0.1)
+    for n in (0, 1, 2, 5):
+        polls(n)
+        for _ in range(3):
+            out, err = s.attend(600, 0.1)
+            nan = torch.isnan(out)
+            assert ((out == right) | nan).all() and (int(err.item()) == 1 or not nan.any())
+            assert n > 0 or nan.all()
+    polls(1 << 18)
+    assert torch.equal(s.run(600, 0.1), right)

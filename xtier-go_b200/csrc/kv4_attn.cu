@@ -446,7 +446,9 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     uint32_t base_low, base_high;   // kept in registers (codes_low)
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(base_low));
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(base_high));
-    uint32_t it = 0;            // chunks of the parts before
+    // chunks of the parts before; once a wait of this warp gave up, from kGivenUp on: it no longer knows the ring's phases
+    uint32_t it = 0;
+    constexpr uint32_t kGivenUp = 1u << 31;
     bool split_after = false;   // the last part goes on in the next CTA
     int x = 0;                  // this warp's next half chunk of the part
     bool more = false;          // the part goes on, its sums so far are in shared memory
@@ -794,7 +796,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // that every row sees
       const int seen_from = a.window > 0 ? tmin - a.window - (kUnit - 1) : -kUnit;
       const int full_from = a.window > 0 ? tmax - a.window : -kUnit, full_to = tmin - (kUnit - 1);
-      const int units = kUnits * p.take;
+      const int units = it < kGivenUp ? kUnits * p.take : 0;
       const int stop = kDirect ? min(units, x + kFold * kWarps) : units;
       bool ok = true;
       for (int p0 = (p.lo + p.c0) * kKv4Page + kUnit * x; x < stop; x += kWarps, p0 += kUnit * kWarps) {
@@ -865,6 +867,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
               to[8] = fmaf(kPair ? y[2] + y[3] : y[e + 2], up[c / 2], oz[j][e][c / 2]);
             }
         }
+      if (!ok) it = kGivenUp;
       more = kDirect && ok && x < units;
       if (more) {   // the same part and rows: no other warp is waited for
         __syncwarp();
