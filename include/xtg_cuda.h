@@ -281,9 +281,9 @@ XTG_CUDA_API int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, vo
                                         void* workspace, int64_t workspace_bytes, void* stream, char* err,
                                         int err_len);
 // How often xtg_cuda_kv4_attention's waits (for its own copies, inside a CTA) look at a barrier before they give up: set
-// for the process's later calls, 0 .. 2^24, the default 2^18 (a second: a look that finds nothing takes 4 us); below 0
-// leaves it. Returns the former value. A call whose wait gave up ends as any other, records 1 in *err and gives NaN for
-// the rows concerned.
+// for the process's later calls, 0 (they give up at once) .. 2^24, the default 2^18 (a second: a look that finds nothing
+// takes 4 us); below 0 leaves it. Returns the former value. A call whose wait gave up ends as any other, records 1 in *err
+// and gives NaN for the rows concerned.
 XTG_CUDA_API int xtg_cuda_kv4_wait_polls(int polls);
 
 // The seeded generators (device; bit-identical with the oracle's xo_gen_*): what 0 normal bf16 (a = stddev),

@@ -270,16 +270,23 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 
 __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)biased << 23); }
 
-// mbarrier wait that gives up: after `polls` looks, or after the first once another wait of the CTA has. The lanes of a warp that
-// wait together may come to different ends: a vote decides for all.
-__device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, uint32_t polls, int* failed, int32_t* err) {
-  for (uint32_t i = 0; i < polls; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*reinterpret_cast<volatile int*>(failed)) break;
-  }
+__device__ __forceinline__ void kv4_give_up(int* failed, int32_t* err) {
   atomicExch(failed, 1);
   if (err) atomicExch(err, 1);
-  return false;
+}
+
+// mbarrier wait that gives up: after `polls` more looks than one, or after one once another wait of the CTA has. The lanes
+// of a warp that wait together may come to different ends: a vote decides for all.
+__device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, uint32_t polls, int* failed, int32_t* err) {
+  uint32_t spins = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    ++spins;
+    if (spins > polls || *reinterpret_cast<volatile int*>(failed)) {
+      kv4_give_up(failed, err);
+      return false;
+    }
+  }
+  return true;
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -397,7 +404,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
     const int64_t page_bytes = (int64_t)a.w.kv_heads * Shape::kBlock;
     int st = pw, next = pw;   // this warp's next stage, and its next chunk of the part
     uint32_t turn = 0;
-    bool ok = true;
+    bool ok = true;   // lane 0, which waits and copies: at once; the others: after 32 chunks
     while (ok && kv4_next<ROWS>(a, walk, p)) {
       const uint8_t* head = a.w.pool + (int64_t)p.h * Shape::kBlock;
       while (ok && next < p.take) {
@@ -406,10 +413,8 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
         const uint64_t mine = page >= 0 ? reinterpret_cast<uint64_t>(head + page * page_bytes) : 0;
         for (int j = 0; j < count; ++j) {
           const void* from = reinterpret_cast<const void*>(__shfl_sync(0xffffffffu, mine, j));
-          if (lane == 0 && turn > 0) ok = kv4_wait(&sm.empty[st], (turn - 1) & 1, a.polls, &sm.failed, a.w.err);
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
-          if (lane == 0) {
+          if (lane == 0 && turn > 0 && ok) ok = kv4_wait(&sm.empty[st], (turn - 1) & 1, a.polls, &sm.failed, a.w.err);
+          if (lane == 0 && ok) {
             sm.present[st] = from != nullptr;
             if (!from) {
               mbar_arrive(&sm.full[st]);
@@ -421,12 +426,14 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
                 bulk_g2s(sm.stage[st], from, Shape::kBlock, &sm.full[st]);
             }
           }
-          st += kProducers;
+          __syncwarp();
+          if (ok) st += kProducers;
           if (st >= kStages) {
             st -= kStages;
             ++turn;
           }
         }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
         next += count * kProducers;
       }
       next -= p.take;
@@ -788,7 +795,7 @@ __global__ void __launch_bounds__(Kv4Shape<D, ROWS>::kThreads, 1)
       // a warp's half of the chunks stays the same.
       static_assert(kWarps % kUnits == 0 && kWarps / kUnits <= kStages, "the ring goes round once between a warp's chunks at most");
       if (!more) x = (int)((warp + kWarps - kUnits * it % kWarps) % kWarps);
-      if (a.polls == 0) kv4_wait(&sm.full[0], 0, 0, &sm.failed, a.w.err);   // a wait that gives up before its first look
+      if (a.polls == 0) kv4_give_up(&sm.failed, a.w.err);   // without a look, and with copies under way
       const int hh = x % kUnits;
       const uint32_t k0 = it + x / kUnits;
       uint32_t st = k0 % kStages, turn = k0 / kStages;
