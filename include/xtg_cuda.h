@@ -275,7 +275,7 @@ XTG_CUDA_API int64_t xtg_cuda_kv4_workspace(int heads, int kv_heads, int head_di
 // calls that may overlap. Sums, softmax and outputs before their last rounding are f32; a call's result does not
 // depend on timing (no atomics). Every 16 q rows of a KV head go through all the pages that the call's rows of the
 // sequence see between them: a prompt longer than its window is faster in calls of 512 to 1024 rows (8192 rows, window
-// 1024, 24 q / 6 KV heads of 128: 1.83 ms in one call, at most 1.16 ms in eight).
+// 1024, 24 q / 6 KV heads of 128: 1.74 ms in one call, at most 1.14 ms in eight).
 XTG_CUDA_API int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, void* out, int dtype, int heads,
                                         int64_t q_row, int64_t q_head, float scale, int window, int rows_per_seq,
                                         void* workspace, int64_t workspace_bytes, void* stream, char* err,

@@ -33,14 +33,14 @@
 // larger blocks would cost more at every part's start and end (64 rows over 8192 positions: blocks of 128 rows 66 us,
 // of 16 rows 52 us). A block's chunks are those that the sequence's rows see between them; those that its own rows do not
 // see are brought and passed over. That is nothing for the rows of a step, half the chunks of a prompt from position 0
-// (4096 rows 1.29 ms), and most of them for a prompt longer than its window (8192 rows, window 1024: 1.83 ms; in eight calls
-// at most 1.16 ms).
+// (4096 rows 1.27 ms), and most of them for a prompt longer than its window (8192 rows, window 1024: 1.74 ms; in eight calls
+// at most 1.14 ms).
 //
 // What bounds it (B200, head dim 128, bf16): with 4 rows about equally the cache's bytes and the instructions (1180 per
 // chunk and head), 64 sequences of 16384 .. 32768 positions in 240 us, 5.6 TB/s, 86 % of a copy's rate (204 us without any
-// computation), and in 278 us, 74 %, in runs of seconds, where the power limit lowers the clock; one sequence of 131072
+// computation), and in 280 us, 74 %, in runs of seconds, where the power limit lowers the clock; one sequence of 131072
 // positions in 28 us, 4.1 TB/s, of which 10 us are the start, the end of the parts and the join. With 16 rows the
-// instructions around the products: 64 rows over 8192 positions in 49 us, 131 TFLOP/s, tensor pipe 35 % and issue slots
+// instructions around the products: 64 rows over 8192 positions in 49 us, 132 TFLOP/s, tensor pipe 35 % and issue slots
 // 55 % busy.
 #include <cuda_bf16.h>
 
