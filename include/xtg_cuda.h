@@ -286,6 +286,87 @@ XTG_CUDA_API int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, vo
 // and gives NaN for the rows concerned.
 XTG_CUDA_API int xtg_cuda_kv4_wait_polls(int polls);
 
+// ---- paged key/value caches in 16 bits (no counterpart in the reference, whose caches are 8-bit) ----
+// k [pages][kv_heads][page][head_dim], v [pages][kv_heads][page][v_dim], bf16 (dtype 1) or f16 (2), `page` positions a page
+// (a power of two, 16 .. 1024), each with strides of its own for pages, heads and slots (in elements, multiples of 8; the
+// dims of a slot are contiguous, pools start on 16-byte boundaries), so that [pages][page][kv_heads][head_dim] serves too.
+// (head_dim, v_dim): (64, 64), (128, 128), (256, 256), or (192, 128), keys with a part of their own that is rotated.
+// A cache of latent vectors has v NULL, kv_heads 1 and head_dim = v_dim + 64, v_dim 256 or 512: a slot holds the latent
+// vector and behind it the 64 dims of a rotated key that all heads share. K of a position is the whole slot, V the latent
+// vector (attention with the heads' projections absorbed into q and into what follows the output).
+//
+// A call covers rows of several sequences as the 4-bit cache's do: rows cu_rows[i] .. cu_rows[i + 1] - 1 of its arrays are
+// sequence i's, at positions pos[i], pos[i] + 1, ...; position p of sequence i is slot p % page of page table[i][p / page].
+// A negative table entry or position holds nothing: an append skips it, attention does not see it. table, pos, cu_rows and
+// err are device memory, read when the call runs on `stream`; the calls allocate nothing and do not wait. A position past
+// the table or a page past the pool is treated as nothing there and recorded in *err (6, 7; 1 when a device wait timed
+// out). Two rows of one append must not write the same slot.
+typedef struct {
+  void* k;
+  void* v;
+  int dtype;
+  int64_t pages;
+  int page, kv_heads, head_dim, v_dim;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+  const int32_t* table;     // [seqs][max_pages]
+  int max_pages, seqs;
+  const int32_t* pos;       // [seqs]
+  const int32_t* cu_rows;   // [seqs + 1], from 0, not decreasing
+  int64_t rows;             // rows of this call's arrays, below 2^31
+  int32_t* err;             // one word, or NULL
+} xtg_cuda_kv16;
+
+// An append's rows: k [rows][kv_heads][head_dim], v [rows][kv_heads][v_dim] and, if given, q [rows][heads][head_dim], f32
+// (dtype 0), bf16 (1) or f16 (2), pointers on 16-byte boundaries, strides in elements (multiples of 16 bytes; the dims
+// are contiguous). Of a latent cache k is [rows][64] (k_head is not used), the keys to rotate, v the latent vectors
+// [rows][v_dim], q [rows][heads][64]. Dims first .. first + rotary - 1 of k's and q's heads are rotated: the pair i of them
+// (dims i and i + rotary / 2, or 2 i and 2 i + 1 where interleaved) by the angle position x freq[i] (f32 radians, device
+// memory, [rotary / 2]), the angle taken in 64 bits, the values in 32, rounded once to the cache's type. rotary 0 (freq may
+// be NULL): none is. rotary and first are multiples of 16 and 8, rotary at most 256. q_out [rows][heads][head_dim] (64 for
+// a latent cache), contiguous, of the cache's type, gets q's rows (zeros where a row is no sequence's).
+typedef struct {
+  const void* k;
+  const void* v;
+  const void* q;            // or NULL
+  void* q_out;
+  int dtype, heads;
+  int64_t k_row, k_head, v_row, v_head, q_row, q_head;
+  const float* freq;
+  int rotary, first, interleaved;
+} xtg_cuda_kv16_rows;
+XTG_CUDA_API int xtg_cuda_kv16_append(const xtg_cuda_kv16* c, const xtg_cuda_kv16_rows* r, void* stream, char* err,
+                                      int err_len);
+
+// Attention of rows q [rows][heads][head_dim] of the cache's type (strides in elements, multiples of 8) over the cached
+// positions up to each row's own (window > 0: the last `window` of these; the row's own position counts, so the call's keys
+// and values are appended first): softmax(scale q . K) V into out [rows][heads][v_dim], contiguous, of the cache's type. Of a
+// latent cache q is [rows][heads][v_dim], q_rot [rows][heads][64] (strides r_row, r_head). heads a multiple of kv_heads, q
+// head j reads KV head j / (heads / kv_heads). A row that sees nothing gives zeros. Keys and values at positions that a row
+// does not see are not read into its result, whatever they are. rows_per_seq >= 1: about how many rows a sequence has; it
+// chooses the tiling only. zero_rest: rows that are no sequence's become zeros, else they are left alone. workspace: device
+// memory of at least xtg_cuda_kv16_workspace bytes, 16-byte aligned, not shared by calls that may overlap. Sums and softmax
+// are f32, the probabilities are rounded to the cache's type; a call's result does not depend on timing (no atomics on
+// values).
+typedef struct {
+  const void* q;
+  const void* q_rot;        // of a latent cache, else NULL
+  void* out;
+  int heads;
+  int64_t q_row, q_head, r_row, r_head;
+  float scale;
+  int window, rows_per_seq, zero_rest;
+  void* workspace;
+  int64_t workspace_bytes;
+} xtg_cuda_kv16_attn;
+XTG_CUDA_API int xtg_cuda_kv16_attention(const xtg_cuda_kv16* c, const xtg_cuda_kv16_attn* a, void* stream, char* err,
+                                         int err_len);
+// Bytes of xtg_cuda_kv16_attention's workspace on the current device (latent != 0: of a latent cache); -1 for bad arguments.
+XTG_CUDA_API int64_t xtg_cuda_kv16_workspace(int heads, int kv_heads, int head_dim, int v_dim, int latent,
+                                             int rows_per_seq);
+// How often xtg_cuda_kv16_attention's waits look at a barrier before they give up, as xtg_cuda_kv4_wait_polls sets it for
+// the 4-bit cache's.
+XTG_CUDA_API int xtg_cuda_kv16_wait_polls(int polls);
+
 // The seeded generators (device; bit-identical with the oracle's xo_gen_*): what 0 normal bf16 (a = stddev),
 // 1 uniform f32 in [a, b), 2 int8 in [-127, 127].
 XTG_CUDA_API int xtg_cuda_gen(int what, uint64_t seed, uint64_t stream_id, float a, float b, void* out, int64_t n, void* stream,

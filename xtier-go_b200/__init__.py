@@ -45,6 +45,31 @@ class Kv4(C.Structure):
                 ("cu_rows", C.c_void_p), ("rows", C.c_int64), ("err", C.c_void_p)]
 
 
+class Kv16(C.Structure):
+    """xtg_cuda_kv16: a 16-bit paged cache and where a call's rows stand in it."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("pages", C.c_int64), ("page", C.c_int),
+                ("kv_heads", C.c_int), ("head_dim", C.c_int), ("v_dim", C.c_int), ("k_page", C.c_int64),
+                ("k_head", C.c_int64), ("k_slot", C.c_int64), ("v_page", C.c_int64), ("v_head", C.c_int64),
+                ("v_slot", C.c_int64), ("table", C.c_void_p), ("max_pages", C.c_int), ("seqs", C.c_int),
+                ("pos", C.c_void_p), ("cu_rows", C.c_void_p), ("rows", C.c_int64), ("err", C.c_void_p)]
+
+
+class Kv16Rows(C.Structure):
+    """xtg_cuda_kv16_rows: the rows of an append."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("q", C.c_void_p), ("q_out", C.c_void_p), ("dtype", C.c_int),
+                ("heads", C.c_int), ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_row", C.c_int64),
+                ("v_head", C.c_int64), ("q_row", C.c_int64), ("q_head", C.c_int64), ("freq", C.c_void_p),
+                ("rotary", C.c_int), ("first", C.c_int), ("interleaved", C.c_int)]
+
+
+class Kv16Attn(C.Structure):
+    """xtg_cuda_kv16_attn: the rows of an attention."""
+    _fields_ = [("q", C.c_void_p), ("q_rot", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int), ("q_row", C.c_int64),
+                ("q_head", C.c_int64), ("r_row", C.c_int64), ("r_head", C.c_int64), ("scale", C.c_float),
+                ("window", C.c_int), ("rows_per_seq", C.c_int), ("zero_rest", C.c_int), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
 class Sampling(C.Structure):
     """xtg_cuda_sampling: Sampler::sample's parameters."""
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("min_p", C.c_float)]
@@ -143,6 +168,14 @@ def lib():
                                              C.c_void_p, E, C.c_int]
         L.xtg_cuda_kv4_wait_polls.restype = C.c_int
         L.xtg_cuda_kv4_wait_polls.argtypes = [C.c_int]
+        L.xtg_cuda_kv16_append.restype = C.c_int
+        L.xtg_cuda_kv16_append.argtypes = [C.POINTER(Kv16), C.POINTER(Kv16Rows), C.c_void_p, E, C.c_int]
+        L.xtg_cuda_kv16_attention.restype = C.c_int
+        L.xtg_cuda_kv16_attention.argtypes = [C.POINTER(Kv16), C.POINTER(Kv16Attn), C.c_void_p, E, C.c_int]
+        L.xtg_cuda_kv16_workspace.restype = C.c_int64
+        L.xtg_cuda_kv16_workspace.argtypes = [C.c_int] * 6
+        L.xtg_cuda_kv16_wait_polls.restype = C.c_int
+        L.xtg_cuda_kv16_wait_polls.argtypes = [C.c_int]
         L.xtg_cuda_gen.restype = C.c_int
         L.xtg_cuda_gen.argtypes = [C.c_int, C.c_uint64, C.c_uint64, C.c_float, C.c_float, C.c_void_p, C.c_int64,
                                    C.c_void_p, E, C.c_int]
@@ -605,28 +638,33 @@ KV4_PAGE = 64
 _KV4_ERRORS = {1: "a device wait timed out", 6: "a position lies past its sequence's page table",
                7: "a page table entry lies past the pool"}
 _kv4_module = None
+_kv16_module = None
 _kv4_dtypes = {}   # torch dtype -> the C ABI's code
 
 
+def _binding(name, *functions):
+    """csrc/<name>_torch.cpp, which checks the tensors and calls the C ABI's functions; raises if it was not built."""
+    import importlib.util
+    import torch   # noqa: F401 (its libraries)
+    path = os.path.join(HERE, f"_{name}_torch.so")
+    if not os.path.exists(path):
+        raise XtgError(f"{path} is missing: build it with xtier-go_b200's Makefile (__graft_entry__.build())")
+    spec = importlib.util.spec_from_file_location(f"_{name}_torch", path)
+    try:
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+    except ImportError as e:   # built for another torch or Python
+        raise XtgError(f"{path} does not load, build it again with xtier-go_b200's Makefile: {e}") from e
+    L = lib()
+    mod.bind(XtgError, *[C.cast(getattr(L, f"xtg_cuda_{name}_{f}"), C.c_void_p).value for f in functions])
+    return mod
+
+
 def _kv4():
-    """csrc/kv4_torch.cpp, which checks the tensors and calls the C ABI; raises if it was not built."""
     global _kv4_module
     if _kv4_module is None:
-        import importlib.util
         import torch
-        path = os.path.join(HERE, "_kv4_torch.so")
-        if not os.path.exists(path):
-            raise XtgError(f"{path} is missing: build it with xtier-go_b200's Makefile (__graft_entry__.build())")
-        spec = importlib.util.spec_from_file_location("_kv4_torch", path)
-        try:
-            mod = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(mod)
-        except ImportError as e:   # built for another torch or Python
-            raise XtgError(f"{path} does not load, build it again with xtier-go_b200's Makefile: {e}") from e
-        L = lib()
-        mod.bind(XtgError, *[C.cast(f, C.c_void_p).value for f in (L.xtg_cuda_kv4_store, L.xtg_cuda_kv4_load,
-                                                                   L.xtg_cuda_kv4_workspace,
-                                                                   L.xtg_cuda_kv4_attention)])
+        mod = _binding("kv4", "store", "load", "workspace", "attention")
         _kv4_dtypes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
         _kv4_module = mod
     return _kv4_module
@@ -667,3 +705,63 @@ def kv4_attention(q, pool, table, pos, cu_rows, scale, window=0, rows_per_seq=No
     calls of 512 to 1024 rows. Rows past cu_rows' last entry are zeros, or
     left as they are in a given out."""
     return _kv4().attention(pool, table, pos, cu_rows, err, q, scale, window, rows_per_seq, out)
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Paged caches in 16 bits (include/xtg_cuda.h: xtg_cuda_kv16_*)
+#
+# k_pool [pages][kv_heads][page][head_dim], v_pool [pages][kv_heads][page][v_dim], bfloat16 or float16, any strides of
+# 16-byte multiples (a transposed view of [pages][page][kv_heads][dim] serves); (head_dim, v_dim) (64, 64), (128, 128),
+# (256, 256) or (192, 128), `page` positions a page (16, 32, .. 1024). A latent cache is one pool [pages][page][latent + 64]
+# (latent 256 or 512): a latent vector, which is both the value and a part of the key, and 64 rotated dims of key that
+# all heads share. table, pos, cu_rows and err are as the 4-bit cache's; kv4_check raises what err holds.
+# ----------------------------------------------------------------------------------------------------------------
+
+def _kv16():
+    global _kv16_module
+    if _kv16_module is None:
+        _kv16_module = _binding("kv16", "append", "workspace", "attention")
+    return _kv16_module
+
+
+def kv16_pool(pages, kv_heads, head_dim, dtype=None, page=64, device="cuda"):
+    """An empty pool of keys or values."""
+    import torch
+    return torch.zeros((pages, kv_heads, page, head_dim), dtype=dtype or torch.bfloat16, device=device)
+
+
+def latent_pool(pages, latent, dtype=None, page=64, device="cuda"):
+    """An empty pool of latent vectors with their rotated keys."""
+    import torch
+    return torch.zeros((pages, page, latent + 64), dtype=dtype or torch.bfloat16, device=device)
+
+
+def kv16_append(k_pool, v_pool, k, v, table, pos, cu_rows, freq=None, q=None, first=0, interleaved=False, err=None):
+    """Write rows k [rows][kv_heads][head_dim] and v [rows][kv_heads][v_dim] (float32, bfloat16 or float16) into the pools.
+    With freq (float32 [rotary / 2], radians a position) dims first .. first + rotary - 1 of k's heads, and of q's, are
+    rotated by their positions: dims i and i + rotary / 2 of these are a pair, or 2 i and 2 i + 1 where interleaved. Angles
+    are taken in 64 bits; a value is rounded once, to the pools' type. Returns q [rows][heads][head_dim] rotated, in the
+    pools' type (zeros for rows past cu_rows' last entry), or None without q."""
+    return _kv16().append(k_pool, v_pool, table, pos, cu_rows, err, k, v, freq, q, first, interleaved)
+
+
+def kv16_attention(q, k_pool, v_pool, table, pos, cu_rows, scale, window=0, rows_per_seq=None, out=None, err=None):
+    """Attention of rows q [rows][heads][head_dim] (the pools' type) over the cached positions up to each row's own
+    (window > 0: the last `window` of these), after the call's rows were appended: [rows][heads][v_dim]. rows_per_seq: about
+    how many rows a sequence has (default rows / seqs); it chooses the tiling only. Rows past cu_rows' last entry are
+    zeros, or left as they are in a given out."""
+    return _kv16().attention(k_pool, v_pool, table, pos, cu_rows, err, q, None, scale, window, rows_per_seq, out)
+
+
+def latent_append(pool, c, k, table, pos, cu_rows, freq=None, q=None, interleaved=False, err=None):
+    """Write latent vectors c [rows][latent] and the keys to rotate k [rows][64] into a latent cache; q [rows][heads][64] is
+    rotated with them and returned in the pool's type. Types, freq and interleaved as kv16_append's."""
+    return _kv16().append(pool, None, table, pos, cu_rows, err, k, c, freq, q, 0, interleaved)
+
+
+def latent_attention(q, q_rot, pool, table, pos, cu_rows, scale, window=0, rows_per_seq=None, out=None, err=None):
+    """Attention over a latent cache in the absorbed form: q [rows][heads][latent] are the queries with the keys' projection
+    multiplied in, q_rot [rows][heads][64] their rotated dims (both of the pool's type); a position's key is its whole slot,
+    its value the latent vector. Returns [rows][heads][latent], which the values' projection is then applied to. The other
+    arguments are kv16_attention's."""
+    return _kv16().attention(pool, None, table, pos, cu_rows, err, q, q_rot, scale, window, rows_per_seq, out)

@@ -15,6 +15,7 @@
 #include "sampling.h"
 #include "fp4mma.cuh"
 #include "kernels.h"
+#include "kv16.h"
 #include "kv4.h"
 
 using namespace xtg;
@@ -423,6 +424,50 @@ void kv4_require_heads(int heads, int kv_heads, int rows_per_seq) {
   XTG_REQUIRE(rows_per_seq >= 1, "kv4: rows_per_seq at least 1");
 }
 
+
+Kv16Cache kv16_cache(const xtg_cuda_kv16* c) {
+  XTG_REQUIRE(c, "kv16: no cache");
+  const bool latent = !c->v;
+  XTG_REQUIRE(c->dtype == kKv16Bf16 || c->dtype == kKv16F16, "kv16: a cache of bf16 (1) or f16 (2)");
+  XTG_REQUIRE(kv16_dims(latent, c->head_dim, c->v_dim),
+              "kv16: (head_dim, v_dim) (64, 64), (128, 128), (192, 128) or (256, 256); of a latent cache (320, 256) or (576, 512)");
+  XTG_REQUIRE(c->kv_heads >= 1 && c->kv_heads <= 65535 && (!latent || c->kv_heads == 1),
+              "kv16: 1..65535 KV heads, one of a latent cache");
+  XTG_REQUIRE(c->page >= 16 && c->page <= 1024 && (c->page & (c->page - 1)) == 0, "kv16: 16, 32, .. 1024 positions a page");
+  XTG_REQUIRE(c->pages >= 1 && c->pages < (1ll << 31) && c->max_pages >= 1,
+              "kv16: at least one page in the pool (fewer than 2^31) and per sequence");
+  XTG_REQUIRE(c->seqs >= 0 && c->rows >= 0 && c->rows < (1ll << 31), "kv16: sequences and rows in 0 .. 2^31 - 1");
+  XTG_REQUIRE((int64_t)c->max_pages * c->page <= (1ll << 31), "kv16: a sequence's table holds at most 2^31 positions");
+  XTG_REQUIRE(c->seqs < (1 << 29), "kv16: fewer than 2^29 sequences");
+  XTG_REQUIRE(c->k && (c->seqs == 0 || (c->table && c->pos && c->cu_rows)), "kv16: null pointer");
+  XTG_REQUIRE(aligned16(c->k) && aligned16(c->v), "kv16: the pools must start on a 16-byte boundary");
+  auto strides = [&](int64_t page, int64_t head, int64_t slot, int dims) {
+    for (const auto& [stride, size] : {std::pair<int64_t, int64_t>(page, c->pages), {head, c->kv_heads}, {slot, c->page}})
+      XTG_REQUIRE(size == 1 || (stride >= dims && stride % 8 == 0 && stride < (1ll << 38)),
+                  "kv16: a pool's strides must be multiples of 16 bytes and at least a slot's dims");
+  };
+  strides(c->k_page, c->k_head, c->k_slot, c->head_dim);
+  if (!latent) strides(c->v_page, c->v_head, c->v_slot, c->v_dim);
+  return {c->k,       c->v,    c->dtype,   latent,      c->pages, c->page,   c->kv_heads, c->head_dim,
+          c->v_dim,   c->k_page, c->k_head, c->k_slot,  c->v_page, c->v_head, c->v_slot,  c->table,
+          c->max_pages, c->seqs, c->pos,    c->cu_rows, c->rows,  c->err};
+}
+
+void kv16_require_rows(std::initializer_list<const void*> pointers, int dtype, std::initializer_list<int64_t> strides) {
+  for (const void* p : pointers) {
+    XTG_REQUIRE(p, "kv16: null pointer");
+    XTG_REQUIRE(aligned16(p), "kv16: rows must start on a 16-byte boundary");
+  }
+  for (int64_t s : strides)
+    XTG_REQUIRE(s >= 0 && s % (dtype == kKv16F32 ? 4 : 8) == 0, "kv16: row and head strides must be multiples of 16 bytes");
+}
+
+void kv16_require_heads(int heads, int kv_heads, int rows_per_seq) {
+  XTG_REQUIRE(heads >= 1 && heads % kv_heads == 0 && heads / kv_heads <= 65535,
+              "kv16: q heads a multiple of KV heads, at most 65535 of each");
+  XTG_REQUIRE(rows_per_seq >= 1, "kv16: rows_per_seq at least 1");
+}
+
 }  // namespace
 
 int xtg_cuda_kv4_store(const xtg_cuda_kv4* c, const void* k, const void* v, int dtype, int64_t k_row, int64_t k_head,
@@ -480,6 +525,70 @@ int xtg_cuda_kv4_attention(const xtg_cuda_kv4* c, const void* q, void* out, int 
     launch_kv4_attention({w, q, out, dtype, q_row, q_head, heads, heads / w.kv_heads, window, scale, rows_per_seq,
                           static_cast<float*>(workspace)},
                          sms, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int xtg_cuda_kv16_append(const xtg_cuda_kv16* cache, const xtg_cuda_kv16_rows* r, void* stream, char* err, int err_len) {
+  return guarded(err, err_len, [&] {
+    const Kv16Cache c = kv16_cache(cache);
+    XTG_REQUIRE(r, "kv16: no rows");
+    XTG_REQUIRE(r->dtype >= kKv16F32 && r->dtype <= kKv16F16, "kv16: rows of f32 (0), bf16 (1) or f16 (2)");
+    const int dims = c.latent ? c.head_dim - c.v_dim : c.head_dim;
+    XTG_REQUIRE(r->rotary >= 0 && r->rotary <= 256 && r->rotary % 16 == 0 && r->first >= 0 && r->first % 8 == 0 &&
+                    (int64_t)r->first + r->rotary <= dims,
+                "kv16: rotary a multiple of 16, first of 8, both within a head");
+    XTG_REQUIRE(r->rotary == 0 || r->freq, "kv16: null pointer (freq)");
+    XTG_REQUIRE(!r->q || (r->heads >= 1 && c.rows * r->heads < (1ll << 31)), "kv16: rows x q heads in 1 .. 2^31 - 1");
+    if (c.rows == 0 || (c.seqs == 0 && !r->q)) return;
+    kv16_require_rows({r->k, r->v}, r->dtype, {r->k_row, c.latent ? 0 : r->k_head, r->v_row, c.latent ? 0 : r->v_head});
+    if (r->q) kv16_require_rows({r->q, r->q_out}, r->dtype, {r->q_row, r->q_head});
+    if (c.seqs == 0) {   // no row is a sequence's
+      XTG_CUDA(cudaMemsetAsync(r->q_out, 0, c.rows * r->heads * dims * 2, static_cast<cudaStream_t>(stream)));
+      return;
+    }
+    launch_kv16_append(c,
+                       {r->k, r->v, r->q, r->q_out, r->dtype, r->heads, r->k_row, c.latent ? 0 : r->k_head, r->v_row,
+                        c.latent ? 0 : r->v_head, r->q_row, r->q_head, r->freq, r->rotary, r->first, r->interleaved != 0},
+                       device_sms(), static_cast<cudaStream_t>(stream));
+  });
+}
+
+int64_t xtg_cuda_kv16_workspace(int heads, int kv_heads, int head_dim, int v_dim, int latent, int rows_per_seq) {
+  int64_t bytes = -1;
+  guarded(nullptr, 0, [&] {
+    XTG_REQUIRE(kv_heads >= 1 && kv16_dims(latent != 0, head_dim, v_dim), "kv16: bad shape");
+    kv16_require_heads(heads, kv_heads, rows_per_seq);
+    bytes = kv16_workspace_bytes(latent != 0, head_dim, v_dim, heads / kv_heads, rows_per_seq, device_sms());
+  });
+  return bytes;
+}
+
+int xtg_cuda_kv16_wait_polls(int polls) { return kv16_wait_polls(polls); }
+
+int xtg_cuda_kv16_attention(const xtg_cuda_kv16* cache, const xtg_cuda_kv16_attn* r, void* stream, char* err, int err_len) {
+  return guarded(err, err_len, [&] {
+    const Kv16Cache c = kv16_cache(cache);
+    XTG_REQUIRE(r, "kv16: no rows");
+    kv16_require_heads(r->heads, c.kv_heads, r->rows_per_seq);
+    XTG_REQUIRE(r->window >= 0, "kv16: window 0 (none) or more");
+    XTG_REQUIRE(std::isfinite(r->scale), "kv16: a finite scale");
+    XTG_REQUIRE(c.rows * r->heads < (1ll << 31), "kv16: rows x heads below 2^31");
+    if (c.rows == 0 || (c.seqs == 0 && !r->zero_rest)) return;
+    kv16_require_rows({r->q, r->out}, c.dtype, {r->q_row, r->q_head});
+    if (c.latent) kv16_require_rows({r->q_rot}, c.dtype, {r->r_row, r->r_head});
+    if (c.seqs == 0) {
+      XTG_CUDA(cudaMemsetAsync(r->out, 0, c.rows * r->heads * c.v_dim * 2, static_cast<cudaStream_t>(stream)));
+      return;
+    }
+    const int sms = device_sms();
+    XTG_REQUIRE(r->workspace && aligned16(r->workspace) &&
+                    r->workspace_bytes >= kv16_workspace_bytes(c.latent, c.head_dim, c.v_dim, r->heads / c.kv_heads,
+                                                               r->rows_per_seq, sms),
+                "kv16: a workspace of xtg_cuda_kv16_workspace bytes on a 16-byte boundary");
+    launch_kv16_attention(c,
+                          {r->q, r->q_rot, r->out, r->heads, r->q_row, r->q_head, r->r_row, r->r_head, r->scale, r->window,
+                           r->rows_per_seq, r->zero_rest != 0, r->workspace},
+                          sms, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -1,0 +1,370 @@
+// The 16-bit paged caches: rows appended with their rotation, and the host side of the attention (kv16_attn.cuh).
+//
+// A row's keys and queries turn by its position: pair i (dims i and i + rotary / 2 of the rotated dims, or 2 i and 2 i + 1)
+// by the angle position x freq[i]. The angle is taken as turns in 64 bits, since 32 would leave a far position's angle
+// 2^-24 of itself off, and only what is past the last whole turn goes to sinpi and cospi in 32 bits. The turned values
+// are rounded once, to the cache's type.
+//
+// One pass: a CTA takes some rows with all their heads, so that a row's angles, its sequence, page and slot are worked out
+// once. 8 dims a thread (two times 8, of a pair's two halves), 16-byte loads and stores.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "kv16_launch.cuh"
+
+namespace xtg {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxRowsPerCta = 4;
+constexpr int kMaxRotary = 256;
+
+struct Stream {   // k's, v's or q's heads of a row
+  const void* src;
+  int64_t row, head;   // strides of src
+  int heads, units, turned;   // units a head, the first `turned` of them rotated
+  int dims, first, rotary;    // rotary 0: copied
+  int64_t out_head;           // q: stride of the output's heads; else the pool's
+};
+
+struct AppendArgs {
+  Stream st[3];   // q, k, v
+  void *q_out, *k, *v;
+  int64_t k_page, k_slot, v_page, v_slot;
+  int k_dim0;   // where k's dims start in its pool's slot
+  const int32_t *table, *pos, *cu_rows;
+  const float* freq;
+  int64_t pages, rows;
+  int max_pages, seqs, page_log2, rows_per_cta, half;
+  int32_t* err;
+};
+
+struct Turn {
+  float c, s;
+};
+
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = kv16::unpack(w[i], T());
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = kv16::pack(x[2 * i], x[2 * i + 1], T());
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The last i with cu_rows[i] <= row, by a warp: 32 entries at a time
+__device__ __forceinline__ int sequence_of(const AppendArgs& a, int64_t row) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = a.seqs;   // cu_rows[lo] <= row or lo == 0, of n entries from lo on
+  while (n > 1) {
+    const int step = (n + 31) / 32, i = lo + lane * step;
+    const bool below = i < lo + n && a.cu_rows[i] <= row;
+    const uint32_t m = __ballot_sync(0xffffffffu, below) | 1u;
+    const int k = 31 - __clz(m);
+    n = min(step, n - k * step);
+    lo += k * step;
+  }
+  return lo;
+}
+
+// X: the rows' type, T: the cache's
+template <class X, class T, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+  __shared__ Turn turn[kMaxRowsPerCta][kMaxRotary / 2];
+  __shared__ struct {
+    int64_t page, slot;   // page -1: nowhere to write
+    int64_t pos;
+    bool live;
+  } at[kMaxRowsPerCta];
+  pdl_wait();
+  pdl_launch_next();
+  const int64_t row0 = (int64_t)blockIdx.x * a.rows_per_cta;
+  const int rows = (int)min((int64_t)a.rows_per_cta, a.rows - row0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < rows) {
+    const int64_t row = row0 + warp;
+    const int s = sequence_of(a, row);
+    const int64_t from = a.cu_rows[s], to = a.cu_rows[s + 1], p = a.pos[s] + (row - from);
+    if (lane == 0) {
+      const bool live = row >= from && row < to;
+      int64_t page = -1;
+      if (live && p >= 0) {
+        const int64_t i = p >> a.page_log2;
+        if (i >= a.max_pages) {
+          if (a.err) atomicExch(a.err, 6);
+        } else {
+          page = a.table[(int64_t)s * a.max_pages + i];
+          if (page >= a.pages) {
+            if (a.err) atomicExch(a.err, 7);
+            page = -1;
+          }
+        }
+      }
+      at[warp] = {page, p & ((1 << a.page_log2) - 1), p, live};
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * a.half; i += kThreads) {
+    const int r = i / a.half, e = i - r * a.half;
+    const double turns = (double)at[r].pos * ((double)a.freq[e] * 0.15915494309189533577);
+    const float half_turns = (float)(2.0 * (turns - rint(turns)));
+    Turn t;
+    sincospif(half_turns, &t.s, &t.c);
+    turn[r][e] = t;
+  }
+  __syncthreads();
+  const int n0 = a.st[0].heads * a.st[0].units, n1 = n0 + a.st[1].heads * a.st[1].units,
+            n = n1 + a.st[2].heads * a.st[2].units;
+  for (int i = threadIdx.x; i < rows * n; i += kThreads) {
+    const int r = i / n;
+    int u = i - r * n;
+    const int which = u < n0 ? 0 : u < n1 ? 1 : 2;
+    u -= which == 0 ? 0 : which == 1 ? n0 : n1;
+    const Stream& st = a.st[which];
+    const int h = u / st.units;
+    u -= h * st.units;
+    const bool live = at[r].live;
+    T* to;
+    if (which == 0) {
+      to = static_cast<T*>(a.q_out) + ((row0 + r) * st.heads + h) * st.dims;
+    } else {
+      if (!live || at[r].page < 0) continue;
+      to = which == 1 ? static_cast<T*>(a.k) + at[r].page * a.k_page + h * st.out_head + at[r].slot * a.k_slot + a.k_dim0
+                      : static_cast<T*>(a.v) + at[r].page * a.v_page + h * st.out_head + at[r].slot * a.v_slot;
+    }
+    const X* from = static_cast<const X*>(st.src) + (row0 + r) * st.row + h * st.head;
+    float x[8];
+    if (u < st.turned) {
+      const Turn* t = turn[r];
+      if (INTERLEAVED) {
+        const int d = st.first + 8 * u;
+        load8(from + d, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const Turn w = t[4 * u + e];
+          const float p = x[2 * e], q = x[2 * e + 1];
+          x[2 * e] = p * w.c - q * w.s;
+          x[2 * e + 1] = q * w.c + p * w.s;
+        }
+        if (!live)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        store8(to + d, x);
+      } else {
+        const int d = st.first + 8 * u;
+        float y[8];
+        load8(from + d, x);
+        load8(from + d + a.half, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const Turn w = t[8 * u + e];
+          const float p = x[e], q = y[e];
+          x[e] = live ? p * w.c - q * w.s : 0.f;
+          y[e] = live ? q * w.c + p * w.s : 0.f;
+        }
+        store8(to + d, x);
+        store8(to + d + a.half, y);
+      }
+    } else {   // the dims before and behind the rotated ones
+      int d = 8 * (u - st.turned);
+      if (d >= st.first && st.rotary) d += st.rotary;
+      load8(from + d, x);
+      if (!live)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+      store8(to + d, x);
+    }
+  }
+}
+
+int log2_of(int page) {
+  int n = 0;
+  while ((1 << n) < page) ++n;
+  return n;
+}
+
+template <class X, class T>
+void launch_append(const AppendArgs& args, bool interleaved, unsigned grid, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  XTG_CUDA(interleaved ? cudaLaunchKernelEx(&cfg, append_kernel<X, T, true>, args)
+                       : cudaLaunchKernelEx(&cfg, append_kernel<X, T, false>, args));
+}
+
+// A pool's map: boxes of 64 dims x `box` slots of a page and KV head
+CUtensorMap pool_map(const void* pool, int dtype, int dims, int page, int heads, int64_t pages, int64_t slot, int64_t head,
+                     int64_t page_stride, int box) {
+  static std::mutex mu;
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!encode) {
+      cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+      void* fn = nullptr;
+      XTG_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+      XTG_REQUIRE(fn && q == cudaDriverEntryPointSuccess, "kv16: no cuTensorMapEncodeTiled in the driver");
+      encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }
+  }
+  CUtensorMap map;
+  const cuuint64_t size[4] = {(cuuint64_t)dims, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)pages};
+  // a stride that nothing steps by may be any
+  const cuuint64_t strides[3] = {(cuuint64_t)(slot * 2), (cuuint64_t)((heads > 1 ? head : dims) * 2),
+                                 (cuuint64_t)((pages > 1 ? page_stride : dims) * 2)};
+  const cuuint32_t boxes[4] = {64u, (cuuint32_t)box, 1u, 1u};
+  const cuuint32_t steps[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = encode(&map, dtype == kKv16Bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                            const_cast<void*>(pool), size, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  XTG_REQUIRE(r == CUDA_SUCCESS, "kv16: cuTensorMapEncodeTiled failed");
+  return map;
+}
+
+// Looks at a barrier before a wait gives up: about a second, no wait begins before the kernels it depends on have ended.
+constexpr uint32_t kPolls = 1u << 18;
+std::atomic<uint32_t> wait_polls{kPolls};
+
+}  // namespace
+
+bool kv16_dims(bool latent, int head_dim, int v_dim) {
+  return kv16::by_shape<__nv_bfloat16>(latent, head_dim, v_dim, 16, [](auto) {});
+}
+
+void launch_kv16_append(const Kv16Cache& c, const Kv16Append& r, int sms, cudaStream_t s) {
+  AppendArgs a = {};
+  auto stream = [&](const void* src, int64_t row, int64_t head, int heads, int dims, bool turned, int64_t out_head) {
+    Stream st = {src, row, head, src ? heads : 0, 0, 0, dims, 0, 0, out_head};
+    if (turned && r.rotary) {
+      st.first = r.first;
+      st.rotary = r.rotary;
+      st.turned = r.interleaved ? r.rotary / 8 : r.rotary / 16;
+    }
+    st.units = st.turned + (dims - st.rotary) / 8;
+    return st;
+  };
+  const int turned_dims = c.latent ? c.head_dim - c.v_dim : c.head_dim;
+  a.st[0] = stream(r.q, r.q_row, r.q_head, r.heads, turned_dims, true, 0);
+  a.st[1] = stream(r.k, r.k_row, r.k_head, c.kv_heads, turned_dims, true, c.k_head);
+  a.st[2] = stream(r.v, r.v_row, r.v_head, c.kv_heads, c.v_dim, false, c.latent ? c.k_head : c.v_head);
+  a.q_out = r.q_out;
+  a.k = c.k;
+  a.v = c.latent ? c.k : c.v;
+  a.k_page = c.k_page;
+  a.k_slot = c.k_slot;
+  a.v_page = c.latent ? c.k_page : c.v_page;
+  a.v_slot = c.latent ? c.k_slot : c.v_slot;
+  a.k_dim0 = c.latent ? c.v_dim : 0;
+  a.table = c.table;
+  a.pos = c.pos;
+  a.cu_rows = c.cu_rows;
+  a.freq = r.freq;
+  a.pages = c.pages;
+  a.rows = c.rows;
+  a.max_pages = c.max_pages;
+  a.seqs = c.seqs;
+  a.page_log2 = log2_of(c.page);
+  a.half = r.rotary / 2;
+  a.err = c.err;
+  // several rows a CTA share its start where there are rows enough to fill the GPU
+  a.rows_per_cta = c.rows >= (int64_t)sms * 8 * kMaxRowsPerCta ? kMaxRowsPerCta : 1;
+  const int64_t grid = (c.rows + a.rows_per_cta - 1) / a.rows_per_cta;
+  auto by_cache = [&](auto x) {
+    using X = decltype(x);
+    if (c.dtype == kKv16Bf16)
+      launch_append<X, __nv_bfloat16>(a, r.interleaved, (unsigned)grid, s);
+    else
+      launch_append<X, __half>(a, r.interleaved, (unsigned)grid, s);
+  };
+  if (r.dtype == kKv16F32)
+    by_cache(float());
+  else if (r.dtype == kKv16Bf16)
+    by_cache(__nv_bfloat16());
+  else
+    by_cache(__half());
+}
+
+int64_t kv16_workspace_bytes(bool latent, int head_dim, int v_dim, int group, int rows_per_seq, int sms) {
+  int64_t bytes = -1;
+  kv16::by_shape<__nv_bfloat16>(latent, head_dim, v_dim, kv16::block_rows(latent, (int64_t)group * rows_per_seq),
+                                [&](auto shape) {
+                                  bytes = kv16::work_bytes<decltype(shape)>(std::min(sms, kv16::kMaxGrid));
+                                });
+  return bytes;
+}
+
+int kv16_wait_polls(int polls) {
+  return (int)(polls < 0 ? wait_polls.load() : wait_polls.exchange(std::min((uint32_t)polls, 1u << 24)));
+}
+
+void launch_kv16_attention(const Kv16Cache& c, const Kv16Attn& r, int sms, cudaStream_t s) {
+  kv16::Params p = {};
+  const int group = r.heads / c.kv_heads;
+  // chunks of 128 positions, of 64 where the keys are wide (Shape::C)
+  const int box = std::min(c.page, c.head_dim <= 192 ? 128 : 64);
+  p.kmap = pool_map(c.k, c.dtype, c.head_dim, c.page, c.kv_heads, c.pages, c.k_slot, c.k_head, c.k_page, box);
+  p.vmap = c.latent ? p.kmap : pool_map(c.v, c.dtype, c.v_dim, c.page, c.kv_heads, c.pages, c.v_slot, c.v_head, c.v_page, box);
+  p.q = r.q;
+  p.q_rot = r.q_rot;
+  p.out = r.out;
+  p.q_row = r.q_row;
+  p.q_head = r.q_head;
+  p.r_row = r.r_row;
+  p.r_head = r.r_head;
+  p.v = static_cast<const uint8_t*>(c.latent ? c.k : c.v);
+  p.v_page = c.latent ? c.k_page : c.v_page;
+  p.v_head = c.latent ? c.k_head : c.v_head;
+  p.v_slot = c.latent ? c.k_slot : c.v_slot;
+  p.table = c.table;
+  p.pos = c.pos;
+  p.cu_rows = c.cu_rows;
+  p.pages = c.pages;
+  p.rows = c.rows;
+  p.max_pages = c.max_pages;
+  p.seqs = c.seqs;
+  p.page_log2 = log2_of(c.page);
+  p.heads = r.heads;
+  p.kv_heads = c.kv_heads;
+  p.group = group;
+  p.window = r.window;
+  p.scale = r.scale;
+  p.zero_rest = r.zero_rest;
+  p.err = c.err;
+  p.work = static_cast<float*>(r.work);
+  p.polls = wait_polls.load(std::memory_order_relaxed);
+  const int rows = kv16::block_rows(c.latent, (int64_t)group * r.rows_per_seq);
+  const int grid = std::min(sms, kv16::kMaxGrid);
+  if (c.dtype == kKv16Bf16)
+    kv16::launch<__nv_bfloat16>(p, c.latent, c.head_dim, c.v_dim, rows, grid, s);
+  else
+    kv16::launch<__half>(p, c.latent, c.head_dim, c.v_dim, rows, grid, s);
+}
+
+}  // namespace xtg

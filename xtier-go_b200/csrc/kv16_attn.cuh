@@ -1,0 +1,959 @@
+// Attention over the 16-bit paged caches: every row sees the cached positions up to its own (with a window only the last
+// `window` of these), and
+//
+//   o[r] = sum_p P[r][p] V[p] / sum_p P[r][p],  P[r][p] = 2^(S[r][p] - m[r]),  S = log2(e) scale q[r] . K[p]
+//
+// Both products run on tcgen05.mma transposed, so that the cache is the wide operand whatever the number of rows:
+// S^T = K Q^T has a chunk's positions as the instruction's M and the rows as its N (16 .. 128), o^T = V^T P^T the dims of V
+// as M. K and V are used as TMA brings them (128-byte swizzle: K as a K-major, V as an MN-major operand), no thread touches
+// them; of a latent cache one tile is both. S^T and o^T lie in tensor memory; a thread of the softmax warps has one position
+// and the rows as columns, so a chunk's sums need no exchange between threads until the part's end. P^T is written back to
+// shared memory as 16-byte pieces (8 rows of a position), the unswizzled MN-major operand.
+//
+// m[r] is a reference that is at most 2^kSlack below the largest score so far: it moves, and o and the sums are scaled, only
+// when a score passes that. P is rounded to the cache's type for the second product and summed up as rounded; sums and o
+// are f32.
+//
+// One CTA per SM takes an equal share of all (sequence, row block, KV head, chunk) items in that order, whatever the
+// sequences' lengths; a part that a share cuts goes to the workspace in f32 and a second kernel joins the parts in order.
+// The warps of a CTA: one walks the share and issues the copies, one issues the products, the others are the softmax's.
+// Every wait is bounded.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "fp4mma.cuh"
+#include "kv16.h"
+
+namespace xtg {
+
+namespace kv16 {
+
+constexpr int kSmem = 232448;      // shared memory of a CTA
+constexpr int kCtrl = 3072;        // of it for barriers and per-row values
+constexpr int kMaxGrid = 256;
+constexpr float kSlack = 6.f;
+constexpr float kFloor = -3.0e38f;   // the least reference of a row that has seen a position
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kPartCost = 1;       // a part's start and end, in chunks, where shares are cut
+
+template <class T_, int DK_, int DV_, bool LATENT_, int N_>
+struct Shape {
+  using T = T_;
+  static constexpr int DK = DK_, DV = DV_, N = N_;
+  static constexpr bool LATENT = LATENT_;
+  static constexpr int C = DK <= 192 ? 128 : 64;   // positions of a chunk: the first product's M
+  static constexpr int WG = N >= 64 ? 2 : 1;       // groups of 4 softmax warps, each with NW of the rows
+  static constexpr int NW = N / WG;
+  static constexpr int kThreads = WG * 128 + 64;
+  static constexpr int kSlotBytes = (DK > DV ? DK : DV) * C * 2;
+  static constexpr int kQBytes = N * DK * 2, kPBytes = N * C * 2;
+  static constexpr int PB = N <= 32 ? 2 : 1;       // buffers of P
+  static constexpr int kFit = (kSmem - kCtrl - kQBytes - PB * kPBytes) / kSlotBytes;
+  static constexpr int R = kFit > 12 ? 12 : kFit;  // slots of the ring
+  static constexpr int kSmemBytes = R * kSlotBytes + kQBytes + PB * kPBytes + kCtrl;
+  static constexpr int MO = DV >= 128 ? 128 : 64, DT = DV / MO;   // the second product's M, and how many of them
+  static constexpr int kO = 2 * N;                 // tensor memory: S^T twice, then o^T
+  static constexpr int kUsed = 2 * N + DT * N;
+  static constexpr int kCols = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
+  static_assert(R >= (LATENT ? 2 : 3) && kUsed <= 512, "shape");
+};
+
+// ---- the walk over a share ----
+
+struct Params {
+  CUtensorMap kmap, vmap;
+  const void *q, *q_rot;
+  void* out;
+  int64_t q_row, q_head, r_row, r_head;
+  const uint8_t* v;   // for values that are not finite
+  int64_t v_page, v_head, v_slot;
+  const int32_t *table, *pos, *cu_rows;
+  int64_t pages, rows;
+  int max_pages, seqs, page_log2, heads, kv_heads, group, window;
+  int slots;   // (sequence, row block) numbers, some of them empty
+  float scale;
+  bool zero_rest;
+  int32_t* err;
+  float* work;
+  uint32_t polls;
+};
+
+// sequence s's first row, within the call's rows (a bad cu_rows shortens sequences, never reaches outside)
+__device__ __forceinline__ int64_t row_bound(const Params& a, int s) {
+  const int64_t c = a.cu_rows[s];
+  return c < 0 ? 0 : c > a.rows ? a.rows : c;
+}
+
+// A row block is N consecutive (row, q head of the KV head's group) pairs of a sequence. Sequence s's blocks have numbers
+// from cu_rows[s] group / N + s on: at least as many as it needs, found without a prefix sum over the sequences.
+struct Block {
+  int s, p0;         // sequence, the position of its first row
+  int64_t row0, f0;  // the call's row of the sequence's first, and the block's first pair in the sequence
+  int count;         // pairs, 0: none
+  int c0, chunks;    // the first chunk that one of its rows sees, and how many
+  int64_t first, last;   // positions of its first and last row
+};
+
+template <class S>
+__device__ __forceinline__ int64_t block_start(const Params& a, int s) {
+  return row_bound(a, s) * a.group / S::N + s;
+}
+
+template <class S>
+__device__ __forceinline__ int find_sequence(const Params& a, int64_t number) {
+  int lo = 0, hi = a.seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (block_start<S>(a, mid) <= number)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+template <class S>
+__device__ __forceinline__ Block block_of(const Params& a, int s, int64_t number) {
+  Block b;
+  b.s = s;
+  b.row0 = row_bound(a, s);
+  const int64_t n = row_bound(a, s + 1) - b.row0, pairs = n > 0 ? n * a.group : 0;
+  b.f0 = (number - block_start<S>(a, s)) * S::N;
+  const int64_t left = pairs - b.f0;
+  b.count = b.f0 < 0 || left <= 0 ? 0 : left < S::N ? (int)left : S::N;
+  b.p0 = a.pos[s];
+  b.chunks = b.c0 = 0;
+  if (b.count == 0) return b;
+  b.first = b.p0 + b.f0 / a.group;
+  b.last = b.p0 + (b.f0 + b.count - 1) / a.group;
+  const int64_t end = (int64_t)a.max_pages << a.page_log2;
+  const int64_t lo = a.window > 0 && b.first - a.window + 1 > 0 ? b.first - a.window + 1 : 0;
+  const int64_t hi = b.last + 1 < end ? b.last + 1 : end;
+  if (lo < hi) {
+    b.c0 = (int)(lo / S::C);
+    b.chunks = (int)((hi + S::C - 1) / S::C) - b.c0;
+  }
+  return b;
+}
+
+struct Part {
+  Block b;
+  int head, from, count;   // KV head, chunks c0 + from .. c0 + from + count - 1
+  int slot;                // of the workspace, -1: the whole item
+};
+
+// What the joining kernel needs about the item that starts in a CTA's share and ends in another's
+struct Cut {
+  int64_t row0, f0;
+  int head, count, last;   // count 0: there is none
+};
+
+template <class S>
+struct Share {   // the part of all items that a CTA takes, in units of chunks
+  int64_t from, to, each;
+  int64_t number, base;   // where it starts: a block's number and the units before it
+};
+
+template <class S>
+__host__ __device__ constexpr int64_t part_floats() {
+  return (int64_t)S::N * (S::DV + 2);
+}
+// workspace: 2 parts a CTA (acc [N][DV], then reference and sum [N][2]), then the cuts
+template <class S>
+__host__ __device__ constexpr int64_t work_bytes(int grid) {
+  return 2 * (int64_t)grid * part_floats<S>() * 4 + (int64_t)grid * (int64_t)sizeof(Cut);
+}
+
+template <class S>
+struct Walk {
+  const Params& a;
+  Share<S> sh;
+  Block b;
+  int s;
+  int64_t number, base;
+  int head;
+  bool have;
+
+  __device__ Walk(const Params& a_, const Share<S>& sh_) : a(a_), sh(sh_), number(sh_.number), base(sh_.base), head(0) {
+    have = sh.from < sh.to;
+    if (have) {
+      s = find_sequence<S>(a, number);
+      b = block_of<S>(a, s, number);
+    }
+  }
+
+  // The next part of the share; cut: filled for an item that goes on in other shares
+  __device__ bool next(Part& p, Cut& cut) {
+    while (have && base < sh.to) {
+      if (b.count > 0 && head < a.kv_heads) {
+        const int64_t at = base + kPartCost;   // the item's first chunk
+        const int64_t from = sh.from - at, to = sh.to - at;
+        const int h = head++;
+        const int64_t here = base;
+        base += kPartCost + b.chunks;
+        if (b.chunks == 0) {
+          if (here < sh.from) continue;
+          p = {b, h, 0, 0, -1};
+          return true;
+        }
+        const int i = from < 0 ? 0 : from > b.chunks ? b.chunks : (int)from;
+        const int j = to < 0 ? 0 : to > b.chunks ? b.chunks : (int)to;
+        if (i >= j) continue;
+        const bool starts = i == 0, ends = j == b.chunks;
+        p = {b, h, i, j - i, starts && ends ? -1 : starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x};
+        if (starts && !ends) cut = {b.row0, b.f0, h, b.count, (int)((at + b.chunks - 1) / sh.each)};
+        return true;
+      }
+      head = 0;
+      if (++number >= a.slots) return have = false;
+      if (s + 1 < a.seqs && block_start<S>(a, s + 1) <= number) ++s;
+      b = block_of<S>(a, s, number);
+    }
+    return false;
+  }
+};
+
+// ---- waits ----
+
+__device__ __forceinline__ void give_up(int* failed, int32_t* err) {
+  atomicExch(failed, 1);
+  if (err) atomicExch(err, 1);
+}
+
+// false: it gave up, after `polls` more looks than one (a look that finds nothing takes about 4 us), or after one once
+// another wait of the CTA has
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t polls, int* failed, int32_t* err) {
+  uint32_t spins = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    ++spins;
+    if (spins > polls || *reinterpret_cast<volatile int*>(failed)) {
+      give_up(failed, err);
+      return false;
+    }
+  }
+  return true;
+}
+
+// whether any of the `threads` threads of named barrier `id` votes yes
+__device__ __forceinline__ bool vote(int id, int threads, bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{ .reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q; }"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"((uint32_t)yes)
+      : "memory");
+  return r != 0;
+}
+
+// ---- tensor memory and operands ----
+
+constexpr uint64_t kSwizzle128 = 2ull << 61;
+__device__ __forceinline__ uint64_t operand(uint32_t saddr, uint32_t lbo, uint32_t sbo, uint64_t swizzle) {
+  return smem_desc(saddr, lbo, sbo) | swizzle;
+}
+
+// the instruction: f32 sums, A and B of type T, M x N; transposed operands are MN-major
+template <class T>
+__host__ __device__ constexpr uint32_t instruction(int m, int n, bool transposed) {
+  const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1 : 0, tr = transposed ? 1 : 0;
+  return (1u << 4) | (type << 7) | (type << 10) | (tr << 15) | (tr << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(
+          d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
+  uint32_t r[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(v[j]);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// a box of the cache: dims x .., slots y .., KV head z, page w
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// ---- values of the cache's type ----
+
+__device__ __forceinline__ uint32_t pack(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi, __half) { return pack_f16x2(lo, hi); }
+__device__ __forceinline__ float2 unpack(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ __nv_bfloat16 narrow(float x, __nv_bfloat16) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ __half narrow(float x, __half) { return __float2half_rn(x); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// floats as integers of the same order (NaN aside), for atomicMax
+__device__ __forceinline__ int ordered(float x) {
+  const int i = __float_as_int(x);
+  return i >= 0 ? i : i ^ 0x7fffffff;
+}
+__device__ __forceinline__ float of_ordered(int i) { return __int_as_float(i >= 0 ? i : i ^ 0x7fffffff); }
+
+// Over the lanes of a warp, each of M values: halves of the set change places at lane distances 16, 8, .. until every lane
+// has M / 32 values (or one, shared by 32 / M lanes). Value j of lane l is then number
+// column(l, j) of the set.
+template <int M, class F>
+__device__ __forceinline__ void spread(float (&v)[M], F f) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 16, m = M; d > 0; d >>= 1) {
+    if (m > 1) {
+      m >>= 1;
+      const bool up = lane & d;
+#pragma unroll
+      for (int j = 0; j < M / 2; ++j)
+        if (j < m) {
+          const float other = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + m], d);
+          v[j] = f(up ? v[j + m] : v[j], other);
+        }
+    } else {
+      v[0] = f(v[0], __shfl_xor_sync(0xffffffffu, v[0], d));
+    }
+  }
+}
+template <int M>
+__device__ __forceinline__ int spread_column(int j) {
+  const int lane = threadIdx.x & 31;
+  int c = j;
+#pragma unroll
+  for (int d = 16, m = M; d > 0; d >>= 1)
+    if (m > 1) {
+      m >>= 1;
+      if (lane & d) c += m;
+    }
+  return c;
+}
+
+// ---- the CTA's shared memory ----
+
+constexpr int kInfo = 16, kQueue = 4;
+
+struct Ctrl {
+  uint64_t full[12], empty[12], sfull[2], sfree[2], pready[2], pdone[2], qready, done, queue_full[kQueue],
+      queue_empty[kQueue];
+  Part queue[kQueue];
+  uint32_t info[kInfo];   // of chunks in turn: the pieces that are there
+  int64_t share_number, share_base, scan[12];
+  uint32_t tmem;
+  int failed;
+  int bad_chunks;                 // chunks with values that are not finite at positions that some rows see: how many
+  int bad_at[4];                  // and which
+  uint32_t bad[4][4];             // their positions
+};
+template <class S>
+struct Rows {
+  float ref[S::N], alpha[S::N];
+  int top[S::N];   // ordered()
+  int place[S::N];   // row in the block << 16 | q head
+};
+
+template <class S>
+struct Where {   // this thread's place among the softmax threads
+  int group, lane4;   // which rows, and the quarter of the tensor memory's lanes
+  int lane, at;       // the position of a chunk that it has
+  bool active;
+};
+
+// Whether position p is seen by the row at position t
+__device__ __forceinline__ bool sees(int64_t t, int64_t p, int window) { return p <= t && (window == 0 || p > t - window); }
+
+template <class S>
+__global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_constant__ Params a) {
+  using T = typename S::T;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* ring = smem;
+  uint8_t* qbuf = smem + S::R * S::kSlotBytes;
+  uint8_t* pbuf = qbuf + S::kQBytes;
+  Ctrl& c = *reinterpret_cast<Ctrl*>(pbuf + S::PB * S::kPBytes);
+  Rows<S>& rows = *reinterpret_cast<Rows<S>*>(&c + 1);
+  static_assert(sizeof(Ctrl) + sizeof(Rows<S>) <= kCtrl, "control block");
+  constexpr int kSoftmaxWarps = 4 * S::WG, kProducer = kSoftmaxWarps, kIssuer = kSoftmaxWarps + 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (warp == kIssuer) tmem_alloc(&c.tmem, S::kCols);
+  if (tid == 0) {
+    for (int i = 0; i < S::R; ++i) {
+      mbar_init(&c.full[i], 1);
+      mbar_init(&c.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&c.sfull[i], 1);
+      mbar_init(&c.sfree[i], kSoftmaxWarps);
+      mbar_init(&c.pready[i], kSoftmaxWarps);
+      mbar_init(&c.pdone[i], 1);
+    }
+    mbar_init(&c.qready, kSoftmaxWarps);
+    mbar_init(&c.done, 1);
+    for (int i = 0; i < kQueue; ++i) {
+      mbar_init(&c.queue_full[i], 1);
+      mbar_init(&c.queue_empty[i], kSoftmaxWarps + 1);
+    }
+    c.failed = 0;
+    mbar_init_fence();
+  }
+  for (int i = tid; i < S::N; i += S::kThreads) rows.top[i] = ordered(-INFINITY);
+
+  // ---- the share: every thread the cost of some blocks, then a sum over the CTA ----
+  pdl_wait();
+  pdl_launch_next();
+  const int each = (a.slots + S::kThreads - 1) / S::kThreads;
+  const int first = min(tid * each, a.slots), last = min(first + each, a.slots);
+  auto cost = [&](const Block& b) { return b.count > 0 ? (int64_t)(b.chunks + kPartCost) * a.kv_heads : (int64_t)0; };
+  auto over_blocks = [&](auto&& f) {
+    if (first >= last) return;
+    int s = find_sequence<S>(a, first);
+    for (int i = first; i < last; ++i) {
+      if (s + 1 < a.seqs && block_start<S>(a, s + 1) <= i) ++s;
+      const Block b = block_of<S>(a, s, i);
+      if (f(i, b)) break;
+    }
+  };
+  int64_t mine = 0;
+  over_blocks([&](int, const Block& b) {
+    if (blockIdx.x == 0 && a.err && b.count > 0 && b.last >= (int64_t)a.max_pages << a.page_log2) atomicExch(a.err, 6);
+    mine += cost(b);
+    return false;
+  });
+  int64_t before = mine;   // over the warp, itself included
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  if (lane == 31) c.scan[warp] = before;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int64_t total = 0;
+  before -= mine;
+#pragma unroll
+  for (int w = 0; w < S::kThreads / 32; ++w) {
+    if (w < warp) before += c.scan[w];
+    total += c.scan[w];
+  }
+  Share<S> sh;
+  sh.each = (total + gridDim.x - 1) / gridDim.x;
+  sh.from = sh.each * blockIdx.x;
+  sh.to = sh.from + sh.each < total ? sh.from + sh.each : total;
+  if (sh.from < sh.to && before <= sh.from && sh.from < before + mine) {
+    int64_t at = before;
+    over_blocks([&](int i, const Block& b) {
+      const int64_t x = cost(b);
+      if (sh.from < at + x) {
+        c.share_number = i;
+        c.share_base = at;
+        return true;
+      }
+      at += x;
+      return false;
+    });
+  }
+  __syncthreads();
+  sh.number = sh.from < sh.to ? c.share_number : 0;
+  sh.base = sh.from < sh.to ? c.share_base : 0;
+  const uint32_t tmem = c.tmem;
+  float* parts = a.work;
+  Cut* cuts = reinterpret_cast<Cut*>(parts + 2 * (int64_t)gridDim.x * part_floats<S>());
+  auto bounded = [&](uint64_t* bar, uint32_t parity) { return wait(bar, parity, a.polls, &c.failed, a.err); };
+
+  if (warp == kProducer) {
+    // ---- the walk and the copies: K of a chunk before V of the chunk before, as the products take them ----
+    constexpr int kSlicesK = S::DK / 64, kSlicesV = S::DV / 64;
+    const int box = min(1 << a.page_log2, S::C), pieces = S::C / box;
+    bool ok = true;
+    if (a.polls == 0) {   // without a look
+      give_up(&c.failed, a.err);
+      ok = false;
+    }
+    uint32_t entry = 0, chunk = 0, queued = 0;
+    Cut cut = {0, 0, 0, 0, 0};
+    Part p;
+    Walk<S> walk(a, sh);
+    auto copy = [&](const CUtensorMap* map, int slices, int head, int slot0, int page, uint32_t there) {
+      const int st = entry % S::R;
+      const uint32_t turn = entry / S::R;
+      if (turn > 0) ok = __all_sync(0xffffffffu, bounded(&c.empty[st], (turn - 1) & 1));
+      if (!ok) return;
+      if (lane == 0) mbar_expect_tx(&c.full[st], (uint32_t)(__popc(there) * slices * box * 128));
+      __syncwarp();
+      const uint32_t to = smem_u32(ring) + st * S::kSlotBytes;
+      for (int i = 0; i < pieces * slices; i += 32) {
+        const int x = i + lane, piece = x % pieces, slice = x / pieces;
+        const int pg = __shfl_sync(0xffffffffu, page, piece);
+        if (slice < slices && (there >> piece & 1))
+          load_box(to + slice * S::C * 128 + piece * box * 128, map, 64 * slice, slot0, head, pg, &c.full[st]);
+      }
+      ++entry;
+    };
+    while (walk.next(p, cut)) {
+      if (ok) {
+        const int qi = queued % kQueue;
+        if (queued >= kQueue) ok = __all_sync(0xffffffffu, bounded(&c.queue_empty[qi], (queued / kQueue - 1) & 1));
+        if (ok && lane == 0) {
+          c.queue[qi] = p;
+          mbar_arrive(&c.queue_full[qi]);
+        }
+        ++queued;
+      }
+      // lane i has the page of piece i; of the next chunk's ahead
+      const int64_t hi = min(p.b.last + 1, (int64_t)a.max_pages << a.page_log2);
+      const int64_t lo = a.window > 0 ? p.b.first - a.window + 1 : 0;
+      auto page_of = [&](int i) {
+        const int64_t at = (int64_t)(p.b.c0 + p.from + i) * S::C + lane * box;
+        if (i >= p.count || lane >= pieces || at >= hi || at + box <= lo) return -1;
+        const int64_t pg = a.table[(int64_t)p.b.s * a.max_pages + (at >> a.page_log2)];
+        if (pg >= a.pages) {
+          if (a.err) atomicExch(a.err, 7);
+          return -1;
+        }
+        return (int)pg;
+      };
+      int page = page_of(0), old_page = -1;
+      uint32_t old_there = 0;
+      int old_slot0 = 0;
+      for (int i = 0; i < p.count && ok; ++i, ++chunk) {
+        const int next_page = page_of(i + 1);
+        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+        const int slot0 = (int)(((int64_t)(p.b.c0 + p.from + i) * S::C) & ((1 << a.page_log2) - 1));
+        if (lane == 0) c.info[chunk % kInfo] = there;
+        copy(&a.kmap, kSlicesK, p.head, slot0, page, there);
+        if (!S::LATENT) {
+          if (i > 0 && ok) copy(&a.vmap, kSlicesV, p.head, old_slot0, old_page, old_there);
+          if (i == p.count - 1 && ok) copy(&a.vmap, kSlicesV, p.head, slot0, page, there);
+        }
+        old_page = page;
+        old_there = there;
+        old_slot0 = slot0;
+        page = next_page;
+      }
+    }
+    if (lane == 0) cuts[blockIdx.x] = cut;
+    if (ok) {   // the end of the queue
+      const int qi = queued % kQueue;
+      if (queued >= kQueue) ok = __all_sync(0xffffffffu, bounded(&c.queue_empty[qi], (queued / kQueue - 1) & 1));
+      if (ok && lane == 0) {
+        c.queue[qi].head = -1;
+        mbar_arrive(&c.queue_full[qi]);
+      }
+    }
+    // no copy is left in flight
+    for (uint32_t e = entry > (uint32_t)S::R ? entry - S::R : 0; e < entry; ++e) {
+      uint32_t spins = 0;
+      while (!mbar_try_wait(&c.full[e % S::R], (e / S::R) & 1))
+        if (++spins > (1u << 18)) break;
+    }
+    __syncwarp();
+  } else if (warp == kIssuer) {
+    // ---- the products, by one thread ----
+    if (lane == 0) {
+      constexpr uint32_t kS = instruction<T>(S::C, S::N, false), kOi = instruction<T>(S::MO, S::N, true);
+      const uint32_t ring0 = smem_u32(ring), q0 = smem_u32(qbuf), pb0 = smem_u32(pbuf);
+      uint32_t entry = 0, chunk = 0, filled = 0;
+      bool ok = a.polls != 0;
+      auto first_product = [&](uint32_t e) {   // S^T of chunk number `chunk`
+        const int st = e % S::R, buf = chunk & 1;
+        ok = ok && bounded(&c.full[st], (e / S::R) & 1);
+        if (chunk >= 2) ok = ok && bounded(&c.sfree[buf], ((chunk >> 1) - 1) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t k0 = ring0 + st * S::kSlotBytes, d = tmem + buf * S::N;
+#pragma unroll
+        for (int x = 0; x < S::DK; x += 16)
+          mma(d, operand(k0 + x / 64 * S::C * 128 + x % 64 * 2, 16, 1024, kSwizzle128),
+              operand(q0 + x / 64 * S::N * 128 + x % 64 * 2, 16, 1024, kSwizzle128), kS, x > 0);
+        tc_commit(&c.sfull[buf]);
+        if (!S::LATENT) tc_commit(&c.empty[st]);
+      };
+      auto second_product = [&](uint32_t e, uint32_t ch, bool accumulate) {   // o^T += of chunk number ch
+        const int st = e % S::R, pb = ch % S::PB;
+        ok = ok && bounded(&c.pready[pb], (ch / S::PB) & 1);
+        ok = ok && bounded(&c.full[st], (e / S::R) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t v0 = ring0 + st * S::kSlotBytes, p0 = pb0 + pb * S::kPBytes;
+#pragma unroll
+        for (int m = 0; m < S::DT; ++m)
+#pragma unroll
+          for (int x = 0; x < S::C; x += 16)
+            mma(tmem + S::kO + m * S::N, operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
+                operand(p0 + x * 16, 128, S::C * 16, 0), kOi, accumulate || x > 0);
+        tc_commit(&c.empty[st]);
+        tc_commit(&c.pdone[pb]);
+      };
+      for (uint32_t part = 0; ok; ++part) {
+        const int qi = part % kQueue;
+        ok = bounded(&c.queue_full[qi], (part / kQueue) & 1);
+        if (!ok) break;
+        const int n = c.queue[qi].count;
+        const bool end = c.queue[qi].head < 0;
+        mbar_arrive(&c.queue_empty[qi]);
+        if (end) break;
+        if (n == 0) continue;
+        ok = bounded(&c.qready, filled & 1);
+        ++filled;
+        tc_fence_after();
+        for (int i = 0; i < n && ok; ++i, ++chunk) {
+          first_product(S::LATENT ? entry + i : i == 0 ? entry : entry + 2 * i - 1);
+          if (i > 0) second_product(S::LATENT ? entry + i - 1 : entry + 2 * i, chunk - 1, i > 1);
+        }
+        if (ok) second_product(S::LATENT ? entry + n - 1 : entry + 2 * n - 1, chunk - 1, n > 1);
+        entry += S::LATENT ? n : 2 * n;
+      }
+      tc_commit(&c.done);
+      uint32_t spins = 0;   // every product has ended before the tensor memory goes back
+      while (!mbar_try_wait(&c.done, 0))
+        if (++spins > (1u << 18)) break;
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax ----
+    const int wg = warp >> 2, quarter = warp & 3, bar = 1 + wg;
+    const bool active = S::C == 128 || lane < 16;
+    const int at = S::C == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);   // this thread's position of a chunk
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
+    float* ref = rows.ref + wg * S::NW;
+    float* alpha = rows.alpha + wg * S::NW;
+    int* top = rows.top + wg * S::NW;
+    int* place = rows.place + wg * S::NW;
+    const int own = tid & 127;
+    const float sc = a.scale * kLog2e;
+    uint32_t chunk = 0, entry = 0;
+    bool bad = false;
+    for (uint32_t part = 0;; ++part) {
+      const int qi = part % kQueue;
+      bad = !__all_sync(0xffffffffu, bounded(&c.queue_full[qi], (part / kQueue) & 1));
+      if (vote(bar, 128, bad)) {
+        bad = true;
+        break;
+      }
+      const Part p = c.queue[qi];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.queue_empty[qi]);
+      if (p.head < 0) break;
+      const int64_t t0 = p.b.f0 / a.group;
+      const int j0 = (int)(p.b.f0 % a.group);
+      // q's rows into the first product's operand, zeros past the last; rows' places and references
+      if (p.count > 0) {
+        constexpr int kUnits = S::DK / 8;   // 16-byte pieces of a row
+        for (int i = tid; i < S::N * kUnits; i += kSoftmaxWarps * 32) {
+          const int r = i / kUnits, u = i % kUnits;
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (r < p.b.count) {
+            const int64_t t = p.b.row0 + t0 + (j0 + r) / a.group;
+            const int64_t h = (int64_t)p.head * a.group + (j0 + r) % a.group;
+            if (S::LATENT && u >= S::DV / 8)
+              x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q_rot) + t * a.r_row + h * a.r_head + 8 * u - S::DV);
+            else
+              x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + t * a.q_row + h * a.q_head + 8 * u);
+          }
+          *reinterpret_cast<uint4*>(qbuf + u / 8 * S::N * 128 + r * 128 + ((u ^ r) & 7) * 16) = x;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.qready);
+      }
+      if (own < S::NW) {
+        const int r = wg * S::NW + own;
+        place[own] = (j0 + r) / a.group << 16 | (j0 + r) % a.group;
+        ref[own] = -INFINITY;
+      }
+      named_bar_sync(bar, 128);
+      float l[S::NW];
+#pragma unroll
+      for (int r = 0; r < S::NW; ++r) l[r] = 0.f;
+
+      for (int i = 0; i < p.count; ++i, ++chunk) {
+        const int buf = chunk & 1;
+        bad = !__all_sync(0xffffffffu, bounded(&c.sfull[buf], (chunk >> 1) & 1)) || bad;
+        tc_fence_after();
+        float y[S::NW];
+        auto load_scores = [&] {
+#pragma unroll
+          for (int r = 0; r < S::NW; r += 16)
+            tmem_ld16(lanes + buf * S::N + wg * S::NW + r, *reinterpret_cast<float(*)[16]>(&y[r]));
+          tmem_ld_wait();
+        };
+        load_scores();
+        const int64_t start = (int64_t)(p.b.c0 + p.from + i) * S::C, pos = start + at;
+        const uint32_t there = c.info[chunk % kInfo];
+        const int box = min(1 << a.page_log2, S::C);
+        const uint32_t all = (1u << (S::C / box)) - 1;
+        const bool clean = there == all && start + S::C - 1 <= p.b.first && (a.window == 0 || start > p.b.last - a.window);
+        const bool here = active && (clean || (there >> (at / box) & 1));
+        // scores less the reference; what a row does not see is -infinity
+        float most = -INFINITY;
+        uint32_t hidden[(S::NW + 31) / 32];
+#pragma unroll
+        for (int r = 0; r < (S::NW + 31) / 32; ++r) hidden[r] = here ? 0u : 0xffffffffu;
+        if (!clean && here) {
+#pragma unroll
+          for (int r = 0; r < S::NW; ++r)
+            if (!sees(p.b.first + (place[r] >> 16), pos, a.window)) hidden[r / 32] |= 1u << (r % 32);
+        }
+        const bool any_hidden = !clean || !active;
+        auto less_reference = [&] {
+#pragma unroll
+          for (int r = 0; r < S::NW; ++r) y[r] = fmaf(y[r], sc, -ref[r]);
+          if (any_hidden)
+#pragma unroll
+            for (int r = 0; r < S::NW; ++r)
+              if (hidden[r / 32] >> (r % 32) & 1) y[r] = -INFINITY;
+        };
+        less_reference();
+#pragma unroll
+        for (int r = 0; r < S::NW; ++r) most = max_nan(most, y[r]);
+        if (vote(bar, 128, bad || !(most <= kSlack))) {
+          // a new reference
+          load_scores();
+#pragma unroll
+          for (int r = 0; r < S::NW; ++r) {
+            y[r] = fmaxf(y[r] * sc, kFloor);
+            if (any_hidden && (hidden[r / 32] >> (r % 32) & 1)) y[r] = -INFINITY;
+          }
+          spread<S::NW>(y, [](float u, float v) { return fmaxf(u, v); });
+#pragma unroll
+          for (int j = 0; j < (S::NW + 31) / 32; ++j) atomicMax(&top[spread_column<S::NW>(j)], ordered(y[j]));
+          if (vote(bar, 128, bad)) {
+            bad = true;
+            break;
+          }
+          if (own < S::NW) {
+            const float old = ref[own], now = fmaxf(old, of_ordered(top[own]));
+            alpha[own] = now == old ? 1.f : ex2_approx(old - now);
+            ref[own] = now;
+            top[own] = ordered(-INFINITY);
+          }
+          named_bar_sync(bar, 128);
+          load_scores();
+          less_reference();
+#pragma unroll
+          for (int r = 0; r < S::NW; ++r) l[r] *= alpha[r];
+          if (i > 0) {   // the sums so far
+            const uint32_t b = (chunk - 1) % S::PB;
+            bad = !__all_sync(0xffffffffu, bounded(&c.pdone[b], ((chunk - 1) / S::PB) & 1));
+            if (!bad) {
+              tc_fence_after();
+#pragma unroll 1
+              for (int m = 0; m < S::DT; ++m)
+#pragma unroll 1
+                for (int r = 0; r < S::NW; r += 16) {
+                  float o[16];
+                  const uint32_t t = lanes + S::kO + m * S::N + wg * S::NW + r;
+                  tmem_ld16(t, o);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) o[j] *= alpha[r + j];
+                  tmem_st16(t, o);
+                }
+              tmem_st_wait();
+              tc_fence_before();
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.sfree[buf]);
+        // P, rounded, and its sums
+        uint32_t w[S::NW / 2];
+#pragma unroll
+        for (int r = 0; r < S::NW; r += 2) {
+          w[r / 2] = pack(ex2_approx(y[r]), ex2_approx(y[r + 1]), T());
+          const float2 f = unpack(w[r / 2], T());
+          l[r] += f.x;
+          l[r + 1] += f.y;
+        }
+        const uint32_t pb = chunk % S::PB;
+        if (chunk >= (uint32_t)S::PB)
+          bad = !__all_sync(0xffffffffu, bounded(&c.pdone[pb], (chunk / S::PB - 1) & 1)) || bad;
+        if (active) {
+          uint8_t* to = pbuf + pb * S::kPBytes + wg * (S::NW / 8) * S::C * 16 + at * 16;
+#pragma unroll
+          for (int r = 0; r < S::NW / 8; ++r)
+            *reinterpret_cast<uint4*>(to + r * S::C * 16) = make_uint4(w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]);
+        }
+        if (!clean && wg == 0) {
+          // V of positions that no row sees is whatever lay there: zeros, since 0 x NaN is no 0
+          const uint32_t e = S::LATENT ? entry + i : i == p.count - 1 ? entry + 2 * p.count - 1 : entry + 2 * i + 2;
+          bad = !__all_sync(0xffffffffu, bounded(&c.full[e % S::R], (e / S::R) & 1)) || bad;
+          const bool seen = here && pos <= p.b.last && (a.window == 0 || pos > p.b.first - a.window);
+          if (active && !seen && !bad) {
+            uint8_t* v = ring + e % S::R * S::kSlotBytes + at * 128;
+            for (int u = 0; u < S::DV / 8; ++u)
+              *reinterpret_cast<uint4*>(v + u / 8 * S::C * 128 + (u % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.pready[pb]);
+      }
+      entry += S::LATENT ? p.count : 2 * p.count;
+
+      // ---- the part's end: the rows' sums over all positions, then o ----
+      if (p.count > 0 && !bad) {
+        const uint32_t b = (chunk - 1) % S::PB;
+        bad = !__all_sync(0xffffffffu, bounded(&c.pdone[b], ((chunk - 1) / S::PB) & 1));
+      }
+      if (vote(bar, 128, bad)) {
+        bad = true;
+        break;
+      }
+      float* sums = reinterpret_cast<float*>(pbuf) + wg * 4 * S::NW;   // P's place
+      spread<S::NW>(l, [](float u, float v) { return u + v; });
+#pragma unroll
+      for (int j = 0; j < (S::NW + 31) / 32; ++j) sums[quarter * S::NW + spread_column<S::NW>(j)] = l[j];
+      named_bar_sync(bar, 128);
+      float* acc = parts + (int64_t)p.slot * part_floats<S>();
+      if (own < S::NW) {
+        const float sum = (sums[own] + sums[S::NW + own]) + (sums[2 * S::NW + own] + sums[3 * S::NW + own]);
+        alpha[own] = ref[own] == -INFINITY ? 0.f : 1.f / sum;
+        if (p.slot >= 0) {
+          float* ml = acc + S::N * S::DV + 2 * (wg * S::NW + own);
+          ml[0] = ref[own];
+          ml[1] = sum;
+        }
+      }
+      named_bar_sync(bar, 128);
+      tc_fence_after();
+      const int mine_rows = min(S::NW, p.b.count - wg * S::NW);
+      const bool has_dim = S::MO == 128 || lane < 16;
+      const int dim0 = S::MO == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);
+#pragma unroll 1
+      for (int m = 0; m < S::DT; ++m)
+#pragma unroll 1
+        for (int r = 0; r < S::NW; r += 16) {
+          if (r >= mine_rows) break;
+          float o[16];
+          if (p.count > 0) {
+            tmem_ld16(lanes + S::kO + m * S::N + wg * S::NW + r, o);
+            tmem_ld_wait();
+          }
+          const int d = m * S::MO + dim0;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (has_dim && r + j < mine_rows) {
+              if (p.slot >= 0) {
+                acc[(int64_t)(wg * S::NW + r + j) * S::DV + d] = o[j];
+              } else {
+                const int64_t t = p.b.row0 + t0 + (place[r + j] >> 16);
+                const int64_t h = (int64_t)p.head * a.group + (place[r + j] & 0xffff);
+                const float f = ref[r + j] == -INFINITY ? 0.f : o[j] * alpha[r + j];
+                static_cast<T*>(a.out)[(t * a.heads + h) * S::DV + d] = narrow(f, T());
+              }
+            }
+        }
+      tc_fence_before();
+    }
+    if (bad) {   // a wait gave up: NaN for the rows of the share
+      Walk<S> walk(a, sh);
+      Part p;
+      Cut cut;
+      while (walk.next(p, cut)) {
+        const int64_t t0 = p.b.f0 / a.group;
+        const int j0 = (int)(p.b.f0 % a.group);
+        for (int r = wg * S::NW; r < min((wg + 1) * S::NW, p.b.count); ++r) {
+          if (p.slot >= 0) {
+            if (own < 2) parts[(int64_t)p.slot * part_floats<S>() + S::N * S::DV + 2 * r + own] = NAN;
+          } else {
+            const int64_t t = p.b.row0 + t0 + (j0 + r) / a.group;
+            const int64_t h = (int64_t)p.head * a.group + (j0 + r) % a.group;
+            for (int d = own; d < S::DV; d += 128) static_cast<T*>(a.out)[(t * a.heads + h) * S::DV + d] = narrow(NAN, T());
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kIssuer) tmem_dealloc(tmem, S::kCols);
+}
+
+// Joins the parts of the item that starts in CTA c's share and ends in another's: one block per (c, row). The blocks past
+// these write zeros for the rows that are no sequence's.
+constexpr int kJoinThreads = 128;
+template <class S>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
+  using T = typename S::T;
+  __shared__ float ref[kMaxGrid], sum[kMaxGrid];
+  pdl_wait();
+  pdl_launch_next();
+  const int tid = threadIdx.x;
+  if (blockIdx.x >= blocks) {
+    const int64_t first = row_bound(a, 0), last = row_bound(a, a.seqs), n = (int64_t)a.heads * S::DV / 8;
+    for (int64_t i = blockIdx.x - blocks; i < first + (a.rows - last); i += gridDim.x - blocks) {
+      uint4* to = reinterpret_cast<uint4*>(a.out) + (i < first ? i : last + (i - first)) * n;
+      for (int64_t x = tid; x < n; x += kJoinThreads) to[x] = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  const float* parts = a.work;
+  const int cta = blockIdx.x / S::N, r = blockIdx.x % S::N;
+  const Cut cut = reinterpret_cast<const Cut*>(parts + 2 * (int64_t)grid * part_floats<S>())[cta];
+  if (r >= cut.count) return;
+  const int n = cut.last - cta + 1;
+  auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * part_floats<S>(); };
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const float2 ml = *reinterpret_cast<const float2*>(part(i) + S::N * S::DV + 2 * r);
+    ref[i] = ml.x;
+    sum[i] = ml.y;
+  }
+  __syncthreads();
+  float top = -INFINITY;
+  for (int i = 0; i < n; ++i) top = max_nan(top, ref[i]);
+  const int64_t t = cut.row0 + (cut.f0 + r) / a.group, h = (int64_t)cut.head * a.group + (cut.f0 + r) % a.group;
+  constexpr int kPer = (S::DV + kJoinThreads - 1) / kJoinThreads;
+  float o[kPer] = {}, total = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    if (ref[i] == -INFINITY) continue;   // saw nothing
+    const float w = ref[i] == top ? 1.f : ex2_approx(ref[i] - top);
+    total = fmaf(w, sum[i], total);
+    const float* acc = part(i) + (int64_t)r * S::DV;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (j * kJoinThreads + tid < S::DV) o[j] = fmaf(w, acc[j * kJoinThreads + tid], o[j]);
+  }
+  const float inv = 1.f / total;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int d = j * kJoinThreads + tid;
+    if (d < S::DV)
+      static_cast<T*>(a.out)[(t * a.heads + h) * S::DV + d] = narrow(top == -INFINITY ? 0.f : o[j] * inv, T());
+  }
+}
+
+}  // namespace kv16
+}  // namespace xtg

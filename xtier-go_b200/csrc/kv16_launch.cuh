@@ -1,0 +1,85 @@
+// Launches of the attention over the 16-bit paged caches, by shape (included once for each type of the cache).
+#pragma once
+
+#include "kv16_attn.cuh"
+
+namespace xtg {
+namespace kv16 {
+
+// Rows of a block, from about how many (row, q head) pairs of a KV head a sequence has: the smallest that holds them.
+// A latent cache's tiles leave room for 64.
+inline int block_rows(bool latent, int64_t pairs) {
+  if (pairs <= 16) return 16;
+  if (pairs <= 32) return 32;
+  return pairs <= 64 || latent ? 64 : 128;
+}
+
+// f(a Shape) for the call's dims; false: there is no kernel for them
+template <class T, class F>
+bool by_shape(bool latent, int head_dim, int v_dim, int rows, F&& f) {
+  auto with = [&](auto dk, auto dv, auto is_latent) {
+    constexpr int DK = decltype(dk)::value, DV = decltype(dv)::value;
+    constexpr bool L = decltype(is_latent)::value;
+    if (rows == 16)
+      f(Shape<T, DK, DV, L, 16>());
+    else if (rows == 32)
+      f(Shape<T, DK, DV, L, 32>());
+    else if (rows == 64 || L)
+      f(Shape<T, DK, DV, L, 64>());
+    else
+      f(Shape<T, DK, DV, L, L ? 64 : 128>());
+    return true;
+  };
+  auto is = [&](bool l, int dk, int dv) { return latent == l && head_dim == dk && v_dim == dv; };
+  using std::integral_constant;
+  using No = std::false_type;
+  using Yes = std::true_type;
+  if (is(false, 64, 64)) return with(integral_constant<int, 64>(), integral_constant<int, 64>(), No());
+  if (is(false, 128, 128)) return with(integral_constant<int, 128>(), integral_constant<int, 128>(), No());
+  if (is(false, 192, 128)) return with(integral_constant<int, 192>(), integral_constant<int, 128>(), No());
+  if (is(false, 256, 256)) return with(integral_constant<int, 256>(), integral_constant<int, 256>(), No());
+  if (is(true, 320, 256)) return with(integral_constant<int, 320>(), integral_constant<int, 256>(), Yes());
+  if (is(true, 576, 512)) return with(integral_constant<int, 576>(), integral_constant<int, 512>(), Yes());
+  return false;
+}
+
+// defined in kv16_bf16.cu and kv16_f16.cu
+template <class T>
+void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int grid, cudaStream_t s);
+
+#ifdef KV16_TYPE
+template <class... P, class... A>
+void launch_dependent(void (*f)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  XTG_CUDA(cudaLaunchKernelEx(&cfg, f, static_cast<P>(args)...));
+}
+
+template <class T>
+void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int grid, cudaStream_t s) {
+  by_shape<T>(latent, head_dim, v_dim, rows, [&](auto shape) {
+    using S = decltype(shape);
+    Params a = p;
+    const int64_t slots = a.rows * a.group / S::N + a.seqs;
+    XTG_REQUIRE(slots < (1ll << 31), "kv16: too many row blocks in one call");
+    a.slots = (int)slots;
+    static std::atomic<uint64_t> optin;
+    ensure_smem_optin(reinterpret_cast<const void*>(&attention_kernel<S>), S::kSmemBytes, optin);
+    launch_dependent(attention_kernel<S>, (unsigned)grid, S::kThreads, S::kSmemBytes, s, a);
+    const unsigned blocks = (unsigned)grid * S::N;
+    launch_dependent(join_kernel<S>, blocks + (a.zero_rest ? 4 : 0), kJoinThreads, 0, s, a, grid, blocks);
+  });
+}
+template void launch<KV16_TYPE>(const Params&, bool, int, int, int, int, cudaStream_t);
+#endif
+
+}  // namespace kv16
+}  // namespace xtg

@@ -2,65 +2,15 @@
 // workspaces allocated by torch on the current stream. A call here costs 4 to 9 us of host time, the launches included;
 // through ctypes it cost 10 to 17, more than the small calls run on the GPU. The C ABI's functions come from the library
 // that the package loaded (bind), so this module links torch only.
-#define PY_SSIZE_T_CLEAN
-#include <Python.h>
-
-#include <ATen/ATen.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <algorithm>
-#include <stdexcept>
-#include <string>
-
-#include "../../include/xtg_cuda.h"
+#define XTG_NAME "kv4"
+#include "torch_call.h"
 
 namespace {
 
-struct Refused : std::runtime_error {
-  using std::runtime_error::runtime_error;
-};
-
-PyObject* error_class = nullptr;
 decltype(&xtg_cuda_kv4_store) store_fn = nullptr;
 decltype(&xtg_cuda_kv4_load) load_fn = nullptr;
 decltype(&xtg_cuda_kv4_workspace) workspace_fn = nullptr;
 decltype(&xtg_cuda_kv4_attention) attention_fn = nullptr;
-
-void require(bool ok, const std::string& why) {
-  if (!ok) throw Refused("kv4: " + why);
-}
-
-const at::Tensor& tensor(PyObject* o, const char* name) {
-  require(THPVariable_Check(o), std::string(name) + " is a tensor");
-  return THPVariable_Unpack(o);
-}
-
-int64_t integer(PyObject* o, const char* name) {
-  const int64_t v = PyLong_AsLongLong(o);
-  if (v == -1 && PyErr_Occurred()) {
-    PyErr_Clear();
-    throw Refused(std::string("kv4: ") + name + " is an integer");
-  }
-  return v;
-}
-
-int small(PyObject* o, const char* name) {
-  const int64_t v = integer(o, name);
-  require(v >= INT32_MIN && v <= INT32_MAX, std::string(name) + " is a 32-bit integer");
-  return (int)v;
-}
-
-int code_of(at::ScalarType t) {
-  return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1;
-}
-
-void require_index(const char* name, const at::Tensor& t, int dims, c10::Device dev) {
-  require(t.scalar_type() == at::kInt && t.dim() == dims && t.device() == dev && t.is_contiguous(),
-          std::string(name) + " is a contiguous int32 tensor of " + std::to_string(dims) +
-              " dimension(s) on the pool's device");
-}
 
 // pool, table, pos, cu_rows, err (a tensor or None) -> the C ABI's descriptor
 xtg_cuda_kv4 where(PyObject* const* args, int64_t rows, c10::Device& dev) {
@@ -96,32 +46,6 @@ int rows_type(const char* name, const at::Tensor& t, int64_t heads, const xtg_cu
           std::string(name) + " is [rows][heads][head_dim] of the pool's head_dim on the pool's device");
   require(t.stride(2) == 1, std::string(name) + "'s head dims must be contiguous");
   return code;
-}
-
-// The stride of dimension d; that of a single row or head, which nothing steps by, may be any number.
-int64_t stride(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
-
-// Runs f (which gets the current stream and a message buffer) with device dev current.
-template <class F>
-void call(c10::Device dev, F&& f) {
-  char why[1024] = "";
-  const c10::cuda::CUDAGuard guard(dev);
-  if (f(c10::cuda::getCurrentCUDAStream(dev.index()).stream(), why, (int)sizeof(why)) != 0) throw Refused(why);
-}
-
-// A METH_FASTCALL function of n arguments; C++ exceptions end here, as the package's error class.
-template <class F>
-PyObject* entry(const char* name, Py_ssize_t given, Py_ssize_t wanted, F&& f) {
-  try {
-    require(attention_fn != nullptr, "bind first");
-    require(given == wanted, std::string(name) + " takes " + std::to_string(wanted) + " arguments");
-    return f();
-  } catch (const std::exception& e) {
-    PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, e.what());
-  } catch (...) {
-    PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, "kv4: unknown error");
-  }
-  return nullptr;
 }
 
 // bind(error class, addresses of the four C functions)
