@@ -37,7 +37,14 @@ namespace kv16 {
 constexpr int kSmem = 232448;      // shared memory of a CTA
 constexpr int kCtrl = 3072;        // of it for barriers and per-row values
 constexpr int kMaxGrid = 256;
-constexpr float kSlack = 6.f;
+// A row's reference is kHead below its largest score when it is set and moves when a score passes kMost above it: P is at
+// most 2^kMost. bf16 has f32's range. f16's normal numbers end at 2^16 and at 2^-14: the head keeps small probabilities
+// among them.
+template <class T>
+constexpr float kHead = std::is_same<T, __half>::value ? 4.f : 0.f;
+template <class T>
+constexpr float kMost = std::is_same<T, __half>::value ? 15.f : 16.f;
+constexpr int kLeastShare = 4;   // chunks of a CTA's share at least: a part costs its start, its end and the join
 constexpr float kFloor = -3.0e38f;   // the least reference of a row that has seen a position
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPartCost = 1;       // a part's start and end, in chunks, where shares are cut
@@ -50,7 +57,7 @@ struct Shape {
   static constexpr int C = DK <= 192 ? 128 : 64;   // positions of a chunk: the first product's M
   static constexpr int WG = N >= 64 ? 2 : 1;       // groups of 4 softmax warps, each with NW of the rows
   static constexpr int NW = N / WG;
-  static constexpr int kThreads = WG * 128 + 64;
+  static constexpr int kThreads = WG == 2 ? 384 : 192;   // with the copies' warp and the products', and two that idle
   static constexpr int kSlotBytes = (DK > DV ? DK : DV) * C * 2;
   static constexpr int kQBytes = N * DK * 2, kPBytes = N * C * 2;
   static constexpr int PB = N <= 32 ? 2 : 1;       // buffers of P
@@ -130,8 +137,8 @@ __device__ __forceinline__ Block block_of(const Params& a, int s, int64_t number
   b.p0 = a.pos[s];
   b.chunks = b.c0 = 0;
   if (b.count == 0) return b;
-  b.first = b.p0 + b.f0 / a.group;
-  b.last = b.p0 + (b.f0 + b.count - 1) / a.group;
+  b.first = (int64_t)b.p0 + (uint32_t)b.f0 / (uint32_t)a.group;   // pairs are below 2^31
+  b.last = (int64_t)b.p0 + (uint32_t)(b.f0 + b.count - 1) / (uint32_t)a.group;
   const int64_t end = (int64_t)a.max_pages << a.page_log2;
   const int64_t lo = a.window > 0 && b.first - a.window + 1 > 0 ? b.first - a.window + 1 : 0;
   const int64_t hi = b.last + 1 < end ? b.last + 1 : end;
@@ -148,6 +155,10 @@ struct Part {
   int slot;                // of the workspace, -1: the whole item
 };
 
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {   // not negative; most are small
+  return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 // What the joining kernel needs about the item that starts in a CTA's share and ends in another's
 struct Cut {
   int64_t row0, f0;
@@ -158,13 +169,14 @@ template <class S>
 struct Share {   // the part of all items that a CTA takes, in units of chunks
   int64_t from, to, each;
   int64_t number, base;   // where it starts: a block's number and the units before it
+  Block block;
 };
 
 template <class S>
 __host__ __device__ constexpr int64_t part_floats() {
   return (int64_t)S::N * (S::DV + 2);
 }
-// workspace: 2 parts a CTA (acc [N][DV], then reference and sum [N][2]), then the cuts
+// workspace: 2 parts a CTA (acc [DV][N], reference [N], sum [N]), then the cuts
 template <class S>
 __host__ __device__ constexpr int64_t work_bytes(int grid) {
   return 2 * (int64_t)grid * part_floats<S>() * 4 + (int64_t)grid * (int64_t)sizeof(Cut);
@@ -182,10 +194,8 @@ struct Walk {
 
   __device__ Walk(const Params& a_, const Share<S>& sh_) : a(a_), sh(sh_), number(sh_.number), base(sh_.base), head(0) {
     have = sh.from < sh.to;
-    if (have) {
-      s = find_sequence<S>(a, number);
-      b = block_of<S>(a, s, number);
-    }
+    b = sh.block;
+    s = b.s;
   }
 
   // The next part of the share; cut: filled for an item that goes on in other shares
@@ -207,7 +217,7 @@ struct Walk {
         if (i >= j) continue;
         const bool starts = i == 0, ends = j == b.chunks;
         p = {b, h, i, j - i, starts && ends ? -1 : starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x};
-        if (starts && !ends) cut = {b.row0, b.f0, h, b.count, (int)((at + b.chunks - 1) / sh.each)};
+        if (starts && !ends) cut = {b.row0, b.f0, h, b.count, (int)divide(at + b.chunks - 1, sh.each)};
         return true;
       }
       head = 0;
@@ -238,6 +248,24 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t po
     }
   }
   return true;
+}
+
+// one look at a barrier, which does not wait; all lanes of the warp
+__device__ __forceinline__ bool passed(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return __all_sync(0xffffffffu, ok != 0);
+}
+
+// One lane of the warp, known to be one: the operands of what it issues then stay in uniform registers. With `lane == 0` each
+// instruction of the products took 49 cycles to issue, more than most of them take to run (32 to 48).
+__device__ __forceinline__ bool elected() {
+  uint32_t r;
+  asm volatile("{ .reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p; }" : "=r"(r));
+  return r != 0;
 }
 
 // whether any of the `threads` threads of named barrier `id` votes yes
@@ -294,6 +322,12 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
+
+// 16 bytes from global to shared memory, zeros where not `live`
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy16_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---- values of the cache's type ----
 
@@ -356,6 +390,42 @@ __device__ __forceinline__ int spread_column(int j) {
   return c;
 }
 
+// Zeros for the infinities and NaN among 8 values; whether there were any
+__device__ __forceinline__ bool drop_unbounded(uint4& x, uint32_t exponent, uint32_t one) {
+  uint32_t* w = &x.x;
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t hit = ((w[i] & exponent) + one) & 0x80008000u;   // a full exponent carries into the sign's bit
+    found = found || hit != 0;
+    w[i] &= ~((hit >> 15) * 0xffffu);
+  }
+  return found;
+}
+__device__ __forceinline__ bool drop_unbounded(uint4& x, __nv_bfloat16) { return drop_unbounded(x, 0x7f807f80u, 0x00800080u); }
+__device__ __forceinline__ bool drop_unbounded(uint4& x, __half) { return drop_unbounded(x, 0x7c007c00u, 0x04000400u); }
+
+// Adds V's infinities and NaN of dim d at the marked positions (drop_unbounded) to the rows r0 .. r0 + 15 of the block that
+// see them: a weight above zero times these is these.
+template <class T>
+__device__ __forceinline__ void add_unbounded(const Params& a, const Part& p, const uint32_t* marks, int d, int r0, uint32_t j0,
+                                           float (&o)[16], T) {
+  for (int bit = 0; bit < 256; ++bit) {
+    if (!(marks[bit >> 5] >> (bit & 31) & 1)) continue;
+    const int64_t pos = bit < 128 ? p.b.first + bit : p.b.first - a.window + (bit - 128);
+    const int64_t page = a.table[(int64_t)p.b.s * a.max_pages + (pos >> a.page_log2)];
+    const int64_t slot = pos & ((1 << a.page_log2) - 1);
+    const float v = static_cast<float>(
+        reinterpret_cast<const T*>(a.v)[page * a.v_page + p.head * a.v_head + slot * a.v_slot + d]);
+    if (fabsf(v) < INFINITY) continue;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int64_t t = p.b.first + (j0 + r0 + j) / (uint32_t)a.group;
+      if (pos <= t && (a.window == 0 || pos > t - a.window)) o[j] += v;
+    }
+  }
+}
+
 // ---- the CTA's shared memory ----
 
 constexpr int kInfo = 16, kQueue = 4;
@@ -366,28 +436,17 @@ struct Ctrl {
   Part queue[kQueue];
   uint32_t info[kInfo];   // of chunks in turn: the pieces that are there
   int64_t share_number, share_base, scan[12];
+  Block share_block;
   uint32_t tmem;
   int failed;
-  int bad_chunks;                 // chunks with values that are not finite at positions that some rows see: how many
-  int bad_at[4];                  // and which
-  uint32_t bad[4][4];             // their positions
+  uint32_t unbounded[2][8];       // of every second part that has chunks: positions seen by some rows, with values that are not finite
 };
 template <class S>
-struct Rows {
+struct __align__(16) Rows {
   float ref[S::N], alpha[S::N];
   int top[S::N];   // ordered()
   int place[S::N];   // row in the block << 16 | q head
 };
-
-template <class S>
-struct Where {   // this thread's place among the softmax threads
-  int group, lane4;   // which rows, and the quarter of the tensor memory's lanes
-  int lane, at;       // the position of a chunk that it has
-  bool active;
-};
-
-// Whether position p is seen by the row at position t
-__device__ __forceinline__ bool sees(int64_t t, int64_t p, int window) { return p <= t && (window == 0 || p > t - window); }
 
 template <class S>
 __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_constant__ Params a) {
@@ -400,7 +459,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   Rows<S>& rows = *reinterpret_cast<Rows<S>*>(&c + 1);
   static_assert(sizeof(Ctrl) + sizeof(Rows<S>) <= kCtrl, "control block");
   constexpr int kSoftmaxWarps = 4 * S::WG, kProducer = kSoftmaxWarps, kIssuer = kSoftmaxWarps + 1;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (warp == kIssuer) tmem_alloc(&c.tmem, S::kCols);
   if (tid == 0) {
@@ -431,13 +490,14 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   const int each = (a.slots + S::kThreads - 1) / S::kThreads;
   const int first = min(tid * each, a.slots), last = min(first + each, a.slots);
   auto cost = [&](const Block& b) { return b.count > 0 ? (int64_t)(b.chunks + kPartCost) * a.kv_heads : (int64_t)0; };
+  Block kept;   // the only one, where each is 1
   auto over_blocks = [&](auto&& f) {
     if (first >= last) return;
     int s = find_sequence<S>(a, first);
     for (int i = first; i < last; ++i) {
       if (s + 1 < a.seqs && block_start<S>(a, s + 1) <= i) ++s;
-      const Block b = block_of<S>(a, s, i);
-      if (f(i, b)) break;
+      kept = block_of<S>(a, s, i);
+      if (f(i, kept)) break;
     }
   };
   int64_t mine = 0;
@@ -464,30 +524,39 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     total += c.scan[w];
   }
   Share<S> sh;
-  sh.each = (total + gridDim.x - 1) / gridDim.x;
+  sh.each = max(divide(total + gridDim.x - 1, gridDim.x), (int64_t)kLeastShare);
   sh.from = sh.each * blockIdx.x;
   sh.to = sh.from + sh.each < total ? sh.from + sh.each : total;
   if (sh.from < sh.to && before <= sh.from && sh.from < before + mine) {
     int64_t at = before;
-    over_blocks([&](int i, const Block& b) {
+    auto start = [&](int i, const Block& b) {
       const int64_t x = cost(b);
       if (sh.from < at + x) {
         c.share_number = i;
         c.share_base = at;
+        c.share_block = b;
         return true;
       }
       at += x;
       return false;
-    });
+    };
+    if (each == 1)
+      start(first, kept);
+    else
+      over_blocks(start);
   }
   __syncthreads();
   sh.number = sh.from < sh.to ? c.share_number : 0;
   sh.base = sh.from < sh.to ? c.share_base : 0;
+  sh.block = c.share_block;
   const uint32_t tmem = c.tmem;
   float* parts = a.work;
   Cut* cuts = reinterpret_cast<Cut*>(parts + 2 * (int64_t)gridDim.x * part_floats<S>());
   auto bounded = [&](uint64_t* bar, uint32_t parity) { return wait(bar, parity, a.polls, &c.failed, a.err); };
 
+  // 384 threads start with 168 registers each: the softmax's 8 warps take 216, the others keep 72
+  if (warp >= kSoftmaxWarps) {
+  if (S::WG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == kProducer) {
     // ---- the walk and the copies: K of a chunk before V of the chunk before, as the products take them ----
     constexpr int kSlicesK = S::DK / 64, kSlicesV = S::DV / 64;
@@ -576,69 +645,91 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     }
     __syncwarp();
   } else if (warp == kIssuer) {
-    // ---- the products, by one thread ----
-    if (lane == 0) {
-      constexpr uint32_t kS = instruction<T>(S::C, S::N, false), kOi = instruction<T>(S::MO, S::N, true);
-      const uint32_t ring0 = smem_u32(ring), q0 = smem_u32(qbuf), pb0 = smem_u32(pbuf);
-      uint32_t entry = 0, chunk = 0, filled = 0;
-      bool ok = a.polls != 0;
-      auto first_product = [&](uint32_t e) {   // S^T of chunk number `chunk`
-        const int st = e % S::R, buf = chunk & 1;
-        ok = ok && bounded(&c.full[st], (e / S::R) & 1);
-        if (chunk >= 2) ok = ok && bounded(&c.sfree[buf], ((chunk >> 1) - 1) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t k0 = ring0 + st * S::kSlotBytes, d = tmem + buf * S::N;
+    // ---- the products: whichever of a chunk's second and the next one's first has its operands ----
+    constexpr uint32_t kS = instruction<T>(S::C, S::N, false), kOi = instruction<T>(S::MO, S::N, true);
+    const uint32_t ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0), q0 = __shfl_sync(0xffffffffu, smem_u32(qbuf), 0),
+                   pb0 = __shfl_sync(0xffffffffu, smem_u32(pbuf), 0), t = __shfl_sync(0xffffffffu, tmem, 0);
+    uint32_t entry = 0, chunk = 0, filled = 0;
+    bool ok = a.polls != 0;
+    for (uint32_t part = 0; ok; ++part) {
+      const int qi = part % kQueue;
+      ok = __all_sync(0xffffffffu, bounded(&c.queue_full[qi], (part / kQueue) & 1));
+      if (!ok) break;
+      const int n = __shfl_sync(0xffffffffu, c.queue[qi].count, 0);
+      const bool end = __shfl_sync(0xffffffffu, c.queue[qi].head, 0) < 0;
+      if (lane == 0) mbar_arrive(&c.queue_empty[qi]);
+      if (end) break;
+      if (n == 0) continue;
+      ok = __all_sync(0xffffffffu, bounded(&c.qready, filled & 1));
+      ++filled;
+      tc_fence_after();
+      uint32_t spins = 0;
+      for (int si = 0, vi = 0; vi < n && ok;) {   // chunks whose first and whose second product were issued
+        bool issued = false;
+        if (vi < si) {
+          const uint32_t e = S::LATENT ? entry + vi : vi == n - 1 ? entry + 2 * n - 1 : entry + 2 * vi + 2;
+          const uint32_t st = e % S::R, ch = chunk + vi, pb = ch % S::PB;
+          if (passed(&c.pready[pb], (ch / S::PB) & 1) && passed(&c.full[st], (e / S::R) & 1)) {
+            tc_fence_after();
+            const uint32_t v0 = ring0 + st * S::kSlotBytes, p0 = pb0 + pb * S::kPBytes;
+            if (elected()) {
 #pragma unroll
-        for (int x = 0; x < S::DK; x += 16)
-          mma(d, operand(k0 + x / 64 * S::C * 128 + x % 64 * 2, 16, 1024, kSwizzle128),
-              operand(q0 + x / 64 * S::N * 128 + x % 64 * 2, 16, 1024, kSwizzle128), kS, x > 0);
-        tc_commit(&c.sfull[buf]);
-        if (!S::LATENT) tc_commit(&c.empty[st]);
-      };
-      auto second_product = [&](uint32_t e, uint32_t ch, bool accumulate) {   // o^T += of chunk number ch
-        const int st = e % S::R, pb = ch % S::PB;
-        ok = ok && bounded(&c.pready[pb], (ch / S::PB) & 1);
-        ok = ok && bounded(&c.full[st], (e / S::R) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t v0 = ring0 + st * S::kSlotBytes, p0 = pb0 + pb * S::kPBytes;
+              for (int m = 0; m < S::DT; ++m)
 #pragma unroll
-        for (int m = 0; m < S::DT; ++m)
-#pragma unroll
-          for (int x = 0; x < S::C; x += 16)
-            mma(tmem + S::kO + m * S::N, operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
-                operand(p0 + x * 16, 128, S::C * 16, 0), kOi, accumulate || x > 0);
-        tc_commit(&c.empty[st]);
-        tc_commit(&c.pdone[pb]);
-      };
-      for (uint32_t part = 0; ok; ++part) {
-        const int qi = part % kQueue;
-        ok = bounded(&c.queue_full[qi], (part / kQueue) & 1);
-        if (!ok) break;
-        const int n = c.queue[qi].count;
-        const bool end = c.queue[qi].head < 0;
-        mbar_arrive(&c.queue_empty[qi]);
-        if (end) break;
-        if (n == 0) continue;
-        ok = bounded(&c.qready, filled & 1);
-        ++filled;
-        tc_fence_after();
-        for (int i = 0; i < n && ok; ++i, ++chunk) {
-          first_product(S::LATENT ? entry + i : i == 0 ? entry : entry + 2 * i - 1);
-          if (i > 0) second_product(S::LATENT ? entry + i - 1 : entry + 2 * i, chunk - 1, i > 1);
+                for (int x = 0; x < S::C; x += 16)
+                  mma(t + S::kO + m * S::N,
+                      operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
+                      operand(p0 + x * 16, 128, S::C * 16, 0), kOi, vi > 0 || x > 0);
+              tc_commit(&c.empty[st]);
+              tc_commit(&c.pdone[pb]);
+            }
+            __syncwarp();
+            ++vi;
+            issued = true;
+          }
         }
-        if (ok) second_product(S::LATENT ? entry + n - 1 : entry + 2 * n - 1, chunk - 1, n > 1);
-        entry += S::LATENT ? n : 2 * n;
+        if (si < n && si < vi + 2) {
+          const uint32_t e = S::LATENT ? entry + si : si == 0 ? entry : entry + 2 * si - 1;
+          const uint32_t st = e % S::R, ch = chunk + si, buf = ch & 1;
+          if (passed(&c.full[st], (e / S::R) & 1) && (ch < 2 || passed(&c.sfree[buf], ((ch >> 1) - 1) & 1))) {
+            tc_fence_after();
+            const uint32_t k0 = ring0 + st * S::kSlotBytes;
+            if (elected()) {
+#pragma unroll
+              for (int x = 0; x < S::DK; x += 16)
+                mma(t + buf * S::N, operand(k0 + x / 64 * S::C * 128 + x % 64 * 2, 16, 1024, kSwizzle128),
+                    operand(q0 + x / 64 * S::N * 128 + x % 64 * 2, 16, 1024, kSwizzle128), kS, x > 0);
+              tc_commit(&c.sfull[buf]);
+              if (!S::LATENT) tc_commit(&c.empty[st]);
+            }
+            __syncwarp();
+            ++si;
+            issued = true;
+          }
+        }
+        if (issued) {
+          spins = 0;
+        } else if (++spins > 32 * a.polls || (spins % 64 == 0 && *reinterpret_cast<volatile int*>(&c.failed))) {
+          // these looks do not wait: some 0.1 us each
+          give_up(&c.failed, a.err);
+          ok = false;
+        }
+        ok = __all_sync(0xffffffffu, ok);
       }
+      entry += S::LATENT ? n : 2 * n;
+      chunk += n;
+    }
+    if (elected()) {
       tc_commit(&c.done);
       uint32_t spins = 0;   // every product has ended before the tensor memory goes back
       while (!mbar_try_wait(&c.done, 0))
         if (++spins > (1u << 18)) break;
     }
     __syncwarp();
+  }
   } else {
     // ---- softmax ----
+    if (S::WG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int wg = warp >> 2, quarter = warp & 3, bar = 1 + wg;
     const bool active = S::C == 128 || lane < 16;
     const int at = S::C == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);   // this thread's position of a chunk
@@ -649,52 +740,73 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     int* place = rows.place + wg * S::NW;
     const int own = tid & 127;
     const float sc = a.scale * kLog2e;
-    uint32_t chunk = 0, entry = 0;
-    bool bad = false;
+    const uint32_t group = (uint32_t)a.group;
+    const int box = min(1 << a.page_log2, S::C);
+    const uint32_t all_pieces = (1u << (S::C / box)) - 1;
+
+    // q's rows into the first product's operand, zeros past the last
+    auto load_q = [&](const Part& p) {
+      constexpr int kUnits = S::DK / 8;   // 16-byte pieces of a row
+      const uint32_t f0 = (uint32_t)p.b.f0;
+      const int64_t row0 = p.b.row0;
+      const int count = p.b.count, head0 = p.head * a.group;
+#pragma unroll 4
+      for (int i = 0; i < (S::NW * kUnits + 127) / 128; ++i) {
+        const int x = i * 128 + own, row = x / kUnits, u = x % kUnits, r = wg * S::NW + row;
+        if (S::NW * kUnits % 128 == 0 || row < S::NW) {
+          const uint32_t pair = f0 + r, rt = pair / group;
+          const int64_t t = row0 + rt, h = head0 + (int)(pair - rt * group);
+          const T* from = S::LATENT && u >= S::DV / 8
+                              ? static_cast<const T*>(a.q_rot) + t * a.r_row + h * a.r_head + (8 * u - S::DV)
+                              : static_cast<const T*>(a.q) + t * a.q_row + h * a.q_head + 8 * u;
+          const bool live = r < count;
+          copy16(smem_u32(qbuf) + u / 8 * S::N * 128 + r * 128 + ((u ^ r) & 7) * 16, live ? from : a.q, live);
+        }
+      }
+    };
+    auto finish_q = [&] {
+      copy16_wait();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.qready);
+    };
+
+    uint32_t chunk = 0, entry = 0, filled = 0;   // filled: parts with chunks
+    bool bad = false, known = false;   // known: the next part is in the queue and its q on the way
     for (uint32_t part = 0;; ++part) {
-      const int qi = part % kQueue;
-      bad = !__all_sync(0xffffffffu, bounded(&c.queue_full[qi], (part / kQueue) & 1));
+      const Part& p = c.queue[part % kQueue];
+      if (!known) bad = !__all_sync(0xffffffffu, bounded(&c.queue_full[part % kQueue], (part / kQueue) & 1)) || bad;
       if (vote(bar, 128, bad)) {
         bad = true;
         break;
       }
-      const Part p = c.queue[qi];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c.queue_empty[qi]);
       if (p.head < 0) break;
-      const int64_t t0 = p.b.f0 / a.group;
-      const int j0 = (int)(p.b.f0 % a.group);
-      // q's rows into the first product's operand, zeros past the last; rows' places and references
-      if (p.count > 0) {
-        constexpr int kUnits = S::DK / 8;   // 16-byte pieces of a row
-        for (int i = tid; i < S::N * kUnits; i += kSoftmaxWarps * 32) {
-          const int r = i / kUnits, u = i % kUnits;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (r < p.b.count) {
-            const int64_t t = p.b.row0 + t0 + (j0 + r) / a.group;
-            const int64_t h = (int64_t)p.head * a.group + (j0 + r) % a.group;
-            if (S::LATENT && u >= S::DV / 8)
-              x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q_rot) + t * a.r_row + h * a.r_head + 8 * u - S::DV);
-            else
-              x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + t * a.q_row + h * a.q_head + 8 * u);
-          }
-          *reinterpret_cast<uint4*>(qbuf + u / 8 * S::N * 128 + r * 128 + ((u ^ r) & 7) * 16) = x;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&c.qready);
+      const int count = p.count;
+      if (!known && count > 0) {
+        load_q(p);
+        finish_q();
       }
+      known = false;
+      const uint32_t t0 = (uint32_t)p.b.f0 / group, j0 = (uint32_t)p.b.f0 - t0 * group;
       if (own < S::NW) {
-        const int r = wg * S::NW + own;
-        place[own] = (j0 + r) / a.group << 16 | (j0 + r) % a.group;
+        const uint32_t r = j0 + wg * S::NW + own;
+        place[own] = (int)(r / group << 16 | r % group);
         ref[own] = -INFINITY;
       }
+      uint32_t* marks = c.unbounded[filled & 1];
+      if (count > 0) {
+        if (wg == 0 && own < 8) marks[own] = 0;
+        ++filled;
+      }
       named_bar_sync(bar, 128);
+      const int64_t first_pos = p.b.first, last_pos = p.b.last;
+      const int64_t start0 = (int64_t)(p.b.c0 + p.from) * S::C;
+      const int pairs = p.b.count;
       float l[S::NW];
 #pragma unroll
       for (int r = 0; r < S::NW; ++r) l[r] = 0.f;
 
-      for (int i = 0; i < p.count; ++i, ++chunk) {
+      for (int i = 0; i < count; ++i, ++chunk) {
         const int buf = chunk & 1;
         bad = !__all_sync(0xffffffffu, bounded(&c.sfull[buf], (chunk >> 1) & 1)) || bad;
         tc_fence_after();
@@ -706,42 +818,61 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
           tmem_ld_wait();
         };
         load_scores();
-        const int64_t start = (int64_t)(p.b.c0 + p.from + i) * S::C, pos = start + at;
+        bool q_coming = false;
+        if (i == count - 1) {   // the last product that reads q is done
+          const uint32_t next = part + 1;
+          bad = !__all_sync(0xffffffffu, bounded(&c.queue_full[next % kQueue], (next / kQueue) & 1)) || bad;
+          if (!bad) {
+            known = true;
+            const Part& np = c.queue[next % kQueue];
+            q_coming = np.head >= 0 && np.count > 0;
+            if (q_coming) load_q(np);
+          }
+        }
+        const int64_t start = start0 + (int64_t)i * S::C, pos = start + at;
         const uint32_t there = c.info[chunk % kInfo];
-        const int box = min(1 << a.page_log2, S::C);
-        const uint32_t all = (1u << (S::C / box)) - 1;
-        const bool clean = there == all && start + S::C - 1 <= p.b.first && (a.window == 0 || start > p.b.last - a.window);
-        const bool here = active && (clean || (there >> (at / box) & 1));
-        // scores less the reference; what a row does not see is -infinity
-        float most = -INFINITY;
-        uint32_t hidden[(S::NW + 31) / 32];
-#pragma unroll
-        for (int r = 0; r < (S::NW + 31) / 32; ++r) hidden[r] = here ? 0u : 0xffffffffu;
-        if (!clean && here) {
+        const bool clean = there == all_pieces && start + S::C - 1 <= first_pos && (a.window == 0 || start > last_pos - a.window);
+        // rows lo .. hi - 1 of the block see this thread's position: their positions t = first_pos + (j0 + r) / group, with
+        // pos - window < t - window + 1 <= pos <= t
+        int lo = 0, hi = S::N;
+        if (!clean) {
+          const int64_t rel = pos - first_pos;
+          const int64_t x = rel * group - j0, z = a.window > 0 ? (rel + a.window) * group - j0 : S::N;
+          lo = x < 0 ? 0 : x > S::N ? S::N : (int)x;
+          hi = z < 0 ? 0 : z > S::N ? S::N : (int)z;
+          if (!active || !(there >> (at / box) & 1)) lo = S::N;
+        }
+        const int lo_own = lo - wg * S::NW, hi_own = hi - wg * S::NW;
+        auto hide = [&] {
 #pragma unroll
           for (int r = 0; r < S::NW; ++r)
-            if (!sees(p.b.first + (place[r] >> 16), pos, a.window)) hidden[r / 32] |= 1u << (r % 32);
-        }
-        const bool any_hidden = !clean || !active;
-        auto less_reference = [&] {
-#pragma unroll
-          for (int r = 0; r < S::NW; ++r) y[r] = fmaf(y[r], sc, -ref[r]);
-          if (any_hidden)
-#pragma unroll
-            for (int r = 0; r < S::NW; ++r)
-              if (hidden[r / 32] >> (r % 32) & 1) y[r] = -INFINITY;
+            if (r < lo_own || r >= hi_own) y[r] = -INFINITY;
         };
-        less_reference();
+        auto less_reference = [&] {   // scores less the reference; what a row does not see is -infinity
 #pragma unroll
-        for (int r = 0; r < S::NW; ++r) most = max_nan(most, y[r]);
-        if (vote(bar, 128, bad || !(most <= kSlack))) {
-          // a new reference
-          load_scores();
-#pragma unroll
-          for (int r = 0; r < S::NW; ++r) {
-            y[r] = fmaxf(y[r] * sc, kFloor);
-            if (any_hidden && (hidden[r / 32] >> (r % 32) & 1)) y[r] = -INFINITY;
+          for (int r = 0; r < S::NW; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(ref + r);
+            y[r] = fmaf(y[r], sc, -f.x);
+            y[r + 1] = fmaf(y[r + 1], sc, -f.y);
+            y[r + 2] = fmaf(y[r + 2], sc, -f.z);
+            y[r + 3] = fmaf(y[r + 3], sc, -f.w);
           }
+          if (!clean) hide();
+        };
+        bool over = false;
+        if (i > 0) {
+          less_reference();
+          float m[4] = {y[0], y[1], y[2], y[3]};
+#pragma unroll
+          for (int r = 4; r < S::NW; ++r) m[r % 4] = max_nan(m[r % 4], y[r]);
+          over = active && !(max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) <= kMost<T>);
+        }
+        if (i == 0 || vote(bar, 128, bad || over)) {
+          // a new reference
+          if (i > 0) load_scores();
+#pragma unroll
+          for (int r = 0; r < S::NW; ++r) y[r] = active ? fmaxf(y[r] * sc, kFloor) : -INFINITY;
+          if (!clean) hide();
           spread<S::NW>(y, [](float u, float v) { return fmaxf(u, v); });
 #pragma unroll
           for (int j = 0; j < (S::NW + 31) / 32; ++j) atomicMax(&top[spread_column<S::NW>(j)], ordered(y[j]));
@@ -750,7 +881,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
             break;
           }
           if (own < S::NW) {
-            const float old = ref[own], now = fmaxf(old, of_ordered(top[own]));
+            const float old = ref[own], now = fmaxf(old, of_ordered(top[own]) - kHead<T>);
             alpha[own] = now == old ? 1.f : ex2_approx(old - now);
             ref[own] = now;
             top[own] = ordered(-INFINITY);
@@ -758,9 +889,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
           named_bar_sync(bar, 128);
           load_scores();
           less_reference();
-#pragma unroll
-          for (int r = 0; r < S::NW; ++r) l[r] *= alpha[r];
           if (i > 0) {   // the sums so far
+#pragma unroll
+            for (int r = 0; r < S::NW; ++r) l[r] *= alpha[r];
             const uint32_t b = (chunk - 1) % S::PB;
             bad = !__all_sync(0xffffffffu, bounded(&c.pdone[b], ((chunk - 1) / S::PB) & 1));
             if (!bad) {
@@ -770,59 +901,74 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
 #pragma unroll 1
                 for (int r = 0; r < S::NW; r += 16) {
                   float o[16];
-                  const uint32_t t = lanes + S::kO + m * S::N + wg * S::NW + r;
-                  tmem_ld16(t, o);
+                  const uint32_t from = lanes + S::kO + m * S::N + wg * S::NW + r;
+                  tmem_ld16(from, o);
                   tmem_ld_wait();
 #pragma unroll
                   for (int j = 0; j < 16; ++j) o[j] *= alpha[r + j];
-                  tmem_st16(t, o);
+                  tmem_st16(from, o);
                 }
               tmem_st_wait();
-              tc_fence_before();
             }
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&c.sfree[buf]);
-        // P, rounded, and its sums
-        uint32_t w[S::NW / 2];
-#pragma unroll
-        for (int r = 0; r < S::NW; r += 2) {
-          w[r / 2] = pack(ex2_approx(y[r]), ex2_approx(y[r + 1]), T());
-          const float2 f = unpack(w[r / 2], T());
-          l[r] += f.x;
-          l[r + 1] += f.y;
+        if (!clean && wg == 0) {
+          // V at positions that no row sees is whatever lay there, and 0 x NaN is no 0: zeros. Where some rows see a
+          // position, what is not finite becomes zeros too and is added to those rows at the part's end.
+          const uint32_t e = S::LATENT ? entry + i : i == count - 1 ? entry + 2 * count - 1 : entry + 2 * i + 2;
+          bad = !__all_sync(0xffffffffu, bounded(&c.full[e % S::R], (e / S::R) & 1)) || bad;
+          const bool seen = lo < min(hi, pairs);
+          if (active && !bad && (!seen || lo > 0 || hi < pairs)) {
+            uint8_t* v = ring + e % S::R * S::kSlotBytes + at * 128;
+            bool found = false;
+            for (int u = 0; u < S::DV / 8; ++u) {
+              uint4* w = reinterpret_cast<uint4*>(v + u / 8 * S::C * 128 + (u % 8) * 16);
+              if (!seen) {
+                *w = make_uint4(0, 0, 0, 0);
+              } else {
+                uint4 x = *w;
+                if (drop_unbounded(x, T())) {
+                  *w = x;
+                  found = true;
+                }
+              }
+            }
+            if (found) {
+              const int bit = pos > first_pos ? (int)(pos - first_pos) : 128 + (int)(pos - (first_pos - a.window));
+              atomicOr(&marks[bit >> 5 & 7], 1u << (bit & 31));
+            }
+          }
         }
+        // P, rounded, and its sums
         const uint32_t pb = chunk % S::PB;
         if (chunk >= (uint32_t)S::PB)
           bad = !__all_sync(0xffffffffu, bounded(&c.pdone[pb], (chunk / S::PB - 1) & 1)) || bad;
-        if (active) {
-          uint8_t* to = pbuf + pb * S::kPBytes + wg * (S::NW / 8) * S::C * 16 + at * 16;
+        uint8_t* to = pbuf + pb * S::kPBytes + wg * (S::NW / 8) * S::C * 16 + at * 16;
 #pragma unroll
-          for (int r = 0; r < S::NW / 8; ++r)
-            *reinterpret_cast<uint4*>(to + r * S::C * 16) = make_uint4(w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]);
-        }
-        if (!clean && wg == 0) {
-          // V of positions that no row sees is whatever lay there: zeros, since 0 x NaN is no 0
-          const uint32_t e = S::LATENT ? entry + i : i == p.count - 1 ? entry + 2 * p.count - 1 : entry + 2 * i + 2;
-          bad = !__all_sync(0xffffffffu, bounded(&c.full[e % S::R], (e / S::R) & 1)) || bad;
-          const bool seen = here && pos <= p.b.last && (a.window == 0 || pos > p.b.first - a.window);
-          if (active && !seen && !bad) {
-            uint8_t* v = ring + e % S::R * S::kSlotBytes + at * 128;
-            for (int u = 0; u < S::DV / 8; ++u)
-              *reinterpret_cast<uint4*>(v + u / 8 * S::C * 128 + (u % 8) * 16) = make_uint4(0, 0, 0, 0);
+        for (int r = 0; r < S::NW; r += 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = pack(ex2_approx(y[r + 2 * j]), ex2_approx(y[r + 2 * j + 1]), T());
+            const float2 f = unpack(w[j], T());
+            l[r + 2 * j] += f.x;
+            l[r + 2 * j + 1] += f.y;
           }
+          if (active) *reinterpret_cast<uint4*>(to + r / 8 * S::C * 16) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&c.pready[pb]);
+        if (q_coming) finish_q();
       }
-      entry += S::LATENT ? p.count : 2 * p.count;
+      entry += S::LATENT ? count : 2 * count;
 
       // ---- the part's end: the rows' sums over all positions, then o ----
-      if (p.count > 0 && !bad) {
+      if (count > 0 && !bad) {
         const uint32_t b = (chunk - 1) % S::PB;
         bad = !__all_sync(0xffffffffu, bounded(&c.pdone[b], ((chunk - 1) / S::PB) & 1));
       }
@@ -830,51 +976,70 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         bad = true;
         break;
       }
-      float* sums = reinterpret_cast<float*>(pbuf) + wg * 4 * S::NW;   // P's place
+      float* sums = reinterpret_cast<float*>(pbuf + wg * (S::NW / 8) * S::C * 16);   // the group's part of P's place
+      if (!active)
+#pragma unroll
+        for (int r = 0; r < S::NW; ++r) l[r] = 0.f;
       spread<S::NW>(l, [](float u, float v) { return u + v; });
 #pragma unroll
       for (int j = 0; j < (S::NW + 31) / 32; ++j) sums[quarter * S::NW + spread_column<S::NW>(j)] = l[j];
       named_bar_sync(bar, 128);
-      float* acc = parts + (int64_t)p.slot * part_floats<S>();
+      const int slot = p.slot;
+      float* acc = parts + (int64_t)slot * part_floats<S>();
       if (own < S::NW) {
         const float sum = (sums[own] + sums[S::NW + own]) + (sums[2 * S::NW + own] + sums[3 * S::NW + own]);
         alpha[own] = ref[own] == -INFINITY ? 0.f : 1.f / sum;
-        if (p.slot >= 0) {
-          float* ml = acc + S::N * S::DV + 2 * (wg * S::NW + own);
+        if (slot >= 0) {
+          float* ml = acc + S::N * S::DV + wg * S::NW + own;
           ml[0] = ref[own];
-          ml[1] = sum;
+          ml[S::N] = sum;
         }
       }
       named_bar_sync(bar, 128);
       tc_fence_after();
-      const int mine_rows = min(S::NW, p.b.count - wg * S::NW);
+      const int mine_rows = min(S::NW, pairs - wg * S::NW);
       const bool has_dim = S::MO == 128 || lane < 16;
       const int dim0 = S::MO == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);
+      // out as pairs of dims: even lanes take one row of two, odd lanes the other. rows x heads are below 2^31.
+      const int out_row = (int)((p.b.row0 + t0) * a.heads + (int64_t)p.head * a.group);
+      T* out = static_cast<T*>(a.out) + (dim0 & ~1);
+      uint32_t unbounded = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) unbounded |= count > 0 ? marks[j] : 0;
 #pragma unroll 1
       for (int m = 0; m < S::DT; ++m)
 #pragma unroll 1
-        for (int r = 0; r < S::NW; r += 16) {
-          if (r >= mine_rows) break;
-          float o[16];
-          if (p.count > 0) {
+        for (int r = 0; r < mine_rows; r += 16) {
+          float o[16] = {};
+          if (count > 0) {
             tmem_ld16(lanes + S::kO + m * S::N + wg * S::NW + r, o);
             tmem_ld_wait();
           }
           const int d = m * S::MO + dim0;
+          if (unbounded != 0 && has_dim) add_unbounded(a, p, marks, d, wg * S::NW + r, j0, o, T());
+          if (slot >= 0) {
+            if (has_dim) {
+              float4* to = reinterpret_cast<float4*>(acc + d * S::N + wg * S::NW + r);
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (has_dim && r + j < mine_rows) {
-              if (p.slot >= 0) {
-                acc[(int64_t)(wg * S::NW + r + j) * S::DV + d] = o[j];
-              } else {
-                const int64_t t = p.b.row0 + t0 + (place[r + j] >> 16);
-                const int64_t h = (int64_t)p.head * a.group + (place[r + j] & 0xffff);
-                const float f = ref[r + j] == -INFINITY ? 0.f : o[j] * alpha[r + j];
-                static_cast<T*>(a.out)[(t * a.heads + h) * S::DV + d] = narrow(f, T());
-              }
+              for (int j = 0; j < 4; ++j) to[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
             }
+          } else {
+            const bool odd = lane & 1;
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              const float2 f = *reinterpret_cast<const float2*>(alpha + r + j);
+              const float even_row = f.x == 0.f ? 0.f : o[j] * f.x, odd_row = f.y == 0.f ? 0.f : o[j + 1] * f.y;
+              const float other = __shfl_xor_sync(0xffffffffu, odd ? even_row : odd_row, 1);
+              const uint32_t w = odd ? pack(other, odd_row, T()) : pack(even_row, other, T());
+              const int x = r + j + odd;
+              const int row = out_row + (place[x] >> 16) * a.heads + (place[x] & 0xffff);
+              if (has_dim && x < mine_rows) *reinterpret_cast<uint32_t*>(out + (int64_t)row * S::DV + m * S::MO) = w;
+            }
+          }
         }
       tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&c.queue_empty[part % kQueue]);
     }
     if (bad) {   // a wait gave up: NaN for the rows of the share
       Walk<S> walk(a, sh);
@@ -885,7 +1050,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         const int j0 = (int)(p.b.f0 % a.group);
         for (int r = wg * S::NW; r < min((wg + 1) * S::NW, p.b.count); ++r) {
           if (p.slot >= 0) {
-            if (own < 2) parts[(int64_t)p.slot * part_floats<S>() + S::N * S::DV + 2 * r + own] = NAN;
+            if (own < 2) parts[(int64_t)p.slot * part_floats<S>() + S::N * (S::DV + own) + r] = NAN;
           } else {
             const int64_t t = p.b.row0 + t0 + (j0 + r) / a.group;
             const int64_t h = (int64_t)p.head * a.group + (j0 + r) % a.group;
@@ -901,16 +1066,25 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   if (warp == kIssuer) tmem_dealloc(tmem, S::kCols);
 }
 
-// Joins the parts of the item that starts in CTA c's share and ends in another's: one block per (c, row). The blocks past
-// these write zeros for the rows that are no sequence's.
-constexpr int kJoinThreads = 128;
+// Joins the parts of the item that starts in CTA c's share and ends in another's: one block per (c, 16 rows, 64 dims). A
+// warp a row for the parts' weights, then a thread 4 rows of a dim, every kGroups-th part. The blocks past these write
+// zeros for the rows that are no sequence's.
+constexpr int kJoinThreads = 512, kJoinRows = 16, kJoinDims = 64;
+template <class S>
+constexpr int join_blocks(int grid) {
+  return grid * (S::N / kJoinRows) * (S::DV / kJoinDims);
+}
 template <class S>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
   using T = typename S::T;
-  __shared__ float ref[kMaxGrid], sum[kMaxGrid];
+  constexpr int kGroups = kJoinThreads / 256;
+  __shared__ __align__(16) float weight[kMaxGrid][kJoinRows];
+  __shared__ float inv[kJoinRows];
+  __shared__ float4 more[kGroups - 1][256];
+  __shared__ __align__(16) T result[kJoinRows][kJoinDims];
   pdl_wait();
   pdl_launch_next();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (blockIdx.x >= blocks) {
     const int64_t first = row_bound(a, 0), last = row_bound(a, a.seqs), n = (int64_t)a.heads * S::DV / 8;
     for (int64_t i = blockIdx.x - blocks; i < first + (a.rows - last); i += gridDim.x - blocks) {
@@ -920,38 +1094,76 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     return;
   }
   const float* parts = a.work;
-  const int cta = blockIdx.x / S::N, r = blockIdx.x % S::N;
+  constexpr int kRowTiles = S::N / kJoinRows, kTiles = kRowTiles * (S::DV / kJoinDims);
+  const int cta = blockIdx.x / kTiles, tile = blockIdx.x % kTiles, r0 = tile % kRowTiles * kJoinRows,
+            d0 = tile / kRowTiles * kJoinDims;
   const Cut cut = reinterpret_cast<const Cut*>(parts + 2 * (int64_t)grid * part_floats<S>())[cta];
-  if (r >= cut.count) return;
+  if (r0 >= cut.count) return;
   const int n = cut.last - cta + 1;
   auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * part_floats<S>(); };
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const float2 ml = *reinterpret_cast<const float2*>(part(i) + S::N * S::DV + 2 * r);
-    ref[i] = ml.x;
-    sum[i] = ml.y;
+  const int group = tid / 256, dim = tid % 256 / 4, rows = tid % 4;
+  const int at = (d0 + dim) * S::N + r0 + 4 * rows;
+  constexpr int kAhead = 8;   // parts requested before their weights are known
+  float4 ahead[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (group + k * kGroups < n) ahead[k] = *reinterpret_cast<const float4*>(part(group + k * kGroups) + at);
+  // a row's weights; NaN where a wait gave up
+  float top = -INFINITY, sum0 = 0.f;
+  for (int i = lane; i < n; i += 32) {
+    const float x = part(i)[S::N * S::DV + r0 + warp];
+    weight[i][warp] = x;
+    if (i < 32) sum0 = part(i)[S::N * (S::DV + 1) + r0 + warp];
+    top = max_nan(top, x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float total = 0.f;
+  for (int i = lane; i < n; i += 32) {
+    const float x = weight[i][warp], w = x == -INFINITY ? 0.f : x == top ? 1.f : ex2_approx(x - top);
+    weight[i][warp] = w;
+    total = fmaf(w, i < 32 ? sum0 : part(i)[S::N * (S::DV + 1) + r0 + warp], total);
+  }
+  total = warp_sum(total);
+  if (lane == 0) inv[warp] = top == -INFINITY ? 0.f : 1.f / total;
+  __syncthreads();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](int i, const float4& x) {
+    const float4 w = *reinterpret_cast<const float4*>(&weight[i][4 * rows]);
+    o.x = fmaf(w.x, x.x, o.x);
+    o.y = fmaf(w.y, x.y, o.y);
+    o.z = fmaf(w.z, x.z, o.z);
+    o.w = fmaf(w.w, x.w, o.w);
+  };
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (group + k * kGroups < n) add(group + k * kGroups, ahead[k]);
+#pragma unroll 8
+  for (int i = group + kAhead * kGroups; i < n; i += kGroups) add(i, *reinterpret_cast<const float4*>(part(i) + at));
+  if (group > 0) more[group - 1][tid % 256] = o;
+  __syncthreads();
+  if (group == 0) {
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) {
+      const float4 x = more[g - 1][tid];
+      o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+    }
+    const float v[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float f = inv[4 * rows + j];
+      result[4 * rows + j][dim] = narrow(f == 0.f ? 0.f : v[j] * f, T());
+    }
   }
   __syncthreads();
-  float top = -INFINITY;
-  for (int i = 0; i < n; ++i) top = max_nan(top, ref[i]);
-  const int64_t t = cut.row0 + (cut.f0 + r) / a.group, h = (int64_t)cut.head * a.group + (cut.f0 + r) % a.group;
-  constexpr int kPer = (S::DV + kJoinThreads - 1) / kJoinThreads;
-  float o[kPer] = {}, total = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    if (ref[i] == -INFINITY) continue;   // saw nothing
-    const float w = ref[i] == top ? 1.f : ex2_approx(ref[i] - top);
-    total = fmaf(w, sum[i], total);
-    const float* acc = part(i) + (int64_t)r * S::DV;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (j * kJoinThreads + tid < S::DV) o[j] = fmaf(w, acc[j * kJoinThreads + tid], o[j]);
-  }
-  const float inv = 1.f / total;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int d = j * kJoinThreads + tid;
-    if (d < S::DV)
-      static_cast<T*>(a.out)[(t * a.heads + h) * S::DV + d] = narrow(top == -INFINITY ? 0.f : o[j] * inv, T());
+  if (tid < kJoinRows * kJoinDims / 8) {
+    const int r = tid / (kJoinDims / 8), u = tid % (kJoinDims / 8);
+    if (r0 + r < cut.count) {
+      const uint32_t pair = (uint32_t)cut.f0 + r0 + r;
+      const int64_t t = cut.row0 + pair / (uint32_t)a.group, h = (int64_t)cut.head * a.group + pair % (uint32_t)a.group;
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (t * a.heads + h) * S::DV + d0 + 8 * u) =
+          *reinterpret_cast<const uint4*>(&result[r][8 * u]);
+    }
   }
 }
 

@@ -74,7 +74,7 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     static std::atomic<uint64_t> optin;
     ensure_smem_optin(reinterpret_cast<const void*>(&attention_kernel<S>), S::kSmemBytes, optin);
     launch_dependent(attention_kernel<S>, (unsigned)grid, S::kThreads, S::kSmemBytes, s, a);
-    const unsigned blocks = (unsigned)grid * S::N;
+    const unsigned blocks = (unsigned)join_blocks<S>(grid);
     launch_dependent(join_kernel<S>, blocks + (a.zero_rest ? 4 : 0), kJoinThreads, 0, s, a, grid, blocks);
   });
 }
