@@ -463,8 +463,8 @@ void kv16_require_rows(std::initializer_list<const void*> pointers, int dtype, s
 }
 
 void kv16_require_heads(int heads, int kv_heads, int rows_per_seq) {
-  XTG_REQUIRE(heads >= 1 && heads % kv_heads == 0 && heads / kv_heads <= 65535,
-              "kv16: q heads a multiple of KV heads, at most 65535 of each");
+  XTG_REQUIRE(heads >= 1 && heads % kv_heads == 0 && heads / kv_heads <= 32768,
+              "kv16: q heads a multiple of KV heads, at most 32768 for each");
   XTG_REQUIRE(rows_per_seq >= 1, "kv16: rows_per_seq at least 1");
 }
 

@@ -353,6 +353,7 @@ void launch_kv16_attention(const Kv16Cache& c, const Kv16Attn& r, int sms, cudaS
   p.heads = r.heads;
   p.kv_heads = c.kv_heads;
   p.group = group;
+  p.group_inv = group > 1 ? (uint32_t)(((1ull << 32) + group - 1) / group) : 0;
   p.window = r.window;
   p.scale = r.scale;
   p.zero_rest = r.zero_rest;
@@ -360,11 +361,11 @@ void launch_kv16_attention(const Kv16Cache& c, const Kv16Attn& r, int sms, cudaS
   p.work = static_cast<float*>(r.work);
   p.polls = wait_polls.load(std::memory_order_relaxed);
   const int rows = kv16::block_rows(c.latent, (int64_t)group * r.rows_per_seq);
-  const int grid = std::min(sms, kv16::kMaxGrid);
+  const int most = std::min(sms, kv16::kMaxGrid);
   if (c.dtype == kKv16Bf16)
-    kv16::launch<__nv_bfloat16>(p, c.latent, c.head_dim, c.v_dim, rows, grid, s);
+    kv16::launch<__nv_bfloat16>(p, c.latent, c.head_dim, c.v_dim, rows, r.rows_per_seq, most, s);
   else
-    kv16::launch<__half>(p, c.latent, c.head_dim, c.v_dim, rows, grid, s);
+    kv16::launch<__half>(p, c.latent, c.head_dim, c.v_dim, rows, r.rows_per_seq, most, s);
 }
 
 }  // namespace xtg

@@ -44,10 +44,8 @@ template <class T>
 constexpr float kHead = std::is_same<T, __half>::value ? 4.f : 0.f;
 template <class T>
 constexpr float kMost = std::is_same<T, __half>::value ? 15.f : 16.f;
-constexpr int kLeastShare = 4;   // chunks of a CTA's share at least: a part costs its start, its end and the join
 constexpr float kFloor = -3.0e38f;   // the least reference of a row that has seen a position
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kPartCost = 1;       // a part's start and end, in chunks, where shares are cut
 
 template <class T_, int DK_, int DV_, bool LATENT_, int N_>
 struct Shape {
@@ -55,12 +53,16 @@ struct Shape {
   static constexpr int DK = DK_, DV = DV_, N = N_;
   static constexpr bool LATENT = LATENT_;
   static constexpr int C = DK <= 192 ? 128 : 64;   // positions of a chunk: the first product's M
-  static constexpr int WG = N >= 64 ? 2 : 1;       // groups of 4 softmax warps, each with NW of the rows
+  static constexpr int WG = N >= 32 ? 2 : 1;       // groups of 4 softmax warps, each with NW of the rows
   static constexpr int NW = N / WG;
+  // Of these a thread has NC: all, or, where the 64 positions of a chunk lie in 16 of a warp's 32 lanes, half of them
+  static constexpr int NC = C == 128 ? NW : NW / 2;
   static constexpr int kThreads = WG == 2 ? 384 : 192;   // with the copies' warp and the products', and two that idle
   static constexpr int kSlotBytes = (DK > DV ? DK : DV) * C * 2;
   static constexpr int kQBytes = N * DK * 2, kPBytes = N * C * 2;
   static constexpr int PB = N <= 32 ? 2 : 1;       // buffers of P
+  // A tile is copied, waited for and released in pieces of 128 dims, the second product's M
+  static constexpr int PK = (DK + 127) / 128, PV = LATENT ? 0 : (DV + 127) / 128, P = PK > PV ? PK : PV;
   static constexpr int kFit = (kSmem - kCtrl - kQBytes - PB * kPBytes) / kSlotBytes;
   static constexpr int R = kFit > 12 ? 12 : kFit;  // slots of the ring
   static constexpr int kSmemBytes = R * kSlotBytes + kQBytes + PB * kPBytes + kCtrl;
@@ -83,6 +85,9 @@ struct Params {
   const int32_t *table, *pos, *cu_rows;
   int64_t pages, rows;
   int max_pages, seqs, page_log2, heads, kv_heads, group, window;
+  uint32_t group_inv;
+  int team;   // CTAs beside each other, a divisor of the grid
+  int part_cost, least_share;   // in chunks: a part's start and end where shares are cut, a share at least
   int slots;   // (sequence, row block) numbers, some of them empty
   float scale;
   bool zero_rest;
@@ -97,10 +102,16 @@ __device__ __forceinline__ int64_t row_bound(const Params& a, int s) {
   return c < 0 ? 0 : c > a.rows ? a.rows : c;
 }
 
-// A row block is N consecutive (row, q head of the KV head's group) pairs of a sequence. Sequence s's blocks have numbers
-// from cu_rows[s] group / N + s on: at least as many as it needs, found without a prefix sum over the sequences.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {   // not negative; most are small
+  return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
+// A row block is N consecutive (row, q head of the KV head's group) pairs of a sequence, one a CTA; `team` CTAs take as many
+// blocks beside each other through the same chunks, so that what the blocks share comes from memory once. Sequence s's
+// blocks of a team have numbers from cu_rows[s] group / (N team) + s on: at least as many as it needs, found without a
+// prefix sum over the sequences.
 struct Block {
-  int s, p0;         // sequence, the position of its first row
+  int s;
   int64_t row0, f0;  // the call's row of the sequence's first, and the block's first pair in the sequence
   int count;         // pairs, 0: none
   int c0, chunks;    // the first chunk that one of its rows sees, and how many
@@ -109,7 +120,7 @@ struct Block {
 
 template <class S>
 __device__ __forceinline__ int64_t block_start(const Params& a, int s) {
-  return row_bound(a, s) * a.group / S::N + s;
+  return divide(row_bound(a, s) * a.group, S::N * a.team) + s;
 }
 
 template <class S>
@@ -125,20 +136,14 @@ __device__ __forceinline__ int find_sequence(const Params& a, int64_t number) {
   return lo;
 }
 
+// Sequence s's pairs f0 .. f0 + count - 1
 template <class S>
-__device__ __forceinline__ Block block_of(const Params& a, int s, int64_t number) {
-  Block b;
-  b.s = s;
-  b.row0 = row_bound(a, s);
-  const int64_t n = row_bound(a, s + 1) - b.row0, pairs = n > 0 ? n * a.group : 0;
-  b.f0 = (number - block_start<S>(a, s)) * S::N;
-  const int64_t left = pairs - b.f0;
-  b.count = b.f0 < 0 || left <= 0 ? 0 : left < S::N ? (int)left : S::N;
-  b.p0 = a.pos[s];
-  b.chunks = b.c0 = 0;
-  if (b.count == 0) return b;
-  b.first = (int64_t)b.p0 + (uint32_t)b.f0 / (uint32_t)a.group;   // pairs are below 2^31
-  b.last = (int64_t)b.p0 + (uint32_t)(b.f0 + b.count - 1) / (uint32_t)a.group;
+__device__ __forceinline__ Block block_at(const Params& a, int s, int64_t row0, int64_t f0, int count) {
+  Block b = {s, row0, f0, count, 0, 0, 0, 0};
+  if (count == 0) return b;
+  const int p0 = a.pos[s];
+  b.first = (int64_t)p0 + (uint32_t)f0 / (uint32_t)a.group;   // pairs are below 2^31
+  b.last = (int64_t)p0 + (uint32_t)(f0 + count - 1) / (uint32_t)a.group;
   const int64_t end = (int64_t)a.max_pages << a.page_log2;
   const int64_t lo = a.window > 0 && b.first - a.window + 1 > 0 ? b.first - a.window + 1 : 0;
   const int64_t hi = b.last + 1 < end ? b.last + 1 : end;
@@ -149,24 +154,32 @@ __device__ __forceinline__ Block block_of(const Params& a, int s, int64_t number
   return b;
 }
 
+// The blocks of a team with this number
+template <class S>
+__device__ __forceinline__ Block block_of(const Params& a, int s, int64_t number) {
+  const int64_t row0 = row_bound(a, s), n = row_bound(a, s + 1) - row0, pairs = n > 0 ? n * a.group : 0;
+  const int most = S::N * a.team;
+  const int64_t f0 = (number - block_start<S>(a, s)) * most, left = pairs - f0;
+  return block_at<S>(a, s, row0, f0, f0 < 0 || left <= 0 ? 0 : left < most ? (int)left : most);
+}
+
 struct Part {
   Block b;
   int head, from, count;   // KV head, chunks c0 + from .. c0 + from + count - 1
-  int slot;                // of the workspace, -1: the whole item
+  int slot;                // of the workspace, -1: the whole block
 };
 
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {   // not negative; most are small
-  return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
-}
+// x / group for x below group + 128, by a multiplication: group_inv = ceil(2^32 / group), group at most 2^15
+__device__ __forceinline__ uint32_t by_group(const Params& a, uint32_t x) { return a.group == 1 ? x : __umulhi(x, a.group_inv); }
 
-// What the joining kernel needs about the item that starts in a CTA's share and ends in another's
+// What the joining kernel needs about the block that starts in a CTA's share and ends in another's
 struct Cut {
   int64_t row0, f0;
-  int head, count, last;   // count 0: there is none
+  int head, count, last;   // count 0: there is none; last: the team that ends it
 };
 
 template <class S>
-struct Share {   // the part of all items that a CTA takes, in units of chunks
+struct Share {   // the part of all items that a team takes, in units of chunks
   int64_t from, to, each;
   int64_t number, base;   // where it starts: a block's number and the units before it
   Block block;
@@ -202,22 +215,30 @@ struct Walk {
   __device__ bool next(Part& p, Cut& cut) {
     while (have && base < sh.to) {
       if (b.count > 0 && head < a.kv_heads) {
-        const int64_t at = base + kPartCost;   // the item's first chunk
+        const int64_t at = base + a.part_cost;   // the item's first chunk
         const int64_t from = sh.from - at, to = sh.to - at;
         const int h = head++;
         const int64_t here = base;
-        base += kPartCost + b.chunks;
+        base += a.part_cost + b.chunks;
+        int i = 0, j = 0;
         if (b.chunks == 0) {
           if (here < sh.from) continue;
-          p = {b, h, 0, 0, -1};
-          return true;
+        } else {
+          i = from < 0 ? 0 : from > b.chunks ? b.chunks : (int)from;
+          j = to < 0 ? 0 : to > b.chunks ? b.chunks : (int)to;
+          if (i >= j) continue;
         }
-        const int i = from < 0 ? 0 : from > b.chunks ? b.chunks : (int)from;
-        const int j = to < 0 ? 0 : to > b.chunks ? b.chunks : (int)to;
-        if (i >= j) continue;
         const bool starts = i == 0, ends = j == b.chunks;
         p = {b, h, i, j - i, starts && ends ? -1 : starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x};
-        if (starts && !ends) cut = {b.row0, b.f0, h, b.count, (int)divide(at + b.chunks - 1, sh.each)};
+        if (a.team > 1) {   // this CTA's block of the team's; it may see fewer chunks, or none of the share's
+          const int before = (int)(blockIdx.x % a.team) * S::N;
+          if (before >= b.count) continue;
+          p.b = block_at<S>(a, s, b.row0, b.f0 + before, min(b.count - before, S::N));
+          const int x = max(b.c0 + i, p.b.c0), y = min(b.c0 + j, p.b.c0 + p.b.chunks);
+          p.from = x - p.b.c0;
+          p.count = max(y - x, 0);
+        }
+        if (starts && !ends) cut = {p.b.row0, p.b.f0, h, p.b.count, (int)divide(at + b.chunks - 1, sh.each)};
         return true;
       }
       head = 0;
@@ -302,6 +323,34 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
       : "memory");
 }
 
+// M columns from `taddr` on, of this warp's 32 lanes; HALVES: columns 0 .. M - 1 of its first 16 lanes for lanes 0 .. 15 and
+// columns M .. 2 M - 1 of the same for lanes 16 .. 31
+template <bool HALVES, int M>
+__device__ __forceinline__ void load_columns(uint32_t taddr, float (&v)[M]) {
+  static_assert(M % 8 == 0 && (HALVES || M % 16 == 0), "columns");
+  uint32_t r[16];
+#pragma unroll
+  for (int c = 0; c < M; c += 16) {
+    if (!HALVES) {
+      tmem_ld16(taddr + c, *reinterpret_cast<float(*)[16]>(&v[c]));
+    } else if (M % 16 == 8) {
+      asm volatile("tcgen05.ld.sync.aligned.16x32bx2.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8], %9;"
+                   : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                   : "r"(taddr + c), "n"(M));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[c + j] = __uint_as_float(r[j]);
+    } else {
+      asm volatile(
+          "tcgen05.ld.sync.aligned.16x32bx2.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16], %17;"
+          : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+            "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+          : "r"(taddr + c), "n"(M));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[c + j] = __uint_as_float(r[j]);
+    }
+  }
+}
+
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
   uint32_t r[16];
 #pragma unroll
@@ -348,6 +397,22 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// sum += a half of a packed pair, without an instruction to unpack it
+__device__ __forceinline__ void add_halves(float& lo, float& hi, uint32_t w, __nv_bfloat16) {
+  asm("{ .reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.bf16 %0, l, %0;\n\tadd.rn.f32.bf16 %1, h, %1; }"
+      : "+f"(lo), "+f"(hi)
+      : "r"(w));
+}
+__device__ __forceinline__ void add_halves(float& lo, float& hi, uint32_t w, __half) {
+  asm("{ .reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.f16 %0, l, %0;\n\tadd.rn.f32.f16 %1, h, %1; }"
+      : "+f"(lo), "+f"(hi)
+      : "r"(w));
+}
 // floats as integers of the same order (NaN aside), for atomicMax
 __device__ __forceinline__ int ordered(float x) {
   const int i = __float_as_int(x);
@@ -355,14 +420,14 @@ __device__ __forceinline__ int ordered(float x) {
 }
 __device__ __forceinline__ float of_ordered(int i) { return __int_as_float(i >= 0 ? i : i ^ 0x7fffffff); }
 
-// Over the lanes of a warp, each of M values: halves of the set change places at lane distances 16, 8, .. until every lane
-// has M / 32 values (or one, shared by 32 / M lanes). Value j of lane l is then number
-// column(l, j) of the set.
-template <int M, class F>
+// Over groups of LANES lanes (32, or 16: the halves of a warp), each of M values: halves of the set change places at lane
+// distances LANES / 2, .. 1 until every lane has spread_left values, which lanes may share. Value j of a lane is then number
+// spread_column(j) of the set.
+template <int M, int LANES, class F>
 __device__ __forceinline__ void spread(float (&v)[M], F f) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int d = 16, m = M; d > 0; d >>= 1) {
+  for (int d = LANES / 2, m = M; d > 0; d >>= 1) {
     if (m > 1) {
       m >>= 1;
       const bool up = lane & d;
@@ -377,12 +442,16 @@ __device__ __forceinline__ void spread(float (&v)[M], F f) {
     }
   }
 }
-template <int M>
+template <int M, int LANES>
+constexpr int spread_left() {
+  return M > LANES ? M / LANES : 1;
+}
+template <int M, int LANES>
 __device__ __forceinline__ int spread_column(int j) {
   const int lane = threadIdx.x & 31;
   int c = j;
 #pragma unroll
-  for (int d = 16, m = M; d > 0; d >>= 1)
+  for (int d = LANES / 2, m = M; d > 0; d >>= 1)
     if (m > 1) {
       m >>= 1;
       if (lane & d) c += m;
@@ -420,7 +489,7 @@ __device__ __forceinline__ void add_unbounded(const Params& a, const Part& p, co
     if (fabsf(v) < INFINITY) continue;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const int64_t t = p.b.first + (j0 + r0 + j) / (uint32_t)a.group;
+      const int64_t t = p.b.first + by_group(a, j0 + r0 + j);
       if (pos <= t && (a.window == 0 || pos > t - a.window)) o[j] += v;
     }
   }
@@ -430,8 +499,9 @@ __device__ __forceinline__ void add_unbounded(const Params& a, const Part& p, co
 
 constexpr int kInfo = 16, kQueue = 4;
 
+template <class S>
 struct Ctrl {
-  uint64_t full[12], empty[12], sfull[2], sfree[2], pready[2], pdone[2], qready, done, queue_full[kQueue],
+  uint64_t full[S::R][S::P], empty[S::R][S::P], sfull[2], sfree[2], pready[2], pdone[2], qready, done, queue_full[kQueue],
       queue_empty[kQueue];
   Part queue[kQueue];
   uint32_t info[kInfo];   // of chunks in turn: the pieces that are there
@@ -445,7 +515,7 @@ template <class S>
 struct __align__(16) Rows {
   float ref[S::N], alpha[S::N];
   int top[S::N];   // ordered()
-  int place[S::N];   // row in the block << 16 | q head
+  int place[S::N];   // the row's place in out
 };
 
 template <class S>
@@ -455,17 +525,17 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   uint8_t* ring = smem;
   uint8_t* qbuf = smem + S::R * S::kSlotBytes;
   uint8_t* pbuf = qbuf + S::kQBytes;
-  Ctrl& c = *reinterpret_cast<Ctrl*>(pbuf + S::PB * S::kPBytes);
+  Ctrl<S>& c = *reinterpret_cast<Ctrl<S>*>(pbuf + S::PB * S::kPBytes);
   Rows<S>& rows = *reinterpret_cast<Rows<S>*>(&c + 1);
-  static_assert(sizeof(Ctrl) + sizeof(Rows<S>) <= kCtrl, "control block");
+  static_assert(sizeof(Ctrl<S>) + sizeof(Rows<S>) <= kCtrl, "control block");
   constexpr int kSoftmaxWarps = 4 * S::WG, kProducer = kSoftmaxWarps, kIssuer = kSoftmaxWarps + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (warp == kIssuer) tmem_alloc(&c.tmem, S::kCols);
   if (tid == 0) {
-    for (int i = 0; i < S::R; ++i) {
-      mbar_init(&c.full[i], 1);
-      mbar_init(&c.empty[i], 1);
+    for (int i = 0; i < S::R * S::P; ++i) {
+      mbar_init(&c.full[0][i], 1);
+      mbar_init(&c.empty[0][i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c.sfull[i], 1);
@@ -489,7 +559,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   pdl_launch_next();
   const int each = (a.slots + S::kThreads - 1) / S::kThreads;
   const int first = min(tid * each, a.slots), last = min(first + each, a.slots);
-  auto cost = [&](const Block& b) { return b.count > 0 ? (int64_t)(b.chunks + kPartCost) * a.kv_heads : (int64_t)0; };
+  auto cost = [&](const Block& b) { return b.count > 0 ? (int64_t)(b.chunks + a.part_cost) * a.kv_heads : (int64_t)0; };
   Block kept;   // the only one, where each is 1
   auto over_blocks = [&](auto&& f) {
     if (first >= last) return;
@@ -524,8 +594,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     total += c.scan[w];
   }
   Share<S> sh;
-  sh.each = max(divide(total + gridDim.x - 1, gridDim.x), (int64_t)kLeastShare);
-  sh.from = sh.each * blockIdx.x;
+  const uint32_t teams = gridDim.x / a.team;
+  sh.each = max(divide(total + teams - 1, teams), (int64_t)(a.part_cost + a.least_share));
+  sh.from = sh.each * (blockIdx.x / a.team);
   sh.to = sh.from + sh.each < total ? sh.from + sh.each : total;
   if (sh.from < sh.to && before <= sh.from && sh.from < before + mine) {
     int64_t at = before;
@@ -570,19 +641,26 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     Cut cut = {0, 0, 0, 0, 0};
     Part p;
     Walk<S> walk(a, sh);
-    auto copy = [&](const CUtensorMap* map, int slices, int head, int slot0, int page, uint32_t there) {
-      const int st = entry % S::R;
-      const uint32_t turn = entry / S::R;
-      if (turn > 0) ok = __all_sync(0xffffffffu, bounded(&c.empty[st], (turn - 1) & 1));
-      if (!ok) return;
-      if (lane == 0) mbar_expect_tx(&c.full[st], (uint32_t)(__popc(there) * slices * box * 128));
-      __syncwarp();
-      const uint32_t to = smem_u32(ring) + st * S::kSlotBytes;
-      for (int i = 0; i < pieces * slices; i += 32) {
-        const int x = i + lane, piece = x % pieces, slice = x / pieces;
-        const int pg = __shfl_sync(0xffffffffu, page, piece);
-        if (slice < slices && (there >> piece & 1))
-          load_box(to + slice * S::C * 128 + piece * box * 128, map, 64 * slice, slot0, head, pg, &c.full[st]);
+    uint32_t begun = 0;   // pieces asked for of a tile that was given up
+    // A tile of K or V into the next slot, piece by piece. A piece that V does not have is passed on empty, so that a slot's
+    // barriers turn alike.
+    auto copy = [&](bool v, int head, int slot0, int page, uint32_t there) {
+      const int st = entry % S::R, slices = v ? kSlicesV : kSlicesK;
+      const CUtensorMap* map = v ? &a.vmap : &a.kmap;
+      const uint32_t turn = entry / S::R, to = smem_u32(ring) + st * S::kSlotBytes;
+      for (int pc = 0; pc < S::P; ++pc) {
+        const int n = max(0, min(2, slices - 2 * pc));
+        if (turn > 0) ok = __all_sync(0xffffffffu, bounded(&c.empty[st][pc], (turn - 1) & 1));
+        if (!ok) {
+          begun = pc;
+          return;
+        }
+        if (lane == 0) mbar_expect_tx(&c.full[st][pc], (uint32_t)(__popc(there) * n * box * 128));
+        __syncwarp();
+        const int x = lane & (pieces - 1), slice = 2 * pc + lane / pieces;   // at most 8 boxes a slice
+        const int pg = __shfl_sync(0xffffffffu, page, x);
+        if (lane < n * pieces && (there >> x & 1))
+          load_box(to + slice * S::C * 128 + x * box * 128, map, 64 * slice, slot0, head, pg, &c.full[st][pc]);
       }
       ++entry;
     };
@@ -617,10 +695,10 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
         const int slot0 = (int)(((int64_t)(p.b.c0 + p.from + i) * S::C) & ((1 << a.page_log2) - 1));
         if (lane == 0) c.info[chunk % kInfo] = there;
-        copy(&a.kmap, kSlicesK, p.head, slot0, page, there);
+        copy(false, p.head, slot0, page, there);
         if (!S::LATENT) {
-          if (i > 0 && ok) copy(&a.vmap, kSlicesV, p.head, old_slot0, old_page, old_there);
-          if (i == p.count - 1 && ok) copy(&a.vmap, kSlicesV, p.head, slot0, page, there);
+          if (i > 0 && ok) copy(true, p.head, old_slot0, old_page, old_there);
+          if (i == p.count - 1 && ok) copy(true, p.head, slot0, page, there);
         }
         old_page = page;
         old_there = there;
@@ -638,11 +716,16 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       }
     }
     // no copy is left in flight
-    for (uint32_t e = entry > (uint32_t)S::R ? entry - S::R : 0; e < entry; ++e) {
-      uint32_t spins = 0;
-      while (!mbar_try_wait(&c.full[e % S::R], (e / S::R) & 1))
-        if (++spins > (1u << 18)) break;
-    }
+    auto landed = [&](uint32_t e, uint32_t n) {
+      for (uint32_t pc = 0; pc < n; ++pc) {
+        uint32_t spins = 0;
+        while (!mbar_try_wait(&c.full[e % S::R][pc], (e / S::R) & 1))
+          if (++spins > (1u << 18)) break;
+      }
+    };
+    landed(entry, begun);
+    for (uint32_t back = 1; back <= min(entry, (uint32_t)S::R); ++back)
+      landed(entry - back, S::P);
     __syncwarp();
   } else if (warp == kIssuer) {
     // ---- the products: whichever of a chunk's second and the next one's first has its operands ----
@@ -664,23 +747,31 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       ++filled;
       tc_fence_after();
       uint32_t spins = 0;
+      int piece = 0;   // of K's tile, the first that the first product has not taken
       for (int si = 0, vi = 0; vi < n && ok;) {   // chunks whose first and whose second product were issued
         bool issued = false;
         if (vi < si) {
           const uint32_t e = S::LATENT ? entry + vi : vi == n - 1 ? entry + 2 * n - 1 : entry + 2 * vi + 2;
           const uint32_t st = e % S::R, ch = chunk + vi, pb = ch % S::PB;
-          if (passed(&c.pready[pb], (ch / S::PB) & 1) && passed(&c.full[st], (e / S::R) & 1)) {
+          bool there = passed(&c.pready[pb], (ch / S::PB) & 1);
+          if (!S::LATENT)   // of a latent cache the first product has waited for the tile
+#pragma unroll
+            for (int m = 0; m < S::PV; ++m) there = there && passed(&c.full[st][m], (e / S::R) & 1);
+          if (there) {
             tc_fence_after();
             const uint32_t v0 = ring0 + st * S::kSlotBytes, p0 = pb0 + pb * S::kPBytes;
             if (elected()) {
 #pragma unroll
-              for (int m = 0; m < S::DT; ++m)
+              for (int m = 0; m < S::DT; ++m) {
 #pragma unroll
                 for (int x = 0; x < S::C; x += 16)
                   mma(t + S::kO + m * S::N,
                       operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
                       operand(p0 + x * 16, 128, S::C * 16, 0), kOi, vi > 0 || x > 0);
-              tc_commit(&c.empty[st]);
+                tc_commit(&c.empty[st][m]);
+              }
+#pragma unroll
+              for (int m = S::DT; m < S::P && !S::LATENT; ++m) tc_commit(&c.empty[st][m]);
               tc_commit(&c.pdone[pb]);
             }
             __syncwarp();
@@ -691,19 +782,30 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         if (si < n && si < vi + 2) {
           const uint32_t e = S::LATENT ? entry + si : si == 0 ? entry : entry + 2 * si - 1;
           const uint32_t st = e % S::R, ch = chunk + si, buf = ch & 1;
-          if (passed(&c.full[st], (e / S::R) & 1) && (ch < 2 || passed(&c.sfree[buf], ((ch >> 1) - 1) & 1))) {
+          if (passed(&c.full[st][piece], (e / S::R) & 1) && (piece > 0 || ch < 2 || passed(&c.sfree[buf], ((ch >> 1) - 1) & 1))) {
             tc_fence_after();
-            const uint32_t k0 = ring0 + st * S::kSlotBytes;
-            if (elected()) {
+            const uint32_t k0 = ring0 + st * S::kSlotBytes + piece * S::C * 256, b0 = q0 + piece * S::N * 256;
+            auto products = [&](auto dims) {
 #pragma unroll
-              for (int x = 0; x < S::DK; x += 16)
+              for (int x = 0; x < decltype(dims)::value; x += 16)
                 mma(t + buf * S::N, operand(k0 + x / 64 * S::C * 128 + x % 64 * 2, 16, 1024, kSwizzle128),
-                    operand(q0 + x / 64 * S::N * 128 + x % 64 * 2, 16, 1024, kSwizzle128), kS, x > 0);
-              tc_commit(&c.sfull[buf]);
-              if (!S::LATENT) tc_commit(&c.empty[st]);
+                    operand(b0 + x / 64 * S::N * 128 + x % 64 * 2, 16, 1024, kSwizzle128), kS, piece > 0 || x > 0);
+            };
+            constexpr int kLast = S::DK - 128 * (S::PK - 1);
+            if (elected()) {
+              if (S::PK > 1 && piece < S::PK - 1)
+                products(std::integral_constant<int, 128>());
+              else
+                products(std::integral_constant<int, kLast>());
+              // K's piece is done with; of a latent cache only the one that is no part of V
+              if (!S::LATENT || piece == S::PK - 1) tc_commit(&c.empty[st][piece]);
+              if (piece == S::PK - 1) tc_commit(&c.sfull[buf]);
             }
             __syncwarp();
-            ++si;
+            if (++piece == S::PK) {
+              piece = 0;
+              ++si;
+            }
             issued = true;
           }
         }
@@ -731,8 +833,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     // ---- softmax ----
     if (S::WG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int wg = warp >> 2, quarter = warp & 3, bar = 1 + wg;
-    const bool active = S::C == 128 || lane < 16;
-    const int at = S::C == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);   // this thread's position of a chunk
+    // this thread's position of a chunk and, from col0 on, its rows of the group's
+    const int at = S::C == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);
+    const int col0 = S::C == 128 ? 0 : (lane >> 4) * S::NC;
     const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
     float* ref = rows.ref + wg * S::NW;
     float* alpha = rows.alpha + wg * S::NW;
@@ -747,14 +850,14 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     // q's rows into the first product's operand, zeros past the last
     auto load_q = [&](const Part& p) {
       constexpr int kUnits = S::DK / 8;   // 16-byte pieces of a row
-      const uint32_t f0 = (uint32_t)p.b.f0;
-      const int64_t row0 = p.b.row0;
+      const uint32_t f0 = (uint32_t)p.b.f0, rt0 = f0 / group, j0 = f0 - rt0 * group;
+      const int64_t row0 = p.b.row0 + rt0;
       const int count = p.b.count, head0 = p.head * a.group;
 #pragma unroll 4
       for (int i = 0; i < (S::NW * kUnits + 127) / 128; ++i) {
         const int x = i * 128 + own, row = x / kUnits, u = x % kUnits, r = wg * S::NW + row;
         if (S::NW * kUnits % 128 == 0 || row < S::NW) {
-          const uint32_t pair = f0 + r, rt = pair / group;
+          const uint32_t pair = j0 + r, rt = by_group(a, pair);
           const int64_t t = row0 + rt, h = head0 + (int)(pair - rt * group);
           const T* from = S::LATENT && u >= S::DV / 8
                               ? static_cast<const T*>(a.q_rot) + t * a.r_row + h * a.r_head + (8 * u - S::DV)
@@ -789,8 +892,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       known = false;
       const uint32_t t0 = (uint32_t)p.b.f0 / group, j0 = (uint32_t)p.b.f0 - t0 * group;
       if (own < S::NW) {
-        const uint32_t r = j0 + wg * S::NW + own;
-        place[own] = (int)(r / group << 16 | r % group);
+        // the row of out, counted over rows and heads (below 2^31)
+        const uint32_t r = j0 + wg * S::NW + own, rt = by_group(a, r);
+        place[own] = (int)((p.b.row0 + t0 + rt) * a.heads + (int64_t)p.head * a.group + (r - rt * group));
         ref[own] = -INFINITY;
       }
       uint32_t* marks = c.unbounded[filled & 1];
@@ -802,19 +906,17 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       const int64_t first_pos = p.b.first, last_pos = p.b.last;
       const int64_t start0 = (int64_t)(p.b.c0 + p.from) * S::C;
       const int pairs = p.b.count;
-      float l[S::NW];
+      float l[S::NC];
 #pragma unroll
-      for (int r = 0; r < S::NW; ++r) l[r] = 0.f;
+      for (int r = 0; r < S::NC; ++r) l[r] = 0.f;
 
       for (int i = 0; i < count; ++i, ++chunk) {
         const int buf = chunk & 1;
         bad = !__all_sync(0xffffffffu, bounded(&c.sfull[buf], (chunk >> 1) & 1)) || bad;
         tc_fence_after();
-        float y[S::NW];
+        float y[S::NC];
         auto load_scores = [&] {
-#pragma unroll
-          for (int r = 0; r < S::NW; r += 16)
-            tmem_ld16(lanes + buf * S::N + wg * S::NW + r, *reinterpret_cast<float(*)[16]>(&y[r]));
+          load_columns<S::C == 64>(lanes + buf * S::N + wg * S::NW, y);
           tmem_ld_wait();
         };
         load_scores();
@@ -840,18 +942,22 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
           const int64_t x = rel * group - j0, z = a.window > 0 ? (rel + a.window) * group - j0 : S::N;
           lo = x < 0 ? 0 : x > S::N ? S::N : (int)x;
           hi = z < 0 ? 0 : z > S::N ? S::N : (int)z;
-          if (!active || !(there >> (at / box) & 1)) lo = S::N;
+          if (!(there >> (at / box) & 1)) lo = S::N;
         }
-        const int lo_own = lo - wg * S::NW, hi_own = hi - wg * S::NW;
+        const int lo_own = lo - wg * S::NW - col0, hi_own = hi - wg * S::NW - col0;
         auto hide = [&] {
 #pragma unroll
-          for (int r = 0; r < S::NW; ++r)
-            if (r < lo_own || r >= hi_own) y[r] = -INFINITY;
+          for (int r = 0; r < S::NC; ++r)
+            if (r < lo_own) y[r] = -INFINITY;
+          if (a.window > 0)
+#pragma unroll
+            for (int r = 0; r < S::NC; ++r)
+              if (r >= hi_own) y[r] = -INFINITY;
         };
         auto less_reference = [&] {   // scores less the reference; what a row does not see is -infinity
 #pragma unroll
-          for (int r = 0; r < S::NW; r += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(ref + r);
+          for (int r = 0; r < S::NC; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(ref + col0 + r);
             y[r] = fmaf(y[r], sc, -f.x);
             y[r + 1] = fmaf(y[r + 1], sc, -f.y);
             y[r + 2] = fmaf(y[r + 2], sc, -f.z);
@@ -864,18 +970,19 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
           less_reference();
           float m[4] = {y[0], y[1], y[2], y[3]};
 #pragma unroll
-          for (int r = 4; r < S::NW; ++r) m[r % 4] = max_nan(m[r % 4], y[r]);
-          over = active && !(max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) <= kMost<T>);
+          for (int r = 4; r + 1 < S::NC; r += 2) m[r / 2 % 4] = max_nan(m[r / 2 % 4], y[r], y[r + 1]);
+          over = !(max_nan(max_nan(m[0], m[1], m[2]), m[3]) <= kMost<T>);
         }
         if (i == 0 || vote(bar, 128, bad || over)) {
           // a new reference
           if (i > 0) load_scores();
 #pragma unroll
-          for (int r = 0; r < S::NW; ++r) y[r] = active ? fmaxf(y[r] * sc, kFloor) : -INFINITY;
+          for (int r = 0; r < S::NC; ++r) y[r] = fmaxf(y[r] * sc, kFloor);
           if (!clean) hide();
-          spread<S::NW>(y, [](float u, float v) { return fmaxf(u, v); });
+          spread<S::NC, S::C / 4>(y, [](float u, float v) { return fmaxf(u, v); });
 #pragma unroll
-          for (int j = 0; j < (S::NW + 31) / 32; ++j) atomicMax(&top[spread_column<S::NW>(j)], ordered(y[j]));
+          for (int j = 0; j < spread_left<S::NC, S::C / 4>(); ++j)
+            atomicMax(&top[col0 + spread_column<S::NC, S::C / 4>(j)], ordered(y[j]));
           if (vote(bar, 128, bad)) {
             bad = true;
             break;
@@ -891,7 +998,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
           less_reference();
           if (i > 0) {   // the sums so far
 #pragma unroll
-            for (int r = 0; r < S::NW; ++r) l[r] *= alpha[r];
+            for (int r = 0; r < S::NC; ++r) l[r] *= alpha[col0 + r];
             const uint32_t b = (chunk - 1) % S::PB;
             bad = !__all_sync(0xffffffffu, bounded(&c.pdone[b], ((chunk - 1) / S::PB) & 1));
             if (!bad) {
@@ -919,12 +1026,18 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
           // V at positions that no row sees is whatever lay there, and 0 x NaN is no 0: zeros. Where some rows see a
           // position, what is not finite becomes zeros too and is added to those rows at the part's end.
           const uint32_t e = S::LATENT ? entry + i : i == count - 1 ? entry + 2 * count - 1 : entry + 2 * i + 2;
-          bad = !__all_sync(0xffffffffu, bounded(&c.full[e % S::R], (e / S::R) & 1)) || bad;
+#pragma unroll
+          for (int m = 0; m < S::PV; ++m)
+            bad = !__all_sync(0xffffffffu, bounded(&c.full[e % S::R][m], (e / S::R) & 1)) || bad;
           const bool seen = lo < min(hi, pairs);
-          if (active && !bad && (!seen || lo > 0 || hi < pairs)) {
+          if (!bad && (!seen || lo > 0 || hi < pairs)) {
             uint8_t* v = ring + e % S::R * S::kSlotBytes + at * 128;
             bool found = false;
-            for (int u = 0; u < S::DV / 8; ++u) {
+            constexpr int kUnits = S::C == 128 ? S::DV / 8 : S::DV / 16;   // two threads have a position where C is 64
+            const int unit0 = S::C == 128 ? 0 : (lane >> 4) * kUnits;
+#pragma unroll 4
+            for (int i = 0; i < kUnits; ++i) {
+              const int u = unit0 + i;
               uint4* w = reinterpret_cast<uint4*>(v + u / 8 * S::C * 128 + (u % 8) * 16);
               if (!seen) {
                 *w = make_uint4(0, 0, 0, 0);
@@ -946,18 +1059,16 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         const uint32_t pb = chunk % S::PB;
         if (chunk >= (uint32_t)S::PB)
           bad = !__all_sync(0xffffffffu, bounded(&c.pdone[pb], (chunk / S::PB - 1) & 1)) || bad;
-        uint8_t* to = pbuf + pb * S::kPBytes + wg * (S::NW / 8) * S::C * 16 + at * 16;
+        uint8_t* to = pbuf + pb * S::kPBytes + (wg * S::NW + col0) / 8 * S::C * 16 + at * 16;
 #pragma unroll
-        for (int r = 0; r < S::NW; r += 8) {
+        for (int r = 0; r < S::NC; r += 8) {
           uint32_t w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             w[j] = pack(ex2_approx(y[r + 2 * j]), ex2_approx(y[r + 2 * j + 1]), T());
-            const float2 f = unpack(w[j], T());
-            l[r + 2 * j] += f.x;
-            l[r + 2 * j + 1] += f.y;
+            add_halves(l[r + 2 * j], l[r + 2 * j + 1], w[j], T());
           }
-          if (active) *reinterpret_cast<uint4*>(to + r / 8 * S::C * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(to + r / 8 * S::C * 16) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -977,12 +1088,10 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         break;
       }
       float* sums = reinterpret_cast<float*>(pbuf + wg * (S::NW / 8) * S::C * 16);   // the group's part of P's place
-      if (!active)
+      spread<S::NC, S::C / 4>(l, [](float u, float v) { return u + v; });
 #pragma unroll
-        for (int r = 0; r < S::NW; ++r) l[r] = 0.f;
-      spread<S::NW>(l, [](float u, float v) { return u + v; });
-#pragma unroll
-      for (int j = 0; j < (S::NW + 31) / 32; ++j) sums[quarter * S::NW + spread_column<S::NW>(j)] = l[j];
+      for (int j = 0; j < spread_left<S::NC, S::C / 4>(); ++j)
+        sums[quarter * S::NW + col0 + spread_column<S::NC, S::C / 4>(j)] = l[j];
       named_bar_sync(bar, 128);
       const int slot = p.slot;
       float* acc = parts + (int64_t)slot * part_floats<S>();
@@ -1000,8 +1109,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       const int mine_rows = min(S::NW, pairs - wg * S::NW);
       const bool has_dim = S::MO == 128 || lane < 16;
       const int dim0 = S::MO == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);
-      // out as pairs of dims: even lanes take one row of two, odd lanes the other. rows x heads are below 2^31.
-      const int out_row = (int)((p.b.row0 + t0) * a.heads + (int64_t)p.head * a.group);
+      // out as pairs of dims: even lanes take one row of two, odd lanes the other
       T* out = static_cast<T*>(a.out) + (dim0 & ~1);
       uint32_t unbounded = 0;
 #pragma unroll
@@ -1028,12 +1136,11 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
               const float2 f = *reinterpret_cast<const float2*>(alpha + r + j);
-              const float even_row = f.x == 0.f ? 0.f : o[j] * f.x, odd_row = f.y == 0.f ? 0.f : o[j + 1] * f.y;
-              const float other = __shfl_xor_sync(0xffffffffu, odd ? even_row : odd_row, 1);
-              const uint32_t w = odd ? pack(other, odd_row, T()) : pack(even_row, other, T());
+              const uint32_t w = pack(o[j] * f.x, o[j + 1] * f.y, T()), other = __shfl_xor_sync(0xffffffffu, w, 1);
               const int x = r + j + odd;
-              const int row = out_row + (place[x] >> 16) * a.heads + (place[x] & 0xffff);
-              if (has_dim && x < mine_rows) *reinterpret_cast<uint32_t*>(out + (int64_t)row * S::DV + m * S::MO) = w;
+              if (has_dim && x < mine_rows)
+                *reinterpret_cast<uint32_t*>(out + (int64_t)place[x] * S::DV + m * S::MO) =
+                    __byte_perm(w, other, odd ? 0x3276 : 0x5410);
             }
           }
         }
@@ -1099,8 +1206,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
             d0 = tile / kRowTiles * kJoinDims;
   const Cut cut = reinterpret_cast<const Cut*>(parts + 2 * (int64_t)grid * part_floats<S>())[cta];
   if (r0 >= cut.count) return;
-  const int n = cut.last - cta + 1;
-  auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i)) * part_floats<S>(); };
+  const int n = cut.last - cta / a.team + 1;
+  auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i * a.team)) * part_floats<S>(); };
   const int group = tid / 256, dim = tid % 256 / 4, rows = tid % 4;
   const int at = (d0 + dim) * S::N + r0 + 4 * rows;
   constexpr int kAhead = 8;   // parts requested before their weights are known

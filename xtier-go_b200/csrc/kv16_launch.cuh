@@ -43,9 +43,12 @@ bool by_shape(bool latent, int head_dim, int v_dim, int rows, F&& f) {
   return false;
 }
 
+// Sequences of more row blocks than this go through their chunks block by block (prompts, whose keys stay in L2 meanwhile).
+constexpr int kMostTeam = 8;
+
 // defined in kv16_bf16.cu and kv16_f16.cu
 template <class T>
-void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int grid, cudaStream_t s);
+void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int rows_per_seq, int sms, cudaStream_t s);
 
 #ifdef KV16_TYPE
 template <class... P, class... A>
@@ -64,11 +67,21 @@ void launch_dependent(void (*f)(P...), unsigned grid, unsigned block, size_t sme
 }
 
 template <class T>
-void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int grid, cudaStream_t s) {
+void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int rows_per_seq, int sms, cudaStream_t s) {
   by_shape<T>(latent, head_dim, v_dim, rows, [&](auto shape) {
     using S = decltype(shape);
     Params a = p;
-    const int64_t slots = a.rows * a.group / S::N + a.seqs;
+    const int64_t blocks_per_seq = ((int64_t)a.group * rows_per_seq + S::N - 1) / S::N;
+    a.team = blocks_per_seq <= kMostTeam ? (int)std::min<int64_t>(blocks_per_seq, sms) : 1;
+    a.part_cost = 2;
+    a.least_share = 2;
+#ifdef KV16_TUNE
+    if (getenv("KP")) a.part_cost = atoi(getenv("KP"));
+    if (getenv("KL")) a.least_share = atoi(getenv("KL"));
+    if (getenv("KT")) a.team = atoi(getenv("KT"));
+#endif
+    const int grid = sms / a.team * a.team;
+    const int64_t slots = a.rows * a.group / (S::N * a.team) + a.seqs;
     XTG_REQUIRE(slots < (1ll << 31), "kv16: too many row blocks in one call");
     a.slots = (int)slots;
     static std::atomic<uint64_t> optin;
@@ -78,7 +91,7 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     launch_dependent(join_kernel<S>, blocks + (a.zero_rest ? 4 : 0), kJoinThreads, 0, s, a, grid, blocks);
   });
 }
-template void launch<KV16_TYPE>(const Params&, bool, int, int, int, int, cudaStream_t);
+template void launch<KV16_TYPE>(const Params&, bool, int, int, int, int, int, cudaStream_t);
 #endif
 
 }  // namespace kv16
