@@ -218,9 +218,11 @@ void launch_append(const AppendArgs& args, bool interleaved, unsigned grid, cuda
                        : cudaLaunchKernelEx(&cfg, append_kernel<X, T, false>, args));
 }
 
-// A pool's map: boxes of 64 dims x `box` slots of a page and KV head
+// A pool's map: boxes of `box` slots x 64 dims of a page and KV head, or of all dims where a box holds a chunk's positions:
+// 64 dims after 64 dims, as the products' operands lie. Few large copies: with boxes of 16 slots (2 KB each) 64 sequences of
+// 16384 .. 32768 positions took 900 us, with 64 slots 730 us.
 CUtensorMap pool_map(const void* pool, int dtype, int dims, int page, int heads, int64_t pages, int64_t slot, int64_t head,
-                     int64_t page_stride, int box) {
+                     int64_t page_stride, int box, bool whole) {
   static std::mutex mu;
   static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
   {
@@ -234,13 +236,13 @@ CUtensorMap pool_map(const void* pool, int dtype, int dims, int page, int heads,
     }
   }
   CUtensorMap map;
-  const cuuint64_t size[4] = {(cuuint64_t)dims, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)pages};
+  const cuuint64_t size[5] = {64u, (cuuint64_t)page, (cuuint64_t)dims / 64, (cuuint64_t)heads, (cuuint64_t)pages};
   // a stride that nothing steps by may be any
-  const cuuint64_t strides[3] = {(cuuint64_t)(slot * 2), (cuuint64_t)((heads > 1 ? head : dims) * 2),
+  const cuuint64_t strides[4] = {(cuuint64_t)(slot * 2), 128u, (cuuint64_t)((heads > 1 ? head : dims) * 2),
                                  (cuuint64_t)((pages > 1 ? page_stride : dims) * 2)};
-  const cuuint32_t boxes[4] = {64u, (cuuint32_t)box, 1u, 1u};
-  const cuuint32_t steps[4] = {1u, 1u, 1u, 1u};
-  const CUresult r = encode(&map, dtype == kKv16Bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+  const cuuint32_t boxes[5] = {64u, (cuuint32_t)box, whole ? (cuuint32_t)dims / 64 : 1u, 1u, 1u};
+  const cuuint32_t steps[5] = {1u, 1u, 1u, 1u, 1u};
+  const CUresult r = encode(&map, dtype == kKv16Bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                             const_cast<void*>(pool), size, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -328,9 +330,12 @@ void launch_kv16_attention(const Kv16Cache& c, const Kv16Attn& r, int sms, cudaS
   kv16::Params p = {};
   const int group = r.heads / c.kv_heads;
   // chunks of 128 positions, of 64 where the keys are wide (Shape::C)
-  const int box = std::min(c.page, c.head_dim <= 192 ? 128 : 64);
-  p.kmap = pool_map(c.k, c.dtype, c.head_dim, c.page, c.kv_heads, c.pages, c.k_slot, c.k_head, c.k_page, box);
-  p.vmap = c.latent ? p.kmap : pool_map(c.v, c.dtype, c.v_dim, c.page, c.kv_heads, c.pages, c.v_slot, c.v_head, c.v_page, box);
+  const int chunk = c.head_dim <= 192 ? 128 : 64, box = std::min(c.page, chunk);
+  p.kmap = pool_map(c.k, c.dtype, c.head_dim, c.page, c.kv_heads, c.pages, c.k_slot, c.k_head, c.k_page, box,
+                    box == chunk);
+  p.vmap = c.latent ? p.kmap
+                    : pool_map(c.v, c.dtype, c.v_dim, c.page, c.kv_heads, c.pages, c.v_slot, c.v_head, c.v_page, box,
+                               box == chunk);
   p.q = r.q;
   p.q_rot = r.q_rot;
   p.out = r.out;

@@ -61,8 +61,6 @@ struct Shape {
   static constexpr int kSlotBytes = (DK > DV ? DK : DV) * C * 2;
   static constexpr int kQBytes = N * DK * 2, kPBytes = N * C * 2;
   static constexpr int PB = N <= 32 ? 2 : 1;       // buffers of P
-  // A tile is copied, waited for and released in pieces of 128 dims, the second product's M
-  static constexpr int PK = (DK + 127) / 128, PV = LATENT ? 0 : (DV + 127) / 128, P = PK > PV ? PK : PV;
   static constexpr int kFit = (kSmem - kCtrl - kQBytes - PB * kPBytes) / kSlotBytes;
   static constexpr int R = kFit > 12 ? 12 : kFit;  // slots of the ring
   static constexpr int kSmemBytes = R * kSlotBytes + kQBytes + PB * kPBytes + kCtrl;
@@ -363,12 +361,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) 
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// a box of the cache: dims x .., slots y .., KV head z, page w
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+// a box of the cache: slots from y on of 64-dim slices from x on, of a KV head z and page w
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int y, int x, int z, int w, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(
           dst),
-      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      "l"(map), "r"(smem_u32(bar)), "r"(0), "r"(y), "r"(x), "r"(z), "r"(w)
       : "memory");
 }
 
@@ -501,7 +499,7 @@ constexpr int kInfo = 16, kQueue = 4;
 
 template <class S>
 struct Ctrl {
-  uint64_t full[S::R][S::P], empty[S::R][S::P], sfull[2], sfree[2], pready[2], pdone[2], qready, done, queue_full[kQueue],
+  uint64_t full[S::R], empty[S::R], sfull[2], sfree[2], pready[2], pdone[2], qready, done, queue_full[kQueue],
       queue_empty[kQueue];
   Part queue[kQueue];
   uint32_t info[kInfo];   // of chunks in turn: the pieces that are there
@@ -533,9 +531,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
 
   if (warp == kIssuer) tmem_alloc(&c.tmem, S::kCols);
   if (tid == 0) {
-    for (int i = 0; i < S::R * S::P; ++i) {
-      mbar_init(&c.full[0][i], 1);
-      mbar_init(&c.empty[0][i], 1);
+    for (int i = 0; i < S::R; ++i) {
+      mbar_init(&c.full[i], 1);
+      mbar_init(&c.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c.sfull[i], 1);
@@ -625,9 +623,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   Cut* cuts = reinterpret_cast<Cut*>(parts + 2 * (int64_t)gridDim.x * part_floats<S>());
   auto bounded = [&](uint64_t* bar, uint32_t parity) { return wait(bar, parity, a.polls, &c.failed, a.err); };
 
-  // 384 threads start with 168 registers each: the softmax's 8 warps take 216, the others keep 72
+  // 384 threads start with 168 registers each: the softmax's 8 warps take 200, the others keep 104
   if (warp >= kSoftmaxWarps) {
-  if (S::WG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (S::WG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == kProducer) {
     // ---- the walk and the copies: K of a chunk before V of the chunk before, as the products take them ----
     constexpr int kSlicesK = S::DK / 64, kSlicesV = S::DV / 64;
@@ -641,26 +639,21 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     Cut cut = {0, 0, 0, 0, 0};
     Part p;
     Walk<S> walk(a, sh);
-    uint32_t begun = 0;   // pieces asked for of a tile that was given up
-    // A tile of K or V into the next slot, piece by piece. A piece that V does not have is passed on empty, so that a slot's
-    // barriers turn alike.
+    // a tile of K or V into the next slot: in one copy where a page holds the chunk, else page by page and 64 dims at a time
     auto copy = [&](bool v, int head, int slot0, int page, uint32_t there) {
       const int st = entry % S::R, slices = v ? kSlicesV : kSlicesK;
       const CUtensorMap* map = v ? &a.vmap : &a.kmap;
       const uint32_t turn = entry / S::R, to = smem_u32(ring) + st * S::kSlotBytes;
-      for (int pc = 0; pc < S::P; ++pc) {
-        const int n = max(0, min(2, slices - 2 * pc));
-        if (turn > 0) ok = __all_sync(0xffffffffu, bounded(&c.empty[st][pc], (turn - 1) & 1));
-        if (!ok) {
-          begun = pc;
-          return;
-        }
-        if (lane == 0) mbar_expect_tx(&c.full[st][pc], (uint32_t)(__popc(there) * n * box * 128));
-        __syncwarp();
-        const int x = lane & (pieces - 1), slice = 2 * pc + lane / pieces;   // at most 8 boxes a slice
-        const int pg = __shfl_sync(0xffffffffu, page, x);
-        if (lane < n * pieces && (there >> x & 1))
-          load_box(to + slice * S::C * 128 + x * box * 128, map, 64 * slice, slot0, head, pg, &c.full[st][pc]);
+      if (turn > 0) ok = __all_sync(0xffffffffu, bounded(&c.empty[st], (turn - 1) & 1));
+      if (!ok) return;
+      if (lane == 0) mbar_expect_tx(&c.full[st], (uint32_t)(__popc(there) * slices * box * 128));
+      __syncwarp();
+      if (pieces == 1) {
+        if (lane == 0 && there) load_box(to, map, slot0, 0, head, page, &c.full[st]);
+      } else {
+        const int x = lane & (pieces - 1), pg = __shfl_sync(0xffffffffu, page, x);   // at most 8 pieces, 9 slices
+        for (int slice = lane / pieces; slice < slices; slice += 32 / pieces)
+          if (there >> x & 1) load_box(to + slice * S::C * 128 + x * box * 128, map, slot0, slice, head, pg, &c.full[st]);
       }
       ++entry;
     };
@@ -716,16 +709,11 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       }
     }
     // no copy is left in flight
-    auto landed = [&](uint32_t e, uint32_t n) {
-      for (uint32_t pc = 0; pc < n; ++pc) {
-        uint32_t spins = 0;
-        while (!mbar_try_wait(&c.full[e % S::R][pc], (e / S::R) & 1))
-          if (++spins > (1u << 18)) break;
-      }
-    };
-    landed(entry, begun);
-    for (uint32_t back = 1; back <= min(entry, (uint32_t)S::R); ++back)
-      landed(entry - back, S::P);
+    for (uint32_t e = entry > (uint32_t)S::R ? entry - S::R : 0; e < entry; ++e) {
+      uint32_t spins = 0;
+      while (!mbar_try_wait(&c.full[e % S::R], (e / S::R) & 1))
+        if (++spins > (1u << 18)) break;
+    }
     __syncwarp();
   } else if (warp == kIssuer) {
     // ---- the products: whichever of a chunk's second and the next one's first has its operands ----
@@ -747,31 +735,24 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       ++filled;
       tc_fence_after();
       uint32_t spins = 0;
-      int piece = 0;   // of K's tile, the first that the first product has not taken
       for (int si = 0, vi = 0; vi < n && ok;) {   // chunks whose first and whose second product were issued
         bool issued = false;
         if (vi < si) {
           const uint32_t e = S::LATENT ? entry + vi : vi == n - 1 ? entry + 2 * n - 1 : entry + 2 * vi + 2;
           const uint32_t st = e % S::R, ch = chunk + vi, pb = ch % S::PB;
-          bool there = passed(&c.pready[pb], (ch / S::PB) & 1);
-          if (!S::LATENT)   // of a latent cache the first product has waited for the tile
-#pragma unroll
-            for (int m = 0; m < S::PV; ++m) there = there && passed(&c.full[st][m], (e / S::R) & 1);
-          if (there) {
+          // (of a latent cache the first product has waited for the tile)
+          if (passed(&c.pready[pb], (ch / S::PB) & 1) && (S::LATENT || passed(&c.full[st], (e / S::R) & 1))) {
             tc_fence_after();
             const uint32_t v0 = ring0 + st * S::kSlotBytes, p0 = pb0 + pb * S::kPBytes;
             if (elected()) {
 #pragma unroll
-              for (int m = 0; m < S::DT; ++m) {
+              for (int m = 0; m < S::DT; ++m)
 #pragma unroll
                 for (int x = 0; x < S::C; x += 16)
                   mma(t + S::kO + m * S::N,
                       operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
                       operand(p0 + x * 16, 128, S::C * 16, 0), kOi, vi > 0 || x > 0);
-                tc_commit(&c.empty[st][m]);
-              }
-#pragma unroll
-              for (int m = S::DT; m < S::P && !S::LATENT; ++m) tc_commit(&c.empty[st][m]);
+              tc_commit(&c.empty[st]);
               tc_commit(&c.pdone[pb]);
             }
             __syncwarp();
@@ -782,30 +763,19 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         if (si < n && si < vi + 2) {
           const uint32_t e = S::LATENT ? entry + si : si == 0 ? entry : entry + 2 * si - 1;
           const uint32_t st = e % S::R, ch = chunk + si, buf = ch & 1;
-          if (passed(&c.full[st][piece], (e / S::R) & 1) && (piece > 0 || ch < 2 || passed(&c.sfree[buf], ((ch >> 1) - 1) & 1))) {
+          if (passed(&c.full[st], (e / S::R) & 1) && (ch < 2 || passed(&c.sfree[buf], ((ch >> 1) - 1) & 1))) {
             tc_fence_after();
-            const uint32_t k0 = ring0 + st * S::kSlotBytes + piece * S::C * 256, b0 = q0 + piece * S::N * 256;
-            auto products = [&](auto dims) {
-#pragma unroll
-              for (int x = 0; x < decltype(dims)::value; x += 16)
-                mma(t + buf * S::N, operand(k0 + x / 64 * S::C * 128 + x % 64 * 2, 16, 1024, kSwizzle128),
-                    operand(b0 + x / 64 * S::N * 128 + x % 64 * 2, 16, 1024, kSwizzle128), kS, piece > 0 || x > 0);
-            };
-            constexpr int kLast = S::DK - 128 * (S::PK - 1);
+            const uint32_t k0 = ring0 + st * S::kSlotBytes;
             if (elected()) {
-              if (S::PK > 1 && piece < S::PK - 1)
-                products(std::integral_constant<int, 128>());
-              else
-                products(std::integral_constant<int, kLast>());
-              // K's piece is done with; of a latent cache only the one that is no part of V
-              if (!S::LATENT || piece == S::PK - 1) tc_commit(&c.empty[st][piece]);
-              if (piece == S::PK - 1) tc_commit(&c.sfull[buf]);
+#pragma unroll
+              for (int x = 0; x < S::DK; x += 16)
+                mma(t + buf * S::N, operand(k0 + x / 64 * S::C * 128 + x % 64 * 2, 16, 1024, kSwizzle128),
+                    operand(q0 + x / 64 * S::N * 128 + x % 64 * 2, 16, 1024, kSwizzle128), kS, x > 0);
+              tc_commit(&c.sfull[buf]);
+              if (!S::LATENT) tc_commit(&c.empty[st]);
             }
             __syncwarp();
-            if (++piece == S::PK) {
-              piece = 0;
-              ++si;
-            }
+            ++si;
             issued = true;
           }
         }
@@ -831,7 +801,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   }
   } else {
     // ---- softmax ----
-    if (S::WG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (S::WG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int wg = warp >> 2, quarter = warp & 3, bar = 1 + wg;
     // this thread's position of a chunk and, from col0 on, its rows of the group's
     const int at = S::C == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);
@@ -1026,9 +996,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
           // V at positions that no row sees is whatever lay there, and 0 x NaN is no 0: zeros. Where some rows see a
           // position, what is not finite becomes zeros too and is added to those rows at the part's end.
           const uint32_t e = S::LATENT ? entry + i : i == count - 1 ? entry + 2 * count - 1 : entry + 2 * i + 2;
-#pragma unroll
-          for (int m = 0; m < S::PV; ++m)
-            bad = !__all_sync(0xffffffffu, bounded(&c.full[e % S::R][m], (e / S::R) & 1)) || bad;
+          bad = !__all_sync(0xffffffffu, bounded(&c.full[e % S::R], (e / S::R) & 1)) || bad;
           const bool seen = lo < min(hi, pairs);
           if (!bad && (!seen || lo > 0 || hi < pairs)) {
             uint8_t* v = ring + e % S::R * S::kSlotBytes + at * 128;
