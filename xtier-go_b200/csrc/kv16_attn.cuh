@@ -57,7 +57,7 @@ struct Shape {
   static constexpr int NW = N / WG;
   // Of these a thread has NC: all, or, where the 64 positions of a chunk lie in 16 of a warp's 32 lanes, half of them
   static constexpr int NC = C == 128 ? NW : NW / 2;
-  static constexpr int kThreads = WG == 2 ? 384 : 192;   // with the copies' warp and the products', and two that idle
+  static constexpr int kThreads = WG == 1 ? 192 : WG * 128 + 128;   // with the copies' warp and the products', and two that idle
   static constexpr int kSlotBytes = (DK > DV ? DK : DV) * C * 2;
   static constexpr int kQBytes = N * DK * 2, kPBytes = N * C * 2;
   static constexpr int PB = N <= 32 ? 2 : 1;       // buffers of P
@@ -992,20 +992,22 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&c.sfree[buf]);
-        if (!clean && wg == 0) {
+        if (!clean) {
           // V at positions that no row sees is whatever lay there, and 0 x NaN is no 0: zeros. Where some rows see a
-          // position, what is not finite becomes zeros too and is added to those rows at the part's end.
+          // position, what is not finite becomes zeros too and is added to those rows at the part's end. The groups take a
+          // share of the dims each.
           const uint32_t e = S::LATENT ? entry + i : i == count - 1 ? entry + 2 * count - 1 : entry + 2 * i + 2;
           bad = !__all_sync(0xffffffffu, bounded(&c.full[e % S::R], (e / S::R) & 1)) || bad;
           const bool seen = lo < min(hi, pairs);
           if (!bad && (!seen || lo > 0 || hi < pairs)) {
             uint8_t* v = ring + e % S::R * S::kSlotBytes + at * 128;
             bool found = false;
-            constexpr int kUnits = S::C == 128 ? S::DV / 8 : S::DV / 16;   // two threads have a position where C is 64
-            const int unit0 = S::C == 128 ? 0 : (lane >> 4) * kUnits;
+            constexpr int kUnits = S::DV / (S::C == 128 ? 8 : 16) / S::WG;   // two threads have a position where C is 64
+            const int unit0 = (S::C == 128 ? wg : 2 * wg + (lane >> 4)) * kUnits;
 #pragma unroll 4
             for (int i = 0; i < kUnits; ++i) {
-              const int u = unit0 + i;
+              // neighbouring positions take different 16-byte columns of the 8 at a time (of kUnits, if fewer)
+              const int u = unit0 + (i ^ (at & (kUnits < 8 ? kUnits - 1 : 7)));
               uint4* w = reinterpret_cast<uint4*>(v + u / 8 * S::C * 128 + (u % 8) * 16);
               if (!seen) {
                 *w = make_uint4(0, 0, 0, 0);
@@ -1144,18 +1146,22 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
 // Joins the parts of the item that starts in CTA c's share and ends in another's: one block per (c, 16 rows, 64 dims). A
 // warp a row for the parts' weights, then a thread 4 rows of a dim, every kGroups-th part. The blocks past these write
 // zeros for the rows that are no sequence's.
-constexpr int kJoinThreads = 512, kJoinRows = 16, kJoinDims = 64;
+constexpr int kJoinRows = 16, kJoinDims = 64;
+// Few rows: the parts are many and the blocks few, so two groups of threads and 8 parts each at once. Else the other way
+// round, and small blocks of which an SM holds many.
+template <class S>
+constexpr int kJoinGroups = S::N == 16 ? 2 : 1;
 template <class S>
 constexpr int join_blocks(int grid) {
   return grid * (S::N / kJoinRows) * (S::DV / kJoinDims);
 }
 template <class S>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
+__global__ void __launch_bounds__(256 * kJoinGroups<S>, kJoinGroups<S> == 2 ? 1 : 5) join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
   using T = typename S::T;
-  constexpr int kGroups = kJoinThreads / 256;
+  constexpr int kGroups = kJoinGroups<S>, kThreads = 256 * kGroups, kWarps = kThreads / 32;
   __shared__ __align__(16) float weight[kMaxGrid][kJoinRows];
   __shared__ float inv[kJoinRows];
-  __shared__ float4 more[kGroups - 1][256];
+  __shared__ float4 more[kGroups > 1 ? kGroups - 1 : 1][256];
   __shared__ __align__(16) T result[kJoinRows][kJoinDims];
   pdl_wait();
   pdl_launch_next();
@@ -1164,7 +1170,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     const int64_t first = row_bound(a, 0), last = row_bound(a, a.seqs), n = (int64_t)a.heads * S::DV / 8;
     for (int64_t i = blockIdx.x - blocks; i < first + (a.rows - last); i += gridDim.x - blocks) {
       uint4* to = reinterpret_cast<uint4*>(a.out) + (i < first ? i : last + (i - first)) * n;
-      for (int64_t x = tid; x < n; x += kJoinThreads) to[x] = make_uint4(0, 0, 0, 0);
+      for (int64_t x = tid; x < n; x += kThreads) to[x] = make_uint4(0, 0, 0, 0);
     }
     return;
   }
@@ -1178,29 +1184,30 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i * a.team)) * part_floats<S>(); };
   const int group = tid / 256, dim = tid % 256 / 4, rows = tid % 4;
   const int at = (d0 + dim) * S::N + r0 + 4 * rows;
-  constexpr int kAhead = 8;   // parts requested before their weights are known
+  constexpr int kAhead = kGroups == 2 ? 8 : 3;   // parts requested before their weights are known
   float4 ahead[kAhead];
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
     if (group + k * kGroups < n) ahead[k] = *reinterpret_cast<const float4*>(part(group + k * kGroups) + at);
   // a row's weights; NaN where a wait gave up
-  float top = -INFINITY, sum0 = 0.f;
-  for (int i = lane; i < n; i += 32) {
-    const float x = part(i)[S::N * S::DV + r0 + warp];
-    weight[i][warp] = x;
-    if (i < 32) sum0 = part(i)[S::N * (S::DV + 1) + r0 + warp];
-    top = max_nan(top, x);
-  }
+  for (int row = warp; row < kJoinRows; row += kWarps) {
+    float top = -INFINITY, sum0 = 0.f, total = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const float x = part(i)[S::N * S::DV + r0 + row];
+      if (i < 32) sum0 = part(i)[S::N * (S::DV + 1) + r0 + row];
+      weight[i][row] = x;
+      top = max_nan(top, x);
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float total = 0.f;
-  for (int i = lane; i < n; i += 32) {
-    const float x = weight[i][warp], w = x == -INFINITY ? 0.f : x == top ? 1.f : ex2_approx(x - top);
-    weight[i][warp] = w;
-    total = fmaf(w, i < 32 ? sum0 : part(i)[S::N * (S::DV + 1) + r0 + warp], total);
+    for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = lane; i < n; i += 32) {
+      const float x = weight[i][row], w = x == -INFINITY ? 0.f : x == top ? 1.f : ex2_approx(x - top);
+      weight[i][row] = w;
+      total = fmaf(w, i < 32 ? sum0 : part(i)[S::N * (S::DV + 1) + r0 + row], total);
+    }
+    total = warp_sum(total);
+    if (lane == 0) inv[row] = top == -INFINITY ? 0.f : 1.f / total;
   }
-  total = warp_sum(total);
-  if (lane == 0) inv[warp] = top == -INFINITY ? 0.f : 1.f / total;
   __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](int i, const float4& x) {
