@@ -472,15 +472,20 @@ __device__ __forceinline__ bool drop_unbounded(uint4& x, uint32_t exponent, uint
 __device__ __forceinline__ bool drop_unbounded(uint4& x, __nv_bfloat16) { return drop_unbounded(x, 0x7f807f80u, 0x00800080u); }
 __device__ __forceinline__ bool drop_unbounded(uint4& x, __half) { return drop_unbounded(x, 0x7c007c00u, 0x04000400u); }
 
-// Adds V's infinities and NaN of dim d at the marked positions (drop_unbounded) to the rows r0 .. r0 + 15 of the block that
-// see them: a weight above zero times these is these.
-template <class T>
-__device__ __forceinline__ void add_unbounded(const Params& a, const Part& p, const uint32_t* marks, int d, int r0, uint32_t j0,
-                                           float (&o)[16], T) {
-  for (int bit = 0; bit < 256; ++bit) {
-    if (!(marks[bit >> 5] >> (bit & 31) & 1)) continue;
-    const int64_t pos = bit < 128 ? p.b.first + bit : p.b.first - a.window + (bit - 128);
+// Adds V's infinities and NaN of dim d, which drop_unbounded has taken out of the part's chunks where some of the block's
+// rows see a position, to the rows r0 .. r0 + 15 that do: a weight above zero times these is these.
+template <class S>
+__device__ __forceinline__ void add_unbounded(const Params& a, const Part& p, int d, int r0, uint32_t j0, float (&o)[16]) {
+  using T = typename S::T;
+  const int64_t from = (int64_t)(p.b.c0 + p.from) * S::C, to = min(from + (int64_t)p.count * S::C, (int64_t)a.max_pages << a.page_log2);
+  const int between = (int)(p.b.last - p.b.first);   // positions that some rows see: behind the first row's, and before
+                                                     // what the last row's window starts with
+  for (int i = 1; i <= 2 * between; ++i) {
+    const int64_t pos = i <= between ? p.b.first + i : p.b.first - a.window + (i - between);
+    if (i > between && (a.window == 0 || pos > p.b.first)) break;
+    if (pos < from || pos >= to) continue;
     const int64_t page = a.table[(int64_t)p.b.s * a.max_pages + (pos >> a.page_log2)];
+    if (page < 0 || page >= a.pages) continue;
     const int64_t slot = pos & ((1 << a.page_log2) - 1);
     const float v = static_cast<float>(
         reinterpret_cast<const T*>(a.v)[page * a.v_page + p.head * a.v_head + slot * a.v_slot + d]);
@@ -498,7 +503,7 @@ __device__ __forceinline__ void add_unbounded(const Params& a, const Part& p, co
 constexpr int kInfo = 16, kQueue = 4;
 
 template <class S>
-struct Ctrl {
+struct __align__(16) Ctrl {
   uint64_t full[S::R], empty[S::R], sfull[2], sfree[2], pready[2], pdone[2], qready, done, queue_full[kQueue],
       queue_empty[kQueue];
   Part queue[kQueue];
@@ -507,7 +512,8 @@ struct Ctrl {
   Block share_block;
   uint32_t tmem;
   int failed;
-  uint32_t unbounded[2][8];       // of every second part that has chunks: positions seen by some rows, with values that are not finite
+  int unbounded[4];   // of every 4th part that has chunks: whether positions that some rows see have values that are not
+                      // finite
 };
 template <class S>
 struct __align__(16) Rows {
@@ -525,7 +531,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   uint8_t* pbuf = qbuf + S::kQBytes;
   Ctrl<S>& c = *reinterpret_cast<Ctrl<S>*>(pbuf + S::PB * S::kPBytes);
   Rows<S>& rows = *reinterpret_cast<Rows<S>*>(&c + 1);
-  static_assert(sizeof(Ctrl<S>) + sizeof(Rows<S>) <= kCtrl, "control block");
+  static_assert(sizeof(Ctrl<S>) % 16 == 0 && sizeof(Ctrl<S>) + sizeof(Rows<S>) <= kCtrl, "control block");
   constexpr int kSoftmaxWarps = 4 * S::WG, kProducer = kSoftmaxWarps, kIssuer = kSoftmaxWarps + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
@@ -542,6 +548,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       mbar_init(&c.pdone[i], 1);
     }
     mbar_init(&c.qready, kSoftmaxWarps);
+    for (int i = 0; i < 4; ++i) c.unbounded[i] = 0;
     mbar_init(&c.done, 1);
     for (int i = 0; i < kQueue; ++i) {
       mbar_init(&c.queue_full[i], 1);
@@ -867,9 +874,10 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         place[own] = (int)((p.b.row0 + t0 + rt) * a.heads + (int64_t)p.head * a.group + (r - rt * group));
         ref[own] = -INFINITY;
       }
-      uint32_t* marks = c.unbounded[filled & 1];
+      volatile int* const unbounded = &c.unbounded[filled % 4];
       if (count > 0) {
-        if (wg == 0 && own < 8) marks[own] = 0;
+        // the other group is in this part or at the end of the one before: a chunk's second product waits for both
+        if (wg == 0 && own == 0) c.unbounded[(filled + 2) % 4] = 0;
         ++filled;
       }
       named_bar_sync(bar, 128);
@@ -1019,10 +1027,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
                 }
               }
             }
-            if (found) {
-              const int bit = pos > first_pos ? (int)(pos - first_pos) : 128 + (int)(pos - (first_pos - a.window));
-              atomicOr(&marks[bit >> 5 & 7], 1u << (bit & 31));
-            }
+            if (found) *unbounded = 1;
           }
         }
         // P, rounded, and its sums
@@ -1081,9 +1086,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       const int dim0 = S::MO == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);
       // out as pairs of dims: even lanes take one row of two, odd lanes the other
       T* out = static_cast<T*>(a.out) + (dim0 & ~1);
-      uint32_t unbounded = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) unbounded |= count > 0 ? marks[j] : 0;
+      const bool add = count > 0 && *unbounded != 0;
 #pragma unroll 1
       for (int m = 0; m < S::DT; ++m)
 #pragma unroll 1
@@ -1094,7 +1097,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
             tmem_ld_wait();
           }
           const int d = m * S::MO + dim0;
-          if (unbounded != 0 && has_dim) add_unbounded(a, p, marks, d, wg * S::NW + r, j0, o, T());
+          if (add && has_dim) add_unbounded<S>(a, p, d, wg * S::NW + r, j0, o);
           if (slot >= 0) {
             if (has_dim) {
               float4* to = reinterpret_cast<float4*>(acc + d * S::N + wg * S::NW + r);
@@ -1147,18 +1150,16 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
 // warp a row for the parts' weights, then a thread 4 rows of a dim, every kGroups-th part. The blocks past these write
 // zeros for the rows that are no sequence's.
 constexpr int kJoinRows = 16, kJoinDims = 64;
-// Few rows: the parts are many and the blocks few, so two groups of threads and 8 parts each at once. Else the other way
+// GROUPS: where an item has many parts and the blocks are few, two groups of threads and 8 parts each at once. Else the other way
 // round, and small blocks of which an SM holds many.
-template <class S>
-constexpr int kJoinGroups = S::N == 16 ? 2 : 1;
 template <class S>
 constexpr int join_blocks(int grid) {
   return grid * (S::N / kJoinRows) * (S::DV / kJoinDims);
 }
-template <class S>
-__global__ void __launch_bounds__(256 * kJoinGroups<S>, kJoinGroups<S> == 2 ? 1 : 5) join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
+template <class S, int GROUPS>
+__global__ void __launch_bounds__(256 * GROUPS, GROUPS == 2 ? 1 : 5) join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
   using T = typename S::T;
-  constexpr int kGroups = kJoinGroups<S>, kThreads = 256 * kGroups, kWarps = kThreads / 32;
+  constexpr int kGroups = GROUPS, kThreads = 256 * kGroups, kWarps = kThreads / 32;
   __shared__ __align__(16) float weight[kMaxGrid][kJoinRows];
   __shared__ float inv[kJoinRows];
   __shared__ float4 more[kGroups > 1 ? kGroups - 1 : 1][256];

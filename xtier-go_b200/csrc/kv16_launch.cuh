@@ -88,7 +88,12 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     ensure_smem_optin(reinterpret_cast<const void*>(&attention_kernel<S>), S::kSmemBytes, optin);
     launch_dependent(attention_kernel<S>, (unsigned)grid, S::kThreads, S::kSmemBytes, s, a);
     const unsigned blocks = (unsigned)join_blocks<S>(grid);
-    launch_dependent(join_kernel<S>, blocks + (a.zero_rest ? 4 : 0), 256 * kJoinGroups<S>, 0, s, a, grid, blocks);
+    const unsigned all = blocks + (a.zero_rest ? 4 : 0);
+    // an item is cut into grid / items parts or so: 2 groups of threads in a block from 4 parts on
+    if (slots * a.kv_heads * a.team * 4 <= grid)
+      launch_dependent(join_kernel<S, 2>, all, 512, 0, s, a, grid, blocks);
+    else
+      launch_dependent(join_kernel<S, 1>, all, 256, 0, s, a, grid, blocks);
   });
 }
 template void launch<KV16_TYPE>(const Params&, bool, int, int, int, int, int, cudaStream_t);
