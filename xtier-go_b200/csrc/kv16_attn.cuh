@@ -85,6 +85,7 @@ struct Params {
   int max_pages, seqs, page_log2, heads, kv_heads, group, window;
   uint32_t group_inv;
   int team;   // CTAs beside each other, a divisor of the grid
+  bool by_item;   // how the cuts are counted
   int part_cost, least_share;   // in chunks: a part's start and end where shares are cut, a share at least
   int slots;   // (sequence, row block) numbers, some of them empty
   float scale;
@@ -109,7 +110,7 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {   // not negat
 // blocks of a team have numbers from cu_rows[s] group / (N team) + s on: at least as many as it needs, found without a
 // prefix sum over the sequences.
 struct Block {
-  int s;
+  int s, p0;         // sequence, the position of its first row
   int64_t row0, f0;  // the call's row of the sequence's first, and the block's first pair in the sequence
   int count;         // pairs, 0: none
   int c0, chunks;    // the first chunk that one of its rows sees, and how many
@@ -134,12 +135,11 @@ __device__ __forceinline__ int find_sequence(const Params& a, int64_t number) {
   return lo;
 }
 
-// Sequence s's pairs f0 .. f0 + count - 1
+// Sequence s's pairs f0 .. f0 + count - 1; p0: the position of its first row
 template <class S>
-__device__ __forceinline__ Block block_at(const Params& a, int s, int64_t row0, int64_t f0, int count) {
-  Block b = {s, row0, f0, count, 0, 0, 0, 0};
+__device__ __forceinline__ Block block_at(const Params& a, int s, int p0, int64_t row0, int64_t f0, int count) {
+  Block b = {s, p0, row0, f0, count, 0, 0, 0, 0};
   if (count == 0) return b;
-  const int p0 = a.pos[s];
   b.first = (int64_t)p0 + (uint32_t)f0 / (uint32_t)a.group;   // pairs are below 2^31
   b.last = (int64_t)p0 + (uint32_t)(f0 + count - 1) / (uint32_t)a.group;
   const int64_t end = (int64_t)a.max_pages << a.page_log2;
@@ -155,10 +155,11 @@ __device__ __forceinline__ Block block_at(const Params& a, int s, int64_t row0, 
 // The blocks of a team with this number
 template <class S>
 __device__ __forceinline__ Block block_of(const Params& a, int s, int64_t number) {
+  const int p0 = a.pos[s];   // all that it needs at once
   const int64_t row0 = row_bound(a, s), n = row_bound(a, s + 1) - row0, pairs = n > 0 ? n * a.group : 0;
   const int most = S::N * a.team;
   const int64_t f0 = (number - block_start<S>(a, s)) * most, left = pairs - f0;
-  return block_at<S>(a, s, row0, f0, f0 < 0 || left <= 0 ? 0 : left < most ? (int)left : most);
+  return block_at<S>(a, s, p0, row0, f0, f0 < 0 || left <= 0 ? 0 : left < most ? (int)left : most);
 }
 
 struct Part {
@@ -173,7 +174,7 @@ __device__ __forceinline__ uint32_t by_group(const Params& a, uint32_t x) { retu
 // What the joining kernel needs about the block that starts in a CTA's share and ends in another's
 struct Cut {
   int64_t row0, f0;
-  int head, count, last;   // count 0: there is none; last: the team that ends it
+  int head, count, first, last;   // count 0: there is none; the CTA that starts it, the team that ends it
 };
 
 template <class S>
@@ -187,7 +188,8 @@ template <class S>
 __host__ __device__ constexpr int64_t part_floats() {
   return (int64_t)S::N * (S::DV + 2);
 }
-// workspace: 2 parts a CTA (acc [DV][N], reference [N], sum [N]), then the cuts
+// workspace: 2 parts a CTA (acc [DV][N], reference [N], sum [N]), then the cuts, by CTA or, where there are fewer, by
+// (block number, KV head, CTA of the team)
 template <class S>
 __host__ __device__ constexpr int64_t work_bytes(int grid) {
   return 2 * (int64_t)grid * part_floats<S>() * 4 + (int64_t)grid * (int64_t)sizeof(Cut);
@@ -209,8 +211,8 @@ struct Walk {
     s = b.s;
   }
 
-  // The next part of the share; cut: filled for an item that goes on in other shares
-  __device__ bool next(Part& p, Cut& cut) {
+  // The next part of the share. The blocks that start in it are noted in `cuts` (if given) for the joining kernel.
+  __device__ bool next(Part& p, Cut* cuts) {
     while (have && base < sh.to) {
       if (b.count > 0 && head < a.kv_heads) {
         const int64_t at = base + a.part_cost;   // the item's first chunk
@@ -228,15 +230,17 @@ struct Walk {
         }
         const bool starts = i == 0, ends = j == b.chunks;
         p = {b, h, i, j - i, starts && ends ? -1 : starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x};
+        const int member = (int)(blockIdx.x % a.team), before = member * S::N;
         if (a.team > 1) {   // this CTA's block of the team's; it may see fewer chunks, or none of the share's
-          const int before = (int)(blockIdx.x % a.team) * S::N;
-          if (before >= b.count) continue;
-          p.b = block_at<S>(a, s, b.row0, b.f0 + before, min(b.count - before, S::N));
+          p.b = block_at<S>(a, s, b.p0, b.row0, b.f0 + before, max(min(b.count - before, S::N), 0));
           const int x = max(b.c0 + i, p.b.c0), y = min(b.c0 + j, p.b.c0 + p.b.chunks);
           p.from = x - p.b.c0;
           p.count = max(y - x, 0);
         }
-        if (starts && !ends) cut = {p.b.row0, p.b.f0, h, p.b.count, (int)divide(at + b.chunks - 1, sh.each)};
+        if (cuts && starts && (a.by_item || !ends))
+          cuts[a.by_item ? (number * a.kv_heads + h) * a.team + member : blockIdx.x] = {
+              p.b.row0, p.b.f0, h, ends ? 0 : p.b.count, (int)blockIdx.x, (int)divide(at + b.chunks - 1, sh.each)};
+        if (p.b.count == 0) continue;
         return true;
       }
       head = 0;
@@ -559,6 +563,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   }
   for (int i = tid; i < S::N; i += S::kThreads) rows.top[i] = ordered(-INFINITY);
 
+  float* parts = a.work;
+  Cut* cuts = reinterpret_cast<Cut*>(parts + 2 * (int64_t)gridDim.x * part_floats<S>());
+
   // ---- the share: every thread the cost of some blocks, then a sum over the CTA ----
   pdl_wait();
   pdl_launch_next();
@@ -576,7 +583,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     }
   };
   int64_t mine = 0;
-  over_blocks([&](int, const Block& b) {
+  over_blocks([&](int i, const Block& b) {
+    if (blockIdx.x == 0 && a.by_item && b.count == 0)   // no share has these
+      for (int x = 0; x < a.kv_heads * a.team; ++x) cuts[(int64_t)i * a.kv_heads * a.team + x].count = 0;
     if (blockIdx.x == 0 && a.err && b.count > 0 && b.last >= (int64_t)a.max_pages << a.page_log2) atomicExch(a.err, 6);
     mine += cost(b);
     return false;
@@ -626,8 +635,6 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   sh.base = sh.from < sh.to ? c.share_base : 0;
   sh.block = c.share_block;
   const uint32_t tmem = c.tmem;
-  float* parts = a.work;
-  Cut* cuts = reinterpret_cast<Cut*>(parts + 2 * (int64_t)gridDim.x * part_floats<S>());
   auto bounded = [&](uint64_t* bar, uint32_t parity) { return wait(bar, parity, a.polls, &c.failed, a.err); };
 
   // 384 threads start with 168 registers each: the softmax's 8 warps take 200, the others keep 104
@@ -643,7 +650,6 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       ok = false;
     }
     uint32_t entry = 0, chunk = 0, queued = 0;
-    Cut cut = {0, 0, 0, 0, 0};
     Part p;
     Walk<S> walk(a, sh);
     // a tile of K or V into the next slot: in one copy where a page holds the chunk, else page by page and 64 dims at a time
@@ -664,7 +670,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       }
       ++entry;
     };
-    while (walk.next(p, cut)) {
+    Cut* const note = lane == 0 ? cuts : nullptr;
+    if (!a.by_item && lane == 0) cuts[blockIdx.x].count = 0;
+    while (walk.next(p, note)) {
       if (ok) {
         const int qi = queued % kQueue;
         if (queued >= kQueue) ok = __all_sync(0xffffffffu, bounded(&c.queue_empty[qi], (queued / kQueue - 1) & 1));
@@ -706,7 +714,6 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         page = next_page;
       }
     }
-    if (lane == 0) cuts[blockIdx.x] = cut;
     if (ok) {   // the end of the queue
       const int qi = queued % kQueue;
       if (queued >= kQueue) ok = __all_sync(0xffffffffu, bounded(&c.queue_empty[qi], (queued / kQueue - 1) & 1));
@@ -1124,8 +1131,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
     if (bad) {   // a wait gave up: NaN for the rows of the share
       Walk<S> walk(a, sh);
       Part p;
-      Cut cut;
-      while (walk.next(p, cut)) {
+      while (walk.next(p, nullptr)) {
         const int64_t t0 = p.b.f0 / a.group;
         const int j0 = (int)(p.b.f0 % a.group);
         for (int r = wg * S::NW; r < min((wg + 1) * S::NW, p.b.count); ++r) {
@@ -1146,18 +1152,18 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   if (warp == kIssuer) tmem_dealloc(tmem, S::kCols);
 }
 
-// Joins the parts of the item that starts in CTA c's share and ends in another's: one block per (c, 16 rows, 64 dims). A
+// Joins the parts of the item that starts in CTA c's share and ends in another's: one block per (cut, 16 rows, 64 dims). A
 // warp a row for the parts' weights, then a thread 4 rows of a dim, every kGroups-th part. The blocks past these write
 // zeros for the rows that are no sequence's.
 constexpr int kJoinRows = 16, kJoinDims = 64;
-// GROUPS: where an item has many parts and the blocks are few, two groups of threads and 8 parts each at once. Else the other way
-// round, and small blocks of which an SM holds many.
+// GROUPS of 256 threads: 4 where the cuts are counted by item, which are few then and have many parts each, else one, and an
+// SM holds several blocks.
 template <class S>
-constexpr int join_blocks(int grid) {
-  return grid * (S::N / kJoinRows) * (S::DV / kJoinDims);
+constexpr unsigned join_blocks(int cuts) {
+  return (unsigned)cuts * (S::N / kJoinRows) * (S::DV / kJoinDims);
 }
 template <class S, int GROUPS>
-__global__ void __launch_bounds__(256 * GROUPS, GROUPS == 2 ? 1 : 5) join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
+__global__ void __launch_bounds__(256 * GROUPS, GROUPS == 4 ? 1 : 5) join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
   using T = typename S::T;
   constexpr int kGroups = GROUPS, kThreads = 256 * kGroups, kWarps = kThreads / 32;
   __shared__ __align__(16) float weight[kMaxGrid][kJoinRows];
@@ -1177,15 +1183,15 @@ __global__ void __launch_bounds__(256 * GROUPS, GROUPS == 2 ? 1 : 5) join_kernel
   }
   const float* parts = a.work;
   constexpr int kRowTiles = S::N / kJoinRows, kTiles = kRowTiles * (S::DV / kJoinDims);
-  const int cta = blockIdx.x / kTiles, tile = blockIdx.x % kTiles, r0 = tile % kRowTiles * kJoinRows,
+  const int which = blockIdx.x / kTiles, tile = blockIdx.x % kTiles, r0 = tile % kRowTiles * kJoinRows,
             d0 = tile / kRowTiles * kJoinDims;
-  const Cut cut = reinterpret_cast<const Cut*>(parts + 2 * (int64_t)grid * part_floats<S>())[cta];
+  const Cut cut = reinterpret_cast<const Cut*>(parts + 2 * (int64_t)grid * part_floats<S>())[which];
   if (r0 >= cut.count) return;
-  const int n = cut.last - cta / a.team + 1;
+  const int cta = cut.first, n = cut.last - cta / a.team + 1;
   auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * cta + 1 : 2 * (cta + i * a.team)) * part_floats<S>(); };
   const int group = tid / 256, dim = tid % 256 / 4, rows = tid % 4;
   const int at = (d0 + dim) * S::N + r0 + 4 * rows;
-  constexpr int kAhead = kGroups == 2 ? 8 : 3;   // parts requested before their weights are known
+  constexpr int kAhead = kGroups == 4 ? 4 : 3;   // parts requested before their weights are known
   float4 ahead[kAhead];
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)

@@ -84,14 +84,14 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     const int64_t slots = a.rows * a.group / (S::N * a.team) + a.seqs;
     XTG_REQUIRE(slots < (1ll << 31), "kv16: too many row blocks in one call");
     a.slots = (int)slots;
+    const int64_t items = slots * a.kv_heads * a.team;
+    a.by_item = items <= grid / 4;
     static std::atomic<uint64_t> optin;
     ensure_smem_optin(reinterpret_cast<const void*>(&attention_kernel<S>), S::kSmemBytes, optin);
     launch_dependent(attention_kernel<S>, (unsigned)grid, S::kThreads, S::kSmemBytes, s, a);
-    const unsigned blocks = (unsigned)join_blocks<S>(grid);
-    const unsigned all = blocks + (a.zero_rest ? 4 : 0);
-    // an item is cut into grid / items parts or so: 2 groups of threads in a block from 4 parts on
-    if (slots * a.kv_heads * a.team * 4 <= grid)
-      launch_dependent(join_kernel<S, 2>, all, 512, 0, s, a, grid, blocks);
+    const unsigned blocks = join_blocks<S>(a.by_item ? (int)items : grid), all = blocks + (a.zero_rest ? 4 : 0);
+    if (a.by_item)
+      launch_dependent(join_kernel<S, 4>, all, 1024, 0, s, a, grid, blocks);
     else
       launch_dependent(join_kernel<S, 1>, all, 256, 0, s, a, grid, blocks);
   });
