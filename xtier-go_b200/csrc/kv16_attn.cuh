@@ -85,6 +85,7 @@ struct Params {
   int max_pages, seqs, page_log2, heads, kv_heads, group, window;
   uint32_t group_inv;
   int team;   // CTAs beside each other, a divisor of the grid
+  uint32_t team_inv;   // ceil(2^32 / team)
   bool by_item;   // how the cuts are counted
   int part_cost, least_share;   // in chunks: a part's start and end where shares are cut, a share at least
   int slots;   // (sequence, row block) numbers, some of them empty
@@ -119,7 +120,8 @@ struct Block {
 
 template <class S>
 __device__ __forceinline__ int64_t block_start(const Params& a, int s) {
-  return divide(row_bound(a, s) * a.group, S::N * a.team) + s;
+  const uint32_t blocks = (uint32_t)(row_bound(a, s) * a.group) / S::N;   // pairs are below 2^31
+  return (a.team == 1 ? blocks : __umulhi(blocks, a.team_inv)) + s;        // blocks / team: below 2^27, team at most 8
 }
 
 template <class S>
@@ -512,8 +514,8 @@ struct __align__(16) Ctrl {
       queue_empty[kQueue];
   Part queue[kQueue];
   uint32_t info[kInfo];   // of chunks in turn: the pieces that are there
-  int64_t share_number, share_base, scan[12];
-  Block share_block;
+  int64_t scan[12];
+  Share<S> share;
   uint32_t tmem;
   int failed;
   int unbounded[4];   // of every 4th part that has chunks: whether positions that some rows see have values that are not
@@ -566,75 +568,88 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   float* parts = a.work;
   Cut* cuts = reinterpret_cast<Cut*>(parts + 2 * (int64_t)gridDim.x * part_floats<S>());
 
-  // ---- the share: every thread the cost of some blocks, then a sum over the CTA ----
-  pdl_wait();
-  pdl_launch_next();
-  const int each = (a.slots + S::kThreads - 1) / S::kThreads;
-  const int first = min(tid * each, a.slots), last = min(first + each, a.slots);
+  // ---- the share: the cost of every block, summed up over `threads` threads, of which this is number `index` ----
   auto cost = [&](const Block& b) { return b.count > 0 ? (int64_t)(b.chunks + a.part_cost) * a.kv_heads : (int64_t)0; };
-  Block kept;   // the only one, where each is 1
-  auto over_blocks = [&](auto&& f) {
-    if (first >= last) return;
-    int s = find_sequence<S>(a, first);
-    for (int i = first; i < last; ++i) {
-      if (s + 1 < a.seqs && block_start<S>(a, s + 1) <= i) ++s;
-      kept = block_of<S>(a, s, i);
-      if (f(i, kept)) break;
+  auto plan = [&](int index, int threads, auto&& sum_before) {
+    const int each = (a.slots + threads - 1) / threads;
+    const int first = min(index * each, a.slots), last = min(first + each, a.slots);
+    Block kept;   // the only one, where each is 1
+    auto over_blocks = [&](auto&& f) {
+      if (first >= last) return;
+      int s = find_sequence<S>(a, first);
+      for (int i = first; i < last; ++i) {
+        if (s + 1 < a.seqs && block_start<S>(a, s + 1) <= i) ++s;
+        kept = block_of<S>(a, s, i);
+        if (f(i, kept)) break;
+      }
+    };
+    int64_t mine = 0, before, total;
+    over_blocks([&](int i, const Block& b) {
+      if (blockIdx.x == 0 && a.by_item && b.count == 0)   // no share has these
+        for (int x = 0; x < a.kv_heads * a.team; ++x) cuts[(int64_t)i * a.kv_heads * a.team + x].count = 0;
+      if (blockIdx.x == 0 && a.err && b.count > 0 && b.last >= (int64_t)a.max_pages << a.page_log2) atomicExch(a.err, 6);
+      mine += cost(b);
+      return false;
+    });
+    sum_before(mine, before, total);
+    const uint32_t teams = gridDim.x / a.team;
+    Share<S> sh;
+    sh.each = max(divide(total + teams - 1, teams), (int64_t)(a.part_cost + a.least_share));
+    sh.from = sh.each * (blockIdx.x / a.team);
+    sh.to = sh.from + sh.each < total ? sh.from + sh.each : total;
+    if (sh.from >= sh.to) {
+      if (index == 0) c.share.from = c.share.to = 0;
+    } else if (before <= sh.from && sh.from < before + mine) {
+      int64_t at = before;
+      auto start = [&](int i, const Block& b) {
+        const int64_t x = cost(b);
+        if (sh.from < at + x) {
+          sh.number = i;
+          sh.base = at;
+          sh.block = b;
+          c.share = sh;
+          return true;
+        }
+        at += x;
+        return false;
+      };
+      if (each == 1)
+        start(first, kept);
+      else
+        over_blocks(start);
     }
   };
-  int64_t mine = 0;
-  over_blocks([&](int i, const Block& b) {
-    if (blockIdx.x == 0 && a.by_item && b.count == 0)   // no share has these
-      for (int x = 0; x < a.kv_heads * a.team; ++x) cuts[(int64_t)i * a.kv_heads * a.team + x].count = 0;
-    if (blockIdx.x == 0 && a.err && b.count > 0 && b.last >= (int64_t)a.max_pages << a.page_log2) atomicExch(a.err, 6);
-    mine += cost(b);
-    return false;
-  });
-  int64_t before = mine;   // over the warp, itself included
+  auto over_warp = [&](int64_t mine, int64_t& upto) {
+    upto = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += x;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+  };
+  // Few blocks: the copies' warp alone, which is the one to wait for it.
+  const bool small_plan = a.slots <= 256;
+  if (!small_plan) {
+    pdl_wait();
+    plan(tid, S::kThreads, [&](int64_t mine, int64_t& before, int64_t& total) {
+      int64_t upto;
+      over_warp(mine, upto);
+      if (lane == 31) c.scan[warp] = upto;
+      __syncthreads();
+      total = 0;
+      before = upto - mine;
+#pragma unroll
+      for (int w = 0; w < S::kThreads / 32; ++w) {
+        if (w < warp) before += c.scan[w];
+        total += c.scan[w];
+      }
+    });
   }
-  if (lane == 31) c.scan[warp] = before;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  int64_t total = 0;
-  before -= mine;
-#pragma unroll
-  for (int w = 0; w < S::kThreads / 32; ++w) {
-    if (w < warp) before += c.scan[w];
-    total += c.scan[w];
-  }
-  Share<S> sh;
-  const uint32_t teams = gridDim.x / a.team;
-  sh.each = max(divide(total + teams - 1, teams), (int64_t)(a.part_cost + a.least_share));
-  sh.from = sh.each * (blockIdx.x / a.team);
-  sh.to = sh.from + sh.each < total ? sh.from + sh.each : total;
-  if (sh.from < sh.to && before <= sh.from && sh.from < before + mine) {
-    int64_t at = before;
-    auto start = [&](int i, const Block& b) {
-      const int64_t x = cost(b);
-      if (sh.from < at + x) {
-        c.share_number = i;
-        c.share_base = at;
-        c.share_block = b;
-        return true;
-      }
-      at += x;
-      return false;
-    };
-    if (each == 1)
-      start(first, kept);
-    else
-      over_blocks(start);
-  }
-  __syncthreads();
-  sh.number = sh.from < sh.to ? c.share_number : 0;
-  sh.base = sh.from < sh.to ? c.share_base : 0;
-  sh.block = c.share_block;
   const uint32_t tmem = c.tmem;
+  bool gave_up = false;
   auto bounded = [&](uint64_t* bar, uint32_t parity) { return wait(bar, parity, a.polls, &c.failed, a.err); };
 
   // 384 threads start with 168 registers each: the softmax's 8 warps take 200, the others keep 104
@@ -643,15 +658,26 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
   if (warp == kProducer) {
     // ---- the walk and the copies: K of a chunk before V of the chunk before, as the products take them ----
     constexpr int kSlicesK = S::DK / 64, kSlicesV = S::DV / 64;
-    const int box = min(1 << a.page_log2, S::C), pieces = S::C / box;
+    const int box = min(1 << a.page_log2, S::C), pieces_log2 = __ffs(S::C / box) - 1, pieces = 1 << pieces_log2;
     bool ok = true;
     if (a.polls == 0) {   // without a look
       give_up(&c.failed, a.err);
       ok = false;
     }
+    pdl_wait();
+    pdl_launch_next();
+    if (small_plan) {
+      plan(lane, 32, [&](int64_t mine, int64_t& before, int64_t& total) {
+        int64_t upto;
+        over_warp(mine, upto);
+        total = __shfl_sync(0xffffffffu, upto, 31);
+        before = upto - mine;
+      });
+      __syncwarp();
+    }
     uint32_t entry = 0, chunk = 0, queued = 0;
     Part p;
-    Walk<S> walk(a, sh);
+    Walk<S> walk(a, c.share);
     // a tile of K or V into the next slot: in one copy where a page holds the chunk, else page by page and 64 dims at a time
     auto copy = [&](bool v, int head, int slot0, int page, uint32_t there) {
       const int st = entry % S::R, slices = v ? kSlicesV : kSlicesK;
@@ -665,62 +691,64 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
         if (lane == 0 && there) load_box(to, map, slot0, 0, head, page, &c.full[st]);
       } else {
         const int x = lane & (pieces - 1), pg = __shfl_sync(0xffffffffu, page, x);   // at most 8 pieces, 9 slices
-        for (int slice = lane / pieces; slice < slices; slice += 32 / pieces)
+        for (int slice = lane >> pieces_log2; slice < slices; slice += 32 >> pieces_log2)
           if (there >> x & 1) load_box(to + slice * S::C * 128 + x * box * 128, map, slot0, slice, head, pg, &c.full[st]);
       }
       ++entry;
     };
     Cut* const note = lane == 0 ? cuts : nullptr;
     if (!a.by_item && lane == 0) cuts[blockIdx.x].count = 0;
-    while (walk.next(p, note)) {
-      if (ok) {
-        const int qi = queued % kQueue;
-        if (queued >= kQueue) ok = __all_sync(0xffffffffu, bounded(&c.queue_empty[qi], (queued / kQueue - 1) & 1));
-        if (ok && lane == 0) {
-          c.queue[qi] = p;
-          mbar_arrive(&c.queue_full[qi]);
-        }
-        ++queued;
+    bool more = true;
+    auto next = [&] {   // the next part into the queue, or its end
+      more = walk.next(p, note);
+      const int qi = queued % kQueue;
+      if (ok && queued >= kQueue) ok = __all_sync(0xffffffffu, bounded(&c.queue_empty[qi], (queued / kQueue - 1) & 1));
+      if (ok && lane == 0) {
+        if (!more) p.head = -1;
+        c.queue[qi] = p;
+        mbar_arrive(&c.queue_full[qi]);
       }
-      // lane i has the page of piece i; of the next chunk's ahead
+      ++queued;
+    };
+    next();
+    while (more) {
+      const int head = p.head, count = p.count, chunk0 = p.b.c0 + p.from;
+      const int32_t* table = a.table + (int64_t)p.b.s * a.max_pages;
       const int64_t hi = min(p.b.last + 1, (int64_t)a.max_pages << a.page_log2);
       const int64_t lo = a.window > 0 ? p.b.first - a.window + 1 : 0;
+      // lane i has the page of piece i; of the next chunk's ahead
       auto page_of = [&](int i) {
-        const int64_t at = (int64_t)(p.b.c0 + p.from + i) * S::C + lane * box;
-        if (i >= p.count || lane >= pieces || at >= hi || at + box <= lo) return -1;
-        const int64_t pg = a.table[(int64_t)p.b.s * a.max_pages + (at >> a.page_log2)];
-        if (pg >= a.pages) {
-          if (a.err) atomicExch(a.err, 7);
-          return -1;
-        }
-        return (int)pg;
+        const int64_t at = (int64_t)(chunk0 + i) * S::C + lane * box;
+        return i >= count || lane >= pieces || at >= hi || at + box <= lo ? -1 : table[at >> a.page_log2];
       };
       int page = page_of(0), old_page = -1;
       uint32_t old_there = 0;
       int old_slot0 = 0;
-      for (int i = 0; i < p.count && ok; ++i, ++chunk) {
-        const int next_page = page_of(i + 1);
+      bool stepped = false;
+      for (int i = 0; i < count && ok; ++i, ++chunk) {
+        const int next_page = page_of(i + 1);   // looked at in the next turn
+        if (page >= a.pages) {
+          if (a.err) atomicExch(a.err, 7);
+          page = -1;
+        }
+        if (i == count - 1) {   // the softmax looks for the next part at this one's last chunk
+          next();
+          stepped = true;
+        }
         const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-        const int slot0 = (int)(((int64_t)(p.b.c0 + p.from + i) * S::C) & ((1 << a.page_log2) - 1));
+        const int slot0 = (int)(((int64_t)(chunk0 + i) * S::C) & ((1 << a.page_log2) - 1));
         if (lane == 0) c.info[chunk % kInfo] = there;
-        copy(false, p.head, slot0, page, there);
+        if (ok) copy(false, head, slot0, page, there);
         if (!S::LATENT) {
-          if (i > 0 && ok) copy(true, p.head, old_slot0, old_page, old_there);
-          if (i == p.count - 1 && ok) copy(true, p.head, slot0, page, there);
+          if (i > 0 && ok) copy(true, head, old_slot0, old_page, old_there);
+          if (i == count - 1 && ok) copy(true, head, slot0, page, there);
         }
         old_page = page;
         old_there = there;
         old_slot0 = slot0;
         page = next_page;
       }
-    }
-    if (ok) {   // the end of the queue
-      const int qi = queued % kQueue;
-      if (queued >= kQueue) ok = __all_sync(0xffffffffu, bounded(&c.queue_empty[qi], (queued / kQueue - 1) & 1));
-      if (ok && lane == 0) {
-        c.queue[qi].head = -1;
-        mbar_arrive(&c.queue_full[qi]);
-      }
+      if (!stepped) next();
     }
     // no copy is left in flight
     for (uint32_t e = entry > (uint32_t)S::R ? entry - S::R : 0; e < entry; ++e) {
@@ -858,6 +886,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       if (lane == 0) mbar_arrive(&c.qready);
     };
 
+    if (small_plan) pdl_wait();   // q and out
     uint32_t chunk = 0, entry = 0, filled = 0;   // filled: parts with chunks
     bool bad = false, known = false;   // known: the next part is in the queue and its q on the way
     for (uint32_t part = 0;; ++part) {
@@ -1128,28 +1157,30 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(&c.queue_empty[part % kQueue]);
     }
-    if (bad) {   // a wait gave up: NaN for the rows of the share
-      Walk<S> walk(a, sh);
-      Part p;
-      while (walk.next(p, nullptr)) {
-        const int64_t t0 = p.b.f0 / a.group;
-        const int j0 = (int)(p.b.f0 % a.group);
-        for (int r = wg * S::NW; r < min((wg + 1) * S::NW, p.b.count); ++r) {
-          if (p.slot >= 0) {
-            if (own < 2) parts[(int64_t)p.slot * part_floats<S>() + S::N * (S::DV + own) + r] = NAN;
-          } else {
-            const int64_t t = p.b.row0 + t0 + (j0 + r) / a.group;
-            const int64_t h = (int64_t)p.head * a.group + (j0 + r) % a.group;
-            for (int d = own; d < S::DV; d += 128) static_cast<T*>(a.out)[(t * a.heads + h) * S::DV + d] = narrow(NAN, T());
-          }
-        }
-      }
-    }
+    gave_up = bad;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == kIssuer) tmem_dealloc(tmem, S::kCols);
+  if (gave_up) {   // a wait of this group gave up: NaN for its rows of the share
+    const int wg = warp >> 2, own = tid & 127;
+    float* const ml = parts + S::N * S::DV;
+    Walk<S> walk(a, c.share);
+    Part p;
+    while (walk.next(p, nullptr)) {
+      const uint32_t group = (uint32_t)a.group, t0 = (uint32_t)p.b.f0 / group, j0 = (uint32_t)p.b.f0 - t0 * group;
+      for (int r = wg * S::NW; r < min((wg + 1) * S::NW, p.b.count); ++r) {
+        if (p.slot >= 0) {
+          if (own < 2) ml[(int64_t)p.slot * part_floats<S>() + own * S::N + r] = NAN;
+        } else {
+          const uint32_t rt = by_group(a, j0 + r);
+          const int64_t row = (p.b.row0 + t0 + rt) * a.heads + (int64_t)p.head * a.group + (j0 + r - rt * group);
+          for (int d = own; d < S::DV; d += 128) static_cast<T*>(a.out)[row * S::DV + d] = narrow(NAN, T());
+        }
+      }
+    }
+  }
 }
 
 // Joins the parts of the item that starts in CTA c's share and ends in another's: one block per (cut, 16 rows, 64 dims). A

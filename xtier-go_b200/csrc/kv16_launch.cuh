@@ -73,13 +73,12 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     Params a = p;
     const int64_t blocks_per_seq = ((int64_t)a.group * rows_per_seq + S::N - 1) / S::N;
     a.team = blocks_per_seq <= kMostTeam ? (int)std::min<int64_t>(blocks_per_seq, sms) : 1;
-    a.part_cost = 2;
-    a.least_share = 2;
-#ifdef KV16_TUNE
-    if (getenv("KP")) a.part_cost = atoi(getenv("KP"));
-    if (getenv("KL")) a.least_share = atoi(getenv("KL"));
-    if (getenv("KT")) a.team = atoi(getenv("KT"));
-#endif
+    // What a part costs besides its chunks, in chunks, which are the shorter the fewer the rows: measured 2 (64 sequences of
+    // 8 rows with a window: 67 us, with 1 or 4 70), 3 for 128 rows (prompts of 2048 rows: 106 us, with 2 122, with 4 107), 4
+    // for 64 rows of a latent cache (28 us, with 2 30).
+    a.part_cost = S::N <= 32 ? 2 : S::LATENT ? 4 : 3;
+    a.least_share = 1;
+    a.team_inv = a.team > 1 ? (uint32_t)(((1ull << 32) + a.team - 1) / a.team) : 0;
     const int grid = sms / a.team * a.team;
     const int64_t slots = a.rows * a.group / (S::N * a.team) + a.seqs;
     XTG_REQUIRE(slots < (1ll << 31), "kv16: too many row blocks in one call");
