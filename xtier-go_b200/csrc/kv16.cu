@@ -22,7 +22,9 @@ namespace xtg {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxRowsPerCta = 4;
+// Rows of a CTA where there are many: they share its start, and a thread its place where it keeps it (interleaved)
+constexpr int kMaxRowsPerCta = 8;
+constexpr int rows_per_cta(bool interleaved) { return interleaved ? kMaxRowsPerCta : 4; }
 constexpr int kMaxRotary = 256;
 
 struct Stream {   // k's, v's or q's heads of a row
@@ -49,17 +51,29 @@ struct Turn {
   float c, s;
 };
 
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+// 8 neighbouring values as they lie in memory
+template <class X>
+struct Raw {
+  uint4 w[sizeof(X) / 2];
+};
+template <class X>
+__device__ __forceinline__ Raw<X> load8(const X* p) {
+  Raw<X> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(X) / 2; ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
 }
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void to_f32(const Raw<float>& r, float (&x)[8]) {
+  const uint4 a = r.w[0], b = r.w[1];
+  x[0] = __uint_as_float(a.x), x[1] = __uint_as_float(a.y), x[2] = __uint_as_float(a.z), x[3] = __uint_as_float(a.w);
+  x[4] = __uint_as_float(b.x), x[5] = __uint_as_float(b.y), x[6] = __uint_as_float(b.z), x[7] = __uint_as_float(b.w);
+}
+template <class X>
+__device__ __forceinline__ void to_f32(const Raw<X>& r, float (&x)[8]) {
+  const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = kv16::unpack(w[i], T());
+    const float2 f = kv16::unpack(w[i], X());
     x[2 * i] = f.x;
     x[2 * i + 1] = f.y;
   }
@@ -89,8 +103,8 @@ __device__ __forceinline__ int sequence_of(const AppendArgs& a, int64_t row) {
 
 // X: the rows' type, T: the cache's
 template <class X, class T, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
-  __shared__ Turn turn[kMaxRowsPerCta][kMaxRotary / 2];
+__global__ void __launch_bounds__(kThreads, INTERLEAVED ? 5 : 7) append_kernel(const __grid_constant__ AppendArgs a) {
+  __shared__ __align__(16) Turn turn[kMaxRowsPerCta][kMaxRotary / 2];
   __shared__ struct {
     int64_t page, slot;   // page -1: nowhere to write
     int64_t pos;
@@ -135,64 +149,100 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   __syncthreads();
   const int n0 = a.st[0].heads * a.st[0].units, n1 = n0 + a.st[1].heads * a.st[1].units,
             n = n1 + a.st[2].heads * a.st[2].units;
-  for (int i = threadIdx.x; i < rows * n; i += kThreads) {
-    const int r = i / n;
-    int u = i - r * n;
+  struct Place {
+    int which, h, u, d;   // q, k or v, head, unit, first dim
+    bool turned;
+  };
+  auto place = [&](int u) {
     const int which = u < n0 ? 0 : u < n1 ? 1 : 2;
-    u -= which == 0 ? 0 : which == 1 ? n0 : n1;
     const Stream& st = a.st[which];
+    u -= which == 0 ? 0 : which == 1 ? n0 : n1;
     const int h = u / st.units;
     u -= h * st.units;
-    const bool live = at[r].live;
-    T* to;
-    if (which == 0) {
-      to = static_cast<T*>(a.q_out) + ((row0 + r) * st.heads + h) * st.dims;
-    } else {
-      if (!live || at[r].page < 0) continue;
-      to = which == 1 ? static_cast<T*>(a.k) + at[r].page * a.k_page + h * st.out_head + at[r].slot * a.k_slot + a.k_dim0
-                      : static_cast<T*>(a.v) + at[r].page * a.v_page + h * st.out_head + at[r].slot * a.v_slot;
+    int d = st.first + 8 * u;
+    if (u >= st.turned) {   // the dims before and behind the rotated ones
+      d = 8 * (u - st.turned);
+      if (d >= st.first && st.rotary) d += st.rotary;
     }
-    const X* from = static_cast<const X*>(st.src) + (row0 + r) * st.row + h * st.head;
-    float x[8];
-    if (u < st.turned) {
-      const Turn* t = turn[r];
-      if (INTERLEAVED) {
-        const int d = st.first + 8 * u;
-        load8(from + d, x);
+    return Place{which, h, u, d, u < st.turned};
+  };
+  auto source = [&](const Place& p, int r) {
+    const Stream& st = a.st[p.which];
+    return static_cast<const X*>(st.src) + (row0 + r) * st.row + p.h * st.head + p.d;
+  };
+  auto target = [&](const Place& p, int r) {
+    const Stream& st = a.st[p.which];
+    if (p.which == 0) return static_cast<T*>(a.q_out) + ((row0 + r) * st.heads + p.h) * st.dims + p.d;
+    return p.which == 1 ? static_cast<T*>(a.k) + at[r].page * a.k_page + p.h * st.out_head + at[r].slot * a.k_slot + a.k_dim0 + p.d
+                        : static_cast<T*>(a.v) + at[r].page * a.v_page + p.h * st.out_head + at[r].slot * a.v_slot + p.d;
+  };
+  auto nowhere = [&](const Place& p, int r) { return p.which > 0 && at[r].page < 0; };
+  if (INTERLEAVED) {
+    // a thread takes the same part of a head in all rows, two at once
+    constexpr int kAtOnce = sizeof(X) == 4 ? 1 : 2;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const Place p = place(i);
+      for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
+        Raw<X> raw[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const Turn w = t[4 * u + e];
-          const float p = x[2 * e], q = x[2 * e + 1];
-          x[2 * e] = p * w.c - q * w.s;
-          x[2 * e + 1] = q * w.c + p * w.s;
+        for (int k = 0; k < kAtOnce; ++k)
+          if (r0 + k < rows) raw[k] = load8(source(p, r0 + k));
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          const int r = r0 + k;
+          if (r >= rows) break;
+          if (nowhere(p, r)) continue;
+          float x[8];
+          to_f32(raw[k], x);
+          if (p.turned) {
+            const Turn* t = turn[r] + 4 * p.u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const Turn w = t[e];
+              const float f = x[2 * e], g = x[2 * e + 1];
+              x[2 * e] = f * w.c - g * w.s;
+              x[2 * e + 1] = g * w.c + f * w.s;
+            }
+          }
+          if (!at[r].live)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+          store8(target(p, r), x);
         }
+      }
+    }
+  } else {
+    // a thread has two pieces on the way as it is: all parts of all rows in turn, with few registers and so many threads (with
+    // the loop above and 95 registers the largest case took 239 us, with 34 it takes 121)
+    for (int i = threadIdx.x; i < rows * n; i += kThreads) {
+      const int r = i / n;
+      const Place p = place(i - r * n);
+      if (nowhere(p, r)) continue;
+      const X* from = source(p, r);
+      T* to = target(p, r);
+      const bool live = at[r].live;
+      float x[8];
+      if (p.turned) {
+        float y[8];
+        to_f32(load8(from), x);
+        to_f32(load8(from + a.half), y);
+        const Turn* t = turn[r] + 8 * p.u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const Turn w = t[e];
+          const float f = x[e], g = y[e];
+          x[e] = live ? f * w.c - g * w.s : 0.f;
+          y[e] = live ? g * w.c + f * w.s : 0.f;
+        }
+        store8(to, x);
+        store8(to + a.half, y);
+      } else {
+        to_f32(load8(from), x);
         if (!live)
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = 0.f;
-        store8(to + d, x);
-      } else {
-        const int d = st.first + 8 * u;
-        float y[8];
-        load8(from + d, x);
-        load8(from + d + a.half, y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const Turn w = t[8 * u + e];
-          const float p = x[e], q = y[e];
-          x[e] = live ? p * w.c - q * w.s : 0.f;
-          y[e] = live ? q * w.c + p * w.s : 0.f;
-        }
-        store8(to + d, x);
-        store8(to + d + a.half, y);
+        store8(to, x);
       }
-    } else {   // the dims before and behind the rotated ones
-      int d = 8 * (u - st.turned);
-      if (d >= st.first && st.rotary) d += st.rotary;
-      load8(from + d, x);
-      if (!live)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f;
-      store8(to + d, x);
     }
   }
 }
@@ -295,8 +345,8 @@ void launch_kv16_append(const Kv16Cache& c, const Kv16Append& r, int sms, cudaSt
   a.page_log2 = log2_of(c.page);
   a.half = r.rotary / 2;
   a.err = c.err;
-  // several rows a CTA share its start where there are rows enough to fill the GPU
-  a.rows_per_cta = c.rows >= (int64_t)sms * 8 * kMaxRowsPerCta ? kMaxRowsPerCta : 1;
+  // as many as leave 8 CTAs for every SM
+  a.rows_per_cta = (int)std::max<int64_t>(1, std::min<int64_t>(c.rows / (8 * sms), rows_per_cta(r.interleaved)));
   const int64_t grid = (c.rows + a.rows_per_cta - 1) / a.rows_per_cta;
   auto by_cache = [&](auto x) {
     using X = decltype(x);
