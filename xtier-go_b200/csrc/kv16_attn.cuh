@@ -254,6 +254,26 @@ struct Walk {
   }
 };
 
+// The positions that some rows of a part's block see, counted from its first chunk on. In the second product they are taken
+// in steps of 16: those of a chunk from `from` to `to`.
+struct Seen {
+  int lo, hi;
+  template <class S>
+  __device__ int from(int chunk) const {
+    return max(lo - chunk * S::C, 0) & ~15;
+  }
+  template <class S>
+  __device__ int to(int chunk) const {
+    return min((hi - chunk * S::C + 15) & ~15, S::C);
+  }
+};
+template <class S>
+__device__ __forceinline__ Seen seen_by(const Params& a, const Part& p) {
+  const int64_t start = (int64_t)(p.b.c0 + p.from) * S::C, hi = p.b.last + 1 - start, most = (int64_t)p.count * S::C;
+  // (a part starts less than a chunk before what its window sees)
+  return {a.window > 0 ? (int)max(p.b.first - a.window + 1 - start, (int64_t)0) : 0, (int)(hi < most ? hi : most)};
+}
+
 // ---- waits ----
 
 __device__ __forceinline__ void give_up(int* failed, int32_t* err) {
@@ -463,20 +483,17 @@ __device__ __forceinline__ int spread_column(int j) {
   return c;
 }
 
-// Zeros for the infinities and NaN among 8 values; whether there were any
-__device__ __forceinline__ bool drop_unbounded(uint4& x, uint32_t exponent, uint32_t one) {
+// Zeros for the infinities and NaN among 8 values
+__device__ __forceinline__ void drop_unbounded(uint4& x, uint32_t exponent, uint32_t one) {
   uint32_t* w = &x.x;
-  bool found = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t hit = ((w[i] & exponent) + one) & 0x80008000u;   // a full exponent carries into the sign's bit
-    found = found || hit != 0;
     w[i] &= ~((hit >> 15) * 0xffffu);
   }
-  return found;
 }
-__device__ __forceinline__ bool drop_unbounded(uint4& x, __nv_bfloat16) { return drop_unbounded(x, 0x7f807f80u, 0x00800080u); }
-__device__ __forceinline__ bool drop_unbounded(uint4& x, __half) { return drop_unbounded(x, 0x7c007c00u, 0x04000400u); }
+__device__ __forceinline__ void drop_unbounded(uint4& x, __nv_bfloat16) { drop_unbounded(x, 0x7f807f80u, 0x00800080u); }
+__device__ __forceinline__ void drop_unbounded(uint4& x, __half) { drop_unbounded(x, 0x7c007c00u, 0x04000400u); }
 
 // Adds V's infinities and NaN of dim d, which drop_unbounded has taken out of the part's chunks where some of the block's
 // rows see a position, to the rows r0 .. r0 + 15 that do: a weight above zero times these is these.
@@ -768,8 +785,12 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       const int qi = part % kQueue;
       ok = __all_sync(0xffffffffu, bounded(&c.queue_full[qi], (part / kQueue) & 1));
       if (!ok) break;
-      const int n = __shfl_sync(0xffffffffu, c.queue[qi].count, 0);
-      const bool end = __shfl_sync(0xffffffffu, c.queue[qi].head, 0) < 0;
+      const Part& p = c.queue[qi];
+      const int n = __shfl_sync(0xffffffffu, p.count, 0);
+      const bool end = __shfl_sync(0xffffffffu, p.head, 0) < 0;
+      Seen seen = seen_by<S>(a, p);
+      seen.lo = __shfl_sync(0xffffffffu, seen.lo, 0);
+      seen.hi = __shfl_sync(0xffffffffu, seen.hi, 0);
       if (lane == 0) mbar_arrive(&c.queue_empty[qi]);
       if (end) break;
       if (n == 0) continue;
@@ -786,14 +807,23 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
           if (passed(&c.pready[pb], (ch / S::PB) & 1) && (S::LATENT || passed(&c.full[st], (e / S::R) & 1))) {
             tc_fence_after();
             const uint32_t v0 = ring0 + st * S::kSlotBytes, p0 = pb0 + pb * S::kPBytes;
+            const int from = seen.from<S>(vi), to = seen.to<S>(vi);
             if (elected()) {
+              auto product = [&](int m, int x, bool accumulate) {
+                mma(t + S::kO + m * S::N, operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
+                    operand(p0 + x * 16, 128, S::C * 16, 0), kOi, accumulate);
+              };
+              if (to - from == S::C) {
 #pragma unroll
-              for (int m = 0; m < S::DT; ++m)
+                for (int m = 0; m < S::DT; ++m)
 #pragma unroll
-                for (int x = 0; x < S::C; x += 16)
-                  mma(t + S::kO + m * S::N,
-                      operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
-                      operand(p0 + x * 16, 128, S::C * 16, 0), kOi, vi > 0 || x > 0);
+                  for (int x = 0; x < S::C; x += 16) product(m, x, vi > 0 || x > 0);
+              } else {
+#pragma unroll 1
+                for (int m = 0; m < S::DT; ++m)
+#pragma unroll 1
+                  for (int x = from; x < to; x += 16) product(m, x, vi > 0 || x > from);
+              }
               tc_commit(&c.empty[st]);
               tc_commit(&c.pdone[pb]);
             }
@@ -920,6 +950,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
       const int64_t first_pos = p.b.first, last_pos = p.b.last;
       const int64_t start0 = (int64_t)(p.b.c0 + p.from) * S::C;
       const int pairs = p.b.count;
+      const Seen part_seen = seen_by<S>(a, p);
       float l[S::NC];
 #pragma unroll
       for (int r = 0; r < S::NC; ++r) l[r] = 0.f;
@@ -1043,25 +1074,35 @@ __global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_
           const uint32_t e = S::LATENT ? entry + i : i == count - 1 ? entry + 2 * count - 1 : entry + 2 * i + 2;
           bad = !__all_sync(0xffffffffu, bounded(&c.full[e % S::R], (e / S::R) & 1)) || bad;
           const bool seen = lo < min(hi, pairs);
-          if (!bad && (!seen || lo > 0 || hi < pairs)) {
+          if (!bad && (!seen || lo > 0 || hi < pairs) && at >= part_seen.from<S>(i) && at < part_seen.to<S>(i)) {
             uint8_t* v = ring + e % S::R * S::kSlotBytes + at * 128;
-            bool found = false;
             constexpr int kUnits = S::DV / (S::C == 128 ? 8 : 16) / S::WG;   // two threads have a position where C is 64
             const int unit0 = (S::C == 128 ? wg : 2 * wg + (lane >> 4)) * kUnits;
-#pragma unroll 4
-            for (int i = 0; i < kUnits; ++i) {
-              // neighbouring positions take different 16-byte columns of the 8 at a time (of kUnits, if fewer)
+            // neighbouring positions take different 16-byte columns of the 8 at a time (of kUnits, if fewer)
+            auto unit = [&](int i) {
               const int u = unit0 + (i ^ (at & (kUnits < 8 ? kUnits - 1 : 7)));
-              uint4* w = reinterpret_cast<uint4*>(v + u / 8 * S::C * 128 + (u % 8) * 16);
-              if (!seen) {
-                *w = make_uint4(0, 0, 0, 0);
-              } else {
-                uint4 x = *w;
-                if (drop_unbounded(x, T())) {
-                  *w = x;
-                  found = true;
-                }
+              return reinterpret_cast<uint4*>(v + u / 8 * S::C * 128 + (u % 8) * 16);
+            };
+            bool found = false;
+            if (!seen) {
+#pragma unroll
+              for (int i = 0; i < kUnits; ++i) *unit(i) = make_uint4(0, 0, 0, 0);
+            } else {
+              uint32_t most = 0;   // of the magnitudes, as 16-bit integers
+#pragma unroll 4
+              for (int i = 0; i < kUnits; ++i) {
+                const uint4 x = *unit(i);
+                most = __vmaxu2(__vmaxu2(most, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu)),
+                                __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
               }
+              constexpr uint32_t kFull = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;   // an exponent of ones
+              found = (most & 0xffffu) >= kFull || (most >> 16) >= kFull;
+              if (found)
+                for (int i = 0; i < kUnits; ++i) {
+                  uint4 x = *unit(i);
+                  drop_unbounded(x, T());
+                  *unit(i) = x;
+                }
             }
             if (found) *unbounded = 1;
           }
