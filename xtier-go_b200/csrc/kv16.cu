@@ -367,7 +367,8 @@ int64_t kv16_workspace_bytes(bool latent, int head_dim, int v_dim, int group, in
   int64_t bytes = -1;
   kv16::by_shape<__nv_bfloat16>(latent, head_dim, v_dim, kv16::block_rows(latent, (int64_t)group * rows_per_seq),
                                 [&](auto shape) {
-                                  bytes = kv16::work_bytes<decltype(shape)>(std::min(sms, kv16::kMaxGrid));
+                                  using S = decltype(shape);
+                                  bytes = kv16::work_bytes<S>(std::min(sms, kv16::kMaxGrid / 2) * S::OCC);
                                 });
   return bytes;
 }
@@ -416,7 +417,7 @@ void launch_kv16_attention(const Kv16Cache& c, const Kv16Attn& r, int sms, cudaS
   p.work = static_cast<float*>(r.work);
   p.polls = wait_polls.load(std::memory_order_relaxed);
   const int rows = kv16::block_rows(c.latent, (int64_t)group * r.rows_per_seq);
-  const int most = std::min(sms, kv16::kMaxGrid);
+  const int most = std::min(sms, kv16::kMaxGrid / 2);
   if (c.dtype == kKv16Bf16)
     kv16::launch<__nv_bfloat16>(p, c.latent, c.head_dim, c.v_dim, rows, r.rows_per_seq, most, s);
   else

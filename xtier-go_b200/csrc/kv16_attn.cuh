@@ -34,9 +34,9 @@ namespace xtg {
 
 namespace kv16 {
 
-constexpr int kSmem = 232448;      // shared memory of a CTA
+constexpr int kSmem = 232448, kSmemHalf = 115200;   // shared memory of a CTA, of one of two
 constexpr int kCtrl = 3072;        // of it for barriers and per-row values
-constexpr int kMaxGrid = 256;
+constexpr int kMaxGrid = 320;
 // A row's reference is kHead below its largest score when it is set and moves when a score passes kMost above it: P is at
 // most 2^kMost. bf16 has f32's range. f16's normal numbers end at 2^16 and at 2^-14: the head keeps small probabilities
 // among them.
@@ -61,7 +61,12 @@ struct Shape {
   static constexpr int kSlotBytes = (DK > DV ? DK : DV) * C * 2;
   static constexpr int kQBytes = N * DK * 2, kPBytes = N * C * 2;
   static constexpr int PB = N <= 32 ? 2 : 1;       // buffers of P
-  static constexpr int kFit = (kSmem - kCtrl - kQBytes - PB * kPBytes) / kSlotBytes;
+  static constexpr int kRest = kCtrl + kQBytes + PB * kPBytes;
+  // Two CTAs an SM for few rows where three tiles fit into half of the memory, so that one's softmax runs beside the other's
+  // (64 sequences of 4096 .. 8192 positions, 8 heads of 64: 166 -> 145 us; 64 of 16384 .. 32768, 24 / 6 heads of 128:
+  // 734 -> 705 us; heads of 256 the same)
+  static constexpr int OCC = N == 16 && C == 128 && (kSmemHalf - kRest) / kSlotBytes >= 3 ? 2 : 1;
+  static constexpr int kFit = ((OCC == 2 ? kSmemHalf : kSmem) - kRest) / kSlotBytes;
   static constexpr int R = kFit > 12 ? 12 : kFit;  // slots of the ring
   static constexpr int kSmemBytes = R * kSlotBytes + kQBytes + PB * kPBytes + kCtrl;
   static constexpr int MO = DV >= 128 ? 128 : 64, DT = DV / MO;   // the second product's M, and how many of them
@@ -546,7 +551,7 @@ struct __align__(16) Rows {
 };
 
 template <class S>
-__global__ void __launch_bounds__(S::kThreads, 1) attention_kernel(const __grid_constant__ Params a) {
+__global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __grid_constant__ Params a) {
   using T = typename S::T;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem;

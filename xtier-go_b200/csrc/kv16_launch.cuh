@@ -79,7 +79,7 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     a.part_cost = S::N <= 32 ? 2 : S::LATENT ? 4 : 3;
     a.least_share = 1;
     a.team_inv = a.team > 1 ? (uint32_t)(((1ull << 32) + a.team - 1) / a.team) : 0;
-    const int grid = sms / a.team * a.team;
+    const int grid = sms * S::OCC / a.team * a.team;
     const int64_t slots = a.rows * a.group / (S::N * a.team) + a.seqs;
     XTG_REQUIRE(slots < (1ll << 31), "kv16: too many row blocks in one call");
     a.slots = (int)slots;
