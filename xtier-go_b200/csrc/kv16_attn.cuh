@@ -7,17 +7,34 @@
 // S^T = K Q^T has a chunk's positions as the instruction's M and the rows as its N (16 .. 128), o^T = V^T P^T the dims of V
 // as M. K and V are used as TMA brings them (128-byte swizzle: K as a K-major, V as an MN-major operand), no thread touches
 // them; of a latent cache one tile is both. S^T and o^T lie in tensor memory; a thread of the softmax warps has one position
-// and the rows as columns, so a chunk's sums need no exchange between threads until the part's end. P^T is written back to
+// and the rows as columns, so that a chunk's sums need no exchange between threads before the part's end. P^T goes back to
 // shared memory as 16-byte pieces (8 rows of a position), the unswizzled MN-major operand.
 //
-// m[r] is a reference that is at most 2^kSlack below the largest score so far: it moves, and o and the sums are scaled, only
-// when a score passes that. P is rounded to the cache's type for the second product and summed up as rounded; sums and o
-// are f32.
+// m[r] is a reference: the row's largest score when it was set (less kHead). It moves, and o and the sums are scaled, when a
+// score passes it by kMost. With a margin of 2^6 a prompt of 2048 rows spent a third of its chunks on that, with 2^16 hardly
+// any. P is rounded to the cache's type, the second product's operand (half a step of it, 2^-8 or 2^-11, which stays below the
+// output's own rounding over more than a few positions), and summed up as rounded, so that a row's largest weight loses
+// nothing; S, the sums and o are f32.
 //
-// One CTA per SM takes an equal share of all (sequence, row block, KV head, chunk) items in that order, whatever the
-// sequences' lengths; a part that a share cuts goes to the workspace in f32 and a second kernel joins the parts in order.
-// The warps of a CTA: one walks the share and issues the copies, one issues the products, the others are the softmax's.
-// Every wait is bounded.
+// A CTA, or a team of them (Block), takes an equal share of all (sequence, row block, KV head, chunk) items in that order,
+// whatever the sequences' lengths; a block that a share cuts goes to the workspace in f32 and a second kernel joins its parts
+// in order. The warps of a CTA: one walks the share and issues the copies, one issues the products, the others are the
+// softmax's. Every wait is bounded.
+//
+// What bounds it (B200, bf16, device time, bytes or flops that cannot be done without against a copy's 6.54 TB/s and 1692
+// TFLOP/s): with few rows the cache's bytes: 64 sequences of 16384 .. 32768 positions, 24 q / 6 KV heads of 128, 715 us, 6.7
+// TB/s; 8 rows each of 64 sequences of 4096 .. 8192 205 us, 6.0 TB/s. With one short sequence latency: 1 x 4096 in 12 us, of
+// which the start and the plan are 2, the first tile and its softmax 3, the others 2, the end 1.5 and the join 3.5. With 128
+// rows a chunk's chain of waits: scores from tensor memory, the vote, exponentials, P back, 1.75 us at heads of 128, of which
+// shared memory needs 0.95 (the products read 128 KB, the copies and P write 96 KB, at 128 bytes a cycle): 8192 rows from
+// position 0 with heads of 192 / 128 492 us, 700 TFLOP/s. A latent cache's tile takes 72 KB and q 72 KB, so there are two
+// slots and a slot's time is copy, first product, softmax, second product one after another: 64 sequences of 8192 .. 16384
+// positions with 16 heads in 164 us, 5.5 TB/s, with 64 in 208, with 128 in 353 us, 620 TFLOP/s (the products alone 170).
+// Tried and not taken: four groups of softmax warps for 64 and 128 rows (within 5 %, mostly slower), blocks of 64 rows side by
+// side in place of 128 (products of 64 rows read shared memory as often for half the work: 185 -> 233 us), tiles in pieces of
+// 128 dims with barriers of their own (20 % slower for latent caches), warps of their own for q (4 % faster for prompts, 4 to
+// 10 % slower for latent caches), two CTAs an SM for 32 rows (window of 1024 66 -> 60 us with pages of 16, 58 -> 63 with
+// pages of 64, the others 2 to 17 % slower).
 #pragma once
 
 #include <cuda.h>
@@ -36,7 +53,7 @@ namespace kv16 {
 
 constexpr int kSmem = 232448, kSmemHalf = 115200;   // shared memory of a CTA, of one of two
 constexpr int kCtrl = 3072;        // of it for barriers and per-row values
-constexpr int kMaxGrid = 320;
+constexpr int kMaxGrid = 320;      // CTAs
 // A row's reference is kHead below its largest score when it is set and moves when a score passes kMost above it: P is at
 // most 2^kMost. bf16 has f32's range. f16's normal numbers end at 2^16 and at 2^-14: the head keeps small probabilities
 // among them.

@@ -43,7 +43,8 @@ bool by_shape(bool latent, int head_dim, int v_dim, int rows, F&& f) {
   return false;
 }
 
-// Sequences of more row blocks than this go through their chunks block by block (prompts, whose keys stay in L2 meanwhile).
+// Sequences of at most so many row blocks have a team of CTAs, which read their chunks side by side; with more (prompts, whose
+// keys stay in L2 meanwhile) the blocks go one after another.
 constexpr int kMostTeam = 8;
 
 // defined in kv16_bf16.cu and kv16_f16.cu
@@ -73,9 +74,9 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     Params a = p;
     const int64_t blocks_per_seq = ((int64_t)a.group * rows_per_seq + S::N - 1) / S::N;
     a.team = blocks_per_seq <= kMostTeam ? (int)std::min<int64_t>(blocks_per_seq, sms) : 1;
-    // What a part costs besides its chunks, in chunks, which are the shorter the fewer the rows: measured 2 (64 sequences of
-    // 8 rows with a window: 67 us, with 1 or 4 70), 3 for 128 rows (prompts of 2048 rows: 106 us, with 2 122, with 4 107), 4
-    // for 64 rows of a latent cache (28 us, with 2 30).
+    // What a part costs besides its chunks, in chunks: 2 for few rows (64 sequences of 8 rows with a window of 1024: 73 us,
+    // with 1 77, with 4 75), 3 for 128 rows (prompts of 2048 rows: 106 us, with 2 122, with 4 108), 4 for 64 rows of a latent
+    // cache (16 x 4 rows: 28 us, with 2 30).
     a.part_cost = S::N <= 32 ? 2 : S::LATENT ? 4 : 3;
     a.least_share = 1;
     a.team_inv = a.team > 1 ? (uint32_t)(((1ull << 32) + a.team - 1) / a.team) : 0;
