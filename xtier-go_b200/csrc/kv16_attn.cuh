@@ -11,8 +11,7 @@
 // shared memory as 16-byte pieces (8 rows of a position), the unswizzled MN-major operand.
 //
 // m[r] is a reference: the row's largest score when it was set (less kHead). It moves, and o and the sums are scaled, when a
-// score passes it by kMost. With a margin of 2^6 a prompt of 2048 rows spent a third of its chunks on that, with 2^16 hardly
-// any. P is rounded to the cache's type, the second product's operand (half a step of it, 2^-8 or 2^-11, which stays below the
+// score passes it by kMost, which later chunks seldom bring about. P is rounded to the cache's type, the second product's operand (half a step of it, 2^-8 or 2^-11, which stays below the
 // output's own rounding over more than a few positions), and summed up as rounded, so that a row's largest weight loses
 // nothing; S, the sums and o are f32.
 //
@@ -29,7 +28,7 @@
 // shared memory needs 0.95 (the products read 128 KB, the copies and P write 96 KB, at 128 bytes a cycle): 8192 rows from
 // position 0 with heads of 192 / 128 492 us, 700 TFLOP/s. A latent cache's tile takes 72 KB and q 72 KB, so there are two
 // slots and a slot's time is copy, first product, softmax, second product one after another: 64 sequences of 8192 .. 16384
-// positions with 16 heads in 164 us, 5.5 TB/s, with 64 in 208, with 128 in 353 us, 620 TFLOP/s (the products alone 170).
+// positions with 16 heads in 164 us, 5.5 TB/s, with 64 in 208, with 128 in 353 us, 620 TFLOP/s (the products alone, at their measured rates, 170).
 // Tried and not taken: four groups of softmax warps for 64 and 128 rows (within 5 %, mostly slower), blocks of 64 rows side by
 // side in place of 128 (products of 64 rows read shared memory as often for half the work: 185 -> 233 us), tiles in pieces of
 // 128 dims with barriers of their own (20 % slower for latent caches), warps of their own for q (4 % faster for prompts, 4 to
