@@ -800,6 +800,7 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
     constexpr uint32_t kS = instruction<T>(S::C, S::N, false), kOi = instruction<T>(S::MO, S::N, true);
     const uint32_t ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0), q0 = __shfl_sync(0xffffffffu, smem_u32(qbuf), 0),
                    pb0 = __shfl_sync(0xffffffffu, smem_u32(pbuf), 0), t = __shfl_sync(0xffffffffu, tmem, 0);
+    if (small_plan) pdl_wait();   // no bounded wait begins before the kernels that this one depends on have ended
     uint32_t entry = 0, chunk = 0, filled = 0;
     bool ok = a.polls != 0;
     for (uint32_t part = 0; ok; ++part) {
@@ -937,7 +938,7 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
       if (lane == 0) mbar_arrive(&c.qready);
     };
 
-    if (small_plan) pdl_wait();   // q and out
+    if (small_plan) pdl_wait();
     uint32_t chunk = 0, entry = 0, filled = 0;   // filled: parts with chunks
     bool bad = false, known = false;   // known: the next part is in the queue and its q on the way
     for (uint32_t part = 0;; ++part) {
