@@ -260,17 +260,10 @@ int log2_of(int page) {
 
 template <class X, class T>
 void launch_append(const AppendArgs& args, bool interleaved, unsigned grid, cudaStream_t s) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  XTG_CUDA(interleaved ? cudaLaunchKernelEx(&cfg, append_kernel<X, T, true>, args)
-                       : cudaLaunchKernelEx(&cfg, append_kernel<X, T, false>, args));
+  if (interleaved)
+    kv16::launch_dependent(append_kernel<X, T, true>, grid, kThreads, 0, s, args);
+  else
+    kv16::launch_dependent(append_kernel<X, T, false>, grid, kThreads, 0, s, args);
 }
 
 // A pool's map: boxes of `box` slots x 64 dims of a page and KV head, or of all dims where a box holds a chunk's positions:

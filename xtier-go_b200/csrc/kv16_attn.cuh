@@ -11,9 +11,9 @@
 // shared memory as 16-byte pieces (8 rows of a position), the unswizzled MN-major operand.
 //
 // m[r] is a reference: the row's largest score when it was set (less kHead). It moves, and o and the sums are scaled, when a
-// score passes it by kMost, which later chunks seldom bring about. P is rounded to the cache's type, the second product's operand (half a step of it, 2^-8 or 2^-11, which stays below the
-// output's own rounding over more than a few positions), and summed up as rounded, so that a row's largest weight loses
-// nothing; S, the sums and o are f32.
+// score passes it by kMost, which later chunks seldom bring about. P is rounded to the cache's type, the second product's
+// operand (half a step of it, 2^-8 or 2^-11, which stays below the output's own rounding over more than a few positions), and
+// summed up as rounded, so that a row's largest weight loses nothing; S, the sums and o are f32.
 //
 // A CTA, or a team of them (Block), takes an equal share of all (sequence, row block, KV head, chunk) items in that order,
 // whatever the sequences' lengths; a block that a share cuts goes to the workspace in f32 and a second kernel joins its parts
@@ -28,7 +28,8 @@
 // shared memory needs 0.95 (the products read 128 KB, the copies and P write 96 KB, at 128 bytes a cycle): 8192 rows from
 // position 0 with heads of 192 / 128 492 us, 700 TFLOP/s. A latent cache's tile takes 72 KB and q 72 KB, so there are two
 // slots and a slot's time is copy, first product, softmax, second product one after another: 64 sequences of 8192 .. 16384
-// positions with 16 heads in 164 us, 5.5 TB/s, with 64 in 208, with 128 in 353 us, 620 TFLOP/s (the products alone, at their measured rates, 170).
+// positions with 16 heads in 164 us, 5.5 TB/s, with 64 in 208, with 128 in 353 us, 620 TFLOP/s (the products alone, at their
+// measured rates, 170).
 // Tried and not taken: four groups of softmax warps for 64 and 128 rows (within 5 %, mostly slower), blocks of 64 rows side by
 // side in place of 128 (products of 64 rows read shared memory as often for half the work: 185 -> 233 us), tiles in pieces of
 // 128 dims with barriers of their own (20 % slower for latent caches), warps of their own for q (4 % faster for prompts, 4 to
@@ -62,6 +63,7 @@ template <class T>
 constexpr float kMost = std::is_same<T, __half>::value ? 15.f : 16.f;
 constexpr float kFloor = -3.0e38f;   // the least reference of a row that has seen a position
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;   // of a thread of the 8 softmax warps and of the 4 others, where there are 12
 
 template <class T_, int DK_, int DV_, bool LATENT_, int N_>
 struct Shape {
@@ -521,7 +523,8 @@ __device__ __forceinline__ void drop_unbounded(uint4& x, __half) { drop_unbounde
 template <class S>
 __device__ __forceinline__ void add_unbounded(const Params& a, const Part& p, int d, int r0, uint32_t j0, float (&o)[16]) {
   using T = typename S::T;
-  const int64_t from = (int64_t)(p.b.c0 + p.from) * S::C, to = min(from + (int64_t)p.count * S::C, (int64_t)a.max_pages << a.page_log2);
+  const int64_t from = (int64_t)(p.b.c0 + p.from) * S::C;
+  const int64_t to = min(from + (int64_t)p.count * S::C, (int64_t)a.max_pages << a.page_log2);
   const int between = (int)(p.b.last - p.b.first);   // positions that some rows see: behind the first row's, and before
                                                      // what the last row's window starts with
   for (int i = 1; i <= 2 * between; ++i) {
@@ -690,212 +693,212 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
   bool gave_up = false;
   auto bounded = [&](uint64_t* bar, uint32_t parity) { return wait(bar, parity, a.polls, &c.failed, a.err); };
 
-  // 384 threads start with 168 registers each: the softmax's 8 warps take 200, the others keep 104
+  // 384 threads start with 168 registers each, which are shared out
   if (warp >= kSoftmaxWarps) {
-  if (S::WG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-  if (warp == kProducer) {
-    // ---- the walk and the copies: K of a chunk before V of the chunk before, as the products take them ----
-    constexpr int kSlicesK = S::DK / 64, kSlicesV = S::DV / 64;
-    const int box = min(1 << a.page_log2, S::C), pieces_log2 = __ffs(S::C / box) - 1, pieces = 1 << pieces_log2;
-    bool ok = true;
-    if (a.polls == 0) {   // without a look
-      give_up(&c.failed, a.err);
-      ok = false;
-    }
-    pdl_wait();
-    pdl_launch_next();
-    if (small_plan) {
-      plan(lane, 32, [&](int64_t mine, int64_t& before, int64_t& total) {
-        int64_t upto;
-        over_warp(mine, upto);
-        total = __shfl_sync(0xffffffffu, upto, 31);
-        before = upto - mine;
-      });
-      __syncwarp();
-    }
-    uint32_t entry = 0, chunk = 0, queued = 0;
-    Part p;
-    Walk<S> walk(a, c.share);
-    // a tile of K or V into the next slot: in one copy where a page holds the chunk, else page by page and 64 dims at a time
-    auto copy = [&](bool v, int head, int slot0, int page, uint32_t there) {
-      const int st = entry % S::R, slices = v ? kSlicesV : kSlicesK;
-      const CUtensorMap* map = v ? &a.vmap : &a.kmap;
-      const uint32_t turn = entry / S::R, to = smem_u32(ring) + st * S::kSlotBytes;
-      if (turn > 0) ok = __all_sync(0xffffffffu, bounded(&c.empty[st], (turn - 1) & 1));
-      if (!ok) return;
-      if (lane == 0) mbar_expect_tx(&c.full[st], (uint32_t)(__popc(there) * slices * box * 128));
-      __syncwarp();
-      if (pieces == 1) {
-        if (lane == 0 && there) load_box(to, map, slot0, 0, head, page, &c.full[st]);
-      } else {
-        const int x = lane & (pieces - 1), pg = __shfl_sync(0xffffffffu, page, x);   // at most 8 pieces, 9 slices
-        for (int slice = lane >> pieces_log2; slice < slices; slice += 32 >> pieces_log2)
-          if (there >> x & 1) load_box(to + slice * S::C * 128 + x * box * 128, map, slot0, slice, head, pg, &c.full[st]);
+    if (S::WG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kProducer) {
+      // ---- the walk and the copies: K of a chunk before V of the chunk before, as the products take them ----
+      constexpr int kSlicesK = S::DK / 64, kSlicesV = S::DV / 64;
+      const int box = min(1 << a.page_log2, S::C), pieces_log2 = __ffs(S::C / box) - 1, pieces = 1 << pieces_log2;
+      bool ok = true;
+      if (a.polls == 0) {   // without a look
+        give_up(&c.failed, a.err);
+        ok = false;
       }
-      ++entry;
-    };
-    Cut* const note = lane == 0 ? cuts : nullptr;
-    if (!a.by_item && lane == 0) cuts[blockIdx.x].count = 0;
-    bool more = true;
-    auto next = [&] {   // the next part into the queue, or its end
-      more = walk.next(p, note);
-      const int qi = queued % kQueue;
-      if (ok && queued >= kQueue) ok = __all_sync(0xffffffffu, bounded(&c.queue_empty[qi], (queued / kQueue - 1) & 1));
-      if (ok && lane == 0) {
-        if (!more) p.head = -1;
-        c.queue[qi] = p;
-        mbar_arrive(&c.queue_full[qi]);
+      pdl_wait();
+      pdl_launch_next();
+      if (small_plan) {
+        plan(lane, 32, [&](int64_t mine, int64_t& before, int64_t& total) {
+          int64_t upto;
+          over_warp(mine, upto);
+          total = __shfl_sync(0xffffffffu, upto, 31);
+          before = upto - mine;
+        });
+        __syncwarp();
       }
-      ++queued;
-    };
-    next();
-    while (more) {
-      const int head = p.head, count = p.count, chunk0 = p.b.c0 + p.from;
-      const int32_t* table = a.table + (int64_t)p.b.s * a.max_pages;
-      const int64_t hi = min(p.b.last + 1, (int64_t)a.max_pages << a.page_log2);
-      const int64_t lo = a.window > 0 ? p.b.first - a.window + 1 : 0;
-      // lane i has the page of piece i; of the next chunk's ahead
-      auto page_of = [&](int i) {
-        const int64_t at = (int64_t)(chunk0 + i) * S::C + lane * box;
-        return i >= count || lane >= pieces || at >= hi || at + box <= lo ? -1 : table[at >> a.page_log2];
+      uint32_t entry = 0, chunk = 0, queued = 0;
+      Part p;
+      Walk<S> walk(a, c.share);
+      // a tile of K or V into the next slot: in one copy where a page holds the chunk, else page by page and 64 dims at a time
+      auto copy = [&](bool v, int head, int slot0, int page, uint32_t there) {
+        const int st = entry % S::R, slices = v ? kSlicesV : kSlicesK;
+        const CUtensorMap* map = v ? &a.vmap : &a.kmap;
+        const uint32_t turn = entry / S::R, to = smem_u32(ring) + st * S::kSlotBytes;
+        if (turn > 0) ok = __all_sync(0xffffffffu, bounded(&c.empty[st], (turn - 1) & 1));
+        if (!ok) return;
+        if (lane == 0) mbar_expect_tx(&c.full[st], (uint32_t)(__popc(there) * slices * box * 128));
+        __syncwarp();
+        if (pieces == 1) {
+          if (lane == 0 && there) load_box(to, map, slot0, 0, head, page, &c.full[st]);
+        } else {
+          const int x = lane & (pieces - 1), pg = __shfl_sync(0xffffffffu, page, x);   // at most 8 pieces, 9 slices
+          for (int slice = lane >> pieces_log2; slice < slices; slice += 32 >> pieces_log2)
+            if (there >> x & 1) load_box(to + slice * S::C * 128 + x * box * 128, map, slot0, slice, head, pg, &c.full[st]);
+        }
+        ++entry;
       };
-      int page = page_of(0), old_page = -1;
-      uint32_t old_there = 0;
-      int old_slot0 = 0;
-      bool stepped = false;
-      for (int i = 0; i < count && ok; ++i, ++chunk) {
-        const int next_page = page_of(i + 1);   // looked at in the next turn
-        if (page >= a.pages) {
-          if (a.err) atomicExch(a.err, 7);
-          page = -1;
+      Cut* const note = lane == 0 ? cuts : nullptr;
+      if (!a.by_item && lane == 0) cuts[blockIdx.x].count = 0;
+      bool more = true;
+      auto next = [&] {   // the next part into the queue, or its end
+        more = walk.next(p, note);
+        const int qi = queued % kQueue;
+        if (ok && queued >= kQueue) ok = __all_sync(0xffffffffu, bounded(&c.queue_empty[qi], (queued / kQueue - 1) & 1));
+        if (ok && lane == 0) {
+          if (!more) p.head = -1;
+          c.queue[qi] = p;
+          mbar_arrive(&c.queue_full[qi]);
         }
-        if (i == count - 1) {   // the softmax looks for the next part at this one's last chunk
-          next();
-          stepped = true;
+        ++queued;
+      };
+      next();
+      while (more) {
+        const int head = p.head, count = p.count, chunk0 = p.b.c0 + p.from;
+        const int32_t* table = a.table + (int64_t)p.b.s * a.max_pages;
+        const int64_t hi = min(p.b.last + 1, (int64_t)a.max_pages << a.page_log2);
+        const int64_t lo = a.window > 0 ? p.b.first - a.window + 1 : 0;
+        // lane i has the page of piece i; of the next chunk's ahead
+        auto page_of = [&](int i) {
+          const int64_t at = (int64_t)(chunk0 + i) * S::C + lane * box;
+          return i >= count || lane >= pieces || at >= hi || at + box <= lo ? -1 : table[at >> a.page_log2];
+        };
+        int page = page_of(0), old_page = -1;
+        uint32_t old_there = 0;
+        int old_slot0 = 0;
+        bool stepped = false;
+        for (int i = 0; i < count && ok; ++i, ++chunk) {
+          const int next_page = page_of(i + 1);   // looked at in the next turn
+          if (page >= a.pages) {
+            if (a.err) atomicExch(a.err, 7);
+            page = -1;
+          }
+          if (i == count - 1) {   // the softmax looks for the next part at this one's last chunk
+            next();
+            stepped = true;
+          }
+          const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+          const int slot0 = (int)(((int64_t)(chunk0 + i) * S::C) & ((1 << a.page_log2) - 1));
+          if (lane == 0) c.info[chunk % kInfo] = there;
+          if (ok) copy(false, head, slot0, page, there);
+          if (!S::LATENT) {
+            if (i > 0 && ok) copy(true, head, old_slot0, old_page, old_there);
+            if (i == count - 1 && ok) copy(true, head, slot0, page, there);
+          }
+          old_page = page;
+          old_there = there;
+          old_slot0 = slot0;
+          page = next_page;
         }
-        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-        const int slot0 = (int)(((int64_t)(chunk0 + i) * S::C) & ((1 << a.page_log2) - 1));
-        if (lane == 0) c.info[chunk % kInfo] = there;
-        if (ok) copy(false, head, slot0, page, there);
-        if (!S::LATENT) {
-          if (i > 0 && ok) copy(true, head, old_slot0, old_page, old_there);
-          if (i == count - 1 && ok) copy(true, head, slot0, page, there);
-        }
-        old_page = page;
-        old_there = there;
-        old_slot0 = slot0;
-        page = next_page;
+        if (!stepped) next();
       }
-      if (!stepped) next();
-    }
-    // no copy is left in flight
-    for (uint32_t e = entry > (uint32_t)S::R ? entry - S::R : 0; e < entry; ++e) {
-      uint32_t spins = 0;
-      while (!mbar_try_wait(&c.full[e % S::R], (e / S::R) & 1))
-        if (++spins > (1u << 18)) break;
-    }
-    __syncwarp();
-  } else if (warp == kIssuer) {
-    // ---- the products: whichever of a chunk's second and the next one's first has its operands ----
-    constexpr uint32_t kS = instruction<T>(S::C, S::N, false), kOi = instruction<T>(S::MO, S::N, true);
-    const uint32_t ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0), q0 = __shfl_sync(0xffffffffu, smem_u32(qbuf), 0),
-                   pb0 = __shfl_sync(0xffffffffu, smem_u32(pbuf), 0), t = __shfl_sync(0xffffffffu, tmem, 0);
-    if (small_plan) pdl_wait();   // no bounded wait begins before the kernels that this one depends on have ended
-    uint32_t entry = 0, chunk = 0, filled = 0;
-    bool ok = a.polls != 0;
-    for (uint32_t part = 0; ok; ++part) {
-      const int qi = part % kQueue;
-      ok = __all_sync(0xffffffffu, bounded(&c.queue_full[qi], (part / kQueue) & 1));
-      if (!ok) break;
-      const Part& p = c.queue[qi];
-      const int n = __shfl_sync(0xffffffffu, p.count, 0);
-      const bool end = __shfl_sync(0xffffffffu, p.head, 0) < 0;
-      Seen seen = seen_by<S>(a, p);
-      seen.lo = __shfl_sync(0xffffffffu, seen.lo, 0);
-      seen.hi = __shfl_sync(0xffffffffu, seen.hi, 0);
-      if (lane == 0) mbar_arrive(&c.queue_empty[qi]);
-      if (end) break;
-      if (n == 0) continue;
-      ok = __all_sync(0xffffffffu, bounded(&c.qready, filled & 1));
-      ++filled;
-      tc_fence_after();
-      uint32_t spins = 0;
-      for (int si = 0, vi = 0; vi < n && ok;) {   // chunks whose first and whose second product were issued
-        bool issued = false;
-        if (vi < si) {
-          const uint32_t e = S::LATENT ? entry + vi : vi == n - 1 ? entry + 2 * n - 1 : entry + 2 * vi + 2;
-          const uint32_t st = e % S::R, ch = chunk + vi, pb = ch % S::PB;
-          // (of a latent cache the first product has waited for the tile)
-          if (passed(&c.pready[pb], (ch / S::PB) & 1) && (S::LATENT || passed(&c.full[st], (e / S::R) & 1))) {
-            tc_fence_after();
-            const uint32_t v0 = ring0 + st * S::kSlotBytes, p0 = pb0 + pb * S::kPBytes;
-            const int from = seen.from<S>(vi), to = seen.to<S>(vi);
-            if (elected()) {
-              auto product = [&](int m, int x, bool accumulate) {
-                mma(t + S::kO + m * S::N, operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
-                    operand(p0 + x * 16, 128, S::C * 16, 0), kOi, accumulate);
-              };
-              if (to - from == S::C) {
+      // no copy is left in flight
+      for (uint32_t e = entry > (uint32_t)S::R ? entry - S::R : 0; e < entry; ++e) {
+        uint32_t spins = 0;
+        while (!mbar_try_wait(&c.full[e % S::R], (e / S::R) & 1))
+          if (++spins > (1u << 18)) break;
+      }
+      __syncwarp();
+    } else if (warp == kIssuer) {
+      // ---- the products: whichever of a chunk's second and the next one's first has its operands ----
+      constexpr uint32_t kS = instruction<T>(S::C, S::N, false), kOi = instruction<T>(S::MO, S::N, true);
+      const uint32_t ring0 = __shfl_sync(0xffffffffu, smem_u32(ring), 0), q0 = __shfl_sync(0xffffffffu, smem_u32(qbuf), 0),
+                     pb0 = __shfl_sync(0xffffffffu, smem_u32(pbuf), 0), t = __shfl_sync(0xffffffffu, tmem, 0);
+      if (small_plan) pdl_wait();   // no bounded wait begins before the kernels that this one depends on have ended
+      uint32_t entry = 0, chunk = 0, filled = 0;
+      bool ok = a.polls != 0;
+      for (uint32_t part = 0; ok; ++part) {
+        const int qi = part % kQueue;
+        ok = __all_sync(0xffffffffu, bounded(&c.queue_full[qi], (part / kQueue) & 1));
+        if (!ok) break;
+        const Part& p = c.queue[qi];
+        const int n = __shfl_sync(0xffffffffu, p.count, 0);
+        const bool end = __shfl_sync(0xffffffffu, p.head, 0) < 0;
+        Seen seen = seen_by<S>(a, p);
+        seen.lo = __shfl_sync(0xffffffffu, seen.lo, 0);
+        seen.hi = __shfl_sync(0xffffffffu, seen.hi, 0);
+        if (lane == 0) mbar_arrive(&c.queue_empty[qi]);
+        if (end) break;
+        if (n == 0) continue;
+        ok = __all_sync(0xffffffffu, bounded(&c.qready, filled & 1));
+        ++filled;
+        tc_fence_after();
+        uint32_t spins = 0;
+        for (int si = 0, vi = 0; vi < n && ok;) {   // chunks whose first and whose second product were issued
+          bool issued = false;
+          if (vi < si) {
+            const uint32_t e = S::LATENT ? entry + vi : vi == n - 1 ? entry + 2 * n - 1 : entry + 2 * vi + 2;
+            const uint32_t st = e % S::R, ch = chunk + vi, pb = ch % S::PB;
+            // (of a latent cache the first product has waited for the tile)
+            if (passed(&c.pready[pb], (ch / S::PB) & 1) && (S::LATENT || passed(&c.full[st], (e / S::R) & 1))) {
+              tc_fence_after();
+              const uint32_t v0 = ring0 + st * S::kSlotBytes, p0 = pb0 + pb * S::kPBytes;
+              const int from = seen.from<S>(vi), to = seen.to<S>(vi);
+              if (elected()) {
+                auto product = [&](int m, int x, bool accumulate) {
+                  mma(t + S::kO + m * S::N, operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
+                      operand(p0 + x * 16, 128, S::C * 16, 0), kOi, accumulate);
+                };
+                if (to - from == S::C) {
 #pragma unroll
-                for (int m = 0; m < S::DT; ++m)
+                  for (int m = 0; m < S::DT; ++m)
 #pragma unroll
-                  for (int x = 0; x < S::C; x += 16) product(m, x, vi > 0 || x > 0);
-              } else {
+                    for (int x = 0; x < S::C; x += 16) product(m, x, vi > 0 || x > 0);
+                } else {
 #pragma unroll 1
-                for (int m = 0; m < S::DT; ++m)
+                  for (int m = 0; m < S::DT; ++m)
 #pragma unroll 1
-                  for (int x = from; x < to; x += 16) product(m, x, vi > 0 || x > from);
+                    for (int x = from; x < to; x += 16) product(m, x, vi > 0 || x > from);
+                }
+                tc_commit(&c.empty[st]);
+                tc_commit(&c.pdone[pb]);
               }
-              tc_commit(&c.empty[st]);
-              tc_commit(&c.pdone[pb]);
+              __syncwarp();
+              ++vi;
+              issued = true;
             }
-            __syncwarp();
-            ++vi;
-            issued = true;
           }
-        }
-        if (si < n && si < vi + 2) {
-          const uint32_t e = S::LATENT ? entry + si : si == 0 ? entry : entry + 2 * si - 1;
-          const uint32_t st = e % S::R, ch = chunk + si, buf = ch & 1;
-          if (passed(&c.full[st], (e / S::R) & 1) && (ch < 2 || passed(&c.sfree[buf], ((ch >> 1) - 1) & 1))) {
-            tc_fence_after();
-            const uint32_t k0 = ring0 + st * S::kSlotBytes;
-            if (elected()) {
+          if (si < n && si < vi + 2) {
+            const uint32_t e = S::LATENT ? entry + si : si == 0 ? entry : entry + 2 * si - 1;
+            const uint32_t st = e % S::R, ch = chunk + si, buf = ch & 1;
+            if (passed(&c.full[st], (e / S::R) & 1) && (ch < 2 || passed(&c.sfree[buf], ((ch >> 1) - 1) & 1))) {
+              tc_fence_after();
+              const uint32_t k0 = ring0 + st * S::kSlotBytes;
+              if (elected()) {
 #pragma unroll
-              for (int x = 0; x < S::DK; x += 16)
-                mma(t + buf * S::N, operand(k0 + x / 64 * S::C * 128 + x % 64 * 2, 16, 1024, kSwizzle128),
-                    operand(q0 + x / 64 * S::N * 128 + x % 64 * 2, 16, 1024, kSwizzle128), kS, x > 0);
-              tc_commit(&c.sfull[buf]);
-              if (!S::LATENT) tc_commit(&c.empty[st]);
+                for (int x = 0; x < S::DK; x += 16)
+                  mma(t + buf * S::N, operand(k0 + x / 64 * S::C * 128 + x % 64 * 2, 16, 1024, kSwizzle128),
+                      operand(q0 + x / 64 * S::N * 128 + x % 64 * 2, 16, 1024, kSwizzle128), kS, x > 0);
+                tc_commit(&c.sfull[buf]);
+                if (!S::LATENT) tc_commit(&c.empty[st]);
+              }
+              __syncwarp();
+              ++si;
+              issued = true;
             }
-            __syncwarp();
-            ++si;
-            issued = true;
           }
+          if (issued) {
+            spins = 0;
+          } else if (++spins > 32 * a.polls || (spins % 64 == 0 && *reinterpret_cast<volatile int*>(&c.failed))) {
+            // these looks do not wait: some 0.1 us each
+            give_up(&c.failed, a.err);
+            ok = false;
+          }
+          ok = __all_sync(0xffffffffu, ok);
         }
-        if (issued) {
-          spins = 0;
-        } else if (++spins > 32 * a.polls || (spins % 64 == 0 && *reinterpret_cast<volatile int*>(&c.failed))) {
-          // these looks do not wait: some 0.1 us each
-          give_up(&c.failed, a.err);
-          ok = false;
-        }
-        ok = __all_sync(0xffffffffu, ok);
+        entry += S::LATENT ? n : 2 * n;
+        chunk += n;
       }
-      entry += S::LATENT ? n : 2 * n;
-      chunk += n;
+      if (elected()) {
+        tc_commit(&c.done);
+        uint32_t spins = 0;   // every product has ended before the tensor memory goes back
+        while (!mbar_try_wait(&c.done, 0))
+          if (++spins > (1u << 18)) break;
+      }
+      __syncwarp();
     }
-    if (elected()) {
-      tc_commit(&c.done);
-      uint32_t spins = 0;   // every product has ended before the tensor memory goes back
-      while (!mbar_try_wait(&c.done, 0))
-        if (++spins > (1u << 18)) break;
-    }
-    __syncwarp();
-  }
   } else {
     // ---- softmax ----
-    if (S::WG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    if (S::WG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int wg = warp >> 2, quarter = warp & 3, bar = 1 + wg;
     // this thread's position of a chunk and, from col0 on, its rows of the group's
     const int at = S::C == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);
@@ -1000,7 +1003,8 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
         }
         const int64_t start = start0 + (int64_t)i * S::C, pos = start + at;
         const uint32_t there = c.info[chunk % kInfo];
-        const bool clean = there == all_pieces && start + S::C - 1 <= first_pos && (a.window == 0 || start > last_pos - a.window);
+        const bool clean = there == all_pieces && start + S::C - 1 <= first_pos &&
+                           (a.window == 0 || start > last_pos - a.window);
         // rows lo .. hi - 1 of the block see this thread's position: their positions t = first_pos + (j0 + r) / group, with
         // pos - window < t - window + 1 <= pos <= t
         int lo = 0, hi = S::N;
@@ -1257,7 +1261,8 @@ constexpr unsigned join_blocks(int cuts) {
   return (unsigned)cuts * (S::N / kJoinRows) * (S::DV / kJoinDims);
 }
 template <class S, int GROUPS>
-__global__ void __launch_bounds__(256 * GROUPS, GROUPS == 4 ? 1 : 5) join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
+__global__ void __launch_bounds__(256 * GROUPS, GROUPS == 4 ? 1 : 5)
+    join_kernel(const __grid_constant__ Params a, int grid, unsigned blocks) {
   using T = typename S::T;
   constexpr int kGroups = GROUPS, kThreads = 256 * kGroups, kWarps = kThreads / 32;
   __shared__ __align__(16) float weight[kMaxGrid][kJoinRows];

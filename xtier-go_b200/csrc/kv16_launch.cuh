@@ -51,7 +51,7 @@ constexpr int kMostTeam = 8;
 template <class T>
 void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int rows_per_seq, int sms, cudaStream_t s);
 
-#ifdef KV16_TYPE
+// A launch that may overlap the end of the kernel before it on the stream; the kernel waits (pdl_wait).
 template <class... P, class... A>
 void launch_dependent(void (*f)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, A&&... args) {
   cudaLaunchConfig_t cfg = {};
@@ -67,6 +67,7 @@ void launch_dependent(void (*f)(P...), unsigned grid, unsigned block, size_t sme
   XTG_CUDA(cudaLaunchKernelEx(&cfg, f, static_cast<P>(args)...));
 }
 
+#ifdef KV16_TYPE
 template <class T>
 void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int rows_per_seq, int sms, cudaStream_t s) {
   by_shape<T>(latent, head_dim, v_dim, rows, [&](auto shape) {
@@ -87,7 +88,19 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     const int64_t items = slots * a.kv_heads * a.team;
     a.by_item = items <= grid / 4;
     static std::atomic<uint64_t> optin;
-    ensure_smem_optin(reinterpret_cast<const void*>(&attention_kernel<S>), S::kSmemBytes, optin);
+    const void* kernel = reinterpret_cast<const void*>(&attention_kernel<S>);
+    ensure_smem_optin(kernel, S::kSmemBytes, optin);
+    if (S::WG == 2) {
+      // setmaxnreg would wait forever in a kernel that starts with fewer registers than its shares were worked out for
+      static std::atomic<int> registers{0};
+      if (registers.load(std::memory_order_relaxed) == 0) {
+        cudaFuncAttributes attr;
+        XTG_CUDA(cudaFuncGetAttributes(&attr, kernel));
+        registers.store(attr.numRegs, std::memory_order_relaxed);
+      }
+      XTG_REQUIRE((registers.load(std::memory_order_relaxed) + 7) / 8 * 8 * S::kThreads >= kSoftmaxRegs * 256 + kOtherRegs * 128,
+                  "kv16: the attention kernel was built with too few registers");
+    }
     launch_dependent(attention_kernel<S>, (unsigned)grid, S::kThreads, S::kSmemBytes, s, a);
     const unsigned blocks = join_blocks<S>(a.by_item ? (int)items : grid), all = blocks + (a.zero_rest ? 4 : 0);
     if (a.by_item)
