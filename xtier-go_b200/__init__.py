@@ -24,7 +24,7 @@ class XtgError(RuntimeError):
 
 def build():
     """Compile libxtg_cuda.so for sm_100a in-tree (nvcc; no GPU needed)."""
-    subprocess.run(["make", "-s", "-C", HERE], check=True)
+    subprocess.run(["make", "-s", f"-j{os.cpu_count() or 1}", "-C", HERE], check=True)
 
 
 LOGITS_FN = C.CFUNCTYPE(None, C.c_int, C.POINTER(C.c_float), C.c_void_p)

@@ -78,7 +78,8 @@ struct Shape {
   static constexpr int kThreads = WG == 1 ? 192 : WG * 128 + 128;   // with the copies' warp and the products', and two that idle
   static constexpr int kSlotBytes = (DK > DV ? DK : DV) * C * 2;
   static constexpr int kQBytes = N * DK * 2, kPBytes = N * C * 2;
-  static constexpr int PB = N <= 32 ? 2 : 1;       // buffers of P
+  // Buffers of P: two, where that leaves tiles enough (64 rows: 2 % faster; 128 rows, with a tile less, 1 % slower)
+  static constexpr int PB = N <= 32 || (N == 64 && !LATENT) ? 2 : 1;
   static constexpr int kRest = kCtrl + kQBytes + PB * kPBytes;
   // Two CTAs an SM for few rows where three tiles fit into half of the memory, so that one's softmax runs beside the other's
   // (64 sequences of 4096 .. 8192 positions, 8 heads of 64: 166 -> 145 us; 64 of 16384 .. 32768, 24 / 6 heads of 128:
