@@ -52,7 +52,7 @@ namespace xtg {
 namespace kv16 {
 
 constexpr int kSmem = 232448, kSmemHalf = 115200;   // shared memory of a CTA, of one of two
-constexpr int kCtrl = 3072;        // of it for barriers and per-row values
+constexpr int kCtrl = 3 * 1024;    // of it for barriers and per-row values
 constexpr int kMaxGrid = 320;      // CTAs
 // A row's reference is kHead below its largest score when it is set and moves when a score passes kMost above it: P is at
 // most 2^kMost. bf16 has f32's range. f16's normal numbers end at 2^16 and at 2^-14: the head keeps small probabilities
