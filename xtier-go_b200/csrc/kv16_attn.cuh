@@ -13,7 +13,7 @@
 // m[r] is a reference: the row's largest score when it was set (less kHead). It moves, and o and the sums are scaled, when a
 // score passes it by kMost, which later chunks seldom bring about. P is rounded to the cache's type, the second product's
 // operand (half a step of it, 2^-8 or 2^-11, which stays below the output's own rounding over more than a few positions), and
-// summed up as rounded, so that a row's largest weight loses nothing; S, the sums and o are f32.
+// summed up as rounded, so that a row's largest weight loses nothing; S, the sums and o are f32, o in stretches (kFoldSteps).
 //
 // A CTA, or a team of them (Block), takes an equal share of all (sequence, row block, KV head, chunk) items in that order,
 // whatever the sequences' lengths; a block that a share cuts goes to the workspace in f32 and a second kernel joins its parts
@@ -63,6 +63,13 @@ template <class T>
 constexpr float kMost = std::is_same<T, __half>::value ? 15.f : 16.f;
 constexpr float kFloor = -3.0e38f;   // the least reference of a row that has seen a position
 constexpr float kLog2e = 1.4426950408889634f;
+// Steps of 16 positions that the matrix unit adds up before its sum goes to f32 sums in the workspace. It cuts its sums off
+// towards zero, about two units of their last place a step: values of one sign came out 7.9e-4 small over 8192 steps (131072
+// positions), 1.6 times half a step of f16. So after 256 steps 2.5e-5, a twentieth of half a step of f16, after 1024 1e-4, a
+// fortieth of half a step of bf16. What it costs: f16 prompts of 128 rows with heads of 256 over 30000 positions 1242 -> 1315 us
+// (128 steps: 1520), over 16383 190 -> 196 (232), 64 sequences of 16384 .. 32768 positions in bf16 702 -> 706 (729).
+template <class T>
+constexpr int kFoldSteps = std::is_same<T, __half>::value ? 256 : 1024;
 constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;   // of a thread of the 8 softmax warps and of the 4 others, where there are 12
 
 template <class T_, int DK_, int DV_, bool LATENT_, int N_>
@@ -89,6 +96,7 @@ struct Shape {
   static constexpr int R = kFit > 12 ? 12 : kFit;  // slots of the ring
   static constexpr int kSmemBytes = R * kSlotBytes + kQBytes + PB * kPBytes + kCtrl;
   static constexpr int MO = DV >= 128 ? 128 : 64, DT = DV / MO;   // the second product's M, and how many of them
+  static constexpr int kFold = kFoldSteps<T> * 16 / C;   // chunks whose second products are added up in the matrix unit
   static constexpr int kO = 2 * N;                 // tensor memory: S^T twice, then o^T
   static constexpr int kUsed = 2 * N + DT * N;
   static constexpr int kCols = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
@@ -214,11 +222,20 @@ template <class S>
 __host__ __device__ constexpr int64_t part_floats() {
   return (int64_t)S::N * (S::DV + 2);
 }
+// what a CTA's softmax threads have added up of o: 128 lanes of tensor memory x N columns for each of its DT tiles
+template <class S>
+__host__ __device__ constexpr int64_t fold_floats() {
+  return (int64_t)S::DT * 128 * S::N;
+}
 // workspace: 2 parts a CTA (acc [DV][N], reference [N], sum [N]), then the cuts, by CTA or, where there are fewer, by
-// (block number, KV head, CTA of the team)
+// (block number, KV head, CTA of the team), then the CTAs' sums of o
+template <class S>
+__host__ __device__ constexpr int64_t fold_offset(int grid) {   // in bytes
+  return 2 * (int64_t)grid * part_floats<S>() * 4 + (int64_t)grid * (int64_t)sizeof(Cut);
+}
 template <class S>
 __host__ __device__ constexpr int64_t work_bytes(int grid) {
-  return 2 * (int64_t)grid * part_floats<S>() * 4 + (int64_t)grid * (int64_t)sizeof(Cut);
+  return fold_offset<S>(grid) + (int64_t)grid * fold_floats<S>() * 4;
 }
 
 template <class S>
@@ -834,6 +851,7 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
               tc_fence_after();
               const uint32_t v0 = ring0 + st * S::kSlotBytes, p0 = pb0 + pb * S::kPBytes;
               const int from = seen.from<S>(vi), to = seen.to<S>(vi);
+              const bool fresh = vi % S::kFold == 0;   // the sum so far is in the workspace
               if (elected()) {
                 auto product = [&](int m, int x, bool accumulate) {
                   mma(t + S::kO + m * S::N, operand(v0 + m * (S::MO / 64) * S::C * 128 + x * 128, S::C * 128, 1024, kSwizzle128),
@@ -843,12 +861,12 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
 #pragma unroll
                   for (int m = 0; m < S::DT; ++m)
 #pragma unroll
-                    for (int x = 0; x < S::C; x += 16) product(m, x, vi > 0 || x > 0);
+                    for (int x = 0; x < S::C; x += 16) product(m, x, !fresh || x > 0);
                 } else {
 #pragma unroll 1
                   for (int m = 0; m < S::DT; ++m)
 #pragma unroll 1
-                    for (int x = from; x < to; x += 16) product(m, x, vi > 0 || x > from);
+                    for (int x = from; x < to; x += 16) product(m, x, !fresh || x > from);
                 }
                 tc_commit(&c.empty[st]);
                 tc_commit(&c.pdone[pb]);
@@ -912,6 +930,10 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
     const int own = tid & 127;
     const float sc = a.scale * kLog2e;
     const uint32_t group = (uint32_t)a.group;
+    // this thread's columns of o's tiles, 4 rows at a time, as far as they were taken from tensor memory
+    float4* const fold = reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(a.work) + fold_offset<S>(gridDim.x)) +
+                         (blockIdx.x * fold_floats<S>() + wg * (S::DT * 128 * S::NW)) / 4 + own;
+    auto folded = [&](int m, int r) { return fold + (m * S::NW + r) / 4 * 128; };
     const int box = min(1 << a.page_log2, S::C);
     const uint32_t all_pieces = (1u << (S::C / box)) - 1;
 
@@ -980,6 +1002,8 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
       float l[S::NC];
 #pragma unroll
       for (int r = 0; r < S::NC; ++r) l[r] = 0.f;
+
+      float kept = -INFINITY;   // of row `own`: the reference of the sums in the workspace
 
       for (int i = 0; i < count; ++i, ++chunk) {
         const int buf = chunk & 1;
@@ -1149,6 +1173,41 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
           }
           *reinterpret_cast<uint4*>(to + r / 8 * S::C * 16) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+        if (i > 0 && i % S::kFold == 0) {   // the second product of this chunk starts a new sum, the last one goes to the others
+          const uint32_t b = (chunk - 1) % S::PB;
+          if (S::PB > 1) bad = !__all_sync(0xffffffffu, bounded(&c.pdone[b], ((chunk - 1) / S::PB) & 1)) || bad;
+          constexpr int kAtOnce = S::NW < 32 ? S::NW : 32;   // rows whose sums are on the way at once
+          named_bar_sync(bar, 128);   // alpha was read
+          if (own < S::NW) {
+            alpha[own] = kept == ref[own] ? 1.f : ex2_approx(kept - ref[own]);
+            kept = ref[own];
+          }
+          named_bar_sync(bar, 128);
+          if (!bad) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int m = 0; m < S::DT; ++m)
+#pragma unroll 1
+              for (int r0 = 0; r0 < S::NW; r0 += kAtOnce) {
+                float4 x[kAtOnce / 4];
+#pragma unroll
+                for (int j = 0; j < kAtOnce / 4; ++j)
+                  x[j] = i == S::kFold ? make_float4(0.f, 0.f, 0.f, 0.f) : *folded(m, r0 + 4 * j);
+#pragma unroll
+                for (int r = 0; r < kAtOnce; r += 16) {
+                  float o[16];
+                  tmem_ld16(lanes + S::kO + m * S::N + wg * S::NW + r0 + r, o);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int j = 0; j < 16; j += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(alpha + r0 + r + j), old = x[(r + j) / 4];
+                    *folded(m, r0 + r + j) = make_float4(fmaf(old.x, f.x, o[j]), fmaf(old.y, f.y, o[j + 1]),
+                                                         fmaf(old.z, f.z, o[j + 2]), fmaf(old.w, f.w, o[j + 3]));
+                  }
+                }
+              }
+          }
+        }
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
@@ -1182,6 +1241,7 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
           ml[0] = ref[own];
           ml[S::N] = sum;
         }
+        ref[own] = kept == ref[own] ? 1.f : ex2_approx(kept - ref[own]);   // what the sums in the workspace are scaled by
       }
       named_bar_sync(bar, 128);
       tc_fence_after();
@@ -1199,6 +1259,13 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
           if (count > 0) {
             tmem_ld16(lanes + S::kO + m * S::N + wg * S::NW + r, o);
             tmem_ld_wait();
+            if (count > S::kFold)
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const float4 x = *folded(m, r + j), f = *reinterpret_cast<const float4*>(ref + r + j);
+                o[j] = fmaf(x.x, f.x, o[j]), o[j + 1] = fmaf(x.y, f.y, o[j + 1]);
+                o[j + 2] = fmaf(x.z, f.z, o[j + 2]), o[j + 3] = fmaf(x.w, f.w, o[j + 3]);
+              }
           }
           const int d = m * S::MO + dim0;
           if (add && has_dim) add_unbounded<S>(a, p, d, wg * S::NW + r, j0, o);
