@@ -322,8 +322,9 @@ typedef struct {
 // [rows][v_dim], q [rows][heads][64]. Dims first .. first + rotary - 1 of k's and q's heads are rotated: the pair i of them
 // (dims i and i + rotary / 2, or 2 i and 2 i + 1 where interleaved) by the angle position x freq[i] (f32 radians, device
 // memory, [rotary / 2]), the angle taken in 64 bits, the values in 32, rounded once to the cache's type. rotary 0 (freq may
-// be NULL): none is. rotary and first are multiples of 16 and 8, rotary at most 256. q_out [rows][heads][head_dim] (64 for
-// a latent cache), contiguous, of the cache's type, gets q's rows (zeros where a row is no sequence's).
+// be NULL): none is. rotary and first are multiples of 16 and 8, rotary at most 256. A row has at most 2^30 values of q, k
+// and v. q_out [rows][heads][head_dim] (64 for a latent cache), contiguous, of the cache's type, gets q's rows (zeros where
+// a row is no sequence's).
 typedef struct {
   const void* k;
   const void* v;

@@ -539,6 +539,9 @@ int xtg_cuda_kv16_append(const xtg_cuda_kv16* cache, const xtg_cuda_kv16_rows* r
                 "kv16: rotary a multiple of 16, first of 8, both within a head");
     XTG_REQUIRE(r->rotary == 0 || r->freq, "kv16: null pointer (freq)");
     XTG_REQUIRE(!r->q || (r->heads >= 1 && c.rows * r->heads < (1ll << 31)), "kv16: rows x q heads in 1 .. 2^31 - 1");
+    // the kernel counts a row's units of 8 values, and those of up to 8 rows, in 32 bits
+    XTG_REQUIRE((r->q ? (int64_t)r->heads : 0) * dims + (int64_t)c.kv_heads * (dims + c.v_dim) <= (1ll << 30),
+                "kv16: at most 2^30 values of q, k and v in a row");
     if (c.rows == 0 || (c.seqs == 0 && !r->q)) return;
     kv16_require_rows({r->k, r->v}, r->dtype, {r->k_row, c.latent ? 0 : r->k_head, r->v_row, c.latent ? 0 : r->v_head});
     if (r->q) kv16_require_rows({r->q, r->q_out}, r->dtype, {r->q_row, r->q_head});
