@@ -686,8 +686,10 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
       if (lane >= o) upto += x;
     }
   };
-  // Few blocks: the copies' warp alone, which is the one to wait for it.
-  const bool small_plan = a.slots <= 256;
+  // Few blocks: the copies' warp alone, which is the one to wait for it (one sequence of 4096 positions 12.4 us, with all warps
+  // 12.7). From some 100 on it is the longer way: 125 blocks 115.6 us and 110.5, 250 blocks 118.0 and 112.1, a prompt of 4096 rows
+  // (129) 214.7 and 210.7.
+  const bool small_plan = a.slots <= 64;
   if (!small_plan) {
     pdl_wait();
     plan(tid, S::kThreads, [&](int64_t mine, int64_t& before, int64_t& total) {

@@ -44,7 +44,9 @@ bool by_shape(bool latent, int head_dim, int v_dim, int rows, F&& f) {
 }
 
 // Sequences of at most so many row blocks have a team of CTAs, which read their chunks side by side; with more (prompts, whose
-// keys stay in L2 meanwhile) the blocks go one after another.
+// keys stay in L2 meanwhile) the blocks go one after another. Without teams and with these: 8 sequences of 256 rows over 32768
+// positions 1233 and 1215 us, 4 of 200 rows over 16384 with heads of 256 352 and 328, 16 of 4 rows over latent caches with 128
+// heads 221 and 202. Teams of up to 16 are within 1 % of these, but for 8 rows of 128 latent heads (477 us and 448).
 constexpr int kMostTeam = 8;
 
 // defined in kv16_bf16.cu and kv16_f16.cu
@@ -76,9 +78,10 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     const int64_t blocks_per_seq = ((int64_t)a.group * rows_per_seq + S::N - 1) / S::N;
     a.team = blocks_per_seq <= kMostTeam ? (int)std::min<int64_t>(blocks_per_seq, sms) : 1;
     // What a part costs besides its chunks, in chunks: 2 for few rows (64 sequences of 8 rows with a window of 1024: 73 us,
-    // with 1 77, with 4 75), 3 for 128 rows (prompts of 2048 rows: 106 us, with 2 122, with 4 108), 4 for 64 rows of a latent
-    // cache (16 x 4 rows: 28 us, with 2 30).
-    a.part_cost = S::N <= 32 ? 2 : S::LATENT ? 4 : 3;
+    // with 1 77, with 4 75), 3 for more (128 rows, prompts of 2048: 108 us, with 2 124, with 4 110; 64 rows, 64 sequences of 16
+    // rows: 78 us, with 1 80), 4 for latent caches (16 x 4 rows: 27.4 us, with 2 29.4; latent 256 with 32 heads, 128 sequences of
+    // 1024 .. 2048: 48.6 us, with 2 51.6; with 16 heads 25.7, with 2 27.7).
+    a.part_cost = S::LATENT ? 4 : S::N <= 32 ? 2 : 3;
     a.least_share = 1;
     a.team_inv = a.team > 1 ? (uint32_t)(((1ull << 32) + a.team - 1) / a.team) : 0;
     const int grid = sms * S::OCC / a.team * a.team;
@@ -86,6 +89,8 @@ void launch(const Params& p, bool latent, int head_dim, int v_dim, int rows, int
     XTG_REQUIRE(slots < (1ll << 31), "kv16: too many row blocks in one call");
     a.slots = (int)slots;
     const int64_t items = slots * a.kv_heads * a.team;
+    // Few items have many parts each, and a join per item is spread over more threads (1 x 4096: 12.4 us, by CTA 14.5; 6 x 4096
+    // with 6 KV heads 16.9 and 19.9); more have few parts (32 latent sequences of 8192: by CTA 77.9 us, by item 81.6).
     a.by_item = items <= grid / 4;
     static std::atomic<uint64_t> optin;
     const void* kernel = reinterpret_cast<const void*>(&attention_kernel<S>);
