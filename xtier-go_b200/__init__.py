@@ -635,8 +635,8 @@ def gen(what, seed, stream_id, a, b, out):
 
 KV4_PAGE = 64
 
-_KV4_ERRORS = {1: "a device wait timed out", 6: "a position lies past its sequence's page table",
-               7: "a page table entry lies past the pool"}
+_CACHE_ERRORS = {1: "a device wait timed out", 6: "a position lies past its sequence's page table",
+                 7: "a page table entry lies past the pool"}
 _kv4_module = None
 _kv16_module = None
 _kv4_dtypes = {}   # torch dtype -> the C ABI's code
@@ -676,12 +676,16 @@ def kv4_pool(pages, kv_heads, head_dim, device="cuda"):
     return torch.zeros((pages, kv_heads, 72 * head_dim), dtype=torch.uint8, device=device)
 
 
-def kv4_check(err):
-    """Wait for err's device, raise XtgError for a recorded error and clear it."""
+def _check(name, err):
     code = int(err.item())
     if code:
         err.zero_()
-        raise XtgError("kv4: " + _KV4_ERRORS.get(code, f"error {code}"))
+        raise XtgError(f"{name}: " + _CACHE_ERRORS.get(code, f"error {code}"))
+
+
+def kv4_check(err):
+    """Wait for err's device, raise XtgError for a recorded error and clear it."""
+    _check("kv4", err)
 
 
 def kv4_store(pool, k, v, table, pos, cu_rows, err=None):
@@ -714,7 +718,7 @@ def kv4_attention(q, pool, table, pos, cu_rows, scale, window=0, rows_per_seq=No
 # 16-byte multiples (a transposed view of [pages][page][kv_heads][dim] serves); (head_dim, v_dim) (64, 64), (128, 128),
 # (256, 256) or (192, 128), `page` positions a page (16, 32, .. 1024). A latent cache is one pool [pages][page][latent + 64]
 # (latent 256 or 512): a latent vector, which is both the value and a part of the key, and 64 rotated dims of key that
-# all heads share. table, pos, cu_rows and err are as the 4-bit cache's; kv4_check raises what err holds.
+# all heads share. table, pos, cu_rows and err are as the 4-bit cache's; kv16_check raises what err holds.
 # ----------------------------------------------------------------------------------------------------------------
 
 def _kv16():
@@ -734,6 +738,11 @@ def latent_pool(pages, latent, dtype=None, page=64, device="cuda"):
     """An empty pool of latent vectors with their rotated keys."""
     import torch
     return torch.zeros((pages, page, latent + 64), dtype=dtype or torch.bfloat16, device=device)
+
+
+def kv16_check(err):
+    """Wait for err's device, raise XtgError for an error that a call on a 16-bit cache recorded and clear it."""
+    _check("kv16", err)
 
 
 def kv16_append(k_pool, v_pool, k, v, table, pos, cu_rows, freq=None, q=None, first=0, interleaved=False, err=None):

@@ -1,4 +1,4 @@
-// Internal interface of the 16-bit paged caches (kv16.cu: append with rotation, kv16_attn.cu: attention).
+// Internal interface of the 16-bit paged caches (kv16.cu: append with rotation, kv16_attn.cuh: attention).
 #pragma once
 
 #include <cuda_runtime.h>

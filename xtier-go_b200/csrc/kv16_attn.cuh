@@ -70,7 +70,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // (128 steps: 1520), over 16383 190 -> 196 (232), 64 sequences of 16384 .. 32768 positions in bf16 702 -> 706 (729).
 template <class T>
 constexpr int kFoldSteps = std::is_same<T, __half>::value ? 256 : 1024;
-constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;   // of a thread of the 8 softmax warps and of the 4 others, where there are 12
+// Registers of a thread of the 8 softmax warps and of the 4 others, where there are 12. The compiler works with the 168 of the
+// launch for all: with 128 rows and chunks of 128 positions it spills 24 bytes.
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
 
 template <class T_, int DK_, int DV_, bool LATENT_, int N_>
 struct Shape {
