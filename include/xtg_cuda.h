@@ -343,8 +343,10 @@ XTG_CUDA_API int xtg_cuda_kv16_append(const xtg_cuda_kv16* c, const xtg_cuda_kv1
 // keys and values are appended first): softmax(scale q . K) V into out [rows][heads][v_dim], contiguous, of the cache's
 // type. Of a latent cache q is [rows][heads][v_dim], q_rot [rows][heads][64] (strides r_row, r_head). heads a multiple
 // of kv_heads (at most 32768 times as many), q head j reads KV head j / (heads / kv_heads). A row that sees nothing
-// gives zeros. Keys and values at positions that a row does not see are not read into its result, whatever they are.
-// rows_per_seq >= 1: about how many rows a sequence has; it chooses the tiling only. zero_rest: rows that are no
+// gives zeros. Keys and values at positions that a row does not see are not read into its result, whatever they are. A dim
+// of a row is finite where the values that it sees are; where one is not, it is an infinity or NaN, which of them is left
+// open: beside a weight that rounded to zero it depends on the tiling. rows_per_seq >= 1: about how many rows a sequence
+// has; it chooses the tiling only. zero_rest: rows that are no
 // sequence's become zeros, else they are left alone. workspace: device memory of at least xtg_cuda_kv16_workspace
 // bytes, 16-byte aligned, not shared by calls that may overlap. Sums and softmax are f32, the probabilities are rounded
 // to the cache's type; a call's result does not depend on timing (no atomics on values).

@@ -539,7 +539,8 @@ __device__ __forceinline__ void drop_unbounded(uint4& x, __nv_bfloat16) { drop_u
 __device__ __forceinline__ void drop_unbounded(uint4& x, __half) { drop_unbounded(x, 0x7c007c00u, 0x04000400u); }
 
 // Adds V's infinities and NaN of dim d, which drop_unbounded has taken out of the part's chunks where some of the block's
-// rows see a position, to the rows r0 .. r0 + 15 that do: a weight above zero times these is these.
+// rows see a position, to the rows r0 .. r0 + 15 that do: a weight above zero times these is these. (Where all rows see them they
+// stay in the product, and a weight that rounded to zero makes NaN of an infinity, as a part's weight of zero does in the join.)
 template <class S>
 __device__ __forceinline__ void add_unbounded(const Params& a, const Part& p, int d, int r0, uint32_t j0, float (&o)[16]) {
   using T = typename S::T;
