@@ -757,8 +757,9 @@ def kv16_append(k_pool, v_pool, k, v, table, pos, cu_rows, freq=None, q=None, fi
 def kv16_attention(q, k_pool, v_pool, table, pos, cu_rows, scale, window=0, rows_per_seq=None, out=None, err=None):
     """Attention of rows q [rows][heads][head_dim] (the pools' type) over the cached positions up to each row's own
     (window > 0: the last `window` of these), after the call's rows were appended: [rows][heads][v_dim]. rows_per_seq: about
-    how many rows a sequence has (default rows / seqs); it chooses the tiling only. Rows past cu_rows' last entry are
-    zeros, or left as they are in a given out."""
+    how many rows a sequence has (default rows / seqs); it chooses one tiling for the whole call, nothing else, so prompts of
+    some thousand rows go in a call of their own rather than beside single tokens. Rows past cu_rows' last entry are zeros,
+    or left as they are in a given out."""
     return _kv16().attention(k_pool, v_pool, table, pos, cu_rows, err, q, None, scale, window, rows_per_seq, out)
 
 
