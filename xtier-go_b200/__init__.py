@@ -630,7 +630,7 @@ def gen(what, seed, stream_id, a, b, out):
 # page table[i][p // 64], and a negative table entry or position holds nothing. table [seqs][max_pages], pos [seqs] and
 # cu_rows [seqs + 1] are int32 CUDA tensors, read when the call runs on the current stream of pool's device. err (an
 # int32 CUDA tensor of one word, or None) records positions past the table and pages past the pool, which hold nothing;
-# kv4_check raises what it holds.
+# kv4_check raises what it holds. The calls are forward only: results carry no gradient, whatever q, k and v require.
 # ----------------------------------------------------------------------------------------------------------------
 
 KV4_PAGE = 64
@@ -719,6 +719,7 @@ def kv4_attention(q, pool, table, pos, cu_rows, scale, window=0, rows_per_seq=No
 # (256, 256) or (192, 128), `page` positions a page (16, 32, .. 1024). A latent cache is one pool [pages][page][latent + 64]
 # (latent 256 or 512): a latent vector, which is both the value and a part of the key, and 64 rotated dims of key that
 # all heads share. table, pos, cu_rows and err are as the 4-bit cache's; kv16_check raises what err holds.
+# The calls are forward only: results carry no gradient, whatever q, k and v require.
 # ----------------------------------------------------------------------------------------------------------------
 
 def _kv16():
