@@ -676,7 +676,7 @@ def kv4_pool(pages, kv_heads, head_dim, device="cuda"):
     return torch.zeros((pages, kv_heads, 72 * head_dim), dtype=torch.uint8, device=device)
 
 
-def _check(name, err):
+def _raise_recorded(name, err):
     code = int(err.item())
     if code:
         err.zero_()
@@ -685,7 +685,7 @@ def _check(name, err):
 
 def kv4_check(err):
     """Wait for err's device, raise XtgError for a recorded error and clear it."""
-    _check("kv4", err)
+    _raise_recorded("kv4", err)
 
 
 def kv4_store(pool, k, v, table, pos, cu_rows, err=None):
@@ -743,7 +743,7 @@ def latent_pool(pages, latent, dtype=None, page=64, device="cuda"):
 
 def kv16_check(err):
     """Wait for err's device, raise XtgError for an error that a call on a 16-bit cache recorded and clear it."""
-    _check("kv16", err)
+    _raise_recorded("kv16", err)
 
 
 def kv16_append(k_pool, v_pool, k, v, table, pos, cu_rows, freq=None, q=None, first=0, interleaved=False, err=None):
