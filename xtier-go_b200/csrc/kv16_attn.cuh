@@ -66,8 +66,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Steps of 16 positions that the matrix unit adds up before its sum goes to f32 sums in the workspace. It cuts its sums off
 // towards zero, about two units of their last place a step: values of one sign came out 7.9e-4 small over 8192 steps (131072
 // positions), 1.6 times half a step of f16. So after 256 steps 2.5e-5, a twentieth of half a step of f16, after 1024 1e-4, a
-// fortieth of half a step of bf16. What it costs: f16 prompts of 128 rows with heads of 256 over 30000 positions 1242 -> 1315 us
-// (128 steps: 1520), over 16383 190 -> 196 (232), 64 sequences of 16384 .. 32768 positions in bf16 702 -> 706 (729).
+// fortieth of half a step of bf16. What it costs: f16 prompts of 128 rows with heads of 256 over 30000 positions 1207 -> 1264 us
+// (with 128 steps 10 % more), over 16383 190 -> 194; the others at most 1 %.
 template <class T>
 constexpr int kFoldSteps = std::is_same<T, __half>::value ? 256 : 1024;
 // Registers of a thread of the 8 softmax warps and of the 4 others, where there are 12. The compiler works with the 168 of the
@@ -566,6 +566,68 @@ __device__ __forceinline__ void add_unbounded(const Params& a, const Part& p, in
   }
 }
 
+// A group's columns of o from tensor memory to its threads' f32 sums, 4 rows of a tile every 128 float4: (first ? 0 : these scaled
+// to the rows' references) + o; unless `bad`. kept: the reference of row `own`'s sums; the new one. Functions of their own: within
+// the kernel they made calls of many short parts 5 % slower (4096 x 1 token over 128 positions 345 -> 361 us, so 355), although none
+// of these comes here.
+template <class S>
+__device__ __noinline__ float take_out(uint32_t taddr, float4* sums, const float* ref, float* scale, float kept, bool first,
+                                       bool bad, int bar) {
+  const int own = threadIdx.x & 127;
+  named_bar_sync(bar, 128);   // what was in `scale` was read
+  if (own < S::NW) {
+    const float now = ref[own];
+    scale[own] = kept == now ? 1.f : ex2_approx(kept - now);
+    kept = now;
+  }
+  named_bar_sync(bar, 128);
+  if (bad) return kept;
+  tc_fence_after();
+  constexpr int kAtOnce = S::NW < 32 ? S::NW : 32;   // rows whose sums are on the way at once
+#pragma unroll 1
+  for (int m = 0; m < S::DT; ++m)
+#pragma unroll 1
+    for (int r0 = 0; r0 < S::NW; r0 += kAtOnce) {
+      float4 x[kAtOnce / 4];
+      float4* const at = sums + (m * S::NW + r0) / 4 * 128;
+#pragma unroll
+      for (int j = 0; j < kAtOnce / 4; ++j) x[j] = first ? make_float4(0.f, 0.f, 0.f, 0.f) : at[j * 128];
+#pragma unroll
+      for (int r = 0; r < kAtOnce; r += 16) {
+        float o[16];
+        tmem_ld16(taddr + m * S::N + r0 + r, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(scale + r0 + r + j), old = x[(r + j) / 4];
+          at[(r + j) / 4 * 128] = make_float4(fmaf(old.x, f.x, o[j]), fmaf(old.y, f.y, o[j + 1]), fmaf(old.z, f.z, o[j + 2]),
+                                              fmaf(old.w, f.w, o[j + 3]));
+        }
+      }
+    }
+  return kept;
+}
+// and back: o + these x scale
+template <class S>
+__device__ __noinline__ void bring_back(uint32_t taddr, const float4* sums, const float* scale) {
+#pragma unroll 1
+  for (int m = 0; m < S::DT; ++m)
+#pragma unroll 1
+    for (int r = 0; r < S::NW; r += 16) {
+      float o[16];
+      tmem_ld16(taddr + m * S::N + r, o);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const float4 x = sums[(m * S::NW + r + j) / 4 * 128], f = *reinterpret_cast<const float4*>(scale + r + j);
+        o[j] = fmaf(x.x, f.x, o[j]), o[j + 1] = fmaf(x.y, f.y, o[j + 1]);
+        o[j + 2] = fmaf(x.z, f.z, o[j + 2]), o[j + 3] = fmaf(x.w, f.w, o[j + 3]);
+      }
+      tmem_st16(taddr + m * S::N + r, o);
+    }
+  tmem_st_wait();
+}
+
 // ---- the CTA's shared memory ----
 
 constexpr int kInfo = 16, kQueue = 4;
@@ -938,7 +1000,6 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
     // this thread's columns of o's tiles, 4 rows at a time, as far as they were taken from tensor memory
     float4* const fold = reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(a.work) + fold_offset<S>(gridDim.x)) +
                          (blockIdx.x * fold_floats<S>() + wg * (S::DT * 128 * S::NW)) / 4 + own;
-    auto folded = [&](int m, int r) { return fold + (m * S::NW + r) / 4 * 128; };
     const int box = min(1 << a.page_log2, S::C);
     const uint32_t all_pieces = (1u << (S::C / box)) - 1;
 
@@ -1181,37 +1242,7 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
         if (i > 0 && i % S::kFold == 0) {   // the second product of this chunk starts a new sum, the last one goes to the others
           const uint32_t b = (chunk - 1) % S::PB;
           if (S::PB > 1) bad = !__all_sync(0xffffffffu, bounded(&c.pdone[b], ((chunk - 1) / S::PB) & 1)) || bad;
-          constexpr int kAtOnce = S::NW < 32 ? S::NW : 32;   // rows whose sums are on the way at once
-          named_bar_sync(bar, 128);   // alpha was read
-          if (own < S::NW) {
-            alpha[own] = kept == ref[own] ? 1.f : ex2_approx(kept - ref[own]);
-            kept = ref[own];
-          }
-          named_bar_sync(bar, 128);
-          if (!bad) {
-            tc_fence_after();
-#pragma unroll 1
-            for (int m = 0; m < S::DT; ++m)
-#pragma unroll 1
-              for (int r0 = 0; r0 < S::NW; r0 += kAtOnce) {
-                float4 x[kAtOnce / 4];
-#pragma unroll
-                for (int j = 0; j < kAtOnce / 4; ++j)
-                  x[j] = i == S::kFold ? make_float4(0.f, 0.f, 0.f, 0.f) : *folded(m, r0 + 4 * j);
-#pragma unroll
-                for (int r = 0; r < kAtOnce; r += 16) {
-                  float o[16];
-                  tmem_ld16(lanes + S::kO + m * S::N + wg * S::NW + r0 + r, o);
-                  tmem_ld_wait();
-#pragma unroll
-                  for (int j = 0; j < 16; j += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(alpha + r0 + r + j), old = x[(r + j) / 4];
-                    *folded(m, r0 + r + j) = make_float4(fmaf(old.x, f.x, o[j]), fmaf(old.y, f.y, o[j + 1]),
-                                                         fmaf(old.z, f.z, o[j + 2]), fmaf(old.w, f.w, o[j + 3]));
-                  }
-                }
-              }
-          }
+          kept = take_out<S>(lanes + S::kO + wg * S::NW, fold, ref, alpha, kept, i == S::kFold, bad, bar);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -1246,10 +1277,11 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
           ml[0] = ref[own];
           ml[S::N] = sum;
         }
-        ref[own] = kept == ref[own] ? 1.f : ex2_approx(kept - ref[own]);   // what the sums in the workspace are scaled by
+        if (count > S::kFold) ref[own] = kept == ref[own] ? 1.f : ex2_approx(kept - ref[own]);   // what the sums in the workspace are scaled by
       }
       named_bar_sync(bar, 128);
       tc_fence_after();
+      if (count > S::kFold) bring_back<S>(lanes + S::kO + wg * S::NW, fold, ref);
       const int mine_rows = min(S::NW, pairs - wg * S::NW);
       const bool has_dim = S::MO == 128 || lane < 16;
       const int dim0 = S::MO == 128 ? 32 * quarter + lane : 16 * quarter + (lane & 15);
@@ -1264,13 +1296,6 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
           if (count > 0) {
             tmem_ld16(lanes + S::kO + m * S::N + wg * S::NW + r, o);
             tmem_ld_wait();
-            if (count > S::kFold)
-#pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const float4 x = *folded(m, r + j), f = *reinterpret_cast<const float4*>(ref + r + j);
-                o[j] = fmaf(x.x, f.x, o[j]), o[j + 1] = fmaf(x.y, f.y, o[j + 1]);
-                o[j + 2] = fmaf(x.z, f.z, o[j + 2]), o[j + 3] = fmaf(x.w, f.w, o[j + 3]);
-              }
           }
           const int d = m * S::MO + dim0;
           if (add && has_dim) add_unbounded<S>(a, p, d, wg * S::NW + r, j0, o);
