@@ -347,9 +347,9 @@ XTG_CUDA_API int xtg_cuda_kv16_append(const xtg_cuda_kv16* c, const xtg_cuda_kv1
 // of a row is finite where the values that it sees are; where one is not, it is an infinity or NaN, which of them is left
 // open: beside a weight that rounded to zero it depends on the tiling. rows_per_seq >= 1: about how many rows a sequence
 // has; it chooses one tiling for all sequences of the call, nothing else. Where it fits few of them calls are slow: a prompt's
-// 2000 rows beside 63 single tokens over 8192 .. 16384 positions (24 q / 6 KV heads of 128) take 971 us with the mean of 33,
-// 382 with 1, and 464 as two calls, prompts apart from single tokens; beside 15 single tokens over 4096 at most 202 with the
-// mean, 179 with 1, 130 as two calls; 512 rows beside 63 370, 371 and 404. So calls with prompts of some thousand rows
+// 2000 rows beside 63 single tokens over 8192 .. 16384 positions (24 q / 6 KV heads of 128) take 970 us with the mean of 33,
+// 380 with 1, and 456 as two calls, prompts apart from single tokens; beside 15 single tokens over 4096 at most 203 with the
+// mean, 174 with 1, 131 as two calls; 512 rows beside 63 366, 364 and 400. So calls with prompts of some thousand rows
 // do well to have them alone. zero_rest: rows that are no sequence's become zeros, else they are left alone. workspace: device
 // memory of at least xtg_cuda_kv16_workspace bytes, 16-byte aligned, not shared by calls that may overlap. Sums and softmax
 // are f32, the probabilities are rounded to the cache's type (f16: those below 2^-29 of a row's largest may become zeros); a

@@ -68,9 +68,9 @@ def test_long_parts(xtg, cuda, d, dv, latent, heads, rows, rise, dtype):
     want, spread = reference(q, k, v, table)
     off = got[0] - want
     # h: half a step. The output's rounding; the weights' (numerator and sum alike, so of the values' spread); the scores' sums
-    # as kv16_ref.tolerance has them, of the spread; ex2 and factors. Sums over positions: the matrix unit adds 256 steps of 16 for f16, 1024
-    # for bf16, each cut off up to four times (by 2^-23); these and the weights are then added in f32 (at most 32 and 1024 of
-    # them, 2^-24).
+    # as kv16_ref.tolerance has them, of the spread; ex2 and factors. Sums over positions: the matrix unit adds 256 steps of 16
+    # for f16, 1024 for bf16, each cut off up to four times (by 2^-23); these and the weights are then added in f32 (at most 32
+    # and 1024 of them, 2^-24).
     h = torch.finfo(dtype).eps / 2
     steps = 256 if dtype == F16 else 1024
     sums = steps * 4 * 2.0 ** -23 + (32 + 1024) * 2.0 ** -24 + 2.0 ** -20

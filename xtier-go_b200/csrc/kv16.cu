@@ -8,10 +8,10 @@
 // One pass: a CTA takes some rows with all their heads, so that a row's angles, its sequence, page and slot are worked out
 // once. 8 dims a thread (two times 8, of a pair's two halves), 16-byte loads and stores.
 //
-// Measured (B200, device time): 8 prompts of 2048 .. 4096 rows with 16 q / 4 KV heads of 256 f16 in 116 us, 5.8 TB/s of what
-// is read and written, 88 % of a copy's rate (128 us, 80 %, in runs on changing data); 4 x 4096 rows of a latent cache with 128
-// q heads, interleaved, in 110 us, 80 %; one row in 3.4 us: one launch, then the row's sequence, page and angles one after
-// another.
+// Measured (B200, device time): 8 prompts of 2048 .. 4096 rows with 16 q / 4 KV heads of 256 f16 in 117 us, 5.8 TB/s of what
+// is read and written, 88 % of a copy's rate (125 to 129 us in runs on changing data), issue slots 71 % busy, interleaved in 124
+// us; 4 x 4096 rows of a latent cache with 128 q heads, interleaved, in 110 us, 80 %; one row in 3.3 us: one launch, then the
+// row's sequence, page and angles one after another.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, INTERLEAVED ? 5 : 7) append_kernel(c
     }
   } else {
     // a thread has two pieces on the way as it is: all parts of all rows in turn, with few registers and so many threads (with
-    // the loop above and 95 registers the largest case took 239 us, with 34 it takes 121)
+    // the loop above and 95 registers the largest case took 239 us, with 32 it takes 117)
     for (int i = threadIdx.x; i < rows * n; i += kThreads) {
       const int r = i / n;
       const Place p = place(i - r * n);

@@ -20,16 +20,17 @@
 // in order. The warps of a CTA: one walks the share and issues the copies, one issues the products, the others are the
 // softmax's. Every wait is bounded.
 //
-// What bounds it (B200, bf16, device time, bytes or flops that cannot be done without against a copy's 6.54 TB/s and 1692
-// TFLOP/s): with few rows the cache's bytes: 64 sequences of 16384 .. 32768 positions, 24 q / 6 KV heads of 128, 715 us, 6.7
-// TB/s; 8 rows each of 64 sequences of 4096 .. 8192 205 us, 6.0 TB/s. With one short sequence latency: 1 x 4096 in 12 us, of
-// which the start and the plan are 2, the first tile and its softmax 3, the others 2, the end 1.5 and the join 3.5. With 128
-// rows a chunk's chain of waits: scores from tensor memory, the vote, exponentials, P back, 1.75 us at heads of 128, of which
-// shared memory needs 0.95 (the products read 128 KB, the copies and P write 96 KB, at 128 bytes a cycle): 8192 rows from
-// position 0 with heads of 192 / 128 492 us, 700 TFLOP/s. A latent cache's tile takes 72 KB and q 72 KB, so there are two
-// slots and a slot's time is copy, first product, softmax, second product one after another: 64 sequences of 8192 .. 16384
-// positions with 16 heads in 164 us, 5.5 TB/s, with 64 in 208, with 128 in 353 us, 620 TFLOP/s (the products alone, at their
-// measured rates, 170).
+// What bounds it (B200, bf16, device time, bytes or flops that cannot be done without against 7.43 TB/s of reading and 1692
+// TFLOP/s): with few rows the cache's bytes: 64 sequences of 16384 .. 32768 positions, 24 q / 6 KV heads of 128, 690 us,
+// 7.0 TB/s; 8 rows each of 64 sequences of 4096 .. 8192 197 us, 6.3 TB/s. With one short sequence latency: 1 x 4096 in 12
+// us, of which the start and the plan are 2, the first tile and its softmax 3, the others 2, the end 1.5 and the join 3.5.
+// With 128 rows a chunk's chain of waits: scores from tensor memory, the vote, exponentials, P back, 1.75 us at heads of
+// 128, of which shared memory needs 0.95 by reckoning (the products read 128 KB, the copies and P write 96 KB, at 128 bytes
+// a cycle); the tensor pipe is busy 23 % of a prompt's time, issue slots 33 %: 8192 rows from position 0 with heads of 192
+// / 128 485 us, 710 TFLOP/s. A latent cache's tile takes 72 KB and q 72 KB, so there are two slots and a slot's time is
+// copy, first product, softmax, second product one after another: 64 sequences of 8192 .. 16384 positions with 16 heads in
+// 163 to 184 us, up to 5.5 TB/s, with 64 in 211, with 128 in 349 us, 620 TFLOP/s (the products alone, at their measured
+// rates, 170).
 // Tried and not taken: four groups of softmax warps for 64 and 128 rows (within 5 %, mostly slower), blocks of 64 rows side by
 // side in place of 128 (products of 64 rows read shared memory as often for half the work: 185 -> 233 us), tiles in pieces of
 // 128 dims with barriers of their own (20 % slower for latent caches), warps of their own for q (4 % faster for prompts, 4 to
@@ -1277,7 +1278,8 @@ __global__ void __launch_bounds__(S::kThreads, S::OCC) attention_kernel(const __
           ml[0] = ref[own];
           ml[S::N] = sum;
         }
-        if (count > S::kFold) ref[own] = kept == ref[own] ? 1.f : ex2_approx(kept - ref[own]);   // what the sums in the workspace are scaled by
+        // what the sums in the workspace are scaled by
+        if (count > S::kFold) ref[own] = kept == ref[own] ? 1.f : ex2_approx(kept - ref[own]);
       }
       named_bar_sync(bar, 128);
       tc_fence_after();
