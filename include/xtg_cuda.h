@@ -343,9 +343,9 @@ XTG_CUDA_API int xtg_cuda_kv16_append(const xtg_cuda_kv16* c, const xtg_cuda_kv1
 // keys and values are appended first): softmax(scale q . K) V into out [rows][heads][v_dim], contiguous, of the cache's
 // type. Of a latent cache q is [rows][heads][v_dim], q_rot [rows][heads][64] (strides r_row, r_head). heads a multiple
 // of kv_heads (at most 32768 times as many), q head j reads KV head j / (heads / kv_heads). A row that sees nothing
-// gives zeros. Keys and values at positions that a row does not see are not read into its result, whatever they are. A dim
-// of a row is finite where the values that it sees are; where one is not, it is an infinity or NaN, which of them is left
-// open: beside a weight that rounded to zero it depends on the tiling. rows_per_seq >= 1: about how many rows a sequence
+// gives zeros. Keys and values at positions that a row does not see are not read into its result, whatever they are. A value
+// that is not finite makes its dim of the rows that see it not finite and nothing else; whether an infinity becomes one or
+// NaN is left open (beside a weight that rounded to zero it depends on the tiling). rows_per_seq >= 1: about how many rows a sequence
 // has; it chooses one tiling for all sequences of the call, nothing else. Where it fits few of them calls are slow: a prompt's
 // 2000 rows beside 63 single tokens over 8192 .. 16384 positions (24 q / 6 KV heads of 128) take 970 us with the mean of 33,
 // 380 with 1, and 456 as two calls, prompts apart from single tokens; beside 15 single tokens over 4096 at most 203 with the

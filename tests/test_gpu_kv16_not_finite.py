@@ -1,5 +1,5 @@
-"""GPU: values of the 16-bit caches that are not finite, where scores lie so far apart that weights round to zero: a dim of a row
-is finite exactly where all the values that the row sees are, whatever the tiling; and what carries no gradient."""
+"""GPU: values of the 16-bit caches that are not finite, where scores lie so far apart that weights round to zero: each makes its
+dim of the rows that see it not finite and nothing else, whatever the tiling; and what carries no gradient."""
 import math
 
 import pytest

@@ -68,7 +68,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // towards zero, about two units of their last place a step: values of one sign came out 7.9e-4 small over 8192 steps (131072
 // positions), 1.6 times half a step of f16. So after 256 steps 2.5e-5, a twentieth of half a step of f16, after 1024 1e-4, a
 // fortieth of half a step of bf16. What it costs: f16 prompts of 128 rows with heads of 256 over 30000 positions 1207 -> 1264 us
-// (with 128 steps 10 % more), over 16383 190 -> 194; the others at most 1 %.
+// (with 128 steps 10 % more), over 16383 190 -> 194; calls of many short parts 3 % (take_out), the others at most 1 %.
 template <class T>
 constexpr int kFoldSteps = std::is_same<T, __half>::value ? 256 : 1024;
 // Registers of a thread of the 8 softmax warps and of the 4 others, where there are 12. The compiler works with the 168 of the
